@@ -827,6 +827,97 @@ size_t pt_mlstm_workspace_bytes(int n_tok, int n_seq, int heads, int dim, int vd
 size_t pt_mlstm_state_floats(int heads, int dim, int vdim, int which);
 int pt_mlstm(const pt_mlstm_args *args, void *stream);
 
+/* ---- speculative steps over the paged caches ---------------------------------------------------------------------------
+ * Several drafted tokens of a sequence run through the model at once, a tree of them: attention (pt_tree_attn), the target's decision
+ * which of them stand (pt_verify_drafts), and the caches put right afterwards (pt_kv_move_rows, pt_kv_copy_pages).
+ *
+ * pt_tree_attn (csrc/tree_attn.cu): row cu[s] + i of the batch is drafted token i of sequence s, behind start[s] cached positions; its
+ * parent is token parent[cu[s] + i] < i of the same sequence, or -1 for one that follows the cached positions (NULL: every token follows
+ * the one before it).  With depth 0 for those and one more than the parent's for the others, token i
+ *   - is cached at position start[s] + i (keys and values are appended before anything is read), and rotated, like its query, by the
+ *     angles of position start[s] + depth: rope as in pt_window_attn; q itself is left as it is;
+ *   - sees its ancestors, itself and every cached position, as far as they are less than `window` positions back (0: all; an ancestor
+ *     counts by its depth).
+ * pool and page_table as in pt_window_attn (grouped heads, key and value widths of their own, at most 256 each); softcap likewise.  A row that
+ * no sequence has (from cu[n_seq] on) is neither read nor written.  A sequence of more than max_tokens_per_seq tokens (at most 256) sets error_flag to 14,
+ * one whose positions reach max_len to 12: its rows are then left as they were.  A parent that is none sets it to 14 and counts as -1.  Values that a row does
+ * not see may be infinite or NaN. */
+typedef struct pt_tree_attn_args {
+  pt_batch_view batch;    /* at most 1024 sequences                                  */
+  int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16: q, k, v, pool and out */
+  int n_head, n_kv, dim, vdim, page_size, max_pages;
+  int max_len;            /* no position reaches this (0 = page_size * max_pages)    */
+  int window;
+  float scale, softcap;
+  const int32_t *parent;
+  const void *q;
+  int q_ld;
+  const void *k, *v;
+  int kv_ld;
+  void *pool;
+  const int32_t *page_table;
+  int rope_dims;
+  const float *rope;
+  void *out;              /* [n_tok, out_ld], columns n_head * vdim .. out_cols - 1 are zeroed (0 = out_ld) */
+  int out_ld, out_cols;
+  int max_tokens_per_seq; /* most drafted tokens of one sequence (0 = n_tok)         */
+  int plain;              /* 1: the kernel for any sizes, whatever the shape         */
+  void *workspace;        /* pt_tree_attn_workspace_bytes, 16-byte aligned; what it holds does not matter */
+  size_t workspace_bytes;
+  int32_t *error_flag;    /* optional; also set to 11 when a bounded wait gave up    */
+} pt_tree_attn_args;
+size_t pt_tree_attn_workspace_bytes(int n_seq, int max_tokens_per_seq, int n_head, int n_kv, int vdim);
+int pt_tree_attn(const pt_tree_attn_args *args, void *stream);
+
+/* pt_verify_drafts (csrc/verify.cu): which drafted tokens the target accepts.  Row cu[s] of the logits belongs to the last known token of
+ * sequence s (the root), the other rows up to cu[s + 1] to its drafted tokens, whose parents are rows of the sequence in front of them
+ * (parent NULL: the row before).  From the root down, the children of a row are looked at in their order; the first that is accepted is
+ * the next row.  With p = softmax(logits / temperature) of the row, child c with token x and random number u = uniform[c]:
+ *   draft != NULL   (children are independent draws from draft[row], a distribution)   accepted if u draft[x] Z < r[x]; r is p for the
+ *                   first child and max(p - S draft, 0) behind others, S the sum of the Z of those before; Z = sum of r
+ *   draft NULL      (children chosen some other way)                                   accepted if u Z < r[x]; r is p without the tokens of
+ *                   the children before
+ *   temperature NULL, or 0 for the sequence: accepted if x is the token of the largest logit (the lowest of equal ones).
+ * Behind the last accepted row one more token follows: the largest logit's, or one drawn from the r that its children left (from p where r
+ * is zero everywhere): the first whose running sum of r, in the order of the vocabulary, exceeds uniform_next[s] Z.
+ * path[s] = the accepted rows (0 = the root, counted from cu[s]), count[s] of them; token[s] = the tokens behind each of them, the last one
+ * drawn; logprob[s] (optional) = their log p (temperature 0: of temperature 1).  The rest of a row of max_path entries is -1 (logprob 0).
+ * A path of max_path rows is not followed further.  Logits may be -inf, and NaN counts as that; equal infinities share all the weight.  A
+ * row that is -inf everywhere accepts nothing and its token is -1.  Sums, residuals and the drawing are in 64 bits.
+ * A token outside the vocabulary, or a parent that is none, is never accepted. */
+typedef struct pt_verify_args {
+  int n_seq, n_tok;
+  const int32_t *cu;      /* [n_seq + 1]; a sequence without rows has count 0        */
+  int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16                      */
+  int vocab, logits_ld;
+  const void *logits;     /* [n_tok]                                                 */
+  const int32_t *token, *parent; /* [n_tok]; the root's entries are not read         */
+  const float *draft;     /* [n_tok, draft_ld] or NULL                               */
+  int draft_ld;
+  const float *temperature; /* [n_seq] or NULL                                       */
+  const float *uniform, *uniform_next; /* [n_tok], [n_seq], in [0, 1); not read at temperature 0 */
+  int max_path;
+  int32_t *path, *count, *out_token; /* [n_seq, max_path], [n_seq], [n_seq, max_path] */
+  float *logprob;
+} pt_verify_args;
+int pt_verify_drafts(const pt_verify_args *args, void *stream);
+
+/* Pages and rows of the caches of several layers that share a page numbering (csrc/pages.cu).  A page of a pool is K [n_kv][page_size][dim] and
+ * then V [n_kv][page_size][vdim]; pools is a host array, read before the call returns.
+ * pt_kv_copy_pages: page dst[i] <- page src[i] of every pool, i < n.  No page is written twice or both read and written in a call, unless it is its
+ *   own source.  Pairs with a negative page are left out; a page from n_pages on sets error_flag to 12 and is left out.
+ * pt_kv_move_rows: position start[s] + i <- position start[s] + path[s][i], i < count[s] (device arrays, as pt_verify_drafts writes them): the accepted
+ *   tokens of a sequence follow its cached positions.  A path that does not increase, or leaves the sequence's new tokens, sets error_flag to 14, positions
+ *   outside the table 12; the sequence is then left as it was. */
+typedef struct pt_kv_pool {
+  void *pool;
+  int n_kv, dim, vdim, elem_bytes;
+} pt_kv_pool;
+int pt_kv_copy_pages(const pt_kv_pool *pools_host, int n_pools, int page_size, int n_pages, const int32_t *src, const int32_t *dst, int n, int32_t *error_flag,
+                     void *stream);
+int pt_kv_move_rows(const pt_kv_pool *pools_host, int n_pools, int page_size, int max_pages, const int32_t *page_table, const pt_batch_view *batch,
+                    const int32_t *path, int path_ld, const int32_t *count, int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

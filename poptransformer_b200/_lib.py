@@ -117,6 +117,23 @@ class SsmArgs(ctypes.Structure):
                [("out_ld", c_int), ("plain", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class TreeAttnArgs(ctypes.Structure):
+    _fields_ = [("batch", BatchView), ("dtype", c_int), ("n_head", c_int), ("n_kv", c_int), ("dim", c_int), ("vdim", c_int), ("page_size", c_int), ("max_pages", c_int),
+                ("max_len", c_int), ("window", c_int), ("scale", c_float), ("softcap", c_float), ("parent", c_void_p), ("q", c_void_p), ("q_ld", c_int), ("k", c_void_p),
+                ("v", c_void_p), ("kv_ld", c_int), ("pool", c_void_p), ("page_table", c_void_p), ("rope_dims", c_int), ("rope", c_void_p), ("out", c_void_p), ("out_ld", c_int),
+                ("out_cols", c_int), ("max_tokens_per_seq", c_int), ("plain", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("error_flag", c_void_p)]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [("n_seq", c_int), ("n_tok", c_int), ("cu", c_void_p), ("dtype", c_int), ("vocab", c_int), ("logits_ld", c_int), ("logits", c_void_p), ("token", c_void_p),
+                ("parent", c_void_p), ("draft", c_void_p), ("draft_ld", c_int), ("temperature", c_void_p), ("uniform", c_void_p), ("uniform_next", c_void_p),
+                ("max_path", c_int), ("path", c_void_p), ("count", c_void_p), ("out_token", c_void_p), ("logprob", c_void_p)]
+
+
+class KvPool(ctypes.Structure):
+    _fields_ = [("pool", c_void_p), ("n_kv", c_int), ("dim", c_int), ("vdim", c_int), ("elem_bytes", c_int)]
+
+
 class MlstmArgs(ctypes.Structure):
     _fields_ = [("batch", BatchView)] + [(n, c_int) for n in ("dtype", "heads", "dim", "vdim")] + [(n, c_float) for n in ("gate_cap", "q_scale", "eps", "out_scale")] + \
                [(n, c_void_p) for n in ("q", "k", "v", "gate")] + [("ld", c_int), ("log_i", c_void_p), ("log_f", c_void_p), ("gate_ld", c_int)] + \
@@ -182,6 +199,11 @@ SIGNATURES = {
     "pt_mlstm_workspace_bytes": (c_size_t, [c_int] * 5),
     "pt_mlstm_state_floats": (c_size_t, [c_int] * 4),
     "pt_mlstm": (c_int, [ctypes.POINTER(MlstmArgs), c_void_p]),
+    "pt_tree_attn_workspace_bytes": (c_size_t, [c_int] * 5),
+    "pt_tree_attn": (c_int, [ctypes.POINTER(TreeAttnArgs), c_void_p]),
+    "pt_verify_drafts": (c_int, [ctypes.POINTER(VerifyArgs), c_void_p]),
+    "pt_kv_copy_pages": (c_int, [ctypes.POINTER(KvPool), c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "pt_kv_move_rows": (c_int, [ctypes.POINTER(KvPool), c_int, c_int, c_int, c_void_p, ctypes.POINTER(BatchView), c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "pt_hyper": (c_int, [ctypes.POINTER(HyperArgs), c_void_p]),
     "pt_window_attn_workspace_bytes": (c_size_t, [c_int] * 7),
     "pt_window_attn": (c_int, [ctypes.POINTER(WindowAttnArgs), c_void_p]),

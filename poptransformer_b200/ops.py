@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import (AttnArgs, BatchView, ContextRows, DenseExt, GemmArgs, HyperArgs, LatentAttnArgs, LatentContextArgs, LatentPrepArgs, LinearArgs, MlstmArgs,
-                   MoeRouteArgs, PostNormArgs, PtError, ShiftNormArgs, SsmArgs, WindowAttnArgs, check)
+                   MoeRouteArgs, PostNormArgs, PtError, ShiftNormArgs, SsmArgs, TreeAttnArgs, VerifyArgs, WindowAttnArgs, check)
 
 W_INT4, W_FP16, W_FP8, W_BF16 = 0, 1, 2, 3
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
@@ -472,6 +472,68 @@ def window_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, window=0, 
     check(_lib.lib().pt_window_attn(ctypes.byref(a), _stream()), "pt_window_attn")
 
 
+def tree_attn_workspace(n_seq, max_tokens_per_seq, n_head, n_kv, vdim, device="cuda"):
+    """Workspace of tree_attn calls that follow one another on a stream (any number of layers)."""
+    return torch.empty(_lib.lib().pt_tree_attn_workspace_bytes(n_seq, max_tokens_per_seq, n_head, n_kv, vdim), dtype=torch.uint8, device=device)
+
+
+def tree_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, parent=None, window=0, softcap=0.0, rope=None, rope_dims=0, max_tokens_per_seq=0, workspace=None,
+              error_flag=None, out_cols=0, plain=False):
+    """Attention of drafted tokens, a tree of them behind every sequence of `view`, over a paged cache (see pt_tree_attn).  qkv rows hold [q | k | v] of a
+    token; k and v are appended at the rows' own positions, the rotation and the window go by a token's depth.  parent: int32 [n_tok], counted
+    from the first token of a sequence, -1 for those that follow its cached positions (None: every token follows the one before)."""
+    a = TreeAttnArgs()
+    es, k = qkv.element_size(), _ptr(qkv)
+    a.batch, a.dtype = view, dtype_code(qkv.dtype)
+    if cache.pool.dtype != qkv.dtype or out.dtype != qkv.dtype:
+        raise PtError(f"tree_attn: rows {qkv.dtype}, cache {cache.pool.dtype}, out {out.dtype}: one type is wanted")
+    if parent is not None and (parent.dtype != torch.int32 or parent.numel() < view.n_tok):
+        raise PtError(f"tree_attn: parent is int32 of {view.n_tok} tokens, got {parent.dtype} {tuple(parent.shape)}")
+    a.n_head, a.n_kv, a.dim, a.vdim = n_head, cache.n_kv, cache.head_dim, cache.v_dim
+    a.page_size, a.max_pages, a.max_len = cache.page_size, cache.page_table.shape[1], cache.max_len
+    a.window, a.scale, a.softcap, a.parent = window, scale, softcap, _ptr(parent)
+    a.q, a.q_ld, a.kv_ld = k, qkv_ld, qkv_ld
+    a.k = k = k + n_head * cache.head_dim * es
+    a.v = k + cache.n_kv * cache.head_dim * es
+    a.pool, a.page_table, a.rope_dims, a.rope = _ptr(cache.pool), _ptr(cache.page_table), rope_dims, _ptr(rope)
+    a.out, a.out_ld, a.out_cols, a.max_tokens_per_seq, a.plain = _ptr(out), out_ld, out_cols, max_tokens_per_seq, 1 if plain else 0
+    a.workspace, a.workspace_bytes, a.error_flag = _ptr(workspace), workspace.numel() if workspace is not None else 0, _ptr(error_flag)
+    check(_lib.lib().pt_tree_attn(ctypes.byref(a), _stream()), "pt_tree_attn")
+    return out
+
+
+def verify_drafts(logits, cu, token, parent=None, max_path=None, draft=None, temperature=None, uniform=None, uniform_next=None, out=None):
+    """Which drafted tokens the target accepts, and the token behind them (see pt_verify_drafts).  logits [rows, vocab]: the first row of a sequence is its last
+    known token's, the others its drafts' in the order of `token` and `parent` (None: chains); cu int32 [n_seq + 1].  draft: fp32 [rows, vocab],
+    the distribution that a row's children were drawn from.  temperature: fp32 [n_seq] (None: greedy), uniform [rows] and uniform_next [n_seq] the
+    random numbers.  Returns (path, count, token, logprob): int32 [n_seq, max_path], [n_seq], [n_seq, max_path], fp32 [n_seq, max_path]
+    (`out`: the four tensors to use)."""
+    rows, vocab = logits.shape
+    n_seq = cu.numel() - 1
+    if token.numel() < rows or (parent is not None and parent.numel() < rows) or (draft is not None and tuple(draft.shape) != (rows, vocab)):
+        raise PtError(f"verify_drafts: {rows} rows of logits over {vocab} tokens, got {token.numel()} tokens, {None if parent is None else parent.numel()} parents, "
+                      f"draft {None if draft is None else tuple(draft.shape)}")
+    if temperature is not None and (uniform is None or uniform_next is None or uniform.numel() < rows or uniform_next.numel() < n_seq or temperature.numel() < n_seq):
+        raise PtError("verify_drafts: sampling needs a temperature and a random number per sequence, and one per row")
+    for name, t, dt in (("cu", cu, torch.int32), ("token", token, torch.int32), ("parent", parent, torch.int32), ("draft", draft, torch.float32),
+                        ("temperature", temperature, torch.float32), ("uniform", uniform, torch.float32), ("uniform_next", uniform_next, torch.float32)):
+        if t is not None and t.dtype != dt:
+            raise PtError(f"verify_drafts: {name} is {dt}, got {t.dtype}")
+    if out is None:
+        max_path = rows if max_path is None else max_path
+        i32 = dict(dtype=torch.int32, device=logits.device)
+        out = (torch.empty((n_seq, max_path), **i32), torch.empty(n_seq, **i32), torch.empty((n_seq, max_path), **i32),
+               torch.empty((n_seq, max_path), dtype=torch.float32, device=logits.device))
+    path, count, said, logprob = out
+    if path.shape != said.shape or path.shape != logprob.shape or path.shape[0] != n_seq or count.numel() != n_seq or (max_path is not None and path.shape[1] != max_path) or \
+            any(t.dtype != torch.int32 for t in out[:3]) or logprob.dtype != torch.float32:
+        raise PtError(f"verify_drafts: out is int32 [{n_seq}, max_path], [{n_seq}], [{n_seq}, max_path] and float32 [{n_seq}, max_path]")
+    a = VerifyArgs(n_seq, rows, _ptr(cu), dtype_code(logits.dtype), vocab, vocab, _ptr(logits), _ptr(token), _ptr(parent), _ptr(draft), vocab, _ptr(temperature), _ptr(uniform),
+                   _ptr(uniform_next), path.shape[1], _ptr(path), _ptr(count), _ptr(said), _ptr(logprob))
+    check(_lib.lib().pt_verify_drafts(ctypes.byref(a), _stream()), "pt_verify_drafts")
+    return out
+
+
 def latent_cache(rows, w, max_len, page_size=64, device="cuda", page_table=None, dtype=torch.bfloat16, n_pages=None):
     """Page pool of a latent attention layer: per position one row [rotated key part | latent] and padding."""
     return PagedKVCache(rows, 1, _lib.lib().pt_latent_row(w.rot_dim, w.rank), max_len, page_size, device, page_table, v_dim=0, dtype=dtype, n_pages=n_pages)
@@ -734,14 +796,17 @@ class PagedKVCache:
     are handed out on demand (cache.SequenceSlots) instead of max_len tokens per row."""
 
     def __init__(self, rows, n_kv, head_dim, max_len, page_size=64, device="cuda", page_table=None, extra_pages=0, v_dim=None, dtype=torch.float16,
-                 n_pages=None):
+                 n_pages=None, pool=None):
+        """pool: memory to use, for instance a layer's part of one tensor (its first dimension is the pages)."""
         self.rows, self.n_kv, self.head_dim, self.page_size = rows, n_kv, head_dim, page_size
         self.v_dim = head_dim if v_dim is None else v_dim
         self.max_len = max_len
         self.max_pages = (max_len + page_size - 1) // page_size
         n_pages = (rows * self.max_pages if n_pages is None else n_pages) + extra_pages
         shape = (n_pages, 2, n_kv, page_size, head_dim) if self.v_dim == head_dim else (n_pages, n_kv * page_size * (head_dim + self.v_dim))
-        self.pool = torch.zeros(shape, dtype=dtype, device=device)
+        if pool is not None and (pool.dtype != dtype or not pool.is_contiguous() or pool[0].numel() != n_kv * page_size * (head_dim + self.v_dim)):
+            raise PtError(f"PagedKVCache: pool {pool.dtype} {tuple(pool.shape)}, expected contiguous {dtype} pages of {n_kv * page_size * (head_dim + self.v_dim)} elements")
+        self.pool = torch.zeros(shape, dtype=dtype, device=device) if pool is None else pool
         if page_table is None:
             page_table = torch.arange(rows * self.max_pages, dtype=torch.int32, device=device).reshape(rows, self.max_pages)
         self.page_table = page_table
@@ -752,6 +817,44 @@ class PagedKVCache:
         check(_lib.lib().pt_kv_export(_ptr(self.pool), _ptr(self.page_table), _ptr(step), self.rows, self.n_kv, self.head_dim,
                                       self.page_size, self.max_pages, max_len, _ptr(out), _stream()), "pt_kv_export")
         return out
+
+
+class PagePools:
+    """The pools of a model's layers, which share one page numbering (and page table): what is copied or moved is copied in all of them by one launch."""
+
+    def __init__(self, caches):
+        caches = list(caches)
+        if not caches:
+            raise PtError("PagePools: no caches")
+        first = caches[0]
+        for c in caches:
+            if c.page_size != first.page_size or c.page_table is not first.page_table and (c.page_table.data_ptr(), c.page_table.shape) != (first.page_table.data_ptr(), first.page_table.shape):
+                raise PtError("PagePools: the caches share neither page size nor page table")
+        self.caches = caches                       # (keeps the pools alive)
+        self.page_size, self.page_table = first.page_size, first.page_table
+        self.n_pages = min(c.pool.shape[0] for c in caches)
+        self._pools = (_lib.KvPool * len(caches))(*[_lib.KvPool(_ptr(c.pool), c.n_kv, c.head_dim, c.v_dim, c.pool.element_size()) for c in caches])
+
+    def copy_pages(self, src, dst, error_flag=None):
+        """Page dst[i] <- page src[i] in every layer (int32 on the device; see pt_kv_copy_pages)."""
+        if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.numel() != dst.numel():
+            raise PtError(f"copy_pages: int32 pages, as many sources as destinations, got {src.dtype} {src.numel()} and {dst.dtype} {dst.numel()}")
+        check(_lib.lib().pt_kv_copy_pages(self._pools, len(self._pools), self.page_size, self.n_pages, _ptr(src), _ptr(dst), src.numel(), _ptr(error_flag), _stream()),
+              "pt_kv_copy_pages")
+
+    def copy(self, pairs):
+        """The same for a list of (source, destination), as SequenceSlots returns it."""
+        if pairs:
+            t = torch.tensor(pairs, dtype=torch.int32).T.contiguous().to(self.page_table.device)
+            self.copy_pages(t[0], t[1])
+
+    def move_rows(self, view, path, count, error_flag=None):
+        """The accepted rows of every sequence of `view` move to the positions behind its cached ones in every layer; path, count as verify_drafts
+        returns them (see pt_kv_move_rows)."""
+        if path.dtype != torch.int32 or count.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != view.n_seq or count.numel() != view.n_seq:
+            raise PtError(f"move_rows: int32 path [{view.n_seq}, max_path] and count [{view.n_seq}], got {path.dtype} {tuple(path.shape)}, {count.dtype} {tuple(count.shape)}")
+        check(_lib.lib().pt_kv_move_rows(self._pools, len(self._pools), self.page_size, self.page_table.shape[1], _ptr(self.page_table), ctypes.byref(view), _ptr(path), path.shape[1],
+                                         _ptr(count), _ptr(error_flag), _stream()), "pt_kv_move_rows")
 
 
 def attn_workspace(batch, n_head, head_dim, max_pages, device="cuda"):
