@@ -9,9 +9,14 @@
 //
 //   tree_prep_kernel      depths; rotates and appends the new keys and values; zeroes the output's padding columns
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
+//   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
 // Scores, softmax and sums are fp32.
+#include <type_traits>
+
 #include "chunk.cuh"
+#include "mbarrier.cuh"
+#include "tmem.cuh"
 
 namespace pt {
 namespace ta {
@@ -37,6 +42,7 @@ struct Params {
   const float2 *rope;
   const int *page_table, *cu, *start, *slot, *parent;
   int *error_flag;
+  bool out16;         // the output can be written in units of 16 bytes
   float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
   float2 *part_ml;    // [2 blocks][rows_tile]
 };
@@ -164,12 +170,15 @@ template <bool MASKS, typename Sync> __device__ __forceinline__ void build_tree(
         }
       }
     } else {
-      for (int u = i; u >= 0; u = t.parent[u], ++d)
+      for (int u = i; u >= 0; ++d) {
         if (MASKS && (p.window == 0 || d < p.window)) {
 #pragma unroll
           for (int k = 0; k < WORDS; ++k)
             if (u >> 5 == k) w[k] |= 1u << (u & 31);
         }
+        const int up = t.parent[u];
+        u = up < u ? up : -1;        // (ends whatever the array holds)
+      }
       --d;
     }
     t.depth[i] = d;
@@ -244,7 +253,7 @@ __device__ __forceinline__ float score2(const Params &p, float s) {
 // ------------------------------------------------------------------------------------------ any sizes
 // Rows and keys of a tile in shared memory as fp32; thread (ty, tx) has rows 2 ty, 2 ty + 1 and keys tx, tx + 8, .. of the scores, and columns 4 tx + 32 j of
 // the output.  What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them.
-constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32;
+constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32, PLAIN_BLOCKS = 2;      // blocks: of an SM
 static size_t plain_smem(int dim, int vdim) { return (size_t)(PROWS + PKEYS) * (dim + 8) * 4 + (size_t)PKEYS * (vdim + 36) * 4 + (size_t)PROWS * (PKEYS + 4) * 4 + PROWS * 8; }
 template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) tree_plain_kernel(const Params p) {
   early_start();
@@ -394,6 +403,466 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
   }
 }
 
+// ------------------------------------------------------------------------------------------ tensor cores
+// One block per SM, 128 query rows against tiles of 128 keys.  S = Q K^T goes to tensor memory (lane = row), the softmax threads, one per row, turn it into
+// weights in place, and O += P V takes those from tensor memory and V, keys outermost as the cache has it, from shared memory.  A row's weights would
+// lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 16 or more, for a second product with V.  Two groups of softmax warps take
+// alternate tiles with sums and an output of their own, so that one group's exponentials run beside the other's products; the two are added at the end.
+//   warps 0-3, 4-7   softmax of even and odd tiles; query rows in, results out
+//   warps 8-11       keys and values: 16-byte asynchronous copies into a ring of tiles in the swizzled layout, a row of a page at a time (any page size)
+//   warp 12          issues the products; owns the tensor memory
+// A tile is 64 KB of keys and values for 1536 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as copies stay in
+// flight (five slots of 32 KB).  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
+// (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
+constexpr int SOFT_WARPS = 8, COPY_WARPS = 4, TENSOR_THREADS = (SOFT_WARPS + COPY_WARPS + 1) * 32, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
+constexpr int RING_BYTES = 160 * 1024, LAG_MAX = 8;
+constexpr float RAISE = 8.f;
+
+struct TcShared {
+  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, group, drained;
+  uint32_t tmem;
+  volatile int abort;
+  int units[MAX_SEQ + 1];
+  Tree tree;
+  float2 stat[2][2][TROWS];      // by piece (a group without tiles is ahead of the other), group
+  // Values that are not finite and that not every row sees, by piece: drafted tokens, and positions from the lowest of any row's window on.  They are
+  // zeroed in shared memory (0 * inf would reach rows that do not see them), and the rows that do see them become NaN.
+  uint32_t bad[8][2 * WORDS];
+  int any_bad[8];
+};
+
+template <typename T> struct Half2;
+template <> struct Half2<__half> {
+  static constexpr float kBias = 7.f;      // weights are 2^7 as large
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u; }
+};
+template <> struct Half2<__nv_bfloat16> {
+  static constexpr float kBias = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
+};
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Values with the keys outermost: 64 columns (128 bytes) of a key are a swizzled row, eight keys 1024 bytes, 64 columns more a block of 128 rows.
+__device__ __forceinline__ uint64_t value_desc(uint32_t addr) { return (tc::smem_desc_sw128(addr) & ~((uint64_t)0x3fff << 16)) | (uint64_t)(TKEYS * 128 >> 4) << 16; }
+__device__ __forceinline__ uint32_t product_desc(bool bf16, int n, bool b_by_rows) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_by_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(TROWS >> 4) << 24;
+}
+// Byte of 16-byte unit c of row r of an operand of rows of 128 swizzled bytes (blocks of 128 rows).
+__device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+__device__ __forceinline__ void cp_wait(int pending) {
+  switch (pending) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+    case 7: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 8;" ::: "memory"); break;
+  }
+}
+
+struct Waits {          // a role's bounded waits: the whole warp goes the same way
+  TcShared &sm;
+  int *error_flag;
+  __device__ __forceinline__ bool operator()(uint64_t &bar, uint32_t parity) const {
+    const uint32_t b = tc::sa(&bar);
+    const bool ok = __all_sync(0xffffffffu, mbar_test(b, parity) || mbar_wait(b, parity, &sm.abort));
+    if (!ok) {
+      if (!sm.abort && error_flag) atomicCAS(error_flag, 0, 11);
+      sm.abort = 1;
+    }
+    return ok;
+  }
+  __device__ __forceinline__ void arrive(uint64_t &bar) const {      // one arrival of the warp
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(tc::sa(&bar));
+  }
+};
+
+// A piece's tile that some rows see in part: keys from `start` on are drafted, those in front of start + n - window are not seen by all.
+__device__ __forceinline__ bool partial(const Params &p, const Seq &x, int j0) { return j0 + TKEYS > x.start || (p.window && x.start + x.n - 1 - j0 >= p.window); }
+// Which of the keys base .. base + 31 token i sees.
+__device__ __forceinline__ uint32_t seen_word(const Params &p, const Seq &x, const uint32_t *seen, int depth, int base) {
+  const int ctx = min(max(x.start - base, 0), 32), low = p.window ? min(max(x.start + depth - p.window + 1 - base, 0), 32) : 0;
+  uint32_t v = ctx == 32 ? 0xffffffffu : (1u << ctx) - 1u;
+  v = low == 32 ? 0u : v & ~((1u << low) - 1u);
+  const int d = base - x.start;      // drafted token of the first key
+  if (d >= 0) {
+    const int k = d >> 5;
+    if (k < WORDS) v |= __funnelshift_r(seen[k], k + 1 < WORDS ? seen[k + 1] : 0u, d & 31);
+  } else if (d > -32) {
+    v |= seen[0] << -d;
+  }
+  return v;
+}
+
+template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const Params p) {
+  early_start();
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char *base = raw + ((1024 - (tc::sa(raw) & 1023)) & 1023);
+  const int kblocks = (p.dim + 63) / 64, vblocks = (p.vdim + 63) / 64, slot_bytes = max(kblocks, vblocks) * TKEYS * 128, slots = min(MAX_SLOTS, RING_BYTES / slot_bytes);
+  unsigned char *Q = base, *ring = base + kblocks * TROWS * 128;
+  TcShared &sm = *reinterpret_cast<TcShared *>(ring + RING_BYTES);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  if (tid == 0) {
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(tc::sa(&sm.full[i]), COPY_WARPS);
+      mbar_init(tc::sa(&sm.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tc::sa(&sm.s_full[i]), 1);
+      mbar_init(tc::sa(&sm.p_full[i]), SOFT_WARPS / 2);
+      mbar_init(tc::sa(&sm.o_done[i]), 1);
+    }
+    mbar_init(tc::sa(&sm.q_full), SOFT_WARPS);
+    mbar_init(tc::sa(&sm.group), SOFT_WARPS);
+    mbar_init(tc::sa(&sm.drained), 1);
+    sm.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int i = tid; i < 8 * 2 * WORDS; i += TENSOR_THREADS) (&sm.bad[0][0])[i] = 0;
+  if (tid < 8) sm.any_bad[tid] = 0;
+  if (warp == SOFT_WARPS + COPY_WARPS) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
+  tc::fence_before();
+  count_units(p, sm.units);      // (ends with a barrier)
+  tc::fence_after();
+  const uint32_t tmem = sm.tmem;
+  const Share sh = share(p, sm.units);
+  const int begin = blockIdx.x * sh.quota, end = min((int)(blockIdx.x + 1) * sh.quota, sh.all);
+  const Waits wait{sm, p.error_flag};
+
+  if (warp >= SOFT_WARPS && warp < SOFT_WARPS + COPY_WARPS) {
+    // ---- keys and values
+    const int w = warp - SOFT_WARPS, lag = min(slots - 2, LAG_MAX);
+    int e = 0, told = 0;                                    // tiles asked for, tiles handed on
+    const int units_row = p.dim / 8, units_val = p.vdim / 8;
+    const int kc = kblocks * 8, vc = vblocks * 8;           // 16-byte units of a row's blocks (8 or 16)
+    int pieces = 0;
+    bool ok = true;
+    auto hand_on = [&](int pending) {
+      cp_wait(pending);
+      tc::fence_operands();
+      wait.arrive(sm.full[told % slots]);
+      ++told;
+    };
+    for (int u = begin; u < end && ok; ++pieces) {
+      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
+      u += k.nt;
+      const Seq x = k.x;
+      const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
+      const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
+      for (int t = 0; t < k.nt && ok; ++t) {
+        const int j0 = (k.t0 + t) * TKEYS, j = j0 + w * 32 + lane;         // this lane's row of the tile
+        const bool in = j >= lowest && j < last;
+        const int phys = in ? table[j / p.page] : 0, place = in ? j % p.page : 0;
+        const T *krow = k_page<T>(p, phys, k.g) + (size_t)place * p.dim, *vrow = v_page<T>(p, phys, k.g) + (size_t)place * p.vdim;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int slot = e % slots;
+          if (e >= slots && !wait(sm.empty[slot], (e / slots + 1) & 1)) { ok = false; break; }
+          unsigned char *to = ring + slot * slot_bytes;
+          const int cols = kv ? vc : kc, have = kv ? units_val : units_row, pad = kv ? (p.vdim + 15) / 16 * 2 : (p.dim + 15) / 16 * 2;
+          const unsigned long long row = (unsigned long long)(kv ? vrow : krow);
+          const int per = 32 / cols, c = lane % cols;                      // rows of a step, this lane's unit
+#pragma unroll 8
+          for (int r0 = 0; r0 < 32; r0 += per) {
+            const int r = r0 + lane / cols;
+            const unsigned long long src = __shfl_sync(0xffffffffu, row, r);
+            const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have;
+            if (c < pad) cp16(to + swizzled(w * 32 + r, c), reinterpret_cast<const T *>(src) + (there ? c * 8 : 0), there);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          ++e;
+          if (kv && partial(p, x, j0)) {
+            // (a tile or two of an item: the copies are waited for here)
+            while (told < e - 1) hand_on(e - 1 - told);
+            cp_wait(0);
+            for (int r0 = 0; r0 < 32; r0 += per) {
+              const int r = r0 + lane / cols, key = j0 + w * 32 + r, d = key - x.start, b = key - lowest;
+              uint4 *at = reinterpret_cast<uint4 *>(to + swizzled(w * 32 + r, c));
+              if (c >= have || key >= last || key < lowest || (d < 0 && (p.window == 0 || b >= MAX_NODES))) continue;
+              const uint4 v = *at;
+              if (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w)) {
+                *at = make_uint4(0u, 0u, 0u, 0u);
+                const int bit = d >= 0 ? d : MAX_NODES + b;
+                atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
+                sm.any_bad[pieces & 7] = 1;
+              }
+            }
+            hand_on(0);
+          } else if (e - told > lag) {
+            hand_on(lag);
+          }
+        }
+      }
+    }
+    while (told < e) hand_on(e - 1 - told);                 // (after a failure too: nothing is in flight when the block ends)
+  } else if (warp == SOFT_WARPS + COPY_WARPS) {
+    // ---- products
+    const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
+    const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
+    const bool one = tc::elect_one();
+    int e = 0, pieces = 0, n_p[2] = {0, 0};                 // tiles used, pieces, weights used of either group
+    bool ok = true;
+    auto scores = [&](int w) {
+      const int slot = e % slots;
+      if (!wait(sm.full[slot], (e / slots) & 1)) return false;
+      tc::fence_after();
+      if (one) {
+        const uint32_t q = tc::sa(Q), kt = tc::sa(ring + slot * slot_bytes);
+        for (int s = 0; s < ksteps; ++s) {
+          const uint32_t at = (uint32_t)((s >> 2) * (128 * 128) + (s & 3) * 32);
+          tc::umma<false>(tmem + w * 128, tc::smem_desc_sw128(q + at), tc::smem_desc_sw128(kt + at), kdesc, s > 0);
+        }
+        tc::umma_commit(tc::sa(&sm.empty[slot]));
+        tc::umma_commit(tc::sa(&sm.s_full[w]));
+      }
+      __syncwarp();
+      return true;
+    };
+    // Tiles come as K V K V ..; the keys of the next tile but one are used after this one's values: e counts keys, values follow them.
+    for (int u = begin; u < end && ok; ++pieces) {
+      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
+      u += k.nt;
+      if (!wait(sm.q_full, pieces & 1)) break;
+      tc::fence_after();
+      const int e0 = e;
+      ok = scores(0);
+      if (ok && k.nt > 1) { e = e0 + 2; ok = scores(1); }
+      for (int t = 0; t < k.nt && ok; ++t) {
+        const int w = t & 1, ev = e0 + 2 * t + 1, slot = ev % slots;
+        if (!wait(sm.p_full[w], n_p[w] & 1) || !wait(sm.full[slot], (ev / slots) & 1)) { ok = false; break; }
+        ++n_p[w];
+        tc::fence_after();
+        if (one) {
+          const uint32_t vt = tc::sa(ring + slot * slot_bytes), o = tmem + 256 + w * 128, pw = tmem + w * 128;
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+              tc::umma_ta(o, pw + (s >> 1) * 32 + part * 16 + (s & 1) * 8, value_desc(vt + s * 2048), vdesc, t > 1 || part > 0 || s > 0);
+          tc::umma_commit(tc::sa(&sm.empty[slot]));
+          if (t + 2 >= k.nt) tc::umma_commit(tc::sa(&sm.o_done[w]));
+        }
+        __syncwarp();
+        if (t + 2 < k.nt) { e = e0 + 2 * t + 4; ok = scores(w); }
+      }
+      e = e0 + 2 * k.nt;
+    }
+    // nothing may be on its way to tensor or shared memory when the block ends
+    if (one) {
+      tc::umma_commit(tc::sa(&sm.drained));
+      mbar_wait_all(tc::sa(&sm.drained), 0);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax
+    const int w = warp >> 2, q = warp & 3, row = q * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16, S = tmem + w * 128 + lanes;
+    int pieces = 0, met = 0, n_s = 0, n_o[2] = {0, 0}, had = -1;
+    const float a1 = p.scale * kLog2e, a2 = CAP ? 2.0f * p.scale * kLog2e / p.softcap : 0.f, b2 = p.softcap * kLog2e;
+    auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };
+    auto meet = [&] {
+      wait.arrive(sm.group);
+      return wait(sm.group, met++ & 1);
+    };
+    for (int u = begin; u < end; ++pieces) {
+      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
+      u += k.nt;
+      const Seq x = k.x;
+      const int r0 = k.rt * TROWS, rows = min(TROWS, x.n * p.qpk - r0);
+      bool ok = true;
+      if (k.s != had) {
+        if (had >= 0 && !meet()) break;                     // (everybody is done with the tree before)
+        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, [&] { if (ok) ok = meet(); });
+        if (!ok) break;
+        had = k.s;
+      }
+      // query rows, rotated
+      {
+        const int cols = kblocks * 8, h = p.rope_half;
+        for (int e = tid; e < TROWS * cols; e += SOFT_WARPS * 32) {
+          const int r = e / cols, c = e - r * cols;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows && c * 8 < p.dim) {
+            const int i = (r0 + r) / p.qpk, head = k.g * p.qpk + (r0 + r) - i * p.qpk;
+            const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)head * p.dim;
+            v = *reinterpret_cast<const uint4 *>(src + c * 8);
+            if (c * 8 < 2 * h) {
+              const int pos = x.start + sm.tree.depth[i];
+              uint32_t *o = reinterpret_cast<uint32_t *>(&v);
+              if (h % 8 == 0) {
+                const bool second = c * 8 >= h;
+                const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? c * 8 - h : c * 8 + h));
+                const uint32_t *y = reinterpret_cast<const uint32_t *>(&other);
+                const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? c * 8 - h : c * 8));
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  const float2 m = Half2<T>::wide(o[z]), t = Half2<T>::wide(y[z]);
+                  const float4 an = __ldg(cs + z);
+                  o[z] = second ? Half2<T>::pack(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : Half2<T>::pack(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
+                }
+              } else {
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[z] = Half2<T>::pack(turned<T>(p, src, c * 8 + 2 * z, pos), turned<T>(p, src, c * 8 + 2 * z + 1, pos));
+              }
+            }
+          }
+          *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
+        }
+        tc::fence_operands();
+        wait.arrive(sm.q_full);
+      }
+      const bool live = q * 32 < rows;                      // (uniform over the warp)
+      const int node = min(r0 + row, x.n * p.qpk - 1) / p.qpk, depth = sm.tree.depth[node];
+      const uint32_t *seen = sm.tree.seen[node];
+      float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to
+      const int mine = (k.nt - w + 1) / 2;
+      for (int t = 0; t < mine && ok; ++t) {
+        if (!wait(sm.s_full[w], n_s & 1)) { ok = false; break; }
+        ++n_s;
+        tc::fence_after();
+        if (live) {
+          const int j0 = (k.t0 + 2 * t + w) * TKEYS;
+          const bool masked = partial(p, x, j0);
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tc::tmem_ld32(S + c * 32, v);
+            const uint32_t vis = masked ? seen_word(p, x, seen, depth, j0 + 32 * c) : 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float s = score(__uint_as_float(v[i]));
+              top = fmaxf(top, vis >> i & 1 ? s : -INFINITY);
+            }
+          }
+          top -= Half2<T>::kBias;
+          // (all keys that went before lie far below, or none was seen: the sums so far are scaled to the new maximum)
+          const bool raise = top > m + (m == -INFINITY ? 0.f : RAISE);
+          if (__any_sync(0xffffffffu, raise && t > 0)) {
+            const float f = raise ? ex2(m - top) : 1.f;     // (m = -inf: 0, of sums that are 0)
+            l *= f;
+            for (int c = 0; c < p.vdim; c += 32) {
+              uint32_t v[32];
+              tc::tmem_ld32(tmem + 256 + w * 128 + lanes + c, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tc::tmem_st32(tmem + 256 + w * 128 + lanes + c, v);
+            }
+          }
+          if (raise) m = top;
+          const float ref = m == -INFINITY ? 0.f : m;
+          float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], o[32];
+            tc::tmem_ld32(S + c * 32, v);
+            const uint32_t vis = masked ? seen_word(p, x, seen, depth, j0 + 32 * c) : 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float a = score(__uint_as_float(v[i])) - ref, b = score(__uint_as_float(v[i + 1])) - ref;
+              a = ex2(vis >> i & 1 ? a : -INFINITY);
+              b = ex2(vis >> (i + 1) & 1 ? b : -INFINITY);
+              add[i & 2] += a;
+              add[(i & 2) + 1] += b;
+              const uint32_t hi = Half2<T>::pack(a, b);
+              const float2 back = Half2<T>::wide(hi);
+              o[i / 2] = hi;
+              o[16 + i / 2] = Half2<T>::pack(a - back.x, b - back.y);
+            }
+            tc::tmem_st32(S + c * 32, o);
+          }
+          l += (add[0] + add[1]) + (add[2] + add[3]);
+          tc::tmem_wait_st();
+          tc::fence_before();
+        }
+        wait.arrive(sm.p_full[w]);
+      }
+      // ---- both groups' sums together; either group takes half of the columns
+      if (!ok) break;
+      sm.stat[pieces & 1][w][row] = make_float2(m, l);
+      if (!meet()) break;
+      if (tid == 0) sm.any_bad[(pieces + 7) & 7] = 0;       // (of the piece before: everybody is past it)
+      if (tid < 2 * WORDS) sm.bad[(pieces + 7) & 7][tid] = 0;
+      if (!wait(sm.o_done[0], n_o[0]++ & 1)) break;
+      if (k.nt > 1 && !wait(sm.o_done[1], n_o[1]++ & 1)) break;
+      tc::fence_after();
+      if (live) {
+        const float2 A = sm.stat[pieces & 1][0][row], B = sm.stat[pieces & 1][1][row];
+        const float top = fmaxf(A.x, B.x), ref = top == -INFINITY ? 0.f : top, fa = ex2(A.x - ref), fb = ex2(B.x - ref);
+        float sum = A.y * fa + B.y * fb;
+        if (sm.any_bad[pieces & 7]) {
+          const uint32_t *bad = sm.bad[pieces & 7];
+          bool hit = false;
+#pragma unroll
+          for (int z = 0; z < WORDS; ++z) hit |= (bad[z] & seen[z]) != 0;
+          if (p.window) {
+            const int low = x.start + depth - p.window + 1 - max(0, x.start - p.window + 1);      // the first of those positions that the token sees
+            for (int z = 0; z < MAX_NODES; ++z) hit |= z >= low && (bad[WORDS + (z >> 5)] >> (z & 31) & 1);
+          }
+          if (hit) sum = NAN;
+        }
+        const float inv = 1.0f / sum;
+        const bool store = row < rows;
+        const int i = (r0 + row) / p.qpk, head = k.g * p.qpk + (r0 + row) - i * p.qpk;
+        T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + i) * p.out_ld + (size_t)head * p.vdim;
+        if (!k.whole && w == 0 && store) p.part_ml[(size_t)k.slot * TROWS + row] = make_float2(top, sum);
+        for (int c = w * 32; c < p.vdim; c += 64) {
+          uint32_t va[32], vb[32];
+          tc::tmem_ld32(tmem + 256 + lanes + c, va);
+          if (k.nt > 1) tc::tmem_ld32(tmem + 384 + lanes + c, vb);
+          float o[32];
+#pragma unroll
+          for (int z = 0; z < 32; ++z) {
+            o[z] = __uint_as_float(va[z]) * fa;
+            if (k.nt > 1) o[z] = fmaf(__uint_as_float(vb[z]), fb, o[z]);
+          }
+          if (!store) continue;
+          if (k.whole) {
+#pragma unroll
+            for (int z = 0; z < 32; z += 8)
+              if (c + z < p.vdim) {
+                uint32_t y[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) y[b] = Half2<T>::pack(o[z + 2 * b] * inv, o[z + 2 * b + 1] * inv);
+                if (p.out16) {
+                  *reinterpret_cast<uint4 *>(out + c + z) = make_uint4(y[0], y[1], y[2], y[3]);
+                } else {
+                  const T *e = reinterpret_cast<const T *>(y);
+#pragma unroll
+                  for (int b = 0; b < 8; ++b) out[c + z + b] = e[b];
+                }
+              }
+          } else {
+#pragma unroll
+            for (int z = 0; z < 32; z += 4)
+              if (c + z < p.vdim)
+                *reinterpret_cast<float4 *>(p.part_o + (((size_t)k.slot * (p.vdim / 4) + (c + z) / 4) * TROWS + row) * 4) = make_float4(o[z], o[z + 1], o[z + 2], o[z + 3]);
+          }
+        }
+        tc::fence_before();
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == SOFT_WARPS + COPY_WARPS) {
+    tc::fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+static size_t tensor_smem(int dim) { return 1024 + (size_t)(dim + 63) / 64 * TROWS * 128 + RING_BYTES + sizeof(TcShared); }
+
 // ------------------------------------------------------------------------------------------ parts of an item
 // Block (x: an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys.
 constexpr int COMBINE_THREADS = 256;
@@ -436,22 +905,37 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
   }
 }
 
-static int max_blocks() { return sm_count() * 4; }
+// Floats of the parts' rows and columns: two of every block of either kernel.
+static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
 
 template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   const size_t smem = plain_smem(p.dim, VJ * 32);
   if (smem > 32 * 1024) PT_CUDA(allow_smem(tree_plain_kernel<T, VJ>, (int)plain_smem(256, VJ * 32), done));
   p.rows_tile = PROWS; p.keys_tile = PKEYS;
-  p.blocks = sm_count() * 2;
+  p.blocks = sm_count() * PLAIN_BLOCKS;
   PT_CUDA(launch_early(tree_plain_kernel<T, VJ>, Grid(p.blocks), PLAIN_THREADS, smem, st, p));
   PT_LAUNCH_CHECK("pt_tree_attn");
   return PT_OK;
 }
-template <typename T> static int run(Params &p, cudaStream_t st) {
+template <typename T, bool CAP> static int launch_tensor(Params &p, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  PT_CUDA(allow_smem(tree_tensor_kernel<T, CAP>, (int)tensor_smem(128), done));
+  p.rows_tile = TROWS; p.keys_tile = TKEYS;
+  p.blocks = sm_count();
+  PT_CUDA(launch_early(tree_tensor_kernel<T, CAP>, Grid(p.blocks), TENSOR_THREADS, tensor_smem(p.dim), st, p));
+  PT_LAUNCH_CHECK("pt_tree_attn");
+  return PT_OK;
+}
+template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   PT_CUDA(launch_early(tree_prep_kernel<T>, Grid(dim3(std::min(p.most, 64), p.n_seq)), PREP_THREADS, 0, st, p));
   PT_LAUNCH_CHECK("pt_tree_attn");
-  const int rc = p.vdim <= 64 ? launch_plain<T, 2>(p, st) : p.vdim <= 128 ? launch_plain<T, 4>(p, st) : launch_plain<T, 8>(p, st);
+  int rc;
+  if constexpr (std::is_same<T, float>::value) tensor = false;
+  if constexpr (!std::is_same<T, float>::value) {
+    if (tensor) rc = p.softcap > 0.f ? launch_tensor<T, true>(p, st) : launch_tensor<T, false>(p, st);
+  }
+  if (!tensor) rc = p.vdim <= 64 ? launch_plain<T, 2>(p, st) : p.vdim <= 128 ? launch_plain<T, 4>(p, st) : launch_plain<T, 8>(p, st);
   if (rc) return rc;
   const int tiles = ceil_div(p.most * p.qpk, p.rows_tile);
   PT_CUDA(launch_early(combine_kernel<T>, Grid(dim3(p.n_kv * tiles, p.n_seq)), COMBINE_THREADS, 0, st, p));
@@ -467,7 +951,7 @@ using namespace pt;
 // (n_seq, max_tokens_per_seq and the heads do not matter to the present kernels: every block has two parts of one tile of rows.)
 extern "C" size_t pt_tree_attn_workspace_bytes(int n_seq, int max_tokens_per_seq, int n_head, int n_kv, int vdim) {
   (void)n_seq; (void)max_tokens_per_seq; (void)n_head; (void)n_kv;
-  return (size_t)2 * ta::max_blocks() * ta::PROWS * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
+  return ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
 }
 
 extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
@@ -502,8 +986,11 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   const size_t need = pt_tree_attn_workspace_bytes(b.n_seq, p.most, a->n_head, a->n_kv, a->vdim);
   PT_REQUIRE(a->workspace && a->workspace_bytes >= need && aligned_to(a->workspace, 16), "pt_tree_attn: %zu workspace bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
   p.part_o = (float *)a->workspace;
-  p.part_ml = (float2 *)(p.part_o + (size_t)2 * ta::max_blocks() * ta::PROWS * ((a->vdim + 3) / 4 * 4));
+  p.part_ml = (float2 *)(p.part_o + ta::part_rows() * ((a->vdim + 3) / 4 * 4));
   cudaStream_t st = as_stream(stream);
-  if (a->dtype == PT_DT_F32) return ta::run<float>(p, st);
-  return a->dtype == PT_DT_F16 ? ta::run<__half>(p, st) : ta::run<__nv_bfloat16>(p, st);
+  p.out16 = a->out_ld % 8 == 0 && aligned_to(a->out, 16);
+  const bool tensor = !a->plain && a->dtype != PT_DT_F32 && a->dim <= 128 && a->vdim <= 128 && a->dim % 8 == 0 && a->vdim % 8 == 0 && a->q_ld % 8 == 0 && aligned_to(a->q, 16) &&
+                      aligned_to(a->pool, 16) && (p.rope_half % 8 || aligned_to(a->rope, 16));
+  if (a->dtype == PT_DT_F32) return ta::run<float>(p, false, st);
+  return a->dtype == PT_DT_F16 ? ta::run<__half>(p, tensor, st) : ta::run<__nv_bfloat16>(p, tensor, st);
 }
