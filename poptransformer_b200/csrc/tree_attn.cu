@@ -12,6 +12,8 @@
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
 // Scores, softmax and sums are fp32.
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "chunk.cuh"
@@ -42,6 +44,7 @@ struct Params {
   const float2 *rope;
   const int *page_table, *cu, *start, *slot, *parent;
   int *error_flag;
+  int box;            // cache rows of a TMA box: the largest power of two up to 128 that divides a page; 0: no boxes
   bool out16;         // the output can be written in units of 16 bytes
   float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
   float2 *part_ml;    // [2 blocks][rows_tile]
@@ -409,17 +412,20 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 // lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 16 or more, for a second product with V.  Two groups of softmax warps take
 // alternate tiles with sums and an output of their own, so that one group's exponentials run beside the other's products; the two are added at the end.
 //   warps 0-3, 4-7   softmax of even and odd tiles; query rows in, results out
-//   warps 8-11       keys and values: 16-byte asynchronous copies into a ring of tiles in the swizzled layout, a row of a page at a time (any page size)
-//   warp 12          issues the products; owns the tensor memory
-// A tile is 64 KB of keys and values for 1536 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as copies stay in
-// flight (five slots of 32 KB).  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
+//   warps 8, 9       keys and values into a ring of tiles in the swizzled layout: whole tiles by TMA, a box per page and 64 columns; tiles that begin or
+//                    end inside (a sequence's last, a window's first), and pages of sizes that no box fits, by 16-byte asynchronous copies of rows.
+//                    (Copies alone deliver 18 bytes a cycle to an SM, memory has 24 for each.)
+//   warp 10          issues the products; owns the tensor memory
+// (Twelve warps: an SM quarter's registers are shared by three.)  Rotated queries would lose 8 bits' worth too, and come in two parts likewise.
+// A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as
+// copies stay in flight.  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
 // (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
-constexpr int SOFT_WARPS = 8, COPY_WARPS = 4, TENSOR_THREADS = (SOFT_WARPS + COPY_WARPS + 1) * 32, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
-constexpr int RING_BYTES = 160 * 1024, LAG_MAX = 8;
+constexpr int SOFT_WARPS = 8, COPY_WARPS = 2, MMA_WARP = SOFT_WARPS + COPY_WARPS, TENSOR_THREADS = 384, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
+constexpr int OPERAND_BYTES = 192 * 1024;      // query rows and the ring
 constexpr float RAISE = 8.f;
 
 struct TcShared {
-  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, group, drained;
+  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, drained;
   uint32_t tmem;
   volatile int abort;
   int units[MAX_SEQ + 1];
@@ -436,12 +442,24 @@ template <> struct Half2<__half> {
   static constexpr float kBias = 7.f;      // weights are 2^7 as large
   static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
   static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+  // a and b in two parts
+  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    hi = pack(a, b);
+    const float2 back = wide(hi);
+    lo = pack(a - back.x, b - back.y);
+  }
   static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u; }
 };
 template <> struct Half2<__nv_bfloat16> {
   static constexpr float kBias = 0.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
   static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+  // (By cutting off bits, which costs no conversion: the upper half of a float is a bf16.  What is lost is below 2^-15 of the value.)
+  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    hi = __byte_perm(x, y, 0x7632);
+    lo = __byte_perm(__float_as_uint(a - __uint_as_float(x & 0xffff0000u)), __float_as_uint(b - __uint_as_float(y & 0xffff0000u)), 0x7632);
+  }
   static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
 };
 __device__ __forceinline__ float ex2(float x) {
@@ -456,18 +474,34 @@ __device__ __forceinline__ uint32_t product_desc(bool bf16, int n, bool b_by_row
 }
 // Byte of 16-byte unit c of row r of an operand of rows of 128 swizzled bytes (blocks of 128 rows).
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
-__device__ __forceinline__ void cp_wait(int pending) {
-  switch (pending) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    case 7: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 8;" ::: "memory"); break;
-  }
+// 16 bytes, zeros where bytes is 0.
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// The barrier gets this thread's arrival when all its copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t &bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::sa(&bar)) : "memory"); }
+__device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t &bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(tc::sa(&bar)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {      // (to be waited for)
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                 "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+                 "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+                 "=r"(v[31])
+               : "r"(taddr)
+               : "memory");
+}
+// (The registers pass through, so that nothing reads them before.)
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
 }
 
 struct Waits {          // a role's bounded waits: the whole warp goes the same way
@@ -475,12 +509,23 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
   int *error_flag;
   __device__ __forceinline__ bool operator()(uint64_t &bar, uint32_t parity) const {
     const uint32_t b = tc::sa(&bar);
-    const bool ok = __all_sync(0xffffffffu, mbar_test(b, parity) || mbar_wait(b, parity, &sm.abort));
+    bool ok = false;
+    for (int i = 0; i < 64 && !ok; ++i) ok = mbar_test(b, parity);      // (a warp that lets itself be suspended wakes late)
+    ok = __all_sync(0xffffffffu, ok || mbar_wait(b, parity, &sm.abort));
     if (!ok) {
       if (!sm.abort && error_flag) atomicCAS(error_flag, 0, 11);
       sm.abort = 1;
     }
     return ok;
+  }
+  __device__ __forceinline__ bool alone(uint64_t &bar, uint32_t parity) const {      // the same for one lane
+    const uint32_t b = tc::sa(&bar);
+    for (int i = 0; i < 64; ++i)
+      if (mbar_test(b, parity)) return true;
+    if (mbar_wait(b, parity, &sm.abort)) return true;
+    if (!sm.abort && error_flag) atomicCAS(error_flag, 0, 11);
+    sm.abort = 1;
+    return false;
   }
   __device__ __forceinline__ void arrive(uint64_t &bar) const {      // one arrival of the warp
     __syncwarp();
@@ -505,18 +550,20 @@ __device__ __forceinline__ uint32_t seen_word(const Params &p, const Seq &x, con
   return v;
 }
 
-template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const Params p) {
+template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
   early_start();
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char *base = raw + ((1024 - (tc::sa(raw) & 1023)) & 1023);
-  const int kblocks = (p.dim + 63) / 64, vblocks = (p.vdim + 63) / 64, slot_bytes = max(kblocks, vblocks) * TKEYS * 128, slots = min(MAX_SLOTS, RING_BYTES / slot_bytes);
-  unsigned char *Q = base, *ring = base + kblocks * TROWS * 128;
-  TcShared &sm = *reinterpret_cast<TcShared *>(ring + RING_BYTES);
+  const int kblocks = (p.dim + 63) / 64, vblocks = (p.vdim + 63) / 64, slot_bytes = max(kblocks, vblocks) * TKEYS * 128, q_bytes = kblocks * TROWS * 128;
+  const bool split_q = p.rope_half > 0;                     // query rows in two parts
+  const int slots = min(MAX_SLOTS, (OPERAND_BYTES - (split_q ? 2 : 1) * q_bytes) / slot_bytes);
+  unsigned char *Q = base, *ring = base + (split_q ? 2 : 1) * q_bytes;
+  TcShared &sm = *reinterpret_cast<TcShared *>(base + OPERAND_BYTES);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (tid == 0) {
     for (int i = 0; i < slots; ++i) {
-      mbar_init(tc::sa(&sm.full[i]), COPY_WARPS);
+      mbar_init(tc::sa(&sm.full[i]), COPY_WARPS * 32);
       mbar_init(tc::sa(&sm.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -525,14 +572,13 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       mbar_init(tc::sa(&sm.o_done[i]), 1);
     }
     mbar_init(tc::sa(&sm.q_full), SOFT_WARPS);
-    mbar_init(tc::sa(&sm.group), SOFT_WARPS);
     mbar_init(tc::sa(&sm.drained), 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = tid; i < 8 * 2 * WORDS; i += TENSOR_THREADS) (&sm.bad[0][0])[i] = 0;
   if (tid < 8) sm.any_bad[tid] = 0;
-  if (warp == SOFT_WARPS + COPY_WARPS) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
+  if (warp == MMA_WARP) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
   tc::fence_before();
   count_units(p, sm.units);      // (ends with a barrier)
   tc::fence_after();
@@ -541,184 +587,194 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
   const int begin = blockIdx.x * sh.quota, end = min((int)(blockIdx.x + 1) * sh.quota, sh.all);
   const Waits wait{sm, p.error_flag};
 
-  if (warp >= SOFT_WARPS && warp < SOFT_WARPS + COPY_WARPS) {
+  if (warp >= SOFT_WARPS && warp < MMA_WARP) {
     // ---- keys and values
-    const int w = warp - SOFT_WARPS, lag = min(slots - 2, LAG_MAX);
-    int e = 0, told = 0;                                    // tiles asked for, tiles handed on
-    const int units_row = p.dim / 8, units_val = p.vdim / 8;
-    const int kc = kblocks * 8, vc = vblocks * 8;           // 16-byte units of a row's blocks (8 or 16)
-    int pieces = 0;
+    const int w = warp - SOFT_WARPS;
+    const int box = p.box, boxes = box ? TKEYS / box : 0;   // rows of a box, and how many make a tile
+    const bool one = tc::elect_one();
+    int e = 0, pieces = 0;                                  // tiles asked for
     bool ok = true;
-    auto hand_on = [&](int pending) {
-      cp_wait(pending);
-      tc::fence_operands();
-      wait.arrive(sm.full[told % slots]);
-      ++told;
-    };
     for (int u = begin; u < end && ok; ++pieces) {
       const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
       u += k.nt;
       const Seq x = k.x;
       const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
       const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
+      auto page_of = [&](int j) { return j >= lowest && j < last ? table[j / p.page] : 0; };
+      auto box_page = [&](int t) { return w == 0 && lane < boxes ? page_of(t * TKEYS + lane * box) : 0; };
+      int ahead = box_page(k.t0);                           // pages of the next tile's boxes, one per lane
       for (int t = 0; t < k.nt && ok; ++t) {
-        const int j0 = (k.t0 + t) * TKEYS, j = j0 + w * 32 + lane;         // this lane's row of the tile
-        const bool in = j >= lowest && j < last;
-        const int phys = in ? table[j / p.page] : 0, place = in ? j % p.page : 0;
-        const T *krow = k_page<T>(p, phys, k.g) + (size_t)place * p.dim, *vrow = v_page<T>(p, phys, k.g) + (size_t)place * p.vdim;
+        const int j0 = (k.t0 + t) * TKEYS, phys = ahead;
+        ahead = box_page(k.t0 + t + 1);
+        const bool whole = box && j0 >= lowest && j0 + TKEYS <= last;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
+        for (int kv = 0; kv < 2; ++kv, ++e) {
           const int slot = e % slots;
           if (e >= slots && !wait(sm.empty[slot], (e / slots + 1) & 1)) { ok = false; break; }
-          unsigned char *to = ring + slot * slot_bytes;
-          const int cols = kv ? vc : kc, have = kv ? units_val : units_row, pad = kv ? (p.vdim + 15) / 16 * 2 : (p.dim + 15) / 16 * 2;
-          const unsigned long long row = (unsigned long long)(kv ? vrow : krow);
-          const int per = 32 / cols, c = lane % cols;                      // rows of a step, this lane's unit
-#pragma unroll 8
-          for (int r0 = 0; r0 < 32; r0 += per) {
-            const int r = r0 + lane / cols;
-            const unsigned long long src = __shfl_sync(0xffffffffu, row, r);
-            const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have;
-            if (c < pad) cp16(to + swizzled(w * 32 + r, c), reinterpret_cast<const T *>(src) + (there ? c * 8 : 0), there);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          ++e;
-          if (kv && partial(p, x, j0)) {
-            // (a tile or two of an item: the copies are waited for here)
-            while (told < e - 1) hand_on(e - 1 - told);
-            cp_wait(0);
-            for (int r0 = 0; r0 < 32; r0 += per) {
-              const int r = r0 + lane / cols, key = j0 + w * 32 + r, d = key - x.start, b = key - lowest;
-              uint4 *at = reinterpret_cast<uint4 *>(to + swizzled(w * 32 + r, c));
-              if (c >= have || key >= last || key < lowest || (d < 0 && (p.window == 0 || b >= MAX_NODES))) continue;
-              const uint4 v = *at;
-              if (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w)) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-                const int bit = d >= 0 ? d : MAX_NODES + b;
-                atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
-                sm.any_bad[pieces & 7] = 1;
+          const uint32_t to = tc::sa(ring + slot * slot_bytes);
+          const int dims = kv ? p.vdim : p.dim, blocks = kv ? vblocks : kblocks, have = dims / 8, pad = (dims + 15) / 16 * 2;
+          if (whole) {
+            if (w == 0) {
+              if (one) mbar_expect_tx(tc::sa(&sm.full[slot]), blocks * TKEYS * 128);
+              for (int i = 0; i < boxes; ++i) {
+                const int page = __shfl_sync(0xffffffffu, phys, i), y = k.g * p.page + (j0 + i * box) % p.page;
+                if (one)
+                  for (int b = 0; b < blocks; ++b) box_load(to + b * (TKEYS * 128) + i * box * 128, kv ? &values : &keys, b * 64, y, page, sm.full[slot]);
               }
             }
-            hand_on(0);
-          } else if (e - told > lag) {
-            hand_on(lag);
+            if (w || !one) mbar_arrive(tc::sa(&sm.full[slot]));
+            continue;
           }
+          for (int h = 0; h < 2; ++h) {
+            const int r0 = w * 64 + h * 32, j = j0 + r0 + lane;
+            const bool in = j >= lowest && j < last;
+            const T *src = (kv ? v_page<T>(p, page_of(j), k.g) : k_page<T>(p, page_of(j), k.g)) + (size_t)(in ? j % p.page : 0) * dims;
+            const int cols = blocks * 8, c = lane % cols;
+            for (int q0 = 0; q0 < 32; q0 += 32 / cols) {
+              const int r = q0 + lane / cols;
+              const unsigned long long from = __shfl_sync(0xffffffffu, (unsigned long long)src, r);
+              const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have;
+              if (c < pad) cp_async(to + swizzled(r0 + r, c), reinterpret_cast<const T *>(from) + (there ? c * 8 : 0), there ? 16 : 0);
+            }
+          }
+          if (kv && partial(p, x, j0)) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int h = 0; h < 2; ++h) {
+              const int cols = blocks * 8, c = lane % cols;
+              for (int q0 = 0; q0 < 32; q0 += 32 / cols) {      // (the units that this lane copied)
+                const int r = w * 64 + h * 32 + q0 + lane / cols, key = j0 + r, d = key - x.start, b = key - lowest;
+                if (c >= have || key >= last || key < lowest || (d < 0 && (p.window == 0 || b >= MAX_NODES))) continue;
+                uint4 *at = reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(r, c));
+                const uint4 v = *at;
+                if (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w)) {
+                  *at = make_uint4(0u, 0u, 0u, 0u);
+                  const int bit = d >= 0 ? d : MAX_NODES + b;
+                  atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
+                  sm.any_bad[pieces & 7] = 1;
+                }
+              }
+            }
+          }
+          cp_arrive(sm.full[slot]);
         }
       }
     }
-    while (told < e) hand_on(e - 1 - told);                 // (after a failure too: nothing is in flight when the block ends)
-  } else if (warp == SOFT_WARPS + COPY_WARPS) {
-    // ---- products
-    const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
-    const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
-    const bool one = tc::elect_one();
-    int e = 0, pieces = 0, n_p[2] = {0, 0};                 // tiles used, pieces, weights used of either group
-    bool ok = true;
-    auto scores = [&](int w) {
-      const int slot = e % slots;
-      if (!wait(sm.full[slot], (e / slots) & 1)) return false;
-      tc::fence_after();
-      if (one) {
-        const uint32_t q = tc::sa(Q), kt = tc::sa(ring + slot * slot_bytes);
-        for (int s = 0; s < ksteps; ++s) {
-          const uint32_t at = (uint32_t)((s >> 2) * (128 * 128) + (s & 3) * 32);
-          tc::umma<false>(tmem + w * 128, tc::smem_desc_sw128(q + at), tc::smem_desc_sw128(kt + at), kdesc, s > 0);
-        }
+    asm volatile("cp.async.wait_all;" ::: "memory");        // nothing is in flight when the block ends, after a failure either
+    if (w == 0 && box) mbar_wait_ring(tc::sa(&sm.full[0]), e, slots);
+  } else if (warp == MMA_WARP) {
+    // ---- products, by one lane
+    if (tc::elect_one()) {
+      const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
+      const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
+      int pieces = 0, n_p[2] = {0, 0}, e0 = 0;              // pieces, weights used of either group, first tile of the piece
+      bool ok = true;
+      const uint64_t q0 = tc::smem_desc_sw128(tc::sa(Q)), q1 = tc::smem_desc_sw128(tc::sa(Q) + q_bytes);
+      auto scores = [&](int w, int e) {
+        const int slot = e % slots;
+        if (!(ok = ok && wait.alone(sm.full[slot], (e / slots) & 1))) return;
+        tc::fence_operands();                               // (what the copies wrote, for the tensor core)
+        tc::fence_after();
+        const uint64_t kt = tc::smem_desc_sw128(tc::sa(ring + slot * slot_bytes));
+        for (int part = 0; part < (split_q ? 2 : 1); ++part)
+#pragma unroll 4
+          for (int s = 0; s < ksteps; ++s) {
+            const uint64_t at = (s >> 2) * (128 * 128 / 16) + (s & 3) * 2;      // (in units of 16 bytes)
+            tc::umma<false>(tmem + w * 128, (part ? q1 : q0) + at, kt + at, kdesc, part > 0 || s > 0);
+          }
         tc::umma_commit(tc::sa(&sm.empty[slot]));
         tc::umma_commit(tc::sa(&sm.s_full[w]));
-      }
-      __syncwarp();
-      return true;
-    };
-    // Tiles come as K V K V ..; the keys of the next tile but one are used after this one's values: e counts keys, values follow them.
-    for (int u = begin; u < end && ok; ++pieces) {
-      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
-      u += k.nt;
-      if (!wait(sm.q_full, pieces & 1)) break;
-      tc::fence_after();
-      const int e0 = e;
-      ok = scores(0);
-      if (ok && k.nt > 1) { e = e0 + 2; ok = scores(1); }
-      for (int t = 0; t < k.nt && ok; ++t) {
-        const int w = t & 1, ev = e0 + 2 * t + 1, slot = ev % slots;
-        if (!wait(sm.p_full[w], n_p[w] & 1) || !wait(sm.full[slot], (ev / slots) & 1)) { ok = false; break; }
-        ++n_p[w];
-        tc::fence_after();
-        if (one) {
-          const uint32_t vt = tc::sa(ring + slot * slot_bytes), o = tmem + 256 + w * 128, pw = tmem + w * 128;
+      };
+      // (Tiles come as K V K V ..; the scores of the next tile but one are asked for behind this one's output.)
+      for (int u = begin; u < end && ok; ++pieces) {
+        const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
+        u += k.nt;
+        if (!(ok = wait.alone(sm.q_full, pieces & 1))) break;
+        scores(0, e0);
+        if (k.nt > 1) scores(1, e0 + 2);
+        for (int t = 0; t < k.nt && ok; ++t) {
+          const int w = t & 1, e = e0 + 2 * t + 1, slot = e % slots;
+          if (!(ok = wait.alone(sm.full[slot], (e / slots) & 1) && wait.alone(sm.p_full[w], n_p[w] & 1))) break;
+          ++n_p[w];
+          tc::fence_operands();
+          tc::fence_after();
+          const uint64_t vt = value_desc(tc::sa(ring + slot * slot_bytes));
+          const uint32_t o = tmem + 256 + w * 128, pw = tmem + w * 128;
 #pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-              tc::umma_ta(o, pw + (s >> 1) * 32 + part * 16 + (s & 1) * 8, value_desc(vt + s * 2048), vdesc, t > 1 || part > 0 || s > 0);
+          for (int s = 0; s < 16; ++s)                      // (hi and lo of 16 keys: 8 columns each)
+            tc::umma_ta(o, pw + (s >> 2) * 32 + (s & 1) * 16 + (s >> 1 & 1) * 8, vt + (s >> 1) * (2048 / 16), vdesc, t > 1 || s > 0);
           tc::umma_commit(tc::sa(&sm.empty[slot]));
           if (t + 2 >= k.nt) tc::umma_commit(tc::sa(&sm.o_done[w]));
+          else scores(w, e + 3);
         }
-        __syncwarp();
-        if (t + 2 < k.nt) { e = e0 + 2 * t + 4; ok = scores(w); }
+        e0 += 2 * k.nt;
       }
-      e = e0 + 2 * k.nt;
-    }
-    // nothing may be on its way to tensor or shared memory when the block ends
-    if (one) {
+      // nothing may be on its way to tensor or shared memory when the block ends
       tc::umma_commit(tc::sa(&sm.drained));
       mbar_wait_all(tc::sa(&sm.drained), 0);
     }
     __syncwarp();
-  } else {
+  } else if (warp < SOFT_WARPS) {
     // ---- softmax
     const int w = warp >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16, S = tmem + w * 128 + lanes;
-    int pieces = 0, met = 0, n_s = 0, n_o[2] = {0, 0}, had = -1;
-    const float a1 = p.scale * kLog2e, a2 = CAP ? 2.0f * p.scale * kLog2e / p.softcap : 0.f, b2 = p.softcap * kLog2e;
-    auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };
-    auto meet = [&] {
-      wait.arrive(sm.group);
-      return wait(sm.group, met++ & 1);
-    };
+    int pieces = 0, n_s = 0, n_o[2] = {0, 0}, had = -1;
+    const float a1 = fabsf(p.scale) * kLog2e, a2 = CAP ? 2.0f * a1 / p.softcap : 0.f, b2 = p.softcap * kLog2e;
+    auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };      // (grows with s)
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory"); };
+    // (After a wait that ran out all go on without waiting: everybody comes to every meeting, and what is computed does not matter.)
     for (int u = begin; u < end; ++pieces) {
       const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
       u += k.nt;
       const Seq x = k.x;
       const int r0 = k.rt * TROWS, rows = min(TROWS, x.n * p.qpk - r0);
-      bool ok = true;
       if (k.s != had) {
-        if (had >= 0 && !meet()) break;                     // (everybody is done with the tree before)
-        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, [&] { if (ok) ok = meet(); });
-        if (!ok) break;
+        if (had >= 0) meet();                               // (everybody is done with the tree before)
+        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, meet);
         had = k.s;
       }
-      // query rows, rotated
+      // query rows, rotated, and negated where the scale is negative
       {
         const int cols = kblocks * 8, h = p.rope_half;
         for (int e = tid; e < TROWS * cols; e += SOFT_WARPS * 32) {
           const int r = e / cols, c = e - r * cols;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
           if (r < rows && c * 8 < p.dim) {
             const int i = (r0 + r) / p.qpk, head = k.g * p.qpk + (r0 + r) - i * p.qpk;
             const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)head * p.dim;
             v = *reinterpret_cast<const uint4 *>(src + c * 8);
+            uint32_t *o = reinterpret_cast<uint32_t *>(&v), *ol = reinterpret_cast<uint32_t *>(&lo);
             if (c * 8 < 2 * h) {
               const int pos = x.start + sm.tree.depth[i];
-              uint32_t *o = reinterpret_cast<uint32_t *>(&v);
+              float2 y[4];
               if (h % 8 == 0) {
                 const bool second = c * 8 >= h;
                 const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? c * 8 - h : c * 8 + h));
-                const uint32_t *y = reinterpret_cast<const uint32_t *>(&other);
+                const uint32_t *z = reinterpret_cast<const uint32_t *>(&other);
                 const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? c * 8 - h : c * 8));
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  const float2 m = Half2<T>::wide(o[z]), t = Half2<T>::wide(y[z]);
-                  const float4 an = __ldg(cs + z);
-                  o[z] = second ? Half2<T>::pack(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : Half2<T>::pack(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
+                for (int i4 = 0; i4 < 4; ++i4) {
+                  const float2 m = Half2<T>::wide(o[i4]), t = Half2<T>::wide(z[i4]);
+                  const float4 an = __ldg(cs + i4);
+                  y[i4] = second ? make_float2(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : make_float2(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
                 }
               } else {
 #pragma unroll
-                for (int z = 0; z < 4; ++z) o[z] = Half2<T>::pack(turned<T>(p, src, c * 8 + 2 * z, pos), turned<T>(p, src, c * 8 + 2 * z + 1, pos));
+                for (int i4 = 0; i4 < 4; ++i4) y[i4] = make_float2(turned<T>(p, src, c * 8 + 2 * i4, pos), turned<T>(p, src, c * 8 + 2 * i4 + 1, pos));
               }
+#pragma unroll
+              for (int i4 = 0; i4 < 4; ++i4) {
+                o[i4] = Half2<T>::pack(y[i4].x, y[i4].y);
+                const float2 back = Half2<T>::wide(o[i4]);
+                ol[i4] = Half2<T>::pack(y[i4].x - back.x, y[i4].y - back.y);
+              }
+            }
+            if (p.scale < 0.f) {
+#pragma unroll
+              for (int i4 = 0; i4 < 4; ++i4) { o[i4] ^= 0x80008000u; ol[i4] ^= 0x80008000u; }
             }
           }
           *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
+          if (split_q) *reinterpret_cast<uint4 *>(Q + q_bytes + swizzled(r, c)) = lo;
         }
         tc::fence_operands();
         wait.arrive(sm.q_full);
@@ -728,75 +784,95 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       const uint32_t *seen = sm.tree.seen[node];
       float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to
       const int mine = (k.nt - w + 1) / 2;
-      for (int t = 0; t < mine && ok; ++t) {
-        if (!wait(sm.s_full[w], n_s & 1)) { ok = false; break; }
-        ++n_s;
+      // Scores of a tile to weights; `vis`: the keys that the row sees.
+      auto weigh = [&](auto masked, bool again, const uint32_t (&vis)[4]) {
+        constexpr bool MASKED = decltype(masked)::value;
+        // (Loops of two steps, not four: a short run of tiles fetches this code once.)
+        uint32_t v[2][32];
+        tmem_load(S, v[0]);
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c2 = 0; c2 < 4; c2 += 2)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t see = MASKED ? (c2 ? vis[2 + b] : vis[b]) : 0;
+            tmem_landed(v[b]);
+            tmem_load(S + (c2 + b + 1 & 3) * 32, v[1 - b]);   // (the last: the first again)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float s = __uint_as_float(v[b][i]);
+              tops[i & 3] = fmaxf(tops[i & 3], !MASKED || see >> i & 1 ? s : -INFINITY);
+            }
+          }
+        tmem_landed(v[0]);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        top = (top == -INFINITY ? top : score(top)) - Half2<T>::kBias;
+        // (keys that went before lie far below, or none was seen: the sums so far are scaled to the new maximum)
+        const bool raise = top > m + (m == -INFINITY ? 0.f : RAISE);
+        if (__any_sync(0xffffffffu, raise && again)) {
+          const float f = raise ? ex2(m - top) : 1.f;        // (m = -inf: 0, of sums that are 0)
+          l *= f;
+          for (int c = 0; c < p.vdim; c += 32) {
+            uint32_t y[32];
+            tc::tmem_ld32(tmem + 256 + w * 128 + lanes + c, y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tc::tmem_st32(tmem + 256 + w * 128 + lanes + c, y);
+          }
+        }
+        if (raise) m = top;
+        const float ref = m == -INFINITY ? 0.f : m;
+        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        tmem_load(S, v[0]);
+#pragma unroll 1
+        for (int c2 = 0; c2 < 4; c2 += 2)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t see = MASKED ? (c2 ? vis[2 + h] : vis[h]) : 0;
+            tmem_landed(v[h]);
+            if (c2 + h < 3) tmem_load(S + (c2 + h + 1) * 32, v[1 - h]);
+            uint32_t o[32];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float a = __uint_as_float(v[h][i]), b = __uint_as_float(v[h][i + 1]);
+              a = CAP ? score(a) - ref : fmaf(a, a1, -ref);
+              b = CAP ? score(b) - ref : fmaf(b, a1, -ref);
+              a = ex2(!MASKED || see >> i & 1 ? a : -INFINITY);
+              b = ex2(!MASKED || see >> (i + 1) & 1 ? b : -INFINITY);
+              add[i & 2] += a;
+              add[(i & 2) + 1] += b;
+              Half2<T>::split(a, b, o[i / 2], o[16 + i / 2]);
+            }
+            tc::tmem_st32(S + (c2 + h) * 32, o);
+          }
+        l += (add[0] + add[1]) + (add[2] + add[3]);
+      };
+      for (int t = 0; t < mine; ++t) {
+        wait(sm.s_full[w], n_s++ & 1);
         tc::fence_after();
         if (live) {
           const int j0 = (k.t0 + 2 * t + w) * TKEYS;
-          const bool masked = partial(p, x, j0);
-          float top = -INFINITY;
+          if (partial(p, x, j0)) {
+            uint32_t vis[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tc::tmem_ld32(S + c * 32, v);
-            const uint32_t vis = masked ? seen_word(p, x, seen, depth, j0 + 32 * c) : 0xffffffffu;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float s = score(__uint_as_float(v[i]));
-              top = fmaxf(top, vis >> i & 1 ? s : -INFINITY);
-            }
+            for (int c = 0; c < 4; ++c) vis[c] = seen_word(p, x, seen, depth, j0 + 32 * c);
+            weigh(std::true_type(), t > 0, vis);
+          } else {
+            uint32_t vis[4] = {};
+            weigh(std::false_type(), t > 0, vis);
           }
-          top -= Half2<T>::kBias;
-          // (all keys that went before lie far below, or none was seen: the sums so far are scaled to the new maximum)
-          const bool raise = top > m + (m == -INFINITY ? 0.f : RAISE);
-          if (__any_sync(0xffffffffu, raise && t > 0)) {
-            const float f = raise ? ex2(m - top) : 1.f;     // (m = -inf: 0, of sums that are 0)
-            l *= f;
-            for (int c = 0; c < p.vdim; c += 32) {
-              uint32_t v[32];
-              tc::tmem_ld32(tmem + 256 + w * 128 + lanes + c, v);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tc::tmem_st32(tmem + 256 + w * 128 + lanes + c, v);
-            }
-          }
-          if (raise) m = top;
-          const float ref = m == -INFINITY ? 0.f : m;
-          float add[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], o[32];
-            tc::tmem_ld32(S + c * 32, v);
-            const uint32_t vis = masked ? seen_word(p, x, seen, depth, j0 + 32 * c) : 0xffffffffu;
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float a = score(__uint_as_float(v[i])) - ref, b = score(__uint_as_float(v[i + 1])) - ref;
-              a = ex2(vis >> i & 1 ? a : -INFINITY);
-              b = ex2(vis >> (i + 1) & 1 ? b : -INFINITY);
-              add[i & 2] += a;
-              add[(i & 2) + 1] += b;
-              const uint32_t hi = Half2<T>::pack(a, b);
-              const float2 back = Half2<T>::wide(hi);
-              o[i / 2] = hi;
-              o[16 + i / 2] = Half2<T>::pack(a - back.x, b - back.y);
-            }
-            tc::tmem_st32(S + c * 32, o);
-          }
-          l += (add[0] + add[1]) + (add[2] + add[3]);
           tc::tmem_wait_st();
           tc::fence_before();
         }
         wait.arrive(sm.p_full[w]);
       }
       // ---- both groups' sums together; either group takes half of the columns
-      if (!ok) break;
       sm.stat[pieces & 1][w][row] = make_float2(m, l);
-      if (!meet()) break;
+      meet();
       if (tid == 0) sm.any_bad[(pieces + 7) & 7] = 0;       // (of the piece before: everybody is past it)
       if (tid < 2 * WORDS) sm.bad[(pieces + 7) & 7][tid] = 0;
-      if (!wait(sm.o_done[0], n_o[0]++ & 1)) break;
-      if (k.nt > 1 && !wait(sm.o_done[1], n_o[1]++ & 1)) break;
+      wait(sm.o_done[0], n_o[0]++ & 1);
+      if (k.nt > 1) wait(sm.o_done[1], n_o[1]++ & 1);
       tc::fence_after();
       if (live) {
         const float2 A = sm.stat[pieces & 1][0][row], B = sm.stat[pieces & 1][1][row];
@@ -856,16 +932,16 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     }
   }
   __syncthreads();
-  if (warp == SOFT_WARPS + COPY_WARPS) {
+  if (warp == MMA_WARP) {
     tc::fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
 }
-static size_t tensor_smem(int dim) { return 1024 + (size_t)(dim + 63) / 64 * TROWS * 128 + RING_BYTES + sizeof(TcShared); }
+static size_t tensor_smem() { return 1024 + OPERAND_BYTES + sizeof(TcShared); }
 
 // ------------------------------------------------------------------------------------------ parts of an item
-// Block (x: an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys.
-constexpr int COMBINE_THREADS = 256;
+// Block (x: eight rows of an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys.
+constexpr int COMBINE_THREADS = 256, COMBINE_ROWS = 8;
 template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const Params p) {
   early_start();
   __shared__ int units[MAX_SEQ + 1];
@@ -873,30 +949,32 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
   const Seq x = sequence(p, s);
   if (!x.n) return;
   const Span y = span(p, x);
-  const int most_tiles = (p.most * p.qpk + p.rows_tile - 1) / p.rows_tile, g = blockIdx.x / most_tiles, rt = blockIdx.x - g * most_tiles;
-  if (rt >= y.row_tiles) return;
+  const int eights = (p.most * p.qpk + COMBINE_ROWS - 1) / COMBINE_ROWS, g = blockIdx.x / eights, r0 = (blockIdx.x - g * eights) * COMBINE_ROWS;   // (first row, of all of the kv head's)
+  const int rows = min(COMBINE_ROWS, x.n * p.qpk - r0), rt = r0 / p.rows_tile;
+  if (rows <= 0) return;
   count_units(p, units);
   const Share sh = share(p, units);
   const int first = units[s] + (g * y.row_tiles + rt) * y.tiles, b0 = first / sh.quota, b1 = (first + y.tiles - 1) / sh.quota;
   if (b0 == b1) return;
-  const int r0 = rt * p.rows_tile, rows = min(p.rows_tile, x.n * p.qpk - r0), v4 = (p.vdim + 3) / 4;
+  const int v4 = (p.vdim + 3) / 4;
   for (int e = tid; e < rows * v4; e += COMBINE_THREADS) {
-    const int r = e / v4, c = e - r * v4;
+    const int r = r0 % p.rows_tile + e / v4, c = e % v4;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int b = b0; b <= b1; ++b) m = fmaxf(m, p.part_ml[(size_t)(2 * b + (b == b0 ? 1 : 0)) * p.rows_tile + r].x);
+    if (m == -INFINITY) m = 0.f;
+#pragma unroll 4
     for (int b = b0; b <= b1; ++b) {
       const size_t slot = 2 * b + (b == b0 ? 1 : 0);
       const float2 ml = p.part_ml[slot * p.rows_tile + r];
       const float4 w = *reinterpret_cast<const float4 *>(p.part_o + ((slot * v4 + c) * p.rows_tile + r) * 4);
-      const float top = fmaxf(m, ml.x);
-      if (top == -INFINITY) continue;
-      const float a = exp2f(m - top), f = exp2f(ml.x - top);
-      o.x = o.x * a + w.x * f; o.y = o.y * a + w.y * f; o.z = o.z * a + w.z * f; o.w = o.w * a + w.w * f;
-      l = l * a + ml.y * f;
-      m = top;
+      const float f = exp2f(ml.x - m);
+      o.x = fmaf(w.x, f, o.x); o.y = fmaf(w.y, f, o.y); o.z = fmaf(w.z, f, o.z); o.w = fmaf(w.w, f, o.w);
+      l = fmaf(ml.y, f, l);
     }
     const float inv = 1.0f / l;
-    const int tok = (r0 + r) / p.qpk, h = g * p.qpk + (r0 + r) % p.qpk;
+    const int row = r0 + e / v4, tok = row / p.qpk, h = g * p.qpk + row % p.qpk;
     T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + tok) * p.out_ld + (size_t)h * p.vdim + 4 * c;
     const float z[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
 #pragma unroll
@@ -905,7 +983,7 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
   }
 }
 
-// Floats of the parts' rows and columns: two of every block of either kernel.
+// Rows of the parts: two tiles of every block of either kernel.
 static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
 
 template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st) {
@@ -918,12 +996,33 @@ template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st
   PT_LAUNCH_CHECK("pt_tree_attn");
   return PT_OK;
 }
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// The rows of all pages' keys or values: [pages][n_kv page][width], boxes of 64 columns of `box` rows of one page.  (How many pages there are is the
+// caller's to know: none that the table does not name is read.)
+static bool page_map(CUtensorMap *map, CUtensorMapDataType dt, const void *base, int width, const Params &p) {
+  static EncodeTiled fn = [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) == cudaSuccess && res == cudaDriverEntryPointSuccess ? (EncodeTiled)ptr : nullptr;
+  }();
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)p.n_kv * p.page, 1u << 30}, strides[2] = {(cuuint64_t)width * 2, (cuuint64_t)p.n_kv * p.page * (p.dim + p.vdim) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.box, 1}, steps[3] = {1, 1, 1};
+  return fn && fn(map, dt, 3, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, bool CAP> static int launch_tensor(Params &p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  PT_CUDA(allow_smem(tree_tensor_kernel<T, CAP>, (int)tensor_smem(128), done));
+  PT_CUDA(allow_smem(tree_tensor_kernel<T, CAP>, (int)tensor_smem(), done));
   p.rows_tile = TROWS; p.keys_tile = TKEYS;
   p.blocks = sm_count();
-  PT_CUDA(launch_early(tree_tensor_kernel<T, CAP>, Grid(p.blocks), TENSOR_THREADS, tensor_smem(p.dim), st, p));
+  CUtensorMap keys{}, values{};
+  p.box = 1;
+  while (p.box < TKEYS && p.page % (2 * p.box) == 0) p.box *= 2;
+  const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (p.box < 8 || !page_map(&keys, dt, p.pool, p.dim, p) || !page_map(&values, dt, (T *)p.pool + (size_t)p.n_kv * p.page * p.dim, p.vdim, p)) p.box = 0;      // (a swizzled box has rows in eights)
+  PT_CUDA(launch_early(tree_tensor_kernel<T, CAP>, Grid(p.blocks), TENSOR_THREADS, tensor_smem(), st, p, keys, values));
   PT_LAUNCH_CHECK("pt_tree_attn");
   return PT_OK;
 }
@@ -937,8 +1036,7 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   }
   if (!tensor) rc = p.vdim <= 64 ? launch_plain<T, 2>(p, st) : p.vdim <= 128 ? launch_plain<T, 4>(p, st) : launch_plain<T, 8>(p, st);
   if (rc) return rc;
-  const int tiles = ceil_div(p.most * p.qpk, p.rows_tile);
-  PT_CUDA(launch_early(combine_kernel<T>, Grid(dim3(p.n_kv * tiles, p.n_seq)), COMBINE_THREADS, 0, st, p));
+  PT_CUDA(launch_early(combine_kernel<T>, Grid(dim3(p.n_kv * ceil_div(p.most * p.qpk, COMBINE_ROWS), p.n_seq)), COMBINE_THREADS, 0, st, p));
   PT_LAUNCH_CHECK("pt_tree_attn");
   return PT_OK;
 }
