@@ -7,7 +7,7 @@
 // (max, sum, unnormalised output) of its keys in the workspace, and combine_kernel adds the parts up in order.  Where the parts lie follows from the
 // lengths alone: no counters, and the same sums on every run.
 //
-//   tree_prep_kernel      depths; rotates and appends the new keys and values; zeroes the output's padding columns
+//   tree_prep_kernel      in front of tree_plain_kernel: depths; rotates and appends the new keys and values; zeroes the output's padding columns
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
@@ -67,8 +67,8 @@ __device__ __forceinline__ Span span(const Params &p, const Seq &x) {
   const int lo = p.window ? max(0, x.start - p.window + 1) / p.keys_tile : 0;
   return Span{lo, (x.start + x.n + p.keys_tile - 1) / p.keys_tile - lo, (x.n * p.qpk + p.rows_tile - 1) / p.rows_tile};
 }
-// Units in front of every sequence (units[n_seq]: all), by the whole block.
-__device__ __forceinline__ void count_units(const Params &p, int *units) {
+// Units in front of every sequence (units[n_seq]: all), by the whole block.  REPORT: sequences that nothing is done for set the flag.
+template <bool REPORT = false> __device__ __forceinline__ void count_units(const Params &p, int *units) {
   __shared__ int warp_sum[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   int base = 0;
@@ -80,6 +80,9 @@ __device__ __forceinline__ void count_units(const Params &p, int *units) {
       if (x.n) {
         const Span y = span(p, x);
         v = p.n_kv * y.row_tiles * y.tiles;
+      } else if (REPORT && blockIdx.x == 0 && p.error_flag) {
+        const int n = p.cu[s + 1] - x.row0;
+        if (n > 0) atomicExch(p.error_flag, n > p.most ? 14 : 12);
       }
     }
     int t = v;
@@ -122,10 +125,10 @@ __device__ __forceinline__ Share share(const Params &p, const int *units) {
 struct Piece {
   int s, g, rt, t0, nt;
   Seq x;
-  bool whole;            // the item's only part
+  bool whole, first;     // the item's only part, its first
   int slot;              // else: where it goes.  A block has at most two such parts: one of an item that began before its run, one that goes on behind it
 };
-__device__ __forceinline__ Piece piece_at(const Params &p, const int *units, const Share &sh, int block, int u) {
+__device__ __noinline__ Piece piece_at(const Params &p, const int *units, const Share &sh, int block, int u) {
   Piece k;
   k.s = seq_of(units, p.n_seq, u);
   k.x = sequence(p, k.s);
@@ -137,7 +140,8 @@ __device__ __forceinline__ Piece piece_at(const Params &p, const int *units, con
   k.t0 = y.first + u - first;
   k.nt = end - u;
   k.whole = k.nt == y.tiles;
-  k.slot = 2 * block + (u == first ? 1 : 0);
+  k.first = u == first;
+  k.slot = 2 * block + (k.first ? 1 : 0);
   return k;
 }
 
@@ -407,30 +411,33 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 }
 
 // ------------------------------------------------------------------------------------------ tensor cores
-// One block per SM, 128 query rows against tiles of 128 keys.  S = Q K^T goes to tensor memory (lane = row), the softmax threads, one per row, turn it into
-// weights in place, and O += P V takes those from tensor memory and V, keys outermost as the cache has it, from shared memory.  A row's weights would
-// lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 16 or more, for a second product with V.  Two groups of softmax warps take
-// alternate tiles with sums and an output of their own, so that one group's exponentials run beside the other's products; the two are added at the end.
-//   warps 0-3, 4-7   softmax of even and odd tiles; query rows in, results out
+// One block per SM, 128 query rows against tiles of 128 keys.  S = Q K^T goes to tensor memory (lane = row), two softmax threads per row, one for each
+// half of the keys, turn it into weights in place, and O += P V takes those from there and V, keys outermost as the cache has it, from shared memory.
+// A row's weights would lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 15 or more, for a second product with V.  Scores
+// have two buffers, so that the products of one tile run beside the exponentials of the other.
+//   warps 0-3, 4-7   softmax of the first and the second 64 keys; query rows in, results out
 //   warps 8, 9       keys and values into a ring of tiles in the swizzled layout: whole tiles by TMA, a box per page and 64 columns; tiles that begin or
 //                    end inside (a sequence's last, a window's first), and pages of sizes that no box fits, by 16-byte asynchronous copies of rows.
 //                    (Copies alone deliver 18 bytes a cycle to an SM, memory has 24 for each.)
-//   warp 10          issues the products; owns the tensor memory
+//   warp 10          issues the products; owns the tensor memory: 2 x 128 columns of scores, 128 of output.  (All 512 are asked for: they begin at 0, and an
+//                    instruction whose operands the compiler knows to be the same in all lanes goes out every 64 cycles, else every 105.)
+// New keys and values come from the caller's rows, not from the cache: whoever has an item's last tile rotates them on their way to shared memory, and
+// the block with the first tile of rows writes them to the pages, which nobody reads in this launch.
 // (Twelve warps: an SM quarter's registers are shared by three.)  Rotated queries would lose 8 bits' worth too, and come in two parts likewise.
 // A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as
 // copies stay in flight.  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
 // (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
 constexpr int SOFT_WARPS = 8, COPY_WARPS = 2, MMA_WARP = SOFT_WARPS + COPY_WARPS, TENSOR_THREADS = 384, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
-constexpr int OPERAND_BYTES = 192 * 1024;      // query rows and the ring
+constexpr int OPERAND_BYTES = 192 * 1024, O_COL = 256;      // query rows and the ring; first column of the output
 constexpr float RAISE = 8.f;
 
 struct TcShared {
   uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, drained;
-  uint32_t tmem;
-  volatile int abort;
+  uint32_t tmem;               // where the tensor memory begins (at 0: all of it is ours)
+  volatile int abort, trees;   // trees: built so far
   int units[MAX_SEQ + 1];
   Tree tree;
-  float2 stat[2][2][TROWS];      // by piece (a group without tiles is ahead of the other), group
+  float top[2][2][TROWS], sum[2][2][TROWS];      // of a half of the keys: by tile, by piece (a warp may be one ahead of its partner)
   // Values that are not finite and that not every row sees, by piece: drafted tokens, and positions from the lowest of any row's window on.  They are
   // zeroed in shared memory (0 * inf would reach rows that do not see them), and the rows that do see them become NaN.
   uint32_t bad[8][2 * WORDS];
@@ -472,14 +479,12 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr) { return (tc::smem
 __device__ __forceinline__ uint32_t product_desc(bool bf16, int n, bool b_by_rows) {
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_by_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(TROWS >> 4) << 24;
 }
-// Byte of 16-byte unit c of row r of an operand of rows of 128 swizzled bytes (blocks of 128 rows).
+// Byte of 16-byte unit c of row r of a tile of rows of 128 swizzled bytes (blocks of 128 rows).
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 // 16 bytes, zeros where bytes is 0.
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// The barrier gets this thread's arrival when all its copies so far have landed.
-__device__ __forceinline__ void cp_arrive(uint64_t &bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::sa(&bar)) : "memory"); }
 __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t &bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(tc::sa(&bar)), "r"(x), "r"(y), "r"(z)
                : "memory");
@@ -504,6 +509,32 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&v)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+
+// Eight neighbouring dimensions d .. d + 7 of a head's row, rotated by the angles of `pos`; `own`: their values.
+template <typename T> __device__ __forceinline__ void turn8(const Params &p, const T *src, int d, int pos, const uint4 &own, float2 (&y)[4]) {
+  const int h = p.rope_half;
+  if (h % 8 == 0) {
+    const bool second = d >= h;
+    const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? d - h : d + h));
+    const uint32_t o[4] = {own.x, own.y, own.z, own.w}, z[4] = {other.x, other.y, other.z, other.w};
+    const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? d - h : d));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 m = Half2<T>::wide(o[i]), t = Half2<T>::wide(z[i]);
+      const float4 an = __ldg(cs + i);
+      y[i] = second ? make_float2(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : make_float2(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = make_float2(turned<T>(p, src, d + 2 * i, pos), turned<T>(p, src, d + 2 * i + 1, pos));
+  }
+}
+
 struct Waits {          // a role's bounded waits: the whole warp goes the same way
   TcShared &sm;
   int *error_flag;
@@ -518,14 +549,15 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
     }
     return ok;
   }
-  __device__ __forceinline__ bool alone(uint64_t &bar, uint32_t parity) const {      // the same for one lane
-    const uint32_t b = tc::sa(&bar);
-    for (int i = 0; i < 64; ++i)
-      if (mbar_test(b, parity)) return true;
-    if (mbar_wait(b, parity, &sm.abort)) return true;
-    if (!sm.abort && error_flag) atomicCAS(error_flag, 0, 11);
-    sm.abort = 1;
-    return false;
+  __device__ __forceinline__ void tree(int n) const {      // the n-th tree of the block
+    int looks = 0;
+    while (sm.trees < n && !sm.abort)
+      if (++looks >= WAIT_LIMIT) {
+        if (error_flag) atomicCAS(error_flag, 0, 11);
+        sm.abort = 1;
+      }
+    __threadfence_block();
+    __syncwarp();
   }
   __device__ __forceinline__ void arrive(uint64_t &bar) const {      // one arrival of the warp
     __syncwarp();
@@ -568,21 +600,21 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tc::sa(&sm.s_full[i]), 1);
-      mbar_init(tc::sa(&sm.p_full[i]), SOFT_WARPS / 2);
+      mbar_init(tc::sa(&sm.p_full[i]), SOFT_WARPS);
       mbar_init(tc::sa(&sm.o_done[i]), 1);
     }
     mbar_init(tc::sa(&sm.q_full), SOFT_WARPS);
     mbar_init(tc::sa(&sm.drained), 1);
     sm.abort = 0;
+    sm.trees = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = tid; i < 8 * 2 * WORDS; i += TENSOR_THREADS) (&sm.bad[0][0])[i] = 0;
   if (tid < 8) sm.any_bad[tid] = 0;
   if (warp == MMA_WARP) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
   tc::fence_before();
-  count_units(p, sm.units);      // (ends with a barrier)
+  count_units<true>(p, sm.units);      // (ends with a barrier)
   tc::fence_after();
-  const uint32_t tmem = sm.tmem;
   const Share sh = share(p, sm.units);
   const int begin = blockIdx.x * sh.quota, end = min((int)(blockIdx.x + 1) * sh.quota, sh.all);
   const Waits wait{sm, p.error_flag};
@@ -592,7 +624,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     const int w = warp - SOFT_WARPS;
     const int box = p.box, boxes = box ? TKEYS / box : 0;   // rows of a box, and how many make a tile
     const bool one = tc::elect_one();
-    int e = 0, pieces = 0;                                  // tiles asked for
+    int e = 0, pieces = 0, trees = 0, had = -1;             // tiles asked for; trees that are built up to here, and of which sequence the last is
     bool ok = true;
     for (int u = begin; u < end && ok; ++pieces) {
       const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
@@ -600,13 +632,15 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       const Seq x = k.x;
       const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
       const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
-      auto page_of = [&](int j) { return j >= lowest && j < last ? table[j / p.page] : 0; };
+      if (k.s != had) ++trees;
+      had = k.s;
+      auto page_of = [&](int j) { return j >= lowest && j < x.start ? table[j / p.page] : 0; };
       auto box_page = [&](int t) { return w == 0 && lane < boxes ? page_of(t * TKEYS + lane * box) : 0; };
       int ahead = box_page(k.t0);                           // pages of the next tile's boxes, one per lane
       for (int t = 0; t < k.nt && ok; ++t) {
         const int j0 = (k.t0 + t) * TKEYS, phys = ahead;
         ahead = box_page(k.t0 + t + 1);
-        const bool whole = box && j0 >= lowest && j0 + TKEYS <= last;
+        const bool whole = box && j0 >= lowest && j0 + TKEYS <= x.start && !partial(p, x, j0);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++e) {
           const int slot = e % slots;
@@ -625,102 +659,147 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
             if (w || !one) mbar_arrive(tc::sa(&sm.full[slot]));
             continue;
           }
+          // rows of the cache, zeros where there are none
           for (int h = 0; h < 2; ++h) {
             const int r0 = w * 64 + h * 32, j = j0 + r0 + lane;
-            const bool in = j >= lowest && j < last;
-            const T *src = (kv ? v_page<T>(p, page_of(j), k.g) : k_page<T>(p, page_of(j), k.g)) + (size_t)(in ? j % p.page : 0) * dims;
+            const bool in = j >= lowest && j < min(last, x.start);
+            const T *src = (kv ? v_page<T>(p, in ? table[j / p.page] : 0, k.g) : k_page<T>(p, in ? table[j / p.page] : 0, k.g)) + (size_t)(in ? j % p.page : 0) * dims;
             const int cols = blocks * 8, c = lane % cols;
             for (int q0 = 0; q0 < 32; q0 += 32 / cols) {
               const int r = q0 + lane / cols;
               const unsigned long long from = __shfl_sync(0xffffffffu, (unsigned long long)src, r);
-              const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have;
-              if (c < pad) cp_async(to + swizzled(r0 + r, c), reinterpret_cast<const T *>(from) + (there ? c * 8 : 0), there ? 16 : 0);
+              const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have, drafted = j0 + r0 + r >= x.start && j0 + r0 + r < last && c < have;
+              if (c < pad && !drafted) cp_async(to + swizzled(r0 + r, c), reinterpret_cast<const T *>(from) + (there ? c * 8 : 0), there ? 16 : 0);
             }
           }
-          if (kv && partial(p, x, j0)) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
+          // drafted rows
+          const int d0 = max(j0 - x.start, 0), d1 = min(x.n, j0 + TKEYS - x.start);      // of the sequence's new tokens
+          if (d1 > d0 && !kv && p.rope_half && p.parent) wait.tree(trees);      // (depths)
+#pragma unroll 2
+          for (int i0 = w * 32 + lane; i0 < (d1 - d0) * have; i0 += COPY_WARPS * 32) {
+            const int d = d0 + i0 / have, c = i0 % have, j = x.start + d;
+            const T *src = reinterpret_cast<const T *>(kv ? p.v : p.k) + (size_t)(x.row0 + d) * p.kv_ld + (size_t)k.g * dims;
+            uint4 v = *reinterpret_cast<const uint4 *>(src + c * 8);
+            if (!kv && c * 8 < 2 * p.rope_half) {
+              float2 y[4];
+              turn8<T>(p, src, c * 8, x.start + (p.parent ? sm.tree.depth[d] : d), v, y);
+              v = make_uint4(Half2<T>::pack(y[0].x, y[0].y), Half2<T>::pack(y[1].x, y[1].y), Half2<T>::pack(y[2].x, y[2].y), Half2<T>::pack(y[3].x, y[3].y));
+            }
+            if (k.rt == 0) {
+              T *row = (kv ? v_page<T>(p, table[j / p.page], k.g) : k_page<T>(p, table[j / p.page], k.g)) + (size_t)(j % p.page) * dims;
+              *reinterpret_cast<uint4 *>(row + c * 8) = v;
+            }
+            if (kv && (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w))) {
+              v = make_uint4(0u, 0u, 0u, 0u);
+              atomicOr(&sm.bad[pieces & 7][d >> 5], 1u << (d & 31));
+              sm.any_bad[pieces & 7] = 1;
+            }
+            *reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(j - j0, c)) = v;
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          if (kv && p.window) {
             for (int h = 0; h < 2; ++h) {
               const int cols = blocks * 8, c = lane % cols;
               for (int q0 = 0; q0 < 32; q0 += 32 / cols) {      // (the units that this lane copied)
-                const int r = w * 64 + h * 32 + q0 + lane / cols, key = j0 + r, d = key - x.start, b = key - lowest;
-                if (c >= have || key >= last || key < lowest || (d < 0 && (p.window == 0 || b >= MAX_NODES))) continue;
+                const int r = w * 64 + h * 32 + q0 + lane / cols, key = j0 + r, b = key - lowest;
+                if (c >= have || key >= min(last, x.start) || key < lowest || b >= MAX_NODES) continue;
                 uint4 *at = reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(r, c));
                 const uint4 v = *at;
                 if (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w)) {
                   *at = make_uint4(0u, 0u, 0u, 0u);
-                  const int bit = d >= 0 ? d : MAX_NODES + b;
+                  const int bit = MAX_NODES + b;
                   atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
                   sm.any_bad[pieces & 7] = 1;
                 }
               }
             }
           }
-          cp_arrive(sm.full[slot]);
+          tc::fence_operands();
+          mbar_arrive(tc::sa(&sm.full[slot]));
         }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");        // nothing is in flight when the block ends, after a failure either
+    // nothing is in flight when the block ends, after a failure either
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (w == 0 && box) mbar_wait_ring(tc::sa(&sm.full[0]), e, slots);
   } else if (warp == MMA_WARP) {
-    // ---- products, by one lane
-    if (tc::elect_one()) {
-      const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
-      const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
-      int pieces = 0, n_p[2] = {0, 0}, e0 = 0;              // pieces, weights used of either group, first tile of the piece
-      bool ok = true;
-      const uint64_t q0 = tc::smem_desc_sw128(tc::sa(Q)), q1 = tc::smem_desc_sw128(tc::sa(Q) + q_bytes);
-      auto scores = [&](int w, int e) {
-        const int slot = e % slots;
-        if (!(ok = ok && wait.alone(sm.full[slot], (e / slots) & 1))) return;
-        tc::fence_operands();                               // (what the copies wrote, for the tensor core)
-        tc::fence_after();
-        const uint64_t kt = tc::smem_desc_sw128(tc::sa(ring + slot * slot_bytes));
-        for (int part = 0; part < (split_q ? 2 : 1); ++part)
-#pragma unroll 4
-          for (int s = 0; s < ksteps; ++s) {
-            const uint64_t at = (s >> 2) * (128 * 128 / 16) + (s & 3) * 2;      // (in units of 16 bytes)
-            tc::umma<false>(tmem + w * 128, (part ? q1 : q0) + at, kt + at, kdesc, part > 0 || s > 0);
+    // ---- products.  (What they take is the same in all lanes, and the compiler knows it: counters that go up by known steps, in loops whose bounds come
+    // out of a reduction.  After a wait that ran out they go on: nobody reads what they give.)
+    const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
+    const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
+    const uint64_t q0 = tc::smem_desc_sw128(tc::sa(Q)), r0 = tc::smem_desc_sw128(tc::sa(ring)), rv0 = value_desc(tc::sa(ring));
+    struct Place { int slot, phase; } at_k{0, 0}, at_v{1, 0};      // of the next tiles of keys and of values
+    auto on = [&](Place &x) {
+      x.slot += 2;
+      if (x.slot >= slots) { x.slot -= slots; x.phase ^= 1; }
+    };
+    int pieces = 0, done = 0;                               // tiles done
+    auto scores = [&](int b) {
+      wait(sm.full[at_k.slot], at_k.phase);
+      tc::fence_after();
+      if (tc::elect_one()) {
+        const uint64_t kt = r0 + (uint64_t)(uint32_t)(at_k.slot * (slot_bytes / 16));
+        for (int part = 0; part < (split_q ? 2 : 1); ++part) {
+          const uint64_t qt = q0 + (part ? (uint32_t)q_bytes / 16 : 0u);
+          if (ksteps == 8) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s) tc::umma<false>(b * 128, qt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
+          } else {
+            for (int s = 0; s < ksteps; ++s) tc::umma<false>(b * 128, qt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
           }
-        tc::umma_commit(tc::sa(&sm.empty[slot]));
-        tc::umma_commit(tc::sa(&sm.s_full[w]));
-      };
-      // (Tiles come as K V K V ..; the scores of the next tile but one are asked for behind this one's output.)
-      for (int u = begin; u < end && ok; ++pieces) {
-        const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
-        u += k.nt;
-        if (!(ok = wait.alone(sm.q_full, pieces & 1))) break;
-        scores(0, e0);
-        if (k.nt > 1) scores(1, e0 + 2);
-        for (int t = 0; t < k.nt && ok; ++t) {
-          const int w = t & 1, e = e0 + 2 * t + 1, slot = e % slots;
-          if (!(ok = wait.alone(sm.full[slot], (e / slots) & 1) && wait.alone(sm.p_full[w], n_p[w] & 1))) break;
-          ++n_p[w];
-          tc::fence_operands();
-          tc::fence_after();
-          const uint64_t vt = value_desc(tc::sa(ring + slot * slot_bytes));
-          const uint32_t o = tmem + 256 + w * 128, pw = tmem + w * 128;
+        }
+        tc::umma_commit(tc::sa(&sm.empty[at_k.slot]));
+        tc::umma_commit(tc::sa(&sm.s_full[b]));
+      }
+      __syncwarp();
+      on(at_k);
+    };
+    // (Tiles come as K V K V ..; the scores of the next tile but one are asked for behind this one's output.)
+    int used0 = 0, used1 = 0;                               // of either buffer
+    const int u1 = __reduce_max_sync(0xffffffffu, end);
+    for (int u = __reduce_max_sync(0xffffffffu, begin); u < u1; ++pieces) {
+      const int nt = __reduce_max_sync(0xffffffffu, piece_at(p, sm.units, sh, blockIdx.x, u).nt);
+      u += nt;
+      wait(sm.q_full, pieces & 1);
+      tc::fence_after();
+      scores(0);
+      if (nt > 1) scores(1);
+      for (int t = 0; t < nt; ++t, ++done) {
+        const int b = t & 1;
+        wait(sm.full[at_v.slot], at_v.phase);
+        wait(sm.p_full[b], (b ? used1++ : used0++) & 1);
+        tc::fence_after();
+        if (tc::elect_one()) {
+          const uint64_t vt = rv0 + (uint64_t)(uint32_t)(at_v.slot * (slot_bytes / 16));
 #pragma unroll
           for (int s = 0; s < 16; ++s)                      // (hi and lo of 16 keys: 8 columns each)
-            tc::umma_ta(o, pw + (s >> 2) * 32 + (s & 1) * 16 + (s >> 1 & 1) * 8, vt + (s >> 1) * (2048 / 16), vdesc, t > 1 || s > 0);
-          tc::umma_commit(tc::sa(&sm.empty[slot]));
-          if (t + 2 >= k.nt) tc::umma_commit(tc::sa(&sm.o_done[w]));
-          else scores(w, e + 3);
+            tc::umma_ta(O_COL, b * 128 + (s >> 2) * 32 + (s & 1) * 16 + (s >> 1 & 1) * 8, vt + (s >> 1) * (2048 / 16), vdesc, t > 0 || s > 0);
+          tc::umma_commit(tc::sa(&sm.empty[at_v.slot]));
+          tc::umma_commit(tc::sa(&sm.o_done[done & 1]));
         }
-        e0 += 2 * k.nt;
+        __syncwarp();
+        on(at_v);
+        if (t + 2 < nt) scores(b);
       }
-      // nothing may be on its way to tensor or shared memory when the block ends
+    }
+    // nothing may be on its way to tensor or shared memory when the block ends
+    if (tc::elect_one()) {
       tc::umma_commit(tc::sa(&sm.drained));
       mbar_wait_all(tc::sa(&sm.drained), 0);
     }
     __syncwarp();
   } else if (warp < SOFT_WARPS) {
     // ---- softmax
-    const int w = warp >> 2, q = warp & 3, row = q * 32 + lane;
-    const uint32_t lanes = (uint32_t)(q * 32) << 16, S = tmem + w * 128 + lanes;
-    int pieces = 0, n_s = 0, n_o[2] = {0, 0}, had = -1;
+    const int half = warp >> 2, q = warp & 3, row = q * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16, S = lanes + half * 64, O = lanes + O_COL;
+    int pieces = 0, n_s[2] = {0, 0}, n_o = 0, had = -1;
     const float a1 = fabsf(p.scale) * kLog2e, a2 = CAP ? 2.0f * a1 / p.softcap : 0.f, b2 = p.softcap * kLog2e;
     auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };      // (grows with s)
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory"); };
+    auto meet_partner = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + q) : "memory"); };       // the warp with the same rows
+    // The output of the block's tile i.  (By turns on two barriers: of either the phase before is done when the scores of tile i are, and the phase behind
+    // needs weights that come later.)
+    auto output_of = [&](int i) { wait(sm.o_done[i & 1], (i >> 1) & 1); };
     // (After a wait that ran out all go on without waiting: everybody comes to every meeting, and what is computed does not matter.)
     for (int u = begin; u < end; ++pieces) {
       const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
@@ -729,49 +808,44 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       const int r0 = k.rt * TROWS, rows = min(TROWS, x.n * p.qpk - r0);
       if (k.s != had) {
         if (had >= 0) meet();                               // (everybody is done with the tree before)
-        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, meet);
+        bool none = false;
+        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, meet, &none);
+        if (none && p.error_flag) atomicExch(p.error_flag, 14);
         had = k.s;
+        if (tid == 0) {
+          __threadfence_block();
+          sm.trees = sm.trees + 1;
+        }
       }
-      // query rows, rotated, and negated where the scale is negative
+      const bool live = q * 32 < rows;                      // (uniform over the warp)
+      const int at = min(r0 + row, x.n * p.qpk - 1), node = at / p.qpk, head = k.g * p.qpk + at - node * p.qpk, depth = sm.tree.depth[node];
+      const uint32_t *seen = sm.tree.seen[node];
+      // query rows, rotated, and negated where the scale is negative (rows that there are none of hold anything: they stay by themselves)
       {
-        const int cols = kblocks * 8, h = p.rope_half;
-        for (int e = tid; e < TROWS * cols; e += SOFT_WARPS * 32) {
-          const int r = e / cols, c = e - r * cols;
+        const int cols = p.dim / 8, pad = (p.dim + 15) / 16 * 2;
+        const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 2
+        for (int e = tid; e < rows * pad; e += SOFT_WARPS * 32) {
+          const int r = e / pad, c = e - r * pad;
           uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
-          if (r < rows && c * 8 < p.dim) {
-            const int i = (r0 + r) / p.qpk, head = k.g * p.qpk + (r0 + r) - i * p.qpk;
-            const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)head * p.dim;
+          if (c < cols) {
+            const int i = (r0 + r) / p.qpk, hd = k.g * p.qpk + (r0 + r) - i * p.qpk;
+            const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)hd * p.dim;
             v = *reinterpret_cast<const uint4 *>(src + c * 8);
-            uint32_t *o = reinterpret_cast<uint32_t *>(&v), *ol = reinterpret_cast<uint32_t *>(&lo);
-            if (c * 8 < 2 * h) {
-              const int pos = x.start + sm.tree.depth[i];
+            if (c * 8 < 2 * p.rope_half) {
               float2 y[4];
-              if (h % 8 == 0) {
-                const bool second = c * 8 >= h;
-                const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? c * 8 - h : c * 8 + h));
-                const uint32_t *z = reinterpret_cast<const uint32_t *>(&other);
-                const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? c * 8 - h : c * 8));
+              uint32_t a[4], b[4];
+              turn8<T>(p, src, c * 8, x.start + sm.tree.depth[i], v, y);
 #pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                  const float2 m = Half2<T>::wide(o[i4]), t = Half2<T>::wide(z[i4]);
-                  const float4 an = __ldg(cs + i4);
-                  y[i4] = second ? make_float2(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : make_float2(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
-                }
-              } else {
-#pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) y[i4] = make_float2(turned<T>(p, src, c * 8 + 2 * i4, pos), turned<T>(p, src, c * 8 + 2 * i4 + 1, pos));
+              for (int z = 0; z < 4; ++z) {
+                a[z] = Half2<T>::pack(y[z].x, y[z].y);
+                const float2 back = Half2<T>::wide(a[z]);
+                b[z] = Half2<T>::pack(y[z].x - back.x, y[z].y - back.y) ^ flip;
               }
-#pragma unroll
-              for (int i4 = 0; i4 < 4; ++i4) {
-                o[i4] = Half2<T>::pack(y[i4].x, y[i4].y);
-                const float2 back = Half2<T>::wide(o[i4]);
-                ol[i4] = Half2<T>::pack(y[i4].x - back.x, y[i4].y - back.y);
-              }
+              v = make_uint4(a[0], a[1], a[2], a[3]);
+              lo = make_uint4(b[0], b[1], b[2], b[3]);
             }
-            if (p.scale < 0.f) {
-#pragma unroll
-              for (int i4 = 0; i4 < 4; ++i4) { o[i4] ^= 0x80008000u; ol[i4] ^= 0x80008000u; }
-            }
+            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
           }
           *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
           if (split_q) *reinterpret_cast<uint4 *>(Q + q_bytes + swizzled(r, c)) = lo;
@@ -779,109 +853,101 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
         tc::fence_operands();
         wait.arrive(sm.q_full);
       }
-      const bool live = q * 32 < rows;                      // (uniform over the warp)
-      const int node = min(r0 + row, x.n * p.qpk - 1) / p.qpk, depth = sm.tree.depth[node];
-      const uint32_t *seen = sm.tree.seen[node];
-      float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to
-      const int mine = (k.nt - w + 1) / 2;
-      // Scores of a tile to weights; `vis`: the keys that the row sees.
-      auto weigh = [&](auto masked, bool again, const uint32_t (&vis)[4]) {
+      // padding columns of the output's rows
+      if (k.g == 0 && half == 0 && row < rows && at == node * p.qpk && k.first)
+        for (int c = p.n_head * p.vdim; c < p.out_cols; ++c) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + node) * p.out_ld + c] = rounded<T>(0.f);
+      float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to; l: of this half
+      // Scores of a tile's half to weights.
+      auto weigh = [&](auto masked, int t) {
         constexpr bool MASKED = decltype(masked)::value;
-        // (Loops of two steps, not four: a short run of tiles fetches this code once.)
-        uint32_t v[2][32];
-        tmem_load(S, v[0]);
+        const uint32_t at = S + (t & 1) * 128;
+        uint32_t v[2][32], see[2] = {0xffffffffu, 0xffffffffu};
+        tmem_load(at, v[0]);
+        tmem_load(at + 32, v[1]);
+        if (MASKED) {
+          const int j0 = (k.t0 + t) * TKEYS + half * 64;
+          see[0] = seen_word(p, x, seen, depth, j0);
+          see[1] = seen_word(p, x, seen, depth, j0 + 32);
+        }
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c2 = 0; c2 < 4; c2 += 2)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t see = MASKED ? (c2 ? vis[2 + b] : vis[b]) : 0;
-            tmem_landed(v[b]);
-            tmem_load(S + (c2 + b + 1 & 3) * 32, v[1 - b]);   // (the last: the first again)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float s = __uint_as_float(v[b][i]);
-              tops[i & 3] = fmaxf(tops[i & 3], !MASKED || see >> i & 1 ? s : -INFINITY);
-            }
-          }
         tmem_landed(v[0]);
+        tmem_landed(v[1]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (MASKED && !(see[b] >> i & 1)) v[b][i] = 0xff800000u;      // -inf
+            tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(v[b][i]));
+          }
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        sm.top[t & 1][half][row] = top;
+        meet_partner();
+        top = fmaxf(top, sm.top[t & 1][1 - half][row]);
         top = (top == -INFINITY ? top : score(top)) - Half2<T>::kBias;
         // (keys that went before lie far below, or none was seen: the sums so far are scaled to the new maximum)
-        const bool raise = top > m + (m == -INFINITY ? 0.f : RAISE);
-        if (__any_sync(0xffffffffu, raise && again)) {
+        const bool raise = row < rows && top > m + (m == -INFINITY ? 0.f : RAISE);
+        if (__any_sync(0xffffffffu, raise) && t > 0) {
           const float f = raise ? ex2(m - top) : 1.f;        // (m = -inf: 0, of sums that are 0)
           l *= f;
-          for (int c = 0; c < p.vdim; c += 32) {
-            uint32_t y[32];
-            tc::tmem_ld32(tmem + 256 + w * 128 + lanes + c, y);
+          output_of(n_o - 1);
+          tc::fence_after();
+          for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
+            uint32_t y[16];
+            tc::tmem_ld16(O + c, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-            tc::tmem_st32(tmem + 256 + w * 128 + lanes + c, y);
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_store16(O + c, y);
           }
         }
         if (raise) m = top;
         const float ref = m == -INFINITY ? 0.f : m;
         float add[4] = {0.f, 0.f, 0.f, 0.f};
-        tmem_load(S, v[0]);
-#pragma unroll 1
-        for (int c2 = 0; c2 < 4; c2 += 2)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t see = MASKED ? (c2 ? vis[2 + h] : vis[h]) : 0;
-            tmem_landed(v[h]);
-            if (c2 + h < 3) tmem_load(S + (c2 + h + 1) * 32, v[1 - h]);
-            uint32_t o[32];
+        for (int b = 0; b < 2; ++b) {
+          uint32_t o[32];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float a = __uint_as_float(v[h][i]), b = __uint_as_float(v[h][i + 1]);
-              a = CAP ? score(a) - ref : fmaf(a, a1, -ref);
-              b = CAP ? score(b) - ref : fmaf(b, a1, -ref);
-              a = ex2(!MASKED || see >> i & 1 ? a : -INFINITY);
-              b = ex2(!MASKED || see >> (i + 1) & 1 ? b : -INFINITY);
-              add[i & 2] += a;
-              add[(i & 2) + 1] += b;
-              Half2<T>::split(a, b, o[i / 2], o[16 + i / 2]);
+          for (int i = 0; i < 32; i += 2) {
+            float a = __uint_as_float(v[b][i]), c = __uint_as_float(v[b][i + 1]);
+            if (CAP) {                                       // (-inf stays what is not seen)
+              a = MASKED && a == -INFINITY ? a : score(a) - ref;
+              c = MASKED && c == -INFINITY ? c : score(c) - ref;
+            } else {
+              a = fmaf(a, a1, -ref);
+              c = fmaf(c, a1, -ref);
             }
-            tc::tmem_st32(S + (c2 + h) * 32, o);
+            a = ex2(a);
+            c = ex2(c);
+            add[i & 2] += a;
+            add[(i & 2) + 1] += c;
+            Half2<T>::split(a, c, o[i / 2], o[16 + i / 2]);
           }
+          tc::tmem_st32(at + b * 32, o);
+        }
         l += (add[0] + add[1]) + (add[2] + add[3]);
       };
-      for (int t = 0; t < mine; ++t) {
-        wait(sm.s_full[w], n_s++ & 1);
+      for (int t = 0; t < k.nt; ++t, ++n_o) {               // (n_o: tiles whose output was asked for before this one)
+        wait(sm.s_full[t & 1], n_s[t & 1]++ & 1);
         tc::fence_after();
         if (live) {
-          const int j0 = (k.t0 + 2 * t + w) * TKEYS;
-          if (partial(p, x, j0)) {
-            uint32_t vis[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) vis[c] = seen_word(p, x, seen, depth, j0 + 32 * c);
-            weigh(std::true_type(), t > 0, vis);
-          } else {
-            uint32_t vis[4] = {};
-            weigh(std::false_type(), t > 0, vis);
-          }
+          if (partial(p, x, (k.t0 + t) * TKEYS)) weigh(std::true_type(), t);
+          else weigh(std::false_type(), t);
           tc::tmem_wait_st();
           tc::fence_before();
         }
-        wait.arrive(sm.p_full[w]);
+        wait.arrive(sm.p_full[t & 1]);
       }
-      // ---- both groups' sums together; either group takes half of the columns
-      sm.stat[pieces & 1][w][row] = make_float2(m, l);
+      // ---- out; either half of the threads takes half of the columns
+      sm.sum[pieces & 1][half][row] = l;
       meet();
       if (tid == 0) sm.any_bad[(pieces + 7) & 7] = 0;       // (of the piece before: everybody is past it)
       if (tid < 2 * WORDS) sm.bad[(pieces + 7) & 7][tid] = 0;
-      wait(sm.o_done[0], n_o[0]++ & 1);
-      if (k.nt > 1) wait(sm.o_done[1], n_o[1]++ & 1);
+      output_of(n_o - 1);
       tc::fence_after();
       if (live) {
-        const float2 A = sm.stat[pieces & 1][0][row], B = sm.stat[pieces & 1][1][row];
-        const float top = fmaxf(A.x, B.x), ref = top == -INFINITY ? 0.f : top, fa = ex2(A.x - ref), fb = ex2(B.x - ref);
-        float sum = A.y * fa + B.y * fb;
+        float sum = sm.sum[pieces & 1][0][row] + sm.sum[pieces & 1][1][row];
         if (sm.any_bad[pieces & 7]) {
           const uint32_t *bad = sm.bad[pieces & 7];
           bool hit = false;
-#pragma unroll
           for (int z = 0; z < WORDS; ++z) hit |= (bad[z] & seen[z]) != 0;
           if (p.window) {
             const int low = x.start + depth - p.window + 1 - max(0, x.start - p.window + 1);      // the first of those positions that the token sees
@@ -889,42 +955,34 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
           }
           if (hit) sum = NAN;
         }
-        const float inv = 1.0f / sum;
         const bool store = row < rows;
-        const int i = (r0 + row) / p.qpk, head = k.g * p.qpk + (r0 + row) - i * p.qpk;
-        T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + i) * p.out_ld + (size_t)head * p.vdim;
-        if (!k.whole && w == 0 && store) p.part_ml[(size_t)k.slot * TROWS + row] = make_float2(top, sum);
-        for (int c = w * 32; c < p.vdim; c += 64) {
-          uint32_t va[32], vb[32];
-          tc::tmem_ld32(tmem + 256 + lanes + c, va);
-          if (k.nt > 1) tc::tmem_ld32(tmem + 384 + lanes + c, vb);
-          float o[32];
-#pragma unroll
-          for (int z = 0; z < 32; ++z) {
-            o[z] = __uint_as_float(va[z]) * fa;
-            if (k.nt > 1) o[z] = fmaf(__uint_as_float(vb[z]), fb, o[z]);
-          }
+        const float inv = k.whole ? 1.0f / sum : 1.0f;
+        T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + node) * p.out_ld + (size_t)head * p.vdim;
+        if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * TROWS + row] = make_float2(m, sum);
+#pragma unroll 1
+        for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
+          uint32_t v[16];
+          tc::tmem_ld16(O + c, v);
           if (!store) continue;
-          if (k.whole) {
 #pragma unroll
-            for (int z = 0; z < 32; z += 8)
-              if (c + z < p.vdim) {
-                uint32_t y[4];
+          for (int z = 0; z < 16; z += 8) {
+            if (c + z >= p.vdim) break;
+            if (k.whole) {
+              uint32_t y[4];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) y[b] = Half2<T>::pack(o[z + 2 * b] * inv, o[z + 2 * b + 1] * inv);
-                if (p.out16) {
-                  *reinterpret_cast<uint4 *>(out + c + z) = make_uint4(y[0], y[1], y[2], y[3]);
-                } else {
-                  const T *e = reinterpret_cast<const T *>(y);
+              for (int b = 0; b < 4; ++b) y[b] = Half2<T>::pack(__uint_as_float(v[z + 2 * b]) * inv, __uint_as_float(v[z + 2 * b + 1]) * inv);
+              if (p.out16) {
+                *reinterpret_cast<uint4 *>(out + c + z) = make_uint4(y[0], y[1], y[2], y[3]);
+              } else {
+                const T *e = reinterpret_cast<const T *>(y);
 #pragma unroll
-                  for (int b = 0; b < 8; ++b) out[c + z + b] = e[b];
-                }
+                for (int b = 0; b < 8; ++b) out[c + z + b] = e[b];
               }
-          } else {
-#pragma unroll
-            for (int z = 0; z < 32; z += 4)
-              if (c + z < p.vdim)
-                *reinterpret_cast<float4 *>(p.part_o + (((size_t)k.slot * (p.vdim / 4) + (c + z) / 4) * TROWS + row) * 4) = make_float4(o[z], o[z + 1], o[z + 2], o[z + 3]);
+            } else {
+              uint4 *to = reinterpret_cast<uint4 *>(p.part_o + (((size_t)k.slot * (p.vdim / 4) + (c + z) / 4) * TROWS + row) * 4);
+              to[0] = make_uint4(v[z], v[z + 1], v[z + 2], v[z + 3]);
+              to[TROWS] = make_uint4(v[z + 4], v[z + 5], v[z + 6], v[z + 7]);
+            }
           }
         }
         tc::fence_before();
@@ -934,7 +992,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
   __syncthreads();
   if (warp == MMA_WARP) {
     tc::fence_after();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(sm.tmem, 512);
   }
 }
 static size_t tensor_smem() { return 1024 + OPERAND_BYTES + sizeof(TcShared); }
@@ -987,6 +1045,8 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
 static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
 
 template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st) {
+  PT_CUDA(launch_early(tree_prep_kernel<T>, Grid(dim3(std::min(p.most, 64), p.n_seq)), PREP_THREADS, 0, st, p));
+  PT_LAUNCH_CHECK("pt_tree_attn");
   static std::atomic<uint64_t> done{0};
   const size_t smem = plain_smem(p.dim, VJ * 32);
   if (smem > 32 * 1024) PT_CUDA(allow_smem(tree_plain_kernel<T, VJ>, (int)plain_smem(256, VJ * 32), done));
@@ -1027,8 +1087,6 @@ template <typename T, bool CAP> static int launch_tensor(Params &p, cudaStream_t
   return PT_OK;
 }
 template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
-  PT_CUDA(launch_early(tree_prep_kernel<T>, Grid(dim3(std::min(p.most, 64), p.n_seq)), PREP_THREADS, 0, st, p));
-  PT_LAUNCH_CHECK("pt_tree_attn");
   int rc;
   if constexpr (std::is_same<T, float>::value) tensor = false;
   if constexpr (!std::is_same<T, float>::value) {
@@ -1087,7 +1145,7 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   p.part_ml = (float2 *)(p.part_o + ta::part_rows() * ((a->vdim + 3) / 4 * 4));
   cudaStream_t st = as_stream(stream);
   p.out16 = a->out_ld % 8 == 0 && aligned_to(a->out, 16);
-  const bool tensor = !a->plain && a->dtype != PT_DT_F32 && a->dim <= 128 && a->vdim <= 128 && a->dim % 8 == 0 && a->vdim % 8 == 0 && a->q_ld % 8 == 0 && aligned_to(a->q, 16) &&
+  const bool tensor = !a->plain && a->dtype != PT_DT_F32 && a->dim <= 128 && a->vdim <= 128 && a->dim % 8 == 0 && a->vdim % 8 == 0 && a->q_ld % 8 == 0 && a->kv_ld % 8 == 0 && aligned_to(a->q, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
                       aligned_to(a->pool, 16) && (p.rope_half % 8 || aligned_to(a->rope, 16));
   if (a->dtype == PT_DT_F32) return ta::run<float>(p, false, st);
   return a->dtype == PT_DT_F16 ? ta::run<__half>(p, tensor, st) : ta::run<__nv_bfloat16>(p, tensor, st);
