@@ -884,7 +884,8 @@ int pt_tree_attn(const pt_tree_attn_args *args, void *stream);
  * drawn; logprob[s] (optional) = their log p (temperature 0: of temperature 1).  The rest of a row of max_path entries is -1 (logprob 0).
  * A path of max_path rows is not followed further.  Logits may be -inf, and NaN counts as that; equal infinities share all the weight.  A
  * row that is -inf everywhere accepts nothing and its token is -1.  Sums, residuals and the drawing are in 64 bits.
- * A token outside the vocabulary, or a parent that is none, is never accepted. */
+ * A token outside the vocabulary, a parent that is none, or a row behind the first 512 of a sequence is never accepted.  A random number of 1 or more
+ * draws like the largest below 1. */
 typedef struct pt_verify_args {
   int n_seq, n_tok;
   const int32_t *cu;      /* [n_seq + 1]; a sequence without rows has count 0        */

@@ -216,3 +216,51 @@ def test_captured_and_given_outputs(cuda):
         got = [t.clone() for t in out]
         want = compare(x[0], counts, x[1], x[2], x[3], [1.0] * 3, x[4], x[5], 8)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("seqs", [1, 3, 20, 200])
+@pytest.mark.parametrize("vocab,mode", [(1025, "drawn"), (16384, "chosen"), (130001, "drawn")])
+def test_batches_share_the_gpu_in_any_way(cuda, seqs, vocab, mode):
+    """The vocabulary is cut by how many sequences there are."""
+    seqs = min(seqs, 2000000 // vocab)
+    counts = [1 + i % 4 for i in range(seqs)]
+    logits, parents, token, q, u, u_next = inputs(cuda, counts, "tree", vocab, torch.float32, seqs)
+    compare(logits, counts, parents, token, q if mode == "drawn" else None, [0.9] * seqs, u, u_next, 4)
+
+
+def test_a_vocabulary_whose_weights_are_not_kept(cuda):
+    """More tokens than a cluster's shared memory has room for: weights are computed again where they are needed."""
+    for dtype in DT.values():
+        for mode in ("drawn", "chosen"):
+            logits, parents, token, q, u, u_next = inputs(cuda, [4, 3], "star", 450001, dtype, 9)
+            compare(logits, [4, 3], parents, token, q if mode == "drawn" else None, [1.0, 0.7], u, u_next, 4)
+
+
+def test_rows_behind_the_first_512(cuda):
+    logits, parents, token, q, u, u_next = inputs(cuda, [600], "star", 40, torch.float32, 10)
+    best = int(logits[0].argmax())
+    token[1:] = (best + 1) % 40
+    token[511] = token[512] = best
+    _, count, said = compare(logits, [600], parents, token, None, None, None, None, 2)
+    assert count.tolist() == [2] and said[0, 0] == best
+    from poptransformer_b200 import ops
+    token[511] = (best + 1) % 40                        # now only the row behind them has the right token
+    path, count, said, _ = ops.verify_drafts(logits, torch.tensor([0, 600], dtype=torch.int32, device=cuda), token, torch.tensor(parents[0], dtype=torch.int32, device=cuda), max_path=2)
+    assert count.tolist() == [1] and said[0].tolist() == [best, -1]
+
+
+def test_strided_and_unaligned_rows(cuda):
+    from poptransformer_b200 import _lib, ops
+    import ctypes
+    logits, parents, token, q, u, u_next = inputs(cuda, [5], "chain", 777, torch.float16, 12)
+    wide = torch.full((5, 801), 50.0, dtype=torch.float16, device=cuda)
+    qw = torch.ones((5, 790), device=cuda)
+    wide[:, 3:780], qw[:, :777] = logits, q
+    temp = torch.ones(1, device=cuda)
+    want = compare(logits, [5], parents, token, q, [1.0], u, u_next, 5)
+    out = [torch.empty_like(t) for t in want]
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=cuda)
+    a = _lib.VerifyArgs(1, 5, cu.data_ptr(), ops.DT_F16, 777, 801, wide.data_ptr() + 6, token.data_ptr(), None, qw.data_ptr(), 790, temp.data_ptr(), u.data_ptr(), u_next.data_ptr(), 5,
+                        out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), None)
+    _lib.check(_lib.lib().pt_verify_drafts(ctypes.byref(a), ops._stream()), "pt_verify_drafts")
+    assert all(torch.equal(x, y) for x, y in zip(out, want))
