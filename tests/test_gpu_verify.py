@@ -264,3 +264,32 @@ def test_strided_and_unaligned_rows(cuda):
                         out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), None)
     _lib.check(_lib.lib().pt_verify_drafts(ctypes.byref(a), ops._stream()), "pt_verify_drafts")
     assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize("t", [1e-30, 1e-12, 1e-5, 1e-3, 50.0, 1e20])
+@pytest.mark.parametrize("mode", ["drawn", "chosen"])
+def test_temperatures_of_any_size(cuda, t, mode):
+    """Next to 0 the largest logit has all the weight (equal ones share it), far above all tokens weigh the same."""
+    for kind in ("chain", "star"):
+        logits, parents, token, q, u, u_next = inputs(cuda, [5, 4], kind, 2000, torch.float32, 13)
+        logits[0, [7, 1500]] = logits[0].max() + 1.0
+        compare(logits, [5, 4], parents, token, q if mode == "drawn" else None, [t, t], u, u_next, 5, chain=kind == "chain")
+
+
+@pytest.mark.parametrize("n", [2, 3, 5, 9, 16, 17, 40])
+@pytest.mark.parametrize("vocab", [40, 2001, 40000])
+def test_chains_of_any_length(cuda, n, vocab):
+    """Chains whose parents are not given take a way of their own; drafts near the target, so that many stand, and greedy ones that all stand."""
+    logits, parents, token, q, u, u_next = inputs(cuda, [n, 1, n // 2], "chain", vocab, torch.bfloat16, n, close=0.02)
+    logits = logits[:, :vocab]
+    for draft in (q, None):
+        for temps in ([1.0, 0.8, 0.0], [0.0, 0.5, 2.0]):
+            compare(logits, [n, 1, n // 2], parents, token, draft, temps, u * 0.3, u_next, n, chain=True)
+    for i in range(1, n):
+        token[i] = int(logits[i - 1].argmax())
+    _, count, _ = compare(logits, [n, 1, n // 2], parents, token, None, None, None, None, n, chain=True)
+    assert int(count[0]) == n
+    token[n // 2] = (int(token[n // 2]) + 1) % vocab
+    logits[n // 3] = -math.inf
+    compare(logits, [n, 1, n // 2], parents, token, None, None, None, None, n, chain=True)
+    compare(logits, [n, 1, n // 2], parents, token, q, [1.0] * 3, u * 0.1, u_next, max(1, n // 2), chain=True)
