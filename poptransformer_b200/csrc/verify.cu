@@ -15,6 +15,8 @@
 // without a meeting in between, and the tests of all children at once; the walk then begins at the last row that stands (32 chains of 6 over 50257 tokens:
 // 70 us walked from the root).  What bounds it is the way down: per row the time of a load, of the 64-bit
 // arithmetic in line (a dependent multiply-add takes several times as long as a 32-bit one) and of a meeting of the cluster; in large batches memory.
+#include <type_traits>
+
 #include "elem.cuh"
 #include "mbarrier.cuh"
 
@@ -116,29 +118,22 @@ template <typename V> __device__ __forceinline__ const V *in_block(const V *p, i
   return reinterpret_cast<const V *>(a);
 }
 
-// Four values from an address on a boundary of four, if `there` (else zeros): loads without a branch, so that several are under way.
+// Four values from an address on a boundary of four, or -inf if not `there`: loads without a branch, so that several are under way.
 __device__ __forceinline__ void load4(const float *p, bool there, float (&v)[4]) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\tmov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.f32 %0, 0fff800000;\n\tmov.f32 %1, 0fff800000;\n\tmov.f32 %2, 0fff800000;\n\tmov.f32 %3, 0fff800000;\n\t"
                "@q ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
                : "=&f"(v[0]), "=&f"(v[1]), "=&f"(v[2]), "=&f"(v[3])
                : "l"(p), "r"((int)there));
 }
 template <typename T> __device__ __forceinline__ void load4(const T *p, bool there, float (&v)[4]) {
+  constexpr uint32_t least = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
   uint2 r;
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@q ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}" : "=&r"(r.x), "=&r"(r.y) : "l"(p), "r"((int)there));
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b32 %0, %4;\n\tmov.b32 %1, %4;\n\t@q ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
+               : "=&r"(r.x), "=&r"(r.y)
+               : "l"(p), "r"((int)there), "n"(least));
   const T *h = reinterpret_cast<const T *>(&r);
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = value(h[k]);
-}
-// What load4 brought from place i of a row, `there` if it lay inside: -inf in front of the row and from hi on.
-template <typename T> __device__ __forceinline__ void settle(const T *row, int i, int vocab, int hi, bool there, float (&v)[4]) {
-  if (!there) {                                       // (the ends of a row that is not on such a boundary)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (i + k >= 0 && i + k < min(hi, vocab)) v[k] = value(row[i + k]);
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = i + k >= 0 && i + k < hi ? v[k] : -INFINITY;
 }
 
 // What a warp does with its part lo .. hi - 1 of a row (from lo on in fours that lie on their boundaries in memory; places below 0 do not exist): the largest logit,
@@ -148,20 +143,24 @@ template <typename T, bool KEEP, bool PLACE> __device__ __forceinline__ Part sum
   float top = -INFINITY;
   int at = 0x7fffffff;
   constexpr int AHEAD = 4;
+  // (Fours are inside a part or outside, but for those at the ends of the row.)
+  const bool ends = lo < 0 || hi == vocab;
+  const int whole = hi == vocab ? lo + (hi - lo) / 4 * 4 : hi;
   for (int i0 = lo; i0 < hi; i0 += AHEAD * 128) {
     float v[AHEAD][4];
-    const bool inside = i0 >= 0 && i0 + AHEAD * 128 <= hi;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u * 128 + lane * 4;
-      load4(row + i, inside || (i >= 0 && i + 4 <= vocab && i < hi), v[u]);
+      load4(row + i, i < whole && i >= 0, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u * 128 + lane * 4;
-      if (!inside) {
-        if (i >= hi) break;
-        settle(row, i, vocab, hi, i >= 0 && i + 4 <= vocab, v[u]);
+      if (i0 + u * 128 >= hi) break;                  // (uniform)
+      if (ends && (i < 0 || i >= whole)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k >= 0 && i + k < hi) v[u][k] = value(row[i + k]);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -172,7 +171,7 @@ template <typename T, bool KEEP, bool PLACE> __device__ __forceinline__ Part sum
           top = fmaxf(top, v[u][k]);
         }
       }
-      if (KEEP) *reinterpret_cast<float4 *>(logits + i - lo) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+      if (KEEP && i < hi) *reinterpret_cast<float4 *>(logits + i - lo) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
     }
   }
   warp_top(top, at);
@@ -289,10 +288,21 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) verify_kerne
         said[lane] = x;
         if (lp) lp[lane] = (float)log_p;
       }
-      if (lane == 0) sm.drawn = stand;
+      // the largest logit's token follows; one that is drawn needs its row's weights
+      const bool over = greedy && (stand < chain - 1 || chain == min(n, p.max_path));
+      if (over && lane == 0) {
+        const Part v = sm.row_all[stand];
+        const bool any = v.top > -INFINITY;
+        path[stand] = stand;
+        said[stand] = any ? v.at : -1;
+        if (lp) lp[stand] = any ? (float)(weigh.log(v.top, v.k) - log(v.sum)) : 0.f;
+      }
+      if (lane == 0) sm.drawn = over ? -stand - 1 : stand;
     }
     stay_for_cluster();
-    at = done = *in_block(&sm.drawn, 0);
+    const int stand = *in_block(&sm.drawn, 0);
+    at = stand < 0 ? -1 : stand;
+    done = stand < 0 ? -stand : stand;
     // (nobody writes sm.drawn before the cluster has met again)
   }
   while (at >= 0) {

@@ -509,25 +509,26 @@ def verify_drafts(logits, cu, token, parent=None, max_path=None, draft=None, tem
     random numbers.  Returns (path, count, token, logprob): int32 [n_seq, max_path], [n_seq], [n_seq, max_path], fp32 [n_seq, max_path]
     (`out`: the four tensors to use)."""
     rows, vocab = logits.shape
-    n_seq = cu.numel() - 1
-    if token.numel() < rows or (parent is not None and parent.numel() < rows) or (draft is not None and tuple(draft.shape) != (rows, vocab)):
-        raise PtError(f"verify_drafts: {rows} rows of logits over {vocab} tokens, got {token.numel()} tokens, {None if parent is None else parent.numel()} parents, "
-                      f"draft {None if draft is None else tuple(draft.shape)}")
-    if temperature is not None and (uniform is None or uniform_next is None or uniform.numel() < rows or uniform_next.numel() < n_seq or temperature.numel() < n_seq):
-        raise PtError("verify_drafts: sampling needs a temperature and a random number per sequence, and one per row")
-    for name, t, dt in (("cu", cu, torch.int32), ("token", token, torch.int32), ("parent", parent, torch.int32), ("draft", draft, torch.float32),
-                        ("temperature", temperature, torch.float32), ("uniform", uniform, torch.float32), ("uniform_next", uniform_next, torch.float32)):
-        if t is not None and t.dtype != dt:
-            raise PtError(f"verify_drafts: {name} is {dt}, got {t.dtype}")
+    n_seq, i32, f32 = cu.shape[0] - 1, torch.int32, torch.float32
+    # (One condition for what is right: a launch takes less time than the checks one by one.)
+    if not (cu.dtype is i32 and token.dtype is i32 and token.numel() >= rows and (parent is None or parent.dtype is i32 and parent.numel() >= rows)
+            and (draft is None or draft.dtype is f32 and draft.shape == logits.shape)
+            and (temperature is None or temperature.dtype is f32 and temperature.numel() >= n_seq and uniform is not None and uniform.dtype is f32 and uniform.numel() >= rows
+                 and uniform_next is not None and uniform_next.dtype is f32 and uniform_next.numel() >= n_seq)):
+        said = ", ".join(f"{k} {None if t is None else (t.dtype, tuple(t.shape))}" for k, t in (("cu", cu), ("token", token), ("parent", parent), ("draft", draft), ("temperature", temperature),
+                                                                                               ("uniform", uniform), ("uniform_next", uniform_next)))
+        raise PtError(f"verify_drafts: {rows} rows over {vocab} tokens want int32 cu, token and parent, float32 draft of the logits' shape, temperature and uniform_next of a sequence "
+                      f"each and uniform of a row each (sampling needs all three), got {said}")
     if out is None:
-        max_path = rows if max_path is None else max_path
-        i32 = dict(dtype=torch.int32, device=logits.device)
-        out = (torch.empty((n_seq, max_path), **i32), torch.empty(n_seq, **i32), torch.empty((n_seq, max_path), **i32),
-               torch.empty((n_seq, max_path), dtype=torch.float32, device=logits.device))
-    path, count, said, logprob = out
-    if path.shape != said.shape or path.shape != logprob.shape or path.shape[0] != n_seq or count.numel() != n_seq or (max_path is not None and path.shape[1] != max_path) or \
-            any(t.dtype != torch.int32 for t in out[:3]) or logprob.dtype != torch.float32:
-        raise PtError(f"verify_drafts: out is int32 [{n_seq}, max_path], [{n_seq}], [{n_seq}, max_path] and float32 [{n_seq}, max_path]")
+        max_path, dev = rows if max_path is None else max_path, logits.device
+        out = (torch.empty((n_seq, max_path), dtype=i32, device=dev), torch.empty(n_seq, dtype=i32, device=dev), torch.empty((n_seq, max_path), dtype=i32, device=dev),
+               torch.empty((n_seq, max_path), dtype=f32, device=dev))
+        path, count, said, logprob = out
+    else:
+        path, count, said, logprob = out
+        if path.shape != said.shape or path.shape != logprob.shape or path.shape[0] != n_seq or count.numel() != n_seq or (max_path is not None and path.shape[1] != max_path) or \
+                any(t.dtype != i32 for t in out[:3]) or logprob.dtype != f32:
+            raise PtError(f"verify_drafts: out is int32 [{n_seq}, max_path], [{n_seq}], [{n_seq}, max_path] and float32 [{n_seq}, max_path]")
     a = VerifyArgs(n_seq, rows, _ptr(cu), dtype_code(logits.dtype), vocab, vocab, _ptr(logits), _ptr(token), _ptr(parent), _ptr(draft), vocab, _ptr(temperature), _ptr(uniform),
                    _ptr(uniform_next), path.shape[1], _ptr(path), _ptr(count), _ptr(said), _ptr(logprob))
     check(_lib.lib().pt_verify_drafts(ctypes.byref(a), _stream()), "pt_verify_drafts")
