@@ -164,25 +164,11 @@ template <bool MASKS, typename Sync> __device__ __forceinline__ void build_tree(
   for (int i = tid; i < x.n; i += threads) t.parent[i] = parent_of(p, x, i, bad);
   sync();
   for (int i = tid; i < x.n; i += threads) {
-    uint32_t w[WORDS] = {};
     int d = 0;
     if (!p.parent) {
       d = i;
-      if (MASKS) {
-        const int lo = p.window ? max(0, i - p.window + 1) : 0;
-#pragma unroll
-        for (int k = 0; k < WORDS; ++k) {
-          const int a = max(lo - 32 * k, 0), b = min(i - 32 * k, 31);      // bits a .. b
-          if (a <= b) w[k] = (0xffffffffu >> (31 - (b - a))) << a;
-        }
-      }
     } else {
       for (int u = i; u >= 0; ++d) {
-        if (MASKS && (p.window == 0 || d < p.window)) {
-#pragma unroll
-          for (int k = 0; k < WORDS; ++k)
-            if (u >> 5 == k) w[k] |= 1u << (u & 31);
-        }
         const int up = t.parent[u];
         u = up < u ? up : -1;        // (ends whatever the array holds)
       }
@@ -190,8 +176,23 @@ template <bool MASKS, typename Sync> __device__ __forceinline__ void build_tree(
     }
     t.depth[i] = d;
     if (MASKS) {
-#pragma unroll
-      for (int k = 0; k < WORDS; ++k) t.seen[i][k] = w[k];
+#pragma unroll 1
+      for (int k = 0; k < WORDS; ++k) {
+        uint32_t w = 0;
+        if (!p.parent) {
+          const int a = max((p.window ? max(0, i - p.window + 1) : 0) - 32 * k, 0), b = min(i - 32 * k, 31);      // bits a .. b
+          if (a <= b) w = (0xffffffffu >> (31 - (b - a))) << a;
+        }
+        t.seen[i][k] = w;
+      }
+      if (p.parent) {
+        int e = 0;
+        for (int u = i; u >= 0; ++e) {
+          if (p.window == 0 || e < p.window) t.seen[i][u >> 5] |= 1u << (u & 31);
+          const int up = t.parent[u];
+          u = up < u ? up : -1;
+        }
+      }
     }
   }
   sync();
@@ -489,26 +490,21 @@ __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, i
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(tc::sa(&bar)), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {      // (to be waited for)
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                 "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-                 "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
-                 "=r"(v[31])
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[16]) {      // (to be waited for)
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                 "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                : "r"(taddr)
                : "memory");
 }
 // (The registers pass through, so that nothing reads them before.)
-__device__ __forceinline__ void tmem_landed(uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
-                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                :
                : "memory");
 }
-
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
@@ -773,7 +769,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
           const uint64_t vt = rv0 + (uint64_t)(uint32_t)(at_v.slot * (slot_bytes / 16));
 #pragma unroll
           for (int s = 0; s < 16; ++s)                      // (hi and lo of 16 keys: 8 columns each)
-            tc::umma_ta(O_COL, b * 128 + (s >> 2) * 32 + (s & 1) * 16 + (s >> 1 & 1) * 8, vt + (s >> 1) * (2048 / 16), vdesc, t > 0 || s > 0);
+            tc::umma_ta(O_COL, b * 128 + (s >> 1) * 16 + (s & 1) * 8, vt + (s >> 1) * (2048 / 16), vdesc, t > 0 || s > 0);
           tc::umma_commit(tc::sa(&sm.empty[at_v.slot]));
           tc::umma_commit(tc::sa(&sm.o_done[done & 1]));
         }
@@ -857,29 +853,39 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       if (k.g == 0 && half == 0 && row < rows && at == node * p.qpk && k.first)
         for (int c = p.n_head * p.vdim; c < p.out_cols; ++c) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + node) * p.out_ld + c] = rounded<T>(0.f);
       float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to; l: of this half
-      // Scores of a tile's half to weights.
-      auto weigh = [&](auto masked, int t) {
-        constexpr bool MASKED = decltype(masked)::value;
+      // Scores of a tile's half to weights.  (In loops of 32 keys: a block that has a tile or two fetches this code once, and waits for it.  Measured with 64 keys
+      // in line and the mask in a copy of it, 5 tokens behind 700: a third of all waiting was for instructions.)
+      auto weigh = [&](int t) {
         const uint32_t at = S + (t & 1) * 128;
-        uint32_t v[2][32], see[2] = {0xffffffffu, 0xffffffffu};
-        tmem_load(at, v[0]);
-        tmem_load(at + 32, v[1]);
-        if (MASKED) {
-          const int j0 = (k.t0 + t) * TKEYS + half * 64;
-          see[0] = seen_word(p, x, seen, depth, j0);
-          see[1] = seen_word(p, x, seen, depth, j0 + 32);
-        }
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_landed(v[0]);
-        tmem_landed(v[1]);
+        const int j0 = (k.t0 + t) * TKEYS;
+        if (partial(p, x, j0)) {
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 16) {
+            uint32_t v[16];
+            tc::tmem_ld16(at + c, v);
+            const uint32_t see = seen_word(p, x, seen, depth, j0 + half * 64 + c);
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (MASKED && !(see[b] >> i & 1)) v[b][i] = 0xff800000u;      // -inf
-            tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(v[b][i]));
+            for (int i = 0; i < 16; ++i)
+              if (!(see >> i & 1)) v[i] = 0xff800000u;       // -inf
+            tmem_store16(at + c, v);
           }
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          tc::tmem_wait_st();
+        }
+        uint32_t a[16], b[16];
+        tmem_load(at, a);
+        float tops[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          tmem_landed(a);
+          tmem_load(at + c + 16, b);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], __uint_as_float(a[i]));
+          tmem_landed(b);
+          tmem_load(at + (c + 32 & 63), a);                  // (the last: the first again)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], __uint_as_float(b[i]));
+        }
+        float top = fmaxf(tops[0], tops[1]);
         sm.top[t & 1][half][row] = top;
         meet_partner();
         top = fmaxf(top, sm.top[t & 1][1 - half][row]);
@@ -891,37 +897,47 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
           l *= f;
           output_of(n_o - 1);
           tc::fence_after();
+          tmem_landed(a);
+#pragma unroll 1
           for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
-            uint32_t y[16];
-            tc::tmem_ld16(O + c, y);
+            tc::tmem_ld16(O + c, b);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-            tmem_store16(O + c, y);
+            for (int i = 0; i < 16; ++i) b[i] = __float_as_uint(__uint_as_float(b[i]) * f);
+            tmem_store16(O + c, b);
           }
         }
         if (raise) m = top;
         const float ref = m == -INFINITY ? 0.f : m;
         float add[4] = {0.f, 0.f, 0.f, 0.f};
+        // 16 keys: eight columns of their weights' first parts, eight of the second
+        auto sixteen = [&](const uint32_t (&v)[16], uint32_t to) {
+          uint32_t o[16];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t o[32];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float a = __uint_as_float(v[b][i]), c = __uint_as_float(v[b][i + 1]);
+          for (int i = 0; i < 16; i += 2) {
+            float y = __uint_as_float(v[i]), z = __uint_as_float(v[i + 1]);
             if (CAP) {                                       // (-inf stays what is not seen)
-              a = MASKED && a == -INFINITY ? a : score(a) - ref;
-              c = MASKED && c == -INFINITY ? c : score(c) - ref;
+              y = y == -INFINITY ? y : score(y) - ref;
+              z = z == -INFINITY ? z : score(z) - ref;
             } else {
-              a = fmaf(a, a1, -ref);
-              c = fmaf(c, a1, -ref);
+              y = fmaf(y, a1, -ref);
+              z = fmaf(z, a1, -ref);
             }
-            a = ex2(a);
-            c = ex2(c);
-            add[i & 2] += a;
-            add[(i & 2) + 1] += c;
-            Half2<T>::split(a, c, o[i / 2], o[16 + i / 2]);
+            y = ex2(y);
+            z = ex2(z);
+            add[i & 2] += y;
+            add[(i & 2) + 1] += z;
+            Half2<T>::split(y, z, o[i / 2], o[8 + i / 2]);
           }
-          tc::tmem_st32(at + b * 32, o);
+          tmem_store16(to, o);
+        };
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          tmem_landed(a);
+          tmem_load(at + c + 16, b);
+          sixteen(a, at + c);
+          tmem_landed(b);
+          if (c == 0) tmem_load(at + 32, a);
+          sixteen(b, at + c + 16);
         }
         l += (add[0] + add[1]) + (add[2] + add[3]);
       };
@@ -929,8 +945,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
         wait(sm.s_full[t & 1], n_s[t & 1]++ & 1);
         tc::fence_after();
         if (live) {
-          if (partial(p, x, (k.t0 + t) * TKEYS)) weigh(std::true_type(), t);
-          else weigh(std::false_type(), t);
+          weigh(t);
           tc::tmem_wait_st();
           tc::fence_before();
         }
