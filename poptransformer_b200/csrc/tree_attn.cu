@@ -2,12 +2,12 @@
 // its ancestors in the tree and itself, each within the window of its own position C + depth(i).
 //
 // Work.  The query rows of a sequence that read the same key/value head g are its tokens times the query heads of the group: row r of them is
-// token r / qpk, head g qpk + r % qpk.  An item is (sequence, kv head, tile of rows), a unit one tile of keys of an item.  The units of all items,
-// in order, are dealt out to the blocks in equal runs, so that sequences of any lengths load all SMs alike; a block that has a part of an item leaves
-// (max, sum, unnormalised output) of its keys in the workspace, and combine_kernel adds the parts up in order.  Where the parts lie follows from the
-// lengths alone: no counters, and the same sums on every run.
+// token r / qpk, head g qpk + r % qpk.  An item is (sequence, kv head, tile of rows); its units are its key tiles, behind `extra` units that stand for what an item costs
+// beside them.  The units of all items, in order, are dealt out to the blocks in equal runs, so that sequences of any lengths load all SMs alike; a block
+// that has a part of an item leaves (max, sum, unnormalised output) of its keys in the workspace, and combine_kernel adds the parts up in order.  Where
+// the parts lie follows from the lengths alone: no counters, and the same sums on every run.
 //
-//   tree_prep_kernel      in front of tree_plain_kernel: depths; rotates and appends the new keys and values; zeroes the output's padding columns
+//   tree_prep_kernel      rotates and appends the new keys and values, writes down what every token sees and who does what
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
@@ -37,7 +37,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(floa
 struct Params {
   int n_seq, n_head, n_kv, qpk, dim, vdim, page, max_pages, max_len, window, most;
   int q_ld, kv_ld, out_ld, out_cols, rope_half;
-  int rows_tile, keys_tile, blocks;        // of an item, of a unit, of the attention kernel
+  int rows_tile, keys_tile, extra, blocks; // of an item, of a unit; units of an item beside its key tiles; blocks of the attention kernel
   float scale, softcap;
   const void *q, *k, *v;
   void *pool, *out;
@@ -46,6 +46,11 @@ struct Params {
   int *error_flag;
   int box;            // cache rows of a TMA box: the largest power of two up to 128 that divides a page; 0: no boxes
   bool out16;         // the output can be written in units of 16 bytes
+  // workspace
+  int *plan;          // units of a block, of all blocks; then the sequence of every block's first unit
+  int *units;         // [n_seq + 1] units in front of a sequence
+  int *depth;         // [n_seq][most]
+  uint32_t *seen;     // [n_seq][most][WORDS]: the tokens that a token sees
   float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
   float2 *part_ml;    // [2 blocks][rows_tile]
 };
@@ -67,20 +72,21 @@ __device__ __forceinline__ Span span(const Params &p, const Seq &x) {
   const int lo = p.window ? max(0, x.start - p.window + 1) / p.keys_tile : 0;
   return Span{lo, (x.start + x.n + p.keys_tile - 1) / p.keys_tile - lo, (x.n * p.qpk + p.rows_tile - 1) / p.rows_tile};
 }
-// Units in front of every sequence (units[n_seq]: all), by the whole block.  REPORT: sequences that nothing is done for set the flag.
-template <bool REPORT = false> __device__ __forceinline__ void count_units(const Params &p, int *units) {
-  __shared__ int warp_sum[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+// Who does what, by one block of tree_prep_kernel.  Sequences that nothing is done for set the flag.
+constexpr int PREP_THREADS = 256;
+__device__ __noinline__ void write_plan(const Params &p) {
+  __shared__ int units[MAX_SEQ + 1], warp_sum[PREP_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int base = 0;
-  for (int s0 = 0; s0 < p.n_seq; s0 += blockDim.x) {
+  for (int s0 = 0; s0 < p.n_seq; s0 += PREP_THREADS) {
     const int s = s0 + tid;
     int v = 0;
     if (s < p.n_seq) {
       const Seq x = sequence(p, s);
       if (x.n) {
         const Span y = span(p, x);
-        v = p.n_kv * y.row_tiles * y.tiles;
-      } else if (REPORT && blockIdx.x == 0 && p.error_flag) {
+        v = p.n_kv * y.row_tiles * (y.tiles + p.extra);
+      } else if (p.error_flag) {
         const int n = p.cu[s + 1] - x.row0;
         if (n > 0) atomicExch(p.error_flag, n > p.most ? 14 : 12);
       }
@@ -95,113 +101,68 @@ template <bool REPORT = false> __device__ __forceinline__ void count_units(const
     if (lane == 31) warp_sum[warp] = t;
     __syncthreads();
     int before = base;
-    for (int i = 0; i < nw; ++i) {
+    for (int i = 0; i < PREP_THREADS / 32; ++i) {
       if (i < warp) before += warp_sum[i];
       base += warp_sum[i];
     }
-    if (s < p.n_seq) units[s] = before + t - v;
+    if (s < p.n_seq) p.units[s] = units[s] = before + t - v;
   }
-  if (tid == 0) units[p.n_seq] = base;
+  if (tid == 0) p.units[p.n_seq] = units[p.n_seq] = base;
   __syncthreads();
-}
-// The sequence of a unit: the last one that begins at or before it and has units.
-__device__ __forceinline__ int seq_of(const int *units, int n_seq, int u) {
-  int lo = 0, hi = n_seq - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (units[mid] <= u) lo = mid;
-    else hi = mid - 1;
+  const int quota = (base + p.blocks - 1) / p.blocks;
+  if (tid == 0) {
+    p.plan[0] = quota;
+    p.plan[1] = base;
   }
-  return lo;
-}
-struct Share {
-  int all, quota;
-};
-__device__ __forceinline__ Share share(const Params &p, const int *units) {
-  const int all = units[p.n_seq];
-  return Share{all, (all + p.blocks - 1) / p.blocks};
+  for (int b = tid; b < p.blocks; b += PREP_THREADS) {
+    // the last sequence that begins at or before the block's first unit
+    const int u = b * quota;
+    int lo = 0, hi = p.n_seq - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (units[mid] <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    p.plan[2 + b] = lo;
+  }
 }
 // A part of an item: key tiles t0 .. t0 + nt - 1 of row tile rt of kv head g of sequence s.
 struct Piece {
-  int s, g, rt, t0, nt;
+  int s, g, rt, t0, nt;    // nt = 0: there is no more
   Seq x;
-  bool whole, first;     // the item's only part, its first
-  int slot;              // else: where it goes.  A block has at most two such parts: one of an item that began before its run, one that goes on behind it
+  bool whole, first;       // the item's only part, its first
+  int slot;                // else: where it goes.  A block has at most two such parts: one of an item that began before its run, one that goes on behind it
 };
-__device__ __noinline__ Piece piece_at(const Params &p, const int *units, const Share &sh, int block, int u) {
-  Piece k;
-  k.s = seq_of(units, p.n_seq, u);
-  k.x = sequence(p, k.s);
-  const Span y = span(p, k.x);
-  const int item = (u - units[k.s]) / y.tiles, first = units[k.s] + item * y.tiles;
-  k.g = item / y.row_tiles;
-  k.rt = item - k.g * y.row_tiles;
-  const int end = min(min(first + y.tiles, (block + 1) * sh.quota), sh.all);
-  k.t0 = y.first + u - first;
-  k.nt = end - u;
-  k.whole = k.nt == y.tiles;
-  k.first = u == first;
-  k.slot = 2 * block + (k.first ? 1 : 0);
-  return k;
-}
-
-// ------------------------------------------------------------------------------------------ trees
-// A token's parent, -1 for one that follows the cached positions (and for a parent that is none: *bad).
-__device__ __forceinline__ int parent_of(const Params &p, const Seq &x, int i, bool *bad = nullptr) {
-  if (!p.parent) return i - 1;
-  const int u = p.parent[x.row0 + i];
-  if (u >= -1 && u < i) return u;
-  if (bad) *bad = true;
-  return -1;
-}
-struct Tree {
-  int parent[MAX_NODES];
-  int depth[MAX_NODES];
-  uint32_t seen[MAX_NODES][WORDS];   // the tokens that a token sees
-};
-// By `threads` threads, between two barriers of theirs (`sync`).  MASKS: also what every token sees.
-template <bool MASKS, typename Sync> __device__ __forceinline__ void build_tree(const Params &p, const Seq &x, Tree &t, int tid, int threads, Sync sync, bool *bad = nullptr) {
-  for (int i = tid; i < x.n; i += threads) t.parent[i] = parent_of(p, x, i, bad);
-  sync();
-  for (int i = tid; i < x.n; i += threads) {
-    int d = 0;
-    if (!p.parent) {
-      d = i;
-    } else {
-      for (int u = i; u >= 0; ++d) {
-        const int up = t.parent[u];
-        u = up < u ? up : -1;        // (ends whatever the array holds)
-      }
-      --d;
-    }
-    t.depth[i] = d;
-    if (MASKS) {
-#pragma unroll 1
-      for (int k = 0; k < WORDS; ++k) {
-        uint32_t w = 0;
-        if (!p.parent) {
-          const int a = max((p.window ? max(0, i - p.window + 1) : 0) - 32 * k, 0), b = min(i - 32 * k, 31);      // bits a .. b
-          if (a <= b) w = (0xffffffffu >> (31 - (b - a))) << a;
-        }
-        t.seen[i][k] = w;
-      }
-      if (p.parent) {
-        int e = 0;
-        for (int u = i; u >= 0; ++e) {
-          if (p.window == 0 || e < p.window) t.seen[i][u >> 5] |= 1u << (u & 31);
-          const int up = t.parent[u];
-          u = up < u ? up : -1;
-        }
-      }
-    }
+struct Cursor {
+  int u, end, quota, s;    // next unit of the block, behind its last one; the sequence of unit u, or one in front of it
+  __device__ __forceinline__ Cursor(const Params &p) : quota(p.plan[0]), s(p.plan[2 + blockIdx.x]) {
+    u = blockIdx.x * quota;
+    end = min(u + quota, p.plan[1]);
   }
-  sync();
-}
-// Whether token i sees position j (below C + n).
-__device__ __forceinline__ bool sees(const Params &p, const Seq &x, const Tree &t, int i, int j) {
-  const int d = j - x.start;
-  if (d >= 0) return t.seen[i][d >> 5] >> (d & 31) & 1;
-  return p.window == 0 || x.start + t.depth[i] - j < p.window;
+};
+__device__ __noinline__ Piece next_piece(const Params &p, Cursor &c) {
+  Piece k;
+  k.nt = 0;
+  while (c.u < c.end) {
+    while (c.u >= p.units[c.s + 1]) ++c.s;
+    const int units = p.units[c.s];
+    k.s = c.s;
+    k.x = sequence(p, k.s);
+    const Span y = span(p, k.x);
+    const int item = (c.u - units) / (y.tiles + p.extra), first = units + item * (y.tiles + p.extra), stop = min(first + y.tiles + p.extra, c.end);
+    const int t0 = max(c.u - first - p.extra, 0), t1 = stop - first - p.extra;
+    c.u = stop;
+    if (t1 <= t0) continue;
+    k.g = item / y.row_tiles;
+    k.rt = item - k.g * y.row_tiles;
+    k.t0 = y.first + t0;
+    k.nt = t1 - t0;
+    k.first = t0 == 0;
+    k.whole = k.first && t1 == y.tiles;
+    k.slot = 2 * blockIdx.x + (k.first ? 1 : 0);
+    break;
+  }
+  return k;
 }
 
 template <typename T> __device__ __forceinline__ T *k_page(const Params &p, int phys, int g) {
@@ -218,28 +179,115 @@ template <typename T> __device__ __forceinline__ float turned(const Params &p, c
   return c < h ? val(row[c]) * a.x - val(row[c + h]) * a.y : val(row[c]) * a.x + val(row[c - h]) * a.y;
 }
 
-constexpr int PREP_THREADS = 256;
-// Block: a sequence's tokens (x strided), one at a time.
-template <typename T> __global__ void __launch_bounds__(PREP_THREADS) tree_prep_kernel(const Params p) {
+// Half: pairs of 16-bit values and fp32
+template <typename T> struct Half2;
+template <> struct Half2<__half> {
+  static constexpr float kBias = 7.f;      // weights are 2^7 as large
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+  // a and b in two parts
+  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    hi = pack(a, b);
+    const float2 back = wide(hi);
+    lo = pack(a - back.x, b - back.y);
+  }
+  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u; }
+};
+template <> struct Half2<__nv_bfloat16> {
+  static constexpr float kBias = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+  // (By cutting off bits, which costs no conversion: the upper half of a float is a bf16.  What is lost is below 2^-15 of the value.)
+  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    hi = __byte_perm(x, y, 0x7632);
+    lo = __byte_perm(__float_as_uint(a - __uint_as_float(x & 0xffff0000u)), __float_as_uint(b - __uint_as_float(y & 0xffff0000u)), 0x7632);
+  }
+  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
+};
+// Eight neighbouring dimensions d .. d + 7 of a head's row, rotated by the angles of `pos`; `own`: their values.
+template <typename T> __device__ __forceinline__ void turn8(const Params &p, const T *src, int d, int pos, const uint4 &own, float2 (&y)[4]) {
+  const int h = p.rope_half;
+  if (h % 8 == 0) {
+    const bool second = d >= h;
+    const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? d - h : d + h));
+    const uint32_t o[4] = {own.x, own.y, own.z, own.w}, z[4] = {other.x, other.y, other.z, other.w};
+    const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? d - h : d));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 m = Half2<T>::wide(o[i]), t = Half2<T>::wide(z[i]);
+      const float4 an = __ldg(cs + i);
+      y[i] = second ? make_float2(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : make_float2(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = make_float2(turned<T>(p, src, d + 2 * i, pos), turned<T>(p, src, d + 2 * i + 1, pos));
+      if (i == 0) y[0] = v; else if (i == 1) y[1] = v; else if (i == 2) y[2] = v; else y[3] = v;
+    }
+  }
+}
+
+// Block: token x of sequence y; one more block writes the plan.  EIGHTS: rows in units of 16 bytes.
+template <typename T, bool EIGHTS> __global__ void __launch_bounds__(PREP_THREADS) tree_prep_kernel(const __grid_constant__ Params p) {
   early_start();
-  __shared__ Tree tree;
-  __shared__ bool bad;
-  const int s = blockIdx.y, tid = threadIdx.x;
-  const Seq x = sequence(p, s);
-  const int n = p.cu[s + 1] - x.row0;
-  if (n <= 0) return;
-  if (!x.n) {
-    if (tid == 0 && blockIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, n > p.most ? 14 : 12);
+  const int s = blockIdx.y, i = blockIdx.x, tid = threadIdx.x;
+  if (s == p.n_seq) {
+    if (i == 0) write_plan(p);
     return;
   }
-  if (tid == 0) bad = false;
-  __syncthreads();
-  build_tree<false>(p, x, tree, tid, PREP_THREADS, [] { __syncthreads(); }, &bad);
-  if (bad && tid == 0 && blockIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 14);
-  const int *table = p.page_table + (size_t)p.slot[s] * p.max_pages;
-  for (int i = blockIdx.x; i < x.n; i += gridDim.x) {
-    const int at = x.start + i, pos = x.start + tree.depth[i], phys = table[at / p.page], place = at % p.page;
-    const T *k = reinterpret_cast<const T *>(p.k) + (size_t)(x.row0 + i) * p.kv_ld, *v = reinterpret_cast<const T *>(p.v) + (size_t)(x.row0 + i) * p.kv_ld;
+  __shared__ int parent[MAX_NODES];
+  __shared__ uint32_t seen[WORDS];
+  __shared__ int depth;
+  const Seq x = sequence(p, s);
+  if (i >= x.n) return;
+  const int at = x.start + i, phys = p.page_table[(size_t)p.slot[s] * p.max_pages + at / p.page], place = at % p.page;
+  if (p.parent) {
+    for (int j = tid; j <= i; j += PREP_THREADS) parent[j] = p.parent[x.row0 + j];
+    if (tid < WORDS) seen[tid] = 0;
+    __syncthreads();
+    if (tid == 0) {
+      // (a parent that is none: the token follows the cached positions)
+      int d = 0;
+      for (int u = i; u >= 0; ++d) {
+        if (p.window == 0 || d < p.window) seen[u >> 5] |= 1u << (u & 31);
+        const int up = parent[u];
+        if (u == i && (up < -1 || up >= i) && p.error_flag) atomicExch(p.error_flag, 14);
+        u = up < u ? max(up, -1) : -1;
+      }
+      depth = d - 1;
+    }
+    __syncthreads();
+  } else {
+    if (tid < WORDS) {
+      const int a = max((p.window ? max(0, i - p.window + 1) : 0) - 32 * tid, 0), b = min(i - 32 * tid, 31);      // bits a .. b
+      seen[tid] = a <= b ? (0xffffffffu >> (31 - (b - a))) << a : 0u;
+    }
+    if (tid == 0) depth = i;
+    __syncthreads();
+  }
+  const int pos = x.start + depth;
+  if (tid < WORDS) p.seen[((size_t)s * p.most + i) * WORDS + tid] = seen[tid];
+  if (tid == WORDS) p.depth[(size_t)s * p.most + i] = depth;
+  const T *k = reinterpret_cast<const T *>(p.k) + (size_t)(x.row0 + i) * p.kv_ld, *v = reinterpret_cast<const T *>(p.v) + (size_t)(x.row0 + i) * p.kv_ld;
+  if constexpr (EIGHTS) {
+    const int nk = p.n_kv * (p.dim / 8), all = nk + p.n_kv * (p.vdim / 8);
+    for (int e = tid; e < all; e += PREP_THREADS) {
+      if (e < nk) {
+        const int per = p.dim / 8, g = e / per, c = (e - g * per) * 8;
+        uint4 w = *reinterpret_cast<const uint4 *>(k + g * p.dim + c);
+        if (c < 2 * p.rope_half) {
+          float2 y[4];
+          turn8<T>(p, k + g * p.dim, c, pos, w, y);
+          w = make_uint4(Half2<T>::pack(y[0].x, y[0].y), Half2<T>::pack(y[1].x, y[1].y), Half2<T>::pack(y[2].x, y[2].y), Half2<T>::pack(y[3].x, y[3].y));
+        }
+        *reinterpret_cast<uint4 *>(k_page<T>(p, phys, g) + (size_t)place * p.dim + c) = w;
+      } else {
+        const int per = p.vdim / 8, g = (e - nk) / per, c = (e - nk - g * per) * 8;
+        *reinterpret_cast<uint4 *>(v_page<T>(p, phys, g) + (size_t)place * p.vdim + c) = *reinterpret_cast<const uint4 *>(v + g * p.vdim + c);
+      }
+    }
+  } else {
     for (int e = tid; e < p.n_kv * p.dim; e += PREP_THREADS) {
       const int g = e / p.dim, c = e - g * p.dim;
       k_page<T>(p, phys, g)[(size_t)place * p.dim + c] = rounded<T>(turned<T>(p, k + g * p.dim, c, pos));
@@ -248,8 +296,8 @@ template <typename T> __global__ void __launch_bounds__(PREP_THREADS) tree_prep_
       const int g = e / p.vdim, c = e - g * p.vdim;
       v_page<T>(p, phys, g)[(size_t)place * p.vdim + c] = v[e];
     }
-    for (int c = p.n_head * p.vdim + tid; c < p.out_cols; c += PREP_THREADS) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + i) * p.out_ld + c] = rounded<T>(0.f);
   }
+  for (int c = p.n_head * p.vdim + tid; c < p.out_cols; c += PREP_THREADS) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + i) * p.out_ld + c] = rounded<T>(0.f);
 }
 
 // Scores in the units of exp2 from raw products.
@@ -263,32 +311,32 @@ __device__ __forceinline__ float score2(const Params &p, float s) {
 // the output.  What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them.
 constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32, PLAIN_BLOCKS = 2;      // blocks: of an SM
 static size_t plain_smem(int dim, int vdim) { return (size_t)(PROWS + PKEYS) * (dim + 8) * 4 + (size_t)PKEYS * (vdim + 36) * 4 + (size_t)PROWS * (PKEYS + 4) * 4 + PROWS * 8; }
-template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) tree_plain_kernel(const Params p) {
+template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) tree_plain_kernel(const __grid_constant__ Params p) {
   early_start();
   extern __shared__ __align__(16) float sm[];
-  __shared__ int units[MAX_SEQ + 1];
-  __shared__ Tree tree;
+  __shared__ int depth[MAX_NODES];
+  __shared__ uint32_t seen[MAX_NODES][WORDS];
   const int d4 = (p.dim + 3) / 4 * 4, v32 = VJ * 32, kld = d4 + 4, vld = v32 + 4, pld = PKEYS + 4;
   float *Q = sm, *K = Q + PROWS * kld, *V = K + PKEYS * kld, *P = V + PKEYS * vld, *corr = P + PROWS * pld, *sum = corr + PROWS;
   const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
-  count_units(p, units);
-  const Share sh = share(p, units);
-  const int end = min((int)(blockIdx.x + 1) * sh.quota, sh.all);
   int had = -1;
-  for (int u = blockIdx.x * sh.quota; u < end;) {
-    const Piece k = piece_at(p, units, sh, blockIdx.x, u);
-    u += k.nt;
+  Cursor cursor(p);
+  for (Piece k = next_piece(p, cursor); k.nt; k = next_piece(p, cursor)) {
     const Seq x = k.x;
     const int rows = min(PROWS, x.n * p.qpk - k.rt * PROWS), r0 = k.rt * PROWS;
     __syncthreads();
-    if (k.s != had) build_tree<true>(p, x, tree, tid, PLAIN_THREADS, [] { __syncthreads(); });
+    if (k.s != had) {
+      for (int i = tid; i < x.n; i += PLAIN_THREADS) depth[i] = p.depth[(size_t)k.s * p.most + i];
+      for (int i = tid; i < x.n * WORDS; i += PLAIN_THREADS) (&seen[0][0])[i] = p.seen[(size_t)k.s * p.most * WORDS + i];
+      __syncthreads();
+    }
     had = k.s;
     for (int e = tid; e < PROWS * d4; e += PLAIN_THREADS) {
       const int r = e / d4, c = e - r * d4;
       float y = 0.f;
       if (r < rows && c < p.dim) {
         const int i = (r0 + r) / p.qpk, h = k.g * p.qpk + (r0 + r) % p.qpk;
-        y = turned<T>(p, reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)h * p.dim, c, x.start + tree.depth[i]);
+        y = turned<T>(p, reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)h * p.dim, c, x.start + depth[i]);
       }
       Q[r * kld + c] = y;
     }
@@ -330,7 +378,9 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 2 * ty + i, key = tx + 8 * j;
-          P[r * pld + key] = r < rows && key < keys && sees(p, x, tree, (r0 + r) / p.qpk, j0 + key) ? score2(p, sc[i][j]) : -INFINITY;
+          const int tok = min((r0 + r) / p.qpk, x.n - 1), d = j0 + key - x.start;      // (drafted token of the key)
+          const bool see = d >= 0 ? seen[tok][min(d, MAX_NODES - 1) >> 5] >> (d & 31) & 1 : p.window == 0 || depth[tok] - d < p.window;
+          P[r * pld + key] = r < rows && key < keys && see ? score2(p, sc[i][j]) : -INFINITY;
         }
       __syncthreads();
       {
@@ -417,13 +467,11 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 // A row's weights would lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 15 or more, for a second product with V.  Scores
 // have two buffers, so that the products of one tile run beside the exponentials of the other.
 //   warps 0-3, 4-7   softmax of the first and the second 64 keys; query rows in, results out
-//   warps 8, 9       keys and values into a ring of tiles in the swizzled layout: whole tiles by TMA, a box per page and 64 columns; tiles that begin or
-//                    end inside (a sequence's last, a window's first), and pages of sizes that no box fits, by 16-byte asynchronous copies of rows.
-//                    (Copies alone deliver 18 bytes a cycle to an SM, memory has 24 for each.)
+//   warps 8, 9       keys and values into a ring of tiles in the swizzled layout, by TMA: a box per page and 64 columns.  (Asynchronous copies of 16 bytes deliver
+//                    18 bytes a cycle to an SM, memory has 24 for each; they serve pages of sizes that no box fits.)  Values that some rows do not see are
+//                    gone over before they are used: zeros where the sequence has none.
 //   warp 10          issues the products; owns the tensor memory: 2 x 128 columns of scores, 128 of output.  (All 512 are asked for: they begin at 0, and an
 //                    instruction whose operands the compiler knows to be the same in all lanes goes out every 64 cycles, else every 105.)
-// New keys and values come from the caller's rows, not from the cache: whoever has an item's last tile rotates them on their way to shared memory, and
-// the block with the first tile of rows writes them to the pages, which nobody reads in this launch.
 // (Twelve warps: an SM quarter's registers are shared by three.)  Rotated queries would lose 8 bits' worth too, and come in two parts likewise.
 // A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as
 // copies stay in flight.  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
@@ -433,11 +481,9 @@ constexpr int OPERAND_BYTES = 192 * 1024, O_COL = 256;      // query rows and th
 constexpr float RAISE = 8.f;
 
 struct TcShared {
-  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, drained;
+  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, landed, drained;
   uint32_t tmem;               // where the tensor memory begins (at 0: all of it is ours)
-  volatile int abort, trees;   // trees: built so far
-  int units[MAX_SEQ + 1];
-  Tree tree;
+  volatile int abort;
   float top[2][2][TROWS], sum[2][2][TROWS];      // of a half of the keys: by tile, by piece (a warp may be one ahead of its partner)
   // Values that are not finite and that not every row sees, by piece: drafted tokens, and positions from the lowest of any row's window on.  They are
   // zeroed in shared memory (0 * inf would reach rows that do not see them), and the rows that do see them become NaN.
@@ -445,31 +491,6 @@ struct TcShared {
   int any_bad[8];
 };
 
-template <typename T> struct Half2;
-template <> struct Half2<__half> {
-  static constexpr float kBias = 7.f;      // weights are 2^7 as large
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
-  static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-  // a and b in two parts
-  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
-    hi = pack(a, b);
-    const float2 back = wide(hi);
-    lo = pack(a - back.x, b - back.y);
-  }
-  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u; }
-};
-template <> struct Half2<__nv_bfloat16> {
-  static constexpr float kBias = 0.f;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
-  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
-  // (By cutting off bits, which costs no conversion: the upper half of a float is a bf16.  What is lost is below 2^-15 of the value.)
-  static __device__ __forceinline__ void split(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-    hi = __byte_perm(x, y, 0x7632);
-    lo = __byte_perm(__float_as_uint(a - __uint_as_float(x & 0xffff0000u)), __float_as_uint(b - __uint_as_float(y & 0xffff0000u)), 0x7632);
-  }
-  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
-};
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -511,26 +532,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&v)
                : "memory");
 }
 
-// Eight neighbouring dimensions d .. d + 7 of a head's row, rotated by the angles of `pos`; `own`: their values.
-template <typename T> __device__ __forceinline__ void turn8(const Params &p, const T *src, int d, int pos, const uint4 &own, float2 (&y)[4]) {
-  const int h = p.rope_half;
-  if (h % 8 == 0) {
-    const bool second = d >= h;
-    const uint4 other = *reinterpret_cast<const uint4 *>(src + (second ? d - h : d + h));
-    const uint32_t o[4] = {own.x, own.y, own.z, own.w}, z[4] = {other.x, other.y, other.z, other.w};
-    const float4 *cs = reinterpret_cast<const float4 *>(p.rope + (size_t)pos * h + (second ? d - h : d));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 m = Half2<T>::wide(o[i]), t = Half2<T>::wide(z[i]);
-      const float4 an = __ldg(cs + i);
-      y[i] = second ? make_float2(m.x * an.x + t.x * an.y, m.y * an.z + t.y * an.w) : make_float2(m.x * an.x - t.x * an.y, m.y * an.z - t.y * an.w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = make_float2(turned<T>(p, src, d + 2 * i, pos), turned<T>(p, src, d + 2 * i + 1, pos));
-  }
-}
-
 struct Waits {          // a role's bounded waits: the whole warp goes the same way
   TcShared &sm;
   int *error_flag;
@@ -544,16 +545,6 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
       sm.abort = 1;
     }
     return ok;
-  }
-  __device__ __forceinline__ void tree(int n) const {      // the n-th tree of the block
-    int looks = 0;
-    while (sm.trees < n && !sm.abort)
-      if (++looks >= WAIT_LIMIT) {
-        if (error_flag) atomicCAS(error_flag, 0, 11);
-        sm.abort = 1;
-      }
-    __threadfence_block();
-    __syncwarp();
   }
   __device__ __forceinline__ void arrive(uint64_t &bar) const {      // one arrival of the warp
     __syncwarp();
@@ -578,7 +569,7 @@ __device__ __forceinline__ uint32_t seen_word(const Params &p, const Seq &x, con
   return v;
 }
 
-template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
+template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
   early_start();
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -600,19 +591,18 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       mbar_init(tc::sa(&sm.o_done[i]), 1);
     }
     mbar_init(tc::sa(&sm.q_full), SOFT_WARPS);
+    mbar_init(tc::sa(&sm.landed), 1);
     mbar_init(tc::sa(&sm.drained), 1);
     sm.abort = 0;
-    sm.trees = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = tid; i < 8 * 2 * WORDS; i += TENSOR_THREADS) (&sm.bad[0][0])[i] = 0;
   if (tid < 8) sm.any_bad[tid] = 0;
   if (warp == MMA_WARP) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
   tc::fence_before();
-  count_units<true>(p, sm.units);      // (ends with a barrier)
+  Cursor cursor(p);
+  __syncthreads();
   tc::fence_after();
-  const Share sh = share(p, sm.units);
-  const int begin = blockIdx.x * sh.quota, end = min((int)(blockIdx.x + 1) * sh.quota, sh.all);
   const Waits wait{sm, p.error_flag};
 
   if (warp >= SOFT_WARPS && warp < MMA_WARP) {
@@ -620,94 +610,84 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     const int w = warp - SOFT_WARPS;
     const int box = p.box, boxes = box ? TKEYS / box : 0;   // rows of a box, and how many make a tile
     const bool one = tc::elect_one();
-    int e = 0, pieces = 0, trees = 0, had = -1;             // tiles asked for; trees that are built up to here, and of which sequence the last is
+    int e = 0, pieces = 0, fixed = 0;                       // tiles asked for; tiles of values gone over
     bool ok = true;
-    for (int u = begin; u < end && ok; ++pieces) {
-      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
-      u += k.nt;
+    for (Piece k = next_piece(p, cursor); k.nt && ok; k = next_piece(p, cursor), ++pieces) {
       const Seq x = k.x;
       const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
       const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
-      if (k.s != had) ++trees;
-      had = k.s;
-      auto page_of = [&](int j) { return j >= lowest && j < x.start ? table[j / p.page] : 0; };
-      auto box_page = [&](int t) { return w == 0 && lane < boxes ? page_of(t * TKEYS + lane * box) : 0; };
+      auto page_of = [&](int j) { return j >= lowest && j < last ? table[j / p.page] : 0; };      // (what is not the sequence's: any page)
+      auto box_page = [&](int t) {
+        const int j = t * TKEYS + lane * box;               // (a box lies in one page)
+        return w == 0 && lane < boxes && j + box > lowest && j < last ? table[j / p.page] : 0;
+      };
       int ahead = box_page(k.t0);                           // pages of the next tile's boxes, one per lane
       for (int t = 0; t < k.nt && ok; ++t) {
         const int j0 = (k.t0 + t) * TKEYS, phys = ahead;
         ahead = box_page(k.t0 + t + 1);
-        const bool whole = box && j0 >= lowest && j0 + TKEYS <= x.start && !partial(p, x, j0);
-#pragma unroll
+        const bool part = partial(p, x, j0);
+#pragma unroll 1
         for (int kv = 0; kv < 2; ++kv, ++e) {
           const int slot = e % slots;
           if (e >= slots && !wait(sm.empty[slot], (e / slots + 1) & 1)) { ok = false; break; }
           const uint32_t to = tc::sa(ring + slot * slot_bytes);
           const int dims = kv ? p.vdim : p.dim, blocks = kv ? vblocks : kblocks, have = dims / 8, pad = (dims + 15) / 16 * 2;
-          if (whole) {
+          const bool look = kv && part;                     // what is seen in part
+          if (box) {
+            uint64_t &bar = look ? sm.landed : sm.full[slot];
             if (w == 0) {
-              if (one) mbar_expect_tx(tc::sa(&sm.full[slot]), blocks * TKEYS * 128);
+              if (one) mbar_expect_tx(tc::sa(&bar), blocks * TKEYS * 128);
+#pragma unroll 1
               for (int i = 0; i < boxes; ++i) {
                 const int page = __shfl_sync(0xffffffffu, phys, i), y = k.g * p.page + (j0 + i * box) % p.page;
                 if (one)
-                  for (int b = 0; b < blocks; ++b) box_load(to + b * (TKEYS * 128) + i * box * 128, kv ? &values : &keys, b * 64, y, page, sm.full[slot]);
+                  for (int b = 0; b < blocks; ++b) box_load(to + b * (TKEYS * 128) + i * box * 128, kv ? &values : &keys, b * 64, y, page, bar);
               }
             }
-            if (w || !one) mbar_arrive(tc::sa(&sm.full[slot]));
-            continue;
-          }
-          // rows of the cache, zeros where there are none
-          for (int h = 0; h < 2; ++h) {
-            const int r0 = w * 64 + h * 32, j = j0 + r0 + lane;
-            const bool in = j >= lowest && j < min(last, x.start);
-            const T *src = (kv ? v_page<T>(p, in ? table[j / p.page] : 0, k.g) : k_page<T>(p, in ? table[j / p.page] : 0, k.g)) + (size_t)(in ? j % p.page : 0) * dims;
-            const int cols = blocks * 8, c = lane % cols;
-            for (int q0 = 0; q0 < 32; q0 += 32 / cols) {
-              const int r = q0 + lane / cols;
-              const unsigned long long from = __shfl_sync(0xffffffffu, (unsigned long long)src, r);
-              const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have, drafted = j0 + r0 + r >= x.start && j0 + r0 + r < last && c < have;
-              if (c < pad && !drafted) cp_async(to + swizzled(r0 + r, c), reinterpret_cast<const T *>(from) + (there ? c * 8 : 0), there ? 16 : 0);
+            if (!look) {
+              if (w || !one) mbar_arrive(tc::sa(&bar));
+              continue;
             }
-          }
-          // drafted rows
-          const int d0 = max(j0 - x.start, 0), d1 = min(x.n, j0 + TKEYS - x.start);      // of the sequence's new tokens
-          if (d1 > d0 && !kv && p.rope_half && p.parent) wait.tree(trees);      // (depths)
-#pragma unroll 2
-          for (int i0 = w * 32 + lane; i0 < (d1 - d0) * have; i0 += COPY_WARPS * 32) {
-            const int d = d0 + i0 / have, c = i0 % have, j = x.start + d;
-            const T *src = reinterpret_cast<const T *>(kv ? p.v : p.k) + (size_t)(x.row0 + d) * p.kv_ld + (size_t)k.g * dims;
-            uint4 v = *reinterpret_cast<const uint4 *>(src + c * 8);
-            if (!kv && c * 8 < 2 * p.rope_half) {
-              float2 y[4];
-              turn8<T>(p, src, c * 8, x.start + (p.parent ? sm.tree.depth[d] : d), v, y);
-              v = make_uint4(Half2<T>::pack(y[0].x, y[0].y), Half2<T>::pack(y[1].x, y[1].y), Half2<T>::pack(y[2].x, y[2].y), Half2<T>::pack(y[3].x, y[3].y));
-            }
-            if (k.rt == 0) {
-              T *row = (kv ? v_page<T>(p, table[j / p.page], k.g) : k_page<T>(p, table[j / p.page], k.g)) + (size_t)(j % p.page) * dims;
-              *reinterpret_cast<uint4 *>(row + c * 8) = v;
-            }
-            if (kv && (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w))) {
-              v = make_uint4(0u, 0u, 0u, 0u);
-              atomicOr(&sm.bad[pieces & 7][d >> 5], 1u << (d & 31));
-              sm.any_bad[pieces & 7] = 1;
-            }
-            *reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(j - j0, c)) = v;
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          if (kv && p.window) {
+            if (!wait(sm.landed, fixed++ & 1)) { ok = false; break; }
+          } else {
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
+              const int r0 = w * 64 + h * 32, j = j0 + r0 + lane;
+              const bool in = j >= lowest && j < last;
+              const T *src = (kv ? v_page<T>(p, page_of(j), k.g) : k_page<T>(p, page_of(j), k.g)) + (size_t)(in ? j % p.page : 0) * dims;
               const int cols = blocks * 8, c = lane % cols;
-              for (int q0 = 0; q0 < 32; q0 += 32 / cols) {      // (the units that this lane copied)
-                const int r = w * 64 + h * 32 + q0 + lane / cols, key = j0 + r, b = key - lowest;
-                if (c >= have || key >= min(last, x.start) || key < lowest || b >= MAX_NODES) continue;
-                uint4 *at = reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(r, c));
+              for (int q0 = 0; q0 < 32; q0 += 32 / cols) {
+                const int r = q0 + lane / cols;
+                const unsigned long long from = __shfl_sync(0xffffffffu, (unsigned long long)src, r);
+                const bool there = __shfl_sync(0xffffffffu, in ? 1 : 0, r) && c < have;
+                if (c < pad) cp_async(to + swizzled(r0 + r, c), reinterpret_cast<const T *>(from) + (there ? c * 8 : 0), there ? 16 : 0);
+              }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+          }
+          if (look) {
+            // rows that the sequence has not: zeros; rows that not all see: finite, or noted
+            const int cols = blocks * 8, c = lane % cols, r1 = w * 64 + 64;
+            int r = w * 64 + lane / cols;
+            if (!p.window) r += max(0, (x.start - j0 - r) / (32 / cols)) * (32 / cols);      // (those in front all see)
+#pragma unroll 2
+            for (; r < r1; r += 32 / cols) {
+              const int key = j0 + r, d = key - x.start, b = key - lowest;
+              if (c >= have || (d < 0 && b >= MAX_NODES)) continue;
+              uint4 *at = reinterpret_cast<uint4 *>(ring + slot * slot_bytes + swizzled(r, c));
+              const bool in = key >= lowest && key < last;
+              if (in) {
                 const uint4 v = *at;
-                if (Half2<T>::bad(v.x) || Half2<T>::bad(v.y) || Half2<T>::bad(v.z) || Half2<T>::bad(v.w)) {
-                  *at = make_uint4(0u, 0u, 0u, 0u);
-                  const int bit = MAX_NODES + b;
+                if (!Half2<T>::bad(v.x) && !Half2<T>::bad(v.y) && !Half2<T>::bad(v.z) && !Half2<T>::bad(v.w)) continue;
+                if (d >= 0 || p.window) {
+                  const int bit = d >= 0 ? d : MAX_NODES + b;
                   atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
                   sm.any_bad[pieces & 7] = 1;
+                } else {
+                  continue;
                 }
               }
+              *at = make_uint4(0u, 0u, 0u, 0u);
             }
           }
           tc::fence_operands();
@@ -717,7 +697,10 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     }
     // nothing is in flight when the block ends, after a failure either
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (w == 0 && box) mbar_wait_ring(tc::sa(&sm.full[0]), e, slots);
+    if (w == 0 && box) {
+      mbar_wait_ring(tc::sa(&sm.full[0]), e, slots);
+      if (!ok && fixed) mbar_wait_all(tc::sa(&sm.landed), (fixed - 1) & 1);
+    }
   } else if (warp == MMA_WARP) {
     // ---- products.  (What they take is the same in all lanes, and the compiler knows it: counters that go up by known steps, in loops whose bounds come
     // out of a reduction.  After a wait that ran out they go on: nobody reads what they give.)
@@ -752,10 +735,9 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     };
     // (Tiles come as K V K V ..; the scores of the next tile but one are asked for behind this one's output.)
     int used0 = 0, used1 = 0;                               // of either buffer
-    const int u1 = __reduce_max_sync(0xffffffffu, end);
-    for (int u = __reduce_max_sync(0xffffffffu, begin); u < u1; ++pieces) {
-      const int nt = __reduce_max_sync(0xffffffffu, piece_at(p, sm.units, sh, blockIdx.x, u).nt);
-      u += nt;
+    for (;; ++pieces) {
+      const int nt = __reduce_max_sync(0xffffffffu, next_piece(p, cursor).nt);
+      if (!nt) break;
       wait(sm.q_full, pieces & 1);
       tc::fence_after();
       scores(0);
@@ -788,7 +770,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     // ---- softmax
     const int half = warp >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16, S = lanes + half * 64, O = lanes + O_COL;
-    int pieces = 0, n_s[2] = {0, 0}, n_o = 0, had = -1;
+    int pieces = 0, n_s[2] = {0, 0}, n_o = 0;
     const float a1 = fabsf(p.scale) * kLog2e, a2 = CAP ? 2.0f * a1 / p.softcap : 0.f, b2 = p.softcap * kLog2e;
     auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };      // (grows with s)
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory"); };
@@ -797,61 +779,47 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     // needs weights that come later.)
     auto output_of = [&](int i) { wait(sm.o_done[i & 1], (i >> 1) & 1); };
     // (After a wait that ran out all go on without waiting: everybody comes to every meeting, and what is computed does not matter.)
-    for (int u = begin; u < end; ++pieces) {
-      const Piece k = piece_at(p, sm.units, sh, blockIdx.x, u);
-      u += k.nt;
+    // Query rows of a piece to shared memory, rotated, and negated where the scale is negative (rows that there are none of hold anything: they stay by themselves).
+    auto stage = [&](const Piece &k) {
+      const int r0 = k.rt * TROWS, rows = min(TROWS, k.x.n * p.qpk - r0), cols = p.dim / 8, pad = (p.dim + 15) / 16 * 2;
+      const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 4
+      for (int e = tid; e < rows * pad; e += SOFT_WARPS * 32) {
+        const int r = e / pad, c = e - r * pad;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
+        if (c < cols) {
+          const int i = (r0 + r) / p.qpk, hd = k.g * p.qpk + (r0 + r) - i * p.qpk;
+          const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(k.x.row0 + i) * p.q_ld + (size_t)hd * p.dim;
+          v = *reinterpret_cast<const uint4 *>(src + c * 8);
+          if (c * 8 < 2 * p.rope_half) {
+            float2 y[4];
+            uint32_t a[4], b[4];
+            turn8<T>(p, src, c * 8, k.x.start + (p.parent ? p.depth[(size_t)k.s * p.most + i] : i), v, y);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              a[z] = Half2<T>::pack(y[z].x, y[z].y);
+              const float2 back = Half2<T>::wide(a[z]);
+              b[z] = Half2<T>::pack(y[z].x - back.x, y[z].y - back.y) ^ flip;
+            }
+            v = make_uint4(a[0], a[1], a[2], a[3]);
+            lo = make_uint4(b[0], b[1], b[2], b[3]);
+          }
+          v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+        }
+        *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
+        if (split_q) *reinterpret_cast<uint4 *>(Q + q_bytes + swizzled(r, c)) = lo;
+      }
+      tc::fence_operands();
+      wait.arrive(sm.q_full);
+    };
+    Piece k = next_piece(p, cursor);
+    if (k.nt) stage(k);
+    for (; k.nt; ++pieces) {
       const Seq x = k.x;
       const int r0 = k.rt * TROWS, rows = min(TROWS, x.n * p.qpk - r0);
-      if (k.s != had) {
-        if (had >= 0) meet();                               // (everybody is done with the tree before)
-        bool none = false;
-        build_tree<true>(p, x, sm.tree, tid, SOFT_WARPS * 32, meet, &none);
-        if (none && p.error_flag) atomicExch(p.error_flag, 14);
-        had = k.s;
-        if (tid == 0) {
-          __threadfence_block();
-          sm.trees = sm.trees + 1;
-        }
-      }
       const bool live = q * 32 < rows;                      // (uniform over the warp)
-      const int at = min(r0 + row, x.n * p.qpk - 1), node = at / p.qpk, head = k.g * p.qpk + at - node * p.qpk, depth = sm.tree.depth[node];
-      const uint32_t *seen = sm.tree.seen[node];
-      // query rows, rotated, and negated where the scale is negative (rows that there are none of hold anything: they stay by themselves)
-      {
-        const int cols = p.dim / 8, pad = (p.dim + 15) / 16 * 2;
-        const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 2
-        for (int e = tid; e < rows * pad; e += SOFT_WARPS * 32) {
-          const int r = e / pad, c = e - r * pad;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
-          if (c < cols) {
-            const int i = (r0 + r) / p.qpk, hd = k.g * p.qpk + (r0 + r) - i * p.qpk;
-            const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)hd * p.dim;
-            v = *reinterpret_cast<const uint4 *>(src + c * 8);
-            if (c * 8 < 2 * p.rope_half) {
-              float2 y[4];
-              uint32_t a[4], b[4];
-              turn8<T>(p, src, c * 8, x.start + sm.tree.depth[i], v, y);
-#pragma unroll
-              for (int z = 0; z < 4; ++z) {
-                a[z] = Half2<T>::pack(y[z].x, y[z].y);
-                const float2 back = Half2<T>::wide(a[z]);
-                b[z] = Half2<T>::pack(y[z].x - back.x, y[z].y - back.y) ^ flip;
-              }
-              v = make_uint4(a[0], a[1], a[2], a[3]);
-              lo = make_uint4(b[0], b[1], b[2], b[3]);
-            }
-            v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-          }
-          *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
-          if (split_q) *reinterpret_cast<uint4 *>(Q + q_bytes + swizzled(r, c)) = lo;
-        }
-        tc::fence_operands();
-        wait.arrive(sm.q_full);
-      }
-      // padding columns of the output's rows
-      if (k.g == 0 && half == 0 && row < rows && at == node * p.qpk && k.first)
-        for (int c = p.n_head * p.vdim; c < p.out_cols; ++c) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + node) * p.out_ld + c] = rounded<T>(0.f);
+      const int at = min(r0 + row, x.n * p.qpk - 1), node = at / p.qpk, head = k.g * p.qpk + at - node * p.qpk, depth = p.parent ? p.depth[(size_t)k.s * p.most + node] : node;
+      const uint32_t *seen = p.seen + ((size_t)k.s * p.most + node) * WORDS;
       float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to; l: of this half
       // Scores of a tile's half to weights.  (In loops of 32 keys: a block that has a tile or two fetches this code once, and waits for it.  Measured with 64 keys
       // in line and the mask in a copy of it, 5 tokens behind 700: a third of all waiting was for instructions.)
@@ -951,7 +919,10 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
         }
         wait.arrive(sm.p_full[t & 1]);
       }
-      // ---- out; either half of the threads takes half of the columns
+      // ---- the next piece's queries (all scores of this one are there: nobody reads its queries any more), then this one out; either half of the threads takes
+      // half of the columns
+      const Piece next = next_piece(p, cursor);
+      if (next.nt) stage(next);
       sm.sum[pieces & 1][half][row] = l;
       meet();
       if (tid == 0) sm.any_bad[(pieces + 7) & 7] = 0;       // (of the piece before: everybody is past it)
@@ -1002,6 +973,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
         }
         tc::fence_before();
       }
+      k = next;
     }
   }
   __syncthreads();
@@ -1015,19 +987,16 @@ static size_t tensor_smem() { return 1024 + OPERAND_BYTES + sizeof(TcShared); }
 // ------------------------------------------------------------------------------------------ parts of an item
 // Block (x: eight rows of an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys.
 constexpr int COMBINE_THREADS = 256, COMBINE_ROWS = 8;
-template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const Params p) {
+template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const __grid_constant__ Params p) {
   early_start();
-  __shared__ int units[MAX_SEQ + 1];
-  const int s = blockIdx.y, tid = threadIdx.x;
+  const int s = blockIdx.y, tid = threadIdx.x, quota = p.plan[0], units = p.units[s];
   const Seq x = sequence(p, s);
   if (!x.n) return;
   const Span y = span(p, x);
   const int eights = (p.most * p.qpk + COMBINE_ROWS - 1) / COMBINE_ROWS, g = blockIdx.x / eights, r0 = (blockIdx.x - g * eights) * COMBINE_ROWS;   // (first row, of all of the kv head's)
   const int rows = min(COMBINE_ROWS, x.n * p.qpk - r0), rt = r0 / p.rows_tile;
   if (rows <= 0) return;
-  count_units(p, units);
-  const Share sh = share(p, units);
-  const int first = units[s] + (g * y.row_tiles + rt) * y.tiles, b0 = first / sh.quota, b1 = (first + y.tiles - 1) / sh.quota;
+  const int first = units + (g * y.row_tiles + rt) * (y.tiles + p.extra) + p.extra, b0 = first / quota, b1 = (first + y.tiles - 1) / quota;
   if (b0 == b1) return;
   const int v4 = (p.vdim + 3) / 4;
   for (int e = tid; e < rows * v4; e += COMBINE_THREADS) {
@@ -1060,13 +1029,9 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
 static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
 
 template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st) {
-  PT_CUDA(launch_early(tree_prep_kernel<T>, Grid(dim3(std::min(p.most, 64), p.n_seq)), PREP_THREADS, 0, st, p));
-  PT_LAUNCH_CHECK("pt_tree_attn");
   static std::atomic<uint64_t> done{0};
   const size_t smem = plain_smem(p.dim, VJ * 32);
   if (smem > 32 * 1024) PT_CUDA(allow_smem(tree_plain_kernel<T, VJ>, (int)plain_smem(256, VJ * 32), done));
-  p.rows_tile = PROWS; p.keys_tile = PKEYS;
-  p.blocks = sm_count() * PLAIN_BLOCKS;
   PT_CUDA(launch_early(tree_plain_kernel<T, VJ>, Grid(p.blocks), PLAIN_THREADS, smem, st, p));
   PT_LAUNCH_CHECK("pt_tree_attn");
   return PT_OK;
@@ -1090,8 +1055,6 @@ static bool page_map(CUtensorMap *map, CUtensorMapDataType dt, const void *base,
 template <typename T, bool CAP> static int launch_tensor(Params &p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   PT_CUDA(allow_smem(tree_tensor_kernel<T, CAP>, (int)tensor_smem(), done));
-  p.rows_tile = TROWS; p.keys_tile = TKEYS;
-  p.blocks = sm_count();
   CUtensorMap keys{}, values{};
   p.box = 1;
   while (p.box < TKEYS && p.page % (2 * p.box) == 0) p.box *= 2;
@@ -1103,7 +1066,17 @@ template <typename T, bool CAP> static int launch_tensor(Params &p, cudaStream_t
 }
 template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   int rc;
+  const Grid prep(dim3(p.most, p.n_seq + 1));
   if constexpr (std::is_same<T, float>::value) tensor = false;
+  if (tensor) {
+    // (A piece beside its tiles costs about as much as two of them: queries in, the last weights and products, the output.)
+    p.rows_tile = TROWS; p.keys_tile = TKEYS; p.extra = 2; p.blocks = sm_count();
+    if constexpr (!std::is_same<T, float>::value) PT_CUDA(launch_early(tree_prep_kernel<T, true>, prep, PREP_THREADS, 0, st, p));
+  } else {
+    p.rows_tile = PROWS; p.keys_tile = PKEYS; p.extra = 0; p.blocks = sm_count() * PLAIN_BLOCKS;
+    PT_CUDA(launch_early(tree_prep_kernel<T, false>, prep, PREP_THREADS, 0, st, p));
+  }
+  PT_LAUNCH_CHECK("pt_tree_attn");
   if constexpr (!std::is_same<T, float>::value) {
     if (tensor) rc = p.softcap > 0.f ? launch_tensor<T, true>(p, st) : launch_tensor<T, false>(p, st);
   }
@@ -1119,10 +1092,13 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
 
 using namespace pt;
 
-// (n_seq, max_tokens_per_seq and the heads do not matter to the present kernels: every block has two parts of one tile of rows.)
+// Workspace: the plan, units, depths and masks of all tokens, then the parts.
+static size_t part_offset(int n_seq, int most) {
+  return (((size_t)(2 + sm_count() * ta::PLAIN_BLOCKS) + n_seq + 1 + (size_t)n_seq * most * (1 + ta::WORDS)) * 4 + 255) / 256 * 256;
+}
 extern "C" size_t pt_tree_attn_workspace_bytes(int n_seq, int max_tokens_per_seq, int n_head, int n_kv, int vdim) {
-  (void)n_seq; (void)max_tokens_per_seq; (void)n_head; (void)n_kv;
-  return ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
+  (void)n_head; (void)n_kv;      // (the parts are two tiles of rows of every block, whatever the heads)
+  return part_offset(n_seq, max_tokens_per_seq) + ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
 }
 
 extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
@@ -1147,7 +1123,7 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   p.most = a->max_tokens_per_seq > 0 ? a->max_tokens_per_seq : b.n_tok;
   PT_REQUIRE(p.most <= ta::MAX_NODES, "pt_tree_attn: %d tokens of one sequence (at most %d)", p.most, ta::MAX_NODES);
   // (a unit is 32 positions of a row tile: their number is an int)
-  PT_REQUIRE((double)b.n_seq * a->n_kv * (p.most * p.qpk / 32 + 1) * (p.max_len / 32 + 2) < 2e9, "pt_tree_attn: %d sequences of up to %d positions and %d heads are too much for one call", b.n_seq,
+  PT_REQUIRE((double)b.n_seq * a->n_kv * (p.most * p.qpk / 32 + 1) * (p.max_len / 32 + 4) < 2e9, "pt_tree_attn: %d sequences of up to %d positions and %d heads are too much for one call", b.n_seq,
              p.max_len, a->n_head);
   p.q_ld = a->q_ld; p.kv_ld = a->kv_ld; p.out_ld = a->out_ld; p.rope_half = a->rope_dims / 2;
   p.out_cols = a->out_cols > 0 ? a->out_cols : a->out_ld;
@@ -1156,7 +1132,11 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   p.page_table = a->page_table; p.cu = b.cu; p.start = b.start; p.slot = b.slot; p.parent = a->parent; p.error_flag = a->error_flag;
   const size_t need = pt_tree_attn_workspace_bytes(b.n_seq, p.most, a->n_head, a->n_kv, a->vdim);
   PT_REQUIRE(a->workspace && a->workspace_bytes >= need && aligned_to(a->workspace, 16), "pt_tree_attn: %zu workspace bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
-  p.part_o = (float *)a->workspace;
+  p.plan = (int *)a->workspace;
+  p.units = p.plan + 2 + sm_count() * ta::PLAIN_BLOCKS;
+  p.depth = p.units + b.n_seq + 1;
+  p.seen = (uint32_t *)(p.depth + (size_t)b.n_seq * p.most);
+  p.part_o = (float *)((char *)a->workspace + part_offset(b.n_seq, p.most));
   p.part_ml = (float2 *)(p.part_o + ta::part_rows() * ((a->vdim + 3) / 4 * 4));
   cudaStream_t st = as_stream(stream);
   p.out16 = a->out_ld % 8 == 0 && aligned_to(a->out, 16);
