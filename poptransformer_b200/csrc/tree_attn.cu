@@ -7,7 +7,8 @@
 // that has a part of an item leaves (max, sum, unnormalised output) of its keys in the workspace, and combine_kernel adds the parts up in order.  Where
 // the parts lie follows from the lengths alone: no counters, and the same sums on every run.
 //
-//   tree_prep_kernel      rotates and appends the new keys and values, writes down what every token sees and who does what
+//   tree_prep_kernel      rotates and appends the new keys and values, writes down what every token sees and who does what, and lays out the queries for the
+//                         tensor cores
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
@@ -51,6 +52,7 @@ struct Params {
   int *units;         // [n_seq + 1] units in front of a sequence
   int *depth;         // [n_seq][most]
   uint32_t *seen;     // [n_seq][most][WORDS]: the tokens that a token sees
+  uint4 *queries;     // of sequence s and kv head g from unit (s most n_head + g rows) 2 dim / 8 on: [part][dim / 8][rows], rows = n qpk
   float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
   float2 *part_ml;    // [2 blocks][rows_tile]
 };
@@ -287,6 +289,33 @@ template <typename T, bool EIGHTS> __global__ void __launch_bounds__(PREP_THREAD
         *reinterpret_cast<uint4 *>(v_page<T>(p, phys, g) + (size_t)place * p.vdim + c) = *reinterpret_cast<const uint4 *>(v + g * p.vdim + c);
       }
     }
+    // queries, rotated (in two parts), and negated where the scale is negative; a row's units lie as far apart as there are rows, so that the threads that have a
+    // row each read them side by side
+    const T *q = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld;
+    const int per = p.dim / 8, rows = x.n * p.qpk;
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    for (int e = tid; e < p.n_head * per; e += PREP_THREADS) {
+      const int head = e / per, c = e - head * per, g = head / p.qpk, r = i * p.qpk + head - g * p.qpk;
+      const T *src = q + (size_t)head * p.dim;
+      uint4 w = *reinterpret_cast<const uint4 *>(src + c * 8), lo = make_uint4(0u, 0u, 0u, 0u);
+      if (c * 8 < 2 * p.rope_half) {
+        float2 y[4];
+        uint32_t a[4], b[4];
+        turn8<T>(p, src, c * 8, pos, w, y);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          a[z] = Half2<T>::pack(y[z].x, y[z].y);
+          const float2 back = Half2<T>::wide(a[z]);
+          b[z] = Half2<T>::pack(y[z].x - back.x, y[z].y - back.y) ^ flip;
+        }
+        w = make_uint4(a[0], a[1], a[2], a[3]);
+        lo = make_uint4(b[0], b[1], b[2], b[3]);
+      }
+      w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+      uint4 *to = p.queries + ((size_t)s * p.most * p.n_head + (size_t)g * rows) * 2 * per + r;
+      to[(size_t)c * rows] = w;
+      if (p.rope_half) to[(size_t)(per + c) * rows] = lo;
+    }
   } else {
     for (int e = tid; e < p.n_kv * p.dim; e += PREP_THREADS) {
       const int g = e / p.dim, c = e - g * p.dim;
@@ -462,22 +491,23 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 }
 
 // ------------------------------------------------------------------------------------------ tensor cores
-// One block per SM, 128 query rows against tiles of 128 keys.  S = Q K^T goes to tensor memory (lane = row), two softmax threads per row, one for each
-// half of the keys, turn it into weights in place, and O += P V takes those from there and V, keys outermost as the cache has it, from shared memory.
-// A row's weights would lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 15 or more, for a second product with V.  Scores
-// have two buffers, so that the products of one tile run beside the exponentials of the other.
+// One block per SM, 128 query rows against tiles of 128 keys.  Queries stay in tensor memory: shared memory is the ring of keys and values, whose depth decides how
+// fast they come (32 KB of queries in two parts cost two of its six slots, and a quarter of the rate behind 60000 positions).  S = Q K^T goes to tensor memory
+// (lane = row), two softmax threads per row, one for each half of the keys, turn it into weights in place, and O += P V takes those from there and V, keys
+// outermost as the cache has it, from shared memory.  A row's weights would lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 15 or
+// more, for a second product with V; rotated queries come in two parts likewise.  Scores have two buffers, so that the products of one tile run beside the
+// exponentials of the other.
 //   warps 0-3, 4-7   softmax of the first and the second 64 keys; query rows in, results out
-//   warps 8, 9       keys and values into a ring of tiles in the swizzled layout, by TMA: a box per page and 64 columns.  (Asynchronous copies of 16 bytes deliver
-//                    18 bytes a cycle to an SM, memory has 24 for each; they serve pages of sizes that no box fits.)  Values that some rows do not see are
-//                    gone over before they are used: zeros where the sequence has none.
-//   warp 10          issues the products; owns the tensor memory: 2 x 128 columns of scores, 128 of output.  (All 512 are asked for: they begin at 0, and an
-//                    instruction whose operands the compiler knows to be the same in all lanes goes out every 64 cycles, else every 105.)
-// (Twelve warps: an SM quarter's registers are shared by three.)  Rotated queries would lose 8 bits' worth too, and come in two parts likewise.
+//   warps 8, 9       keys and values into a ring of tiles in the swizzled layout, by TMA: a box per page and 64 columns; pages of sizes that no box fits by
+//                    asynchronous copies of 16 bytes.  Values that some rows do not see are gone over before they are used: zeros where the sequence has none.
+//   warp 10          issues the products; owns the tensor memory: 2 x 128 columns of scores, 128 of output, 2 x 64 of queries.  (All 512 are asked for: they
+//                    begin at 0.)
+// (Twelve warps: an SM quarter's registers are shared by three.)
 // A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as
 // copies stay in flight.  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
 // (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
 constexpr int SOFT_WARPS = 8, COPY_WARPS = 2, MMA_WARP = SOFT_WARPS + COPY_WARPS, TENSOR_THREADS = 384, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
-constexpr int OPERAND_BYTES = 192 * 1024, O_COL = 256;      // query rows and the ring; first column of the output
+constexpr int RING_BYTES = 192 * 1024, O_COL = 256, Q_COL = 384, Q_LOW = 64;      // columns of output and queries, from there of the queries' second part
 constexpr float RAISE = 8.f;
 
 struct TcShared {
@@ -574,11 +604,11 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char *base = raw + ((1024 - (tc::sa(raw) & 1023)) & 1023);
-  const int kblocks = (p.dim + 63) / 64, vblocks = (p.vdim + 63) / 64, slot_bytes = max(kblocks, vblocks) * TKEYS * 128, q_bytes = kblocks * TROWS * 128;
+  const int kblocks = (p.dim + 63) / 64, vblocks = (p.vdim + 63) / 64, slot_bytes = max(kblocks, vblocks) * TKEYS * 128;
   const bool split_q = p.rope_half > 0;                     // query rows in two parts
-  const int slots = min(MAX_SLOTS, (OPERAND_BYTES - (split_q ? 2 : 1) * q_bytes) / slot_bytes);
-  unsigned char *Q = base, *ring = base + (split_q ? 2 : 1) * q_bytes;
-  TcShared &sm = *reinterpret_cast<TcShared *>(base + OPERAND_BYTES);
+  const int slots = min(MAX_SLOTS, RING_BYTES / slot_bytes);
+  unsigned char *ring = base;
+  TcShared &sm = *reinterpret_cast<TcShared *>(base + RING_BYTES);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (tid == 0) {
     for (int i = 0; i < slots; ++i) {
@@ -706,7 +736,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     // out of a reduction.  After a wait that ran out they go on: nobody reads what they give.)
     const int ksteps = (p.dim + 15) / 16, vcols = (p.vdim + 15) / 16 * 16;
     const uint32_t kdesc = product_desc(BF16, TKEYS, false), vdesc = product_desc(BF16, vcols, true);
-    const uint64_t q0 = tc::smem_desc_sw128(tc::sa(Q)), r0 = tc::smem_desc_sw128(tc::sa(ring)), rv0 = value_desc(tc::sa(ring));
+    const uint64_t r0 = tc::smem_desc_sw128(tc::sa(ring)), rv0 = value_desc(tc::sa(ring));
     struct Place { int slot, phase; } at_k{0, 0}, at_v{1, 0};      // of the next tiles of keys and of values
     auto on = [&](Place &x) {
       x.slot += 2;
@@ -719,12 +749,12 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       if (tc::elect_one()) {
         const uint64_t kt = r0 + (uint64_t)(uint32_t)(at_k.slot * (slot_bytes / 16));
         for (int part = 0; part < (split_q ? 2 : 1); ++part) {
-          const uint64_t qt = q0 + (part ? (uint32_t)q_bytes / 16 : 0u);
+          const uint32_t qt = Q_COL + part * Q_LOW;
           if (ksteps == 8) {
 #pragma unroll
-            for (int s = 0; s < 8; ++s) tc::umma<false>(b * 128, qt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
+            for (int s = 0; s < 8; ++s) tc::umma_ta(b * 128, qt + s * 8, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
           } else {
-            for (int s = 0; s < ksteps; ++s) tc::umma<false>(b * 128, qt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
+            for (int s = 0; s < ksteps; ++s) tc::umma_ta(b * 128, qt + s * 8, kt + (s >> 2) * (128 * 128 / 16) + (s & 3) * 2, kdesc, part > 0 || s > 0);
           }
         }
         tc::umma_commit(tc::sa(&sm.empty[at_k.slot]));
@@ -779,37 +809,24 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     // needs weights that come later.)
     auto output_of = [&](int i) { wait(sm.o_done[i & 1], (i >> 1) & 1); };
     // (After a wait that ran out all go on without waiting: everybody comes to every meeting, and what is computed does not matter.)
-    // Query rows of a piece to shared memory, rotated, and negated where the scale is negative (rows that there are none of hold anything: they stay by themselves).
+    // Query rows of a piece to tensor memory, 64 dimensions a thread (rows that there are none of hold anything: they stay by themselves).
     auto stage = [&](const Piece &k) {
-      const int r0 = k.rt * TROWS, rows = min(TROWS, k.x.n * p.qpk - r0), cols = p.dim / 8, pad = (p.dim + 15) / 16 * 2;
-      const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
-      for (int e = tid; e < rows * pad; e += SOFT_WARPS * 32) {
-        const int r = e / pad, c = e - r * pad;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u), lo = v;
-        if (c < cols) {
-          const int i = (r0 + r) / p.qpk, hd = k.g * p.qpk + (r0 + r) - i * p.qpk;
-          const T *src = reinterpret_cast<const T *>(p.q) + (size_t)(k.x.row0 + i) * p.q_ld + (size_t)hd * p.dim;
-          v = *reinterpret_cast<const uint4 *>(src + c * 8);
-          if (c * 8 < 2 * p.rope_half) {
-            float2 y[4];
-            uint32_t a[4], b[4];
-            turn8<T>(p, src, c * 8, k.x.start + (p.parent ? p.depth[(size_t)k.s * p.most + i] : i), v, y);
+      const int all = k.x.n * p.qpk, r0 = k.rt * TROWS, per = p.dim / 8;
+      if (q * 32 < all - r0 && half * 64 < p.dim) {
+        const uint4 *from = p.queries + ((size_t)k.s * p.most * p.n_head + (size_t)k.g * all) * 2 * per + min(r0 + row, all - 1);
+        for (int part = 0; part < (split_q ? 2 : 1); ++part) {
+          uint32_t v[32];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              a[z] = Half2<T>::pack(y[z].x, y[z].y);
-              const float2 back = Half2<T>::wide(a[z]);
-              b[z] = Half2<T>::pack(y[z].x - back.x, y[z].y - back.y) ^ flip;
-            }
-            v = make_uint4(a[0], a[1], a[2], a[3]);
-            lo = make_uint4(b[0], b[1], b[2], b[3]);
+          for (int c = 0; c < 8; ++c) {
+            const int d = half * 8 + c;
+            const uint4 w = d < per ? __ldcg(from + (size_t)(part * per + d) * all) : make_uint4(0u, 0u, 0u, 0u);
+            v[4 * c] = w.x; v[4 * c + 1] = w.y; v[4 * c + 2] = w.z; v[4 * c + 3] = w.w;
           }
-          v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+          tc::tmem_st32(lanes + Q_COL + part * Q_LOW + half * 32, v);
         }
-        *reinterpret_cast<uint4 *>(Q + swizzled(r, c)) = v;
-        if (split_q) *reinterpret_cast<uint4 *>(Q + q_bytes + swizzled(r, c)) = lo;
+        tc::tmem_wait_st();
+        tc::fence_before();
       }
-      tc::fence_operands();
       wait.arrive(sm.q_full);
     };
     Piece k = next_piece(p, cursor);
@@ -982,7 +999,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     tc::tmem_dealloc(sm.tmem, 512);
   }
 }
-static size_t tensor_smem() { return 1024 + OPERAND_BYTES + sizeof(TcShared); }
+static size_t tensor_smem() { return 1024 + RING_BYTES + sizeof(TcShared); }
 
 // ------------------------------------------------------------------------------------------ parts of an item
 // Block (x: eight rows of an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys.
@@ -1092,13 +1109,12 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
 
 using namespace pt;
 
-// Workspace: the plan, units, depths and masks of all tokens, then the parts.
-static size_t part_offset(int n_seq, int most) {
-  return (((size_t)(2 + sm_count() * ta::PLAIN_BLOCKS) + n_seq + 1 + (size_t)n_seq * most * (1 + ta::WORDS)) * 4 + 255) / 256 * 256;
-}
+// Workspace: the plan, units, depths and masks of all tokens; the queries as the tensor cores take them (widths up to 128 in two parts of 16 bits); the parts.
+static size_t queries_offset(int n_seq, int most) { return (((size_t)(2 + sm_count() * ta::PLAIN_BLOCKS) + n_seq + 1 + (size_t)n_seq * most * (1 + ta::WORDS)) * 4 + 255) / 256 * 256; }
+static size_t part_offset(int n_seq, int most, int n_head) { return queries_offset(n_seq, most) + (size_t)n_seq * most * n_head * 128 * 4; }
 extern "C" size_t pt_tree_attn_workspace_bytes(int n_seq, int max_tokens_per_seq, int n_head, int n_kv, int vdim) {
-  (void)n_head; (void)n_kv;      // (the parts are two tiles of rows of every block, whatever the heads)
-  return part_offset(n_seq, max_tokens_per_seq) + ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
+  (void)n_kv;
+  return part_offset(n_seq, max_tokens_per_seq, n_head) + ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
 }
 
 extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
@@ -1136,7 +1152,8 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   p.units = p.plan + 2 + sm_count() * ta::PLAIN_BLOCKS;
   p.depth = p.units + b.n_seq + 1;
   p.seen = (uint32_t *)(p.depth + (size_t)b.n_seq * p.most);
-  p.part_o = (float *)((char *)a->workspace + part_offset(b.n_seq, p.most));
+  p.queries = (uint4 *)((char *)a->workspace + queries_offset(b.n_seq, p.most));
+  p.part_o = (float *)((char *)a->workspace + part_offset(b.n_seq, p.most, a->n_head));
   p.part_ml = (float2 *)(p.part_o + ta::part_rows() * ((a->vdim + 3) / 4 * 4));
   cudaStream_t st = as_stream(stream);
   p.out16 = a->out_ld % 8 == 0 && aligned_to(a->out, 16);
