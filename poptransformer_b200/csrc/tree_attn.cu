@@ -640,38 +640,43 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     const int w = warp - SOFT_WARPS;
     const int box = p.box, boxes = box ? TKEYS / box : 0;   // rows of a box, and how many make a tile
     const bool one = tc::elect_one();
-    int e = 0, pieces = 0, fixed = 0;                       // tiles asked for; tiles of values gone over
+    int slot = 0, phase = 1, e = 0, pieces = 0, fixed = 0;  // where the next tile goes; tiles asked for; tiles of values gone over
     bool ok = true;
     for (Piece k = next_piece(p, cursor); k.nt && ok; k = next_piece(p, cursor), ++pieces) {
       const Seq x = k.x;
       const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
       const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
       auto page_of = [&](int j) { return j >= lowest && j < last ? table[j / p.page] : 0; };      // (what is not the sequence's: any page)
-      auto box_page = [&](int t) {
-        const int j = t * TKEYS + lane * box;               // (a box lies in one page)
-        return w == 0 && lane < boxes && j + box > lowest && j < last ? table[j / p.page] : 0;
+      // Page and row in it of a tile's boxes, one per lane, looked up a tile ahead (here and not where they are used: a division takes as long as a box)
+      auto box_at = [&](int t) {
+        const int j = t * TKEYS + lane * box, page = box ? j / p.page : 0;      // (a box lies in one page)
+        return make_int2(w == 0 && lane < boxes && j + box > lowest && j < last ? table[page] : 0, k.g * p.page + j - page * p.page);
       };
-      int ahead = box_page(k.t0);                           // pages of the next tile's boxes, one per lane
+      int2 ahead = box_at(k.t0);
       for (int t = 0; t < k.nt && ok; ++t) {
-        const int j0 = (k.t0 + t) * TKEYS, phys = ahead;
-        ahead = box_page(k.t0 + t + 1);
+        const int j0 = (k.t0 + t) * TKEYS;
+        const int2 here = ahead;
+        ahead = box_at(k.t0 + t + 1);
         const bool part = partial(p, x, j0);
 #pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv, ++e) {
-          const int slot = e % slots;
-          if (e >= slots && !wait(sm.empty[slot], (e / slots + 1) & 1)) { ok = false; break; }
+        for (int kv = 0; kv < 2; ++kv, ++e, phase ^= ++slot == slots, slot = slot == slots ? 0 : slot) {
+          if (e >= slots && !wait(sm.empty[slot], phase)) { ok = false; break; }
           const uint32_t to = tc::sa(ring + slot * slot_bytes);
           const int dims = kv ? p.vdim : p.dim, blocks = kv ? vblocks : kblocks, have = dims / 8, pad = (dims + 15) / 16 * 2;
           const bool look = kv && part;                     // what is seen in part
           if (box) {
             uint64_t &bar = look ? sm.landed : sm.full[slot];
             if (w == 0) {
-              if (one) mbar_expect_tx(tc::sa(&bar), blocks * TKEYS * 128);
+              if (tc::elect_one()) mbar_expect_tx(tc::sa(&bar), blocks * TKEYS * 128);
+              __syncwarp();
 #pragma unroll 1
               for (int i = 0; i < boxes; ++i) {
-                const int page = __shfl_sync(0xffffffffu, phys, i), y = k.g * p.page + (j0 + i * box) % p.page;
-                if (one)
-                  for (int b = 0; b < blocks; ++b) box_load(to + b * (TKEYS * 128) + i * box * 128, kv ? &values : &keys, b * 64, y, page, bar);
+                const int page = __shfl_sync(0xffffffffu, here.x, i), y = __shfl_sync(0xffffffffu, here.y, i);
+                if (tc::elect_one()) {                      // (said here, so that the compiler knows that one lane goes in: the instruction wants its operands the same in all)
+                  box_load(to + i * box * 128, kv ? &values : &keys, 0, y, page, bar);
+                  if (blocks > 1) box_load(to + TKEYS * 128 + i * box * 128, kv ? &values : &keys, 64, y, page, bar);
+                }
+                __syncwarp();
               }
             }
             if (!look) {
