@@ -482,22 +482,18 @@ def tree_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, parent=None,
     """Attention of drafted tokens, a tree of them behind every sequence of `view`, over a paged cache (see pt_tree_attn).  qkv rows hold [q | k | v] of a
     token; k and v are appended at the rows' own positions, the rotation and the window go by a token's depth.  parent: int32 [n_tok], counted
     from the first token of a sequence, -1 for those that follow its cached positions (None: every token follows the one before)."""
-    a = TreeAttnArgs()
-    es, k = qkv.element_size(), _ptr(qkv)
-    a.batch, a.dtype = view, dtype_code(qkv.dtype)
-    if cache.pool.dtype != qkv.dtype or out.dtype != qkv.dtype:
-        raise PtError(f"tree_attn: rows {qkv.dtype}, cache {cache.pool.dtype}, out {out.dtype}: one type is wanted")
+    pool, table, dtype = cache.pool, cache.page_table, qkv.dtype
+    if pool.dtype != dtype or out.dtype != dtype:
+        raise PtError(f"tree_attn: rows {dtype}, cache {pool.dtype}, out {out.dtype}: one type is wanted")
     if parent is not None and (parent.dtype != torch.int32 or parent.numel() < view.n_tok):
         raise PtError(f"tree_attn: parent is int32 of {view.n_tok} tokens, got {parent.dtype} {tuple(parent.shape)}")
-    a.n_head, a.n_kv, a.dim, a.vdim = n_head, cache.n_kv, cache.head_dim, cache.v_dim
-    a.page_size, a.max_pages, a.max_len = cache.page_size, cache.page_table.shape[1], cache.max_len
-    a.window, a.scale, a.softcap, a.parent = window, scale, softcap, _ptr(parent)
-    a.q, a.q_ld, a.kv_ld = k, qkv_ld, qkv_ld
-    a.k = k = k + n_head * cache.head_dim * es
-    a.v = k + cache.n_kv * cache.head_dim * es
-    a.pool, a.page_table, a.rope_dims, a.rope = _ptr(cache.pool), _ptr(cache.page_table), rope_dims, _ptr(rope)
-    a.out, a.out_ld, a.out_cols, a.max_tokens_per_seq, a.plain = _ptr(out), out_ld, out_cols, max_tokens_per_seq, 1 if plain else 0
-    a.workspace, a.workspace_bytes, a.error_flag = _ptr(workspace), workspace.numel() if workspace is not None else 0, _ptr(error_flag)
+    n_kv, dim, vdim, es = cache.n_kv, cache.head_dim, cache.v_dim, qkv.element_size()
+    q = _ptr(qkv)
+    k = q + n_head * dim * es
+    # (In the order of the structure: setting its fields one by one takes 4 us more.)
+    a = TreeAttnArgs(view, dtype_code(dtype), n_head, n_kv, dim, vdim, cache.page_size, table.shape[1], cache.max_len, window, scale, softcap, _ptr(parent), q, qkv_ld, k, k + n_kv * dim * es,
+                     qkv_ld, _ptr(pool), _ptr(table), rope_dims, _ptr(rope), _ptr(out), out_ld, out_cols, max_tokens_per_seq, 1 if plain else 0, _ptr(workspace),
+                     0 if workspace is None else workspace.numel(), _ptr(error_flag))
     check(_lib.lib().pt_tree_attn(ctypes.byref(a), _stream()), "pt_tree_attn")
     return out
 
@@ -520,10 +516,11 @@ def verify_drafts(logits, cu, token, parent=None, max_path=None, draft=None, tem
         raise PtError(f"verify_drafts: {rows} rows over {vocab} tokens want int32 cu, token and parent, float32 draft of the logits' shape, temperature and uniform_next of a sequence "
                       f"each and uniform of a row each (sampling needs all three), got {said}")
     if out is None:
-        max_path, dev = rows if max_path is None else max_path, logits.device
-        out = (torch.empty((n_seq, max_path), dtype=i32, device=dev), torch.empty(n_seq, dtype=i32, device=dev), torch.empty((n_seq, max_path), dtype=i32, device=dev),
-               torch.empty((n_seq, max_path), dtype=f32, device=dev))
-        path, count, said, logprob = out
+        shape = (n_seq, rows if max_path is None else max_path)
+        path, count = cu.new_empty(shape), cu.new_empty(n_seq)
+        said = torch.empty_like(path)
+        out = path, count, said, torch.empty_like(path, dtype=f32)
+        logprob = out[3]
     else:
         path, count, said, logprob = out
         if path.shape != said.shape or path.shape != logprob.shape or path.shape[0] != n_seq or count.numel() != n_seq or (max_path is not None and path.shape[1] != max_path) or \
@@ -831,9 +828,9 @@ class PagePools:
         for c in caches:
             if c.page_size != first.page_size or c.page_table is not first.page_table and (c.page_table.data_ptr(), c.page_table.shape) != (first.page_table.data_ptr(), first.page_table.shape):
                 raise PtError("PagePools: the caches share neither page size nor page table")
-        self.caches = caches                       # (keeps the pools alive)
+        self.pools = [c.pool for c in caches]      # (keeps them alive)
         self.page_size, self.page_table = first.page_size, first.page_table
-        self.n_pages = min(c.pool.shape[0] for c in caches)
+        self.n_pages = min(t.shape[0] for t in self.pools)
         self._pools = (_lib.KvPool * len(caches))(*[_lib.KvPool(_ptr(c.pool), c.n_kv, c.head_dim, c.v_dim, c.pool.element_size()) for c in caches])
 
     def copy_pages(self, src, dst, error_flag=None):
