@@ -38,7 +38,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(floa
 struct Params {
   int n_seq, n_head, n_kv, qpk, dim, vdim, page, max_pages, max_len, window, most;
   int q_ld, kv_ld, out_ld, out_cols, rope_half;
-  int rows_tile, keys_tile, extra, blocks; // of an item, of a unit; units of an item beside its key tiles; blocks of the attention kernel
+  int rows_tile, keys_tile, extra, blocks; // of an item, of a unit (powers of two); units of an item beside its key tiles; blocks of the attention kernel
+  int rows_shift, keys_shift;
   float scale, softcap;
   const void *q, *k, *v;
   void *pool, *out;
@@ -48,11 +49,12 @@ struct Params {
   int box;            // cache rows of a TMA box: the largest power of two up to 128 that divides a page; 0: no boxes
   bool out16;         // the output can be written in units of 16 bytes
   // workspace
-  int *plan;          // units of a block, of all blocks; then the sequence of every block's first unit
+  int *plan;          // units of a block, of all blocks; from PLAN_HEAD on a Start of every block
   int *units;         // [n_seq + 1] units in front of a sequence
   int *depth;         // [n_seq][most]
   uint32_t *seen;     // [n_seq][most][WORDS]: the tokens that a token sees
-  uint4 *queries;     // of sequence s and kv head g from unit (s most n_head + g rows) 2 dim / 8 on: [part][dim / 8][rows], rows = n qpk
+  uint4 *queries;     // tensor cores: of sequence s and kv head g from unit (s most n_head + g rows) 2 dim / 8 on: [part][dim / 8][rows], rows = n qpk;
+                      // plain: [n_seq][most][n_head][dim up to a multiple of 4] as fp32
   float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
   float2 *part_ml;    // [2 blocks][rows_tile]
 };
@@ -71,9 +73,16 @@ struct Span {
   int first, tiles, row_tiles;      // key tiles of an item, items per kv head
 };
 __device__ __forceinline__ Span span(const Params &p, const Seq &x) {
-  const int lo = p.window ? max(0, x.start - p.window + 1) / p.keys_tile : 0;
-  return Span{lo, (x.start + x.n + p.keys_tile - 1) / p.keys_tile - lo, (x.n * p.qpk + p.rows_tile - 1) / p.rows_tile};
+  const int lo = p.window ? max(0, x.start - p.window + 1) >> p.keys_shift : 0;
+  return Span{lo, ((x.start + x.n + p.keys_tile - 1) >> p.keys_shift) - lo, (x.n * p.qpk + p.rows_tile - 1) >> p.rows_shift};
 }
+// What a block has to know of the sequence of its first unit, in one place: two loads instead of a chain of five.
+struct __align__(16) Start {
+  int s, units, next, slot;      // next: the next sequence's first unit
+  Seq x;
+  int unused;
+};
+constexpr int PLAN_HEAD = 4;
 // Who does what, by one block of tree_prep_kernel.  Sequences that nothing is done for set the flag.
 constexpr int PREP_THREADS = 256;
 __device__ __noinline__ void write_plan(const Params &p) {
@@ -125,31 +134,41 @@ __device__ __noinline__ void write_plan(const Params &p) {
       if (units[mid] <= u) lo = mid;
       else hi = mid - 1;
     }
-    p.plan[2 + b] = lo;
+    *reinterpret_cast<Start *>(p.plan + PLAN_HEAD + b * (sizeof(Start) / 4)) = Start{lo, units[lo], units[lo + 1], p.slot[lo], sequence(p, lo), 0};
   }
 }
 // A part of an item: key tiles t0 .. t0 + nt - 1 of row tile rt of kv head g of sequence s.
 struct Piece {
   int s, g, rt, t0, nt;    // nt = 0: there is no more
   Seq x;
+  int table;               // the sequence's row of the page table
   bool whole, first;       // the item's only part, its first
   int slot;                // else: where it goes.  A block has at most two such parts: one of an item that began before its run, one that goes on behind it
 };
 struct Cursor {
-  int u, end, quota, s;    // next unit of the block, behind its last one; the sequence of unit u, or one in front of it
-  __device__ __forceinline__ Cursor(const Params &p) : quota(p.plan[0]), s(p.plan[2 + blockIdx.x]) {
-    u = blockIdx.x * quota;
-    end = min(u + quota, p.plan[1]);
+  int u, end;              // next unit of the block, behind its last one
+  Start at;                // the sequence of unit u, or one in front of it
+  __device__ __forceinline__ Cursor(const Params &p) {
+    const int2 all = *reinterpret_cast<const int2 *>(p.plan);
+    const int4 *from = reinterpret_cast<const int4 *>(p.plan + PLAN_HEAD) + 2 * blockIdx.x, a = from[0], b = from[1];
+    at = Start{a.x, a.y, a.z, a.w, Seq{b.x, b.y, b.z}, 0};
+    u = blockIdx.x * all.x;
+    end = min(u + all.x, all.y);
   }
 };
 __device__ __noinline__ Piece next_piece(const Params &p, Cursor &c) {
   Piece k;
   k.nt = 0;
   while (c.u < c.end) {
-    while (c.u >= p.units[c.s + 1]) ++c.s;
-    const int units = p.units[c.s];
-    k.s = c.s;
-    k.x = sequence(p, k.s);
+    if (c.u >= c.at.next) {
+      do c.at.units = c.at.next, c.at.next = p.units[++c.at.s + 1]; while (c.u >= c.at.next);
+      c.at.x = sequence(p, c.at.s);
+      c.at.slot = p.slot[c.at.s];
+    }
+    const int units = c.at.units;
+    k.s = c.at.s;
+    k.x = c.at.x;
+    k.table = c.at.slot;
     const Span y = span(p, k.x);
     const int item = (c.u - units) / (y.tiles + p.extra), first = units + item * (y.tiles + p.extra), stop = min(first + y.tiles + p.extra, c.end);
     const int t0 = max(c.u - first - p.extra, 0), t1 = stop - first - p.extra;
@@ -325,6 +344,13 @@ template <typename T, bool EIGHTS> __global__ void __launch_bounds__(PREP_THREAD
       const int g = e / p.vdim, c = e - g * p.vdim;
       v_page<T>(p, phys, g)[(size_t)place * p.vdim + c] = v[e];
     }
+    const T *q = reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld;
+    const int d4 = (p.dim + 3) / 4 * 4;
+    float *to = reinterpret_cast<float *>(p.queries) + ((size_t)s * p.most + i) * p.n_head * d4;
+    for (int e = tid; e < p.n_head * d4; e += PREP_THREADS) {
+      const int head = e / d4, c = e - head * d4;
+      to[e] = c < p.dim ? turned<T>(p, q + (size_t)head * p.dim, c, pos) : 0.f;
+    }
   }
   for (int c = p.n_head * p.vdim + tid; c < p.out_cols; c += PREP_THREADS) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + i) * p.out_ld + c] = rounded<T>(0.f);
 }
@@ -337,9 +363,23 @@ __device__ __forceinline__ float score2(const Params &p, float s) {
 
 // ------------------------------------------------------------------------------------------ any sizes
 // Rows and keys of a tile in shared memory as fp32; thread (ty, tx) has rows 2 ty, 2 ty + 1 and keys tx, tx + 8, .. of the scores, and columns 4 tx + 32 j of
-// the output.  What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them.
+// the output.  The next keys come in behind the scores, the next values behind the output, four threads a row; fp32 rows of whole 16 bytes by asynchronous copies.
+// What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them.
 constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32, PLAIN_BLOCKS = 2;      // blocks: of an SM
 static size_t plain_smem(int dim, int vdim) { return (size_t)(PROWS + PKEYS) * (dim + 8) * 4 + (size_t)PKEYS * (vdim + 36) * 4 + (size_t)PROWS * (PKEYS + 4) * 4 + PROWS * 8; }
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// This thread's part of a row of `have` elements (zeros, where it is not `there`) to `to`, up to a multiple of four.
+template <typename T> __device__ __noinline__ void row_in(float *to, const T *from, bool there, int have, bool async) {
+  const int part = threadIdx.x & 3;
+  if (std::is_same<T, float>::value && async) {
+    for (int c = 4 * part; c < have; c += 16) cp_async(tc::sa(to + c), from + (there ? c : 0), there ? 16 : 0);
+    return;
+  }
+#pragma unroll 4
+  for (int c = part; c < (have + 3) / 4 * 4; c += 4) to[c] = there && c < have ? val(from[c]) : 0.f;
+}
 template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) tree_plain_kernel(const __grid_constant__ Params p) {
   early_start();
   extern __shared__ __align__(16) float sm[];
@@ -347,28 +387,35 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
   __shared__ uint32_t seen[MAX_NODES][WORDS];
   const int d4 = (p.dim + 3) / 4 * 4, v32 = VJ * 32, kld = d4 + 4, vld = v32 + 4, pld = PKEYS + 4;
   float *Q = sm, *K = Q + PROWS * kld, *V = K + PKEYS * kld, *P = V + PKEYS * vld, *corr = P + PROWS * pld, *sum = corr + PROWS;
-  const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
+  const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3, mine = tid >> 2;      // mine: the row that the thread brings in and whose softmax it shares
+  const bool async = p.dim % 4 == 0 && p.vdim % 4 == 0 && (reinterpret_cast<uintptr_t>(p.pool) & 15) == 0;
   int had = -1;
   Cursor cursor(p);
   for (Piece k = next_piece(p, cursor); k.nt; k = next_piece(p, cursor)) {
     const Seq x = k.x;
-    const int rows = min(PROWS, x.n * p.qpk - k.rt * PROWS), r0 = k.rt * PROWS;
+    const int rows = min(PROWS, x.n * p.qpk - k.rt * PROWS), r0 = k.rt * PROWS, last = x.start + x.n, lowest = p.window ? max(0, x.start - p.window + 1) : 0;
+    const int *table = p.page_table + (size_t)k.table * p.max_pages;
+    // the thread's row of a tile: its page (-1: it is not the sequence's, or nobody sees it), looked up a tile ahead, and its place in the page
+    auto page_of = [&](int t, int &in) {
+      const int j = t * PKEYS + mine, page = j / p.page;
+      in = j - page * p.page;
+      return t < k.t0 + k.nt && j >= lowest && j < last ? table[page] : -1;
+    };
+    int in, in_next, phys = page_of(k.t0, in), phys_next = page_of(k.t0 + 1, in_next);
+    auto keys_in = [&](int phys, int in) { row_in<T>(K + mine * kld, k_page<T>(p, max(phys, 0), k.g) + (size_t)in * p.dim, phys >= 0, p.dim, async); };
+    auto values_in = [&](int phys, int in) { row_in<T>(V + mine * vld, v_page<T>(p, max(phys, 0), k.g) + (size_t)in * p.vdim, phys >= 0, p.vdim, async); };
+    const int row = min(r0 + mine, x.n * p.qpk - 1), tok = row / p.qpk;      // (rows behind the last: anything)
     __syncthreads();
+    row_in<float>(Q + mine * kld, reinterpret_cast<const float *>(p.queries) + (((size_t)k.s * p.most + tok) * p.n_head + k.g * p.qpk + row - tok * p.qpk) * d4, true, d4, true);
+    keys_in(phys, in);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    values_in(phys, in);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (k.s != had) {
       for (int i = tid; i < x.n; i += PLAIN_THREADS) depth[i] = p.depth[(size_t)k.s * p.most + i];
       for (int i = tid; i < x.n * WORDS; i += PLAIN_THREADS) (&seen[0][0])[i] = p.seen[(size_t)k.s * p.most * WORDS + i];
-      __syncthreads();
     }
     had = k.s;
-    for (int e = tid; e < PROWS * d4; e += PLAIN_THREADS) {
-      const int r = e / d4, c = e - r * d4;
-      float y = 0.f;
-      if (r < rows && c < p.dim) {
-        const int i = (r0 + r) / p.qpk, h = k.g * p.qpk + (r0 + r) % p.qpk;
-        y = turned<T>(p, reinterpret_cast<const T *>(p.q) + (size_t)(x.row0 + i) * p.q_ld + (size_t)h * p.dim, c, x.start + depth[i]);
-      }
-      Q[r * kld + c] = y;
-    }
     float o[2][VJ][4];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -377,18 +424,10 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[a][j][e] = 0.f;
     float m = -INFINITY, l = 0.f;        // of row tid / 4, the same in its four threads
-    const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
     for (int t = k.t0; t < k.t0 + k.nt; ++t) {
-      const int j0 = t * PKEYS, keys = min(PKEYS, x.start + x.n - j0);
-      __syncthreads();
-      for (int e = tid; e < PKEYS * d4; e += PLAIN_THREADS) {
-        const int r = e / d4, c = e - r * d4, j = j0 + r;
-        K[r * kld + c] = r < keys && c < p.dim ? val(k_page<T>(p, table[j / p.page], k.g)[(size_t)(j % p.page) * p.dim + c]) : 0.f;
-      }
-      for (int e = tid; e < PKEYS * v32; e += PLAIN_THREADS) {
-        const int r = e / v32, c = e - r * v32, j = j0 + r;
-        V[r * vld + c] = r < keys && c < p.vdim ? val(v_page<T>(p, table[j / p.page], k.g)[(size_t)(j % p.page) * p.vdim + c]) : 0.f;
-      }
+      const int j0 = t * PKEYS;
+      const bool all_seen = j0 + PKEYS <= x.start && (p.window == 0 || last - 1 - j0 < p.window);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
       float sc[2][4] = {};
       for (int c = 0; c < d4; c += 4) {
@@ -407,30 +446,39 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 2 * ty + i, key = tx + 8 * j;
-          const int tok = min((r0 + r) / p.qpk, x.n - 1), d = j0 + key - x.start;      // (drafted token of the key)
-          const bool see = d >= 0 ? seen[tok][min(d, MAX_NODES - 1) >> 5] >> (d & 31) & 1 : p.window == 0 || depth[tok] - d < p.window;
-          P[r * pld + key] = r < rows && key < keys && see ? score2(p, sc[i][j]) : -INFINITY;
+          bool see = all_seen;
+          if (!all_seen) {
+            const int tok = min((r0 + r) / p.qpk, x.n - 1), d = j0 + key - x.start;      // (drafted token of the key)
+            see = j0 + key < last && (d >= 0 ? seen[tok][min(d, MAX_NODES - 1) >> 5] >> (d & 31) & 1 : p.window == 0 || depth[tok] - d < p.window);
+          }
+          P[r * pld + key] = see ? score2(p, sc[i][j]) : -INFINITY;
         }
       __syncthreads();
+      in = in_next;
+      phys = phys_next;
+      phys_next = page_of(t + 2, in_next);
+      if (t + 1 < k.t0 + k.nt) keys_in(phys, in);
+      asm volatile("cp.async.commit_group;" ::: "memory");
       {
-        float *row = P + (tid >> 2) * pld + (tid & 3) * 8, top = m, add = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, row[j]);
+        float4 *row = reinterpret_cast<float4 *>(P + mine * pld + (tid & 3) * 8);
+        float4 y = row[0], z = row[1];
+        float top = fmaxf(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)), fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)));
+        top = fmaxf(top, m);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = exp2f(row[j] - base);
-          row[j] = w;
-          add += w;
-        }
+        y.x = exp2f(y.x - base); y.y = exp2f(y.y - base); y.z = exp2f(y.z - base); y.w = exp2f(y.w - base);
+        z.x = exp2f(z.x - base); z.y = exp2f(z.y - base); z.z = exp2f(z.z - base); z.w = exp2f(z.w - base);
+        row[0] = y;
+        row[1] = z;
+        float add = ((y.x + y.y) + (y.z + y.w)) + ((z.x + z.y) + (z.z + z.w));
         add += __shfl_xor_sync(0xffffffffu, add, 1);
         add += __shfl_xor_sync(0xffffffffu, add, 2);
         l = l * f + add;
         m = top;
-        if ((tid & 3) == 0) corr[tid >> 2] = f;
+        if ((tid & 3) == 0) corr[mine] = f;
       }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -440,28 +488,29 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
       }
-      // (a value that a row does not see may be infinite or NaN: it is left out, not multiplied by zero)
-      const bool all_seen = j0 + keys <= x.start && (p.window == 0 || x.start + x.n - 1 - j0 < p.window);
-      for (int key = 0; key < keys; ++key) {
-        const float w0 = P[2 * ty * pld + key], w1 = P[(2 * ty + 1) * pld + key];
-        if (!all_seen) {
+#pragma unroll 1
+      for (int k4 = 0; k4 < PKEYS; k4 += 4) {
+        const float4 a4 = *reinterpret_cast<const float4 *>(P + 2 * ty * pld + k4), b4 = *reinterpret_cast<const float4 *>(P + (2 * ty + 1) * pld + k4);
+        const float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-          for (int j = 0; j < VJ; ++j)
+        for (int z = 0; z < 4; ++z) {
+          // (a value that a row does not see may be infinite or NaN: it is left out, not multiplied by zero)
+          const bool first = all_seen || a[z] != 0.f, second = all_seen || b[z] != 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = V[key * vld + 4 * tx + 32 * j + e];
-              if (w0 != 0.f) o[0][j][e] = fmaf(w0, y, o[0][j][e]);
-              if (w1 != 0.f) o[1][j][e] = fmaf(w1, y, o[1][j][e]);
+          for (int j = 0; j < VJ; ++j) {
+            const float4 y = *reinterpret_cast<const float4 *>(V + (k4 + z) * vld + 4 * tx + 32 * j);
+            if (first) {
+              o[0][j][0] = fmaf(a[z], y.x, o[0][j][0]); o[0][j][1] = fmaf(a[z], y.y, o[0][j][1]); o[0][j][2] = fmaf(a[z], y.z, o[0][j][2]); o[0][j][3] = fmaf(a[z], y.w, o[0][j][3]);
             }
-          continue;
-        }
-#pragma unroll
-        for (int j = 0; j < VJ; ++j) {
-          const float4 y = *reinterpret_cast<const float4 *>(V + key * vld + 4 * tx + 32 * j);
-          o[0][j][0] = fmaf(w0, y.x, o[0][j][0]); o[0][j][1] = fmaf(w0, y.y, o[0][j][1]); o[0][j][2] = fmaf(w0, y.z, o[0][j][2]); o[0][j][3] = fmaf(w0, y.w, o[0][j][3]);
-          o[1][j][0] = fmaf(w1, y.x, o[1][j][0]); o[1][j][1] = fmaf(w1, y.y, o[1][j][1]); o[1][j][2] = fmaf(w1, y.z, o[1][j][2]); o[1][j][3] = fmaf(w1, y.w, o[1][j][3]);
+            if (second) {
+              o[1][j][0] = fmaf(b[z], y.x, o[1][j][0]); o[1][j][1] = fmaf(b[z], y.y, o[1][j][1]); o[1][j][2] = fmaf(b[z], y.z, o[1][j][2]); o[1][j][3] = fmaf(b[z], y.w, o[1][j][3]);
+            }
+          }
         }
       }
+      __syncthreads();
+      if (t + 1 < k.t0 + k.nt) values_in(phys, in);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
     if ((tid & 3) == 0) {
       sum[tid >> 2] = l;
@@ -534,9 +583,6 @@ __device__ __forceinline__ uint32_t product_desc(bool bf16, int n, bool b_by_row
 // Byte of 16-byte unit c of row r of a tile of rows of 128 swizzled bytes (blocks of 128 rows).
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 // 16 bytes, zeros where bytes is 0.
-__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t &bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(tc::sa(&bar)), "r"(x), "r"(y), "r"(z)
                : "memory");
@@ -644,7 +690,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     bool ok = true;
     for (Piece k = next_piece(p, cursor); k.nt && ok; k = next_piece(p, cursor), ++pieces) {
       const Seq x = k.x;
-      const int *table = p.page_table + (size_t)p.slot[k.s] * p.max_pages;
+      const int *table = p.page_table + (size_t)k.table * p.max_pages;
       const int lowest = p.window ? max(0, x.start - p.window + 1) : 0, last = x.start + x.n;
       auto page_of = [&](int j) { return j >= lowest && j < last ? table[j / p.page] : 0; };      // (what is not the sequence's: any page)
       // Page and row in it of a tile's boxes, one per lane, looked up a tile ahead (here and not where they are used: a division takes as long as a box)
@@ -1016,13 +1062,13 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
   if (!x.n) return;
   const Span y = span(p, x);
   const int eights = (p.most * p.qpk + COMBINE_ROWS - 1) / COMBINE_ROWS, g = blockIdx.x / eights, r0 = (blockIdx.x - g * eights) * COMBINE_ROWS;   // (first row, of all of the kv head's)
-  const int rows = min(COMBINE_ROWS, x.n * p.qpk - r0), rt = r0 / p.rows_tile;
+  const int rows = min(COMBINE_ROWS, x.n * p.qpk - r0), rt = r0 >> p.rows_shift;
   if (rows <= 0) return;
   const int first = units + (g * y.row_tiles + rt) * (y.tiles + p.extra) + p.extra, b0 = first / quota, b1 = (first + y.tiles - 1) / quota;
   if (b0 == b1) return;
   const int v4 = (p.vdim + 3) / 4;
   for (int e = tid; e < rows * v4; e += COMBINE_THREADS) {
-    const int r = r0 % p.rows_tile + e / v4, c = e % v4;
+    const int r = (r0 & (p.rows_tile - 1)) + e / v4, c = e % v4;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -1047,6 +1093,7 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
   }
 }
 
+static size_t plan_ints() { return PLAN_HEAD + (size_t)sm_count() * PLAIN_BLOCKS * (sizeof(Start) / 4); }
 // Rows of the parts: two tiles of every block of either kernel.
 static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
 
@@ -1092,10 +1139,10 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   if constexpr (std::is_same<T, float>::value) tensor = false;
   if (tensor) {
     // (A piece beside its tiles costs about as much as two of them: queries in, the last weights and products, the output.)
-    p.rows_tile = TROWS; p.keys_tile = TKEYS; p.extra = 2; p.blocks = sm_count();
+    p.rows_tile = TROWS; p.keys_tile = TKEYS; p.rows_shift = p.keys_shift = 7; p.extra = 2; p.blocks = sm_count();
     if constexpr (!std::is_same<T, float>::value) PT_CUDA(launch_early(tree_prep_kernel<T, true>, prep, PREP_THREADS, 0, st, p));
   } else {
-    p.rows_tile = PROWS; p.keys_tile = PKEYS; p.extra = 0; p.blocks = sm_count() * PLAIN_BLOCKS;
+    p.rows_tile = PROWS; p.keys_tile = PKEYS; p.rows_shift = p.keys_shift = 5; p.extra = 0; p.blocks = sm_count() * PLAIN_BLOCKS;
     PT_CUDA(launch_early(tree_prep_kernel<T, false>, prep, PREP_THREADS, 0, st, p));
   }
   PT_LAUNCH_CHECK("pt_tree_attn");
@@ -1114,9 +1161,10 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
 
 using namespace pt;
 
-// Workspace: the plan, units, depths and masks of all tokens; the queries as the tensor cores take them (widths up to 128 in two parts of 16 bits); the parts.
-static size_t queries_offset(int n_seq, int most) { return (((size_t)(2 + sm_count() * ta::PLAIN_BLOCKS) + n_seq + 1 + (size_t)n_seq * most * (1 + ta::WORDS)) * 4 + 255) / 256 * 256; }
-static size_t part_offset(int n_seq, int most, int n_head) { return queries_offset(n_seq, most) + (size_t)n_seq * most * n_head * 128 * 4; }
+// Workspace: the plan, units, depths and masks of all tokens; the queries as the attention kernel takes them (fp32, or of widths up to 128 two
+// parts of 16 bits); the parts.
+static size_t queries_offset(int n_seq, int most) { return ((ta::plan_ints() + n_seq + 1 + (size_t)n_seq * most * (1 + ta::WORDS)) * 4 + 255) / 256 * 256; }
+static size_t part_offset(int n_seq, int most, int n_head) { return queries_offset(n_seq, most) + (size_t)n_seq * most * n_head * 256 * 4; }
 extern "C" size_t pt_tree_attn_workspace_bytes(int n_seq, int max_tokens_per_seq, int n_head, int n_kv, int vdim) {
   (void)n_kv;
   return part_offset(n_seq, max_tokens_per_seq, n_head) + ta::part_rows() * (sizeof(float2) + (size_t)(vdim + 3) / 4 * 16);
@@ -1154,7 +1202,7 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   const size_t need = pt_tree_attn_workspace_bytes(b.n_seq, p.most, a->n_head, a->n_kv, a->vdim);
   PT_REQUIRE(a->workspace && a->workspace_bytes >= need && aligned_to(a->workspace, 16), "pt_tree_attn: %zu workspace bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
   p.plan = (int *)a->workspace;
-  p.units = p.plan + 2 + sm_count() * ta::PLAIN_BLOCKS;
+  p.units = p.plan + ta::plan_ints();
   p.depth = p.units + b.n_seq + 1;
   p.seen = (uint32_t *)(p.depth + (size_t)b.n_seq * p.most);
   p.queries = (uint4 *)((char *)a->workspace + queries_offset(b.n_seq, p.most));
