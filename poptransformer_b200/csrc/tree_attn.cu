@@ -39,7 +39,7 @@ struct Params {
   int n_seq, n_head, n_kv, qpk, dim, vdim, page, max_pages, max_len, window, most;
   int q_ld, kv_ld, out_ld, out_cols, rope_half;
   int rows_tile, keys_tile, extra, blocks; // of an item, of a unit (powers of two); units of an item beside its key tiles; blocks of the attention kernel
-  int rows_shift, keys_shift;
+  int rows_shift, keys_shift, part_ld;      // part_ld: rows of a part in the workspace
   float scale, softcap;
   const void *q, *k, *v;
   void *pool, *out;
@@ -55,8 +55,8 @@ struct Params {
   uint32_t *seen;     // [n_seq][most][WORDS]: the tokens that a token sees
   uint4 *queries;     // tensor cores: of sequence s and kv head g from unit (s most n_head + g rows) 2 dim / 8 on: [part][dim / 8][rows], rows = n qpk;
                       // plain: [n_seq][most][n_head][dim up to a multiple of 4] as fp32
-  float *part_o;      // [2 blocks][vdim / 4][rows_tile][4]
-  float2 *part_ml;    // [2 blocks][rows_tile]
+  float *part_o;      // [2 blocks][vdim / 4][part_ld][4]
+  float2 *part_ml;    // [2 blocks][part_ld]
 };
 
 // ------------------------------------------------------------------------------------------ the work and its parts
@@ -355,10 +355,33 @@ template <typename T, bool EIGHTS> __global__ void __launch_bounds__(PREP_THREAD
   for (int c = p.n_head * p.vdim + tid; c < p.out_cols; c += PREP_THREADS) reinterpret_cast<T *>(p.out)[(size_t)(x.row0 + i) * p.out_ld + c] = rounded<T>(0.f);
 }
 
-// Scores in the units of exp2 from raw products.
-__device__ __forceinline__ float score2(const Params &p, float s) {
-  s *= p.scale;
-  return (p.softcap > 0.f ? p.softcap * tanhf(s / p.softcap) : s) * kLog2e;
+// Which of the keys base .. base + 31 token i sees.
+__device__ __forceinline__ uint32_t seen_word(const Params &p, const Seq &x, const uint32_t *seen, int depth, int base) {
+  const int ctx = min(max(x.start - base, 0), 32), low = p.window ? min(max(x.start + depth - p.window + 1 - base, 0), 32) : 0;
+  uint32_t v = ctx == 32 ? 0xffffffffu : (1u << ctx) - 1u;
+  v = low == 32 ? 0u : v & ~((1u << low) - 1u);
+  const int d = base - x.start;      // drafted token of the first key
+  if (d >= 0) {
+    const int k = d >> 5;
+    if (k < WORDS) v |= __funnelshift_r(seen[k], k + 1 < WORDS ? seen[k + 1] : 0u, d & 31);
+  } else if (d > -32) {
+    v |= seen[0] << -d;
+  }
+  return v;
+}
+
+// tanh without a branch: below 0.55 its Taylor series (the coefficients are 2^2n (2^2n - 1) B_2n / (2n)!; what is left out is below 2^-24 of it), else
+// 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float tanh_of(float x) {
+  const float y = x * x;
+  float t = -929569.f / 638512875.f;
+  t = fmaf(t, y, 21844.f / 6081075.f);
+  t = fmaf(t, y, -1382.f / 155925.f);
+  t = fmaf(t, y, 62.f / 2835.f);
+  t = fmaf(t, y, -17.f / 315.f);
+  t = fmaf(t, y, 2.f / 15.f);
+  t = fmaf(t, y, -1.f / 3.f);
+  return fabsf(x) < 0.55f ? fmaf(x * y, t, x) : 1.0f - __fdividef(2.0f, exp2f(2.0f * kLog2e * x) + 1.0f);
 }
 
 // ------------------------------------------------------------------------------------------ any sizes
@@ -383,13 +406,11 @@ template <typename T> __device__ __noinline__ void row_in(float *to, const T *fr
 template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) tree_plain_kernel(const __grid_constant__ Params p) {
   early_start();
   extern __shared__ __align__(16) float sm[];
-  __shared__ int depth[MAX_NODES];
-  __shared__ uint32_t seen[MAX_NODES][WORDS];
   const int d4 = (p.dim + 3) / 4 * 4, v32 = VJ * 32, kld = d4 + 4, vld = v32 + 4, pld = PKEYS + 4;
   float *Q = sm, *K = Q + PROWS * kld, *V = K + PKEYS * kld, *P = V + PKEYS * vld, *corr = P + PROWS * pld, *sum = corr + PROWS;
   const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3, mine = tid >> 2;      // mine: the row that the thread brings in and whose softmax it shares
   const bool async = p.dim % 4 == 0 && p.vdim % 4 == 0 && (reinterpret_cast<uintptr_t>(p.pool) & 15) == 0;
-  int had = -1;
+  const float inv_cap = p.softcap > 0.f ? 1.0f / p.softcap : 0.f;
   Cursor cursor(p);
   for (Piece k = next_piece(p, cursor); k.nt; k = next_piece(p, cursor)) {
     const Seq x = k.x;
@@ -411,11 +432,8 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
     asm volatile("cp.async.commit_group;" ::: "memory");
     values_in(phys, in);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (k.s != had) {
-      for (int i = tid; i < x.n; i += PLAIN_THREADS) depth[i] = p.depth[(size_t)k.s * p.most + i];
-      for (int i = tid; i < x.n * WORDS; i += PLAIN_THREADS) (&seen[0][0])[i] = p.seen[(size_t)k.s * p.most * WORDS + i];
-    }
-    had = k.s;
+    const int depth = p.depth[(size_t)k.s * p.most + tok];
+    const uint32_t *seen = p.seen + ((size_t)k.s * p.most + tok) * WORDS;
     float o[2][VJ][4];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -429,7 +447,9 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
       const bool all_seen = j0 + PKEYS <= x.start && (p.window == 0 || last - 1 - j0 < p.window);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
+      const uint32_t see = all_seen ? 0xffffffffu : seen_word(p, x, seen, depth, j0) >> (tid & 3) * 8;      // of the eight keys whose weights the thread works out
       float sc[2][4] = {};
+#pragma unroll 2
       for (int c = 0; c < d4; c += 4) {
         float4 a[2], b[4];
 #pragma unroll
@@ -444,15 +464,7 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 2 * ty + i, key = tx + 8 * j;
-          bool see = all_seen;
-          if (!all_seen) {
-            const int tok = min((r0 + r) / p.qpk, x.n - 1), d = j0 + key - x.start;      // (drafted token of the key)
-            see = j0 + key < last && (d >= 0 ? seen[tok][min(d, MAX_NODES - 1) >> 5] >> (d & 31) & 1 : p.window == 0 || depth[tok] - d < p.window);
-          }
-          P[r * pld + key] = see ? score2(p, sc[i][j]) : -INFINITY;
-        }
+        for (int j = 0; j < 4; ++j) P[(2 * ty + i) * pld + tx + 8 * j] = sc[i][j] * p.scale;
       __syncthreads();
       in = in_next;
       phys = phys_next;
@@ -461,17 +473,27 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
       asm volatile("cp.async.commit_group;" ::: "memory");
       {
         float4 *row = reinterpret_cast<float4 *>(P + mine * pld + (tid & 3) * 8);
-        float4 y = row[0], z = row[1];
-        float top = fmaxf(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)), fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)));
-        top = fmaxf(top, m);
+        const float4 y = row[0], z = row[1];
+        float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w}, top = m, add = 0.f;
+        if (p.softcap > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = p.softcap * tanh_of(w[i] * inv_cap);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] = see >> i & 1 ? w[i] * kLog2e : -INFINITY;
+          top = fmaxf(top, w[i]);
+        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float base = top == -INFINITY ? 0.f : top, f = exp2f(m - base);
-        y.x = exp2f(y.x - base); y.y = exp2f(y.y - base); y.z = exp2f(y.z - base); y.w = exp2f(y.w - base);
-        z.x = exp2f(z.x - base); z.y = exp2f(z.y - base); z.z = exp2f(z.z - base); z.w = exp2f(z.w - base);
-        row[0] = y;
-        row[1] = z;
-        float add = ((y.x + y.y) + (y.z + y.w)) + ((z.x + z.y) + (z.z + z.w));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] = exp2f(w[i] - base);
+          add += w[i];
+        }
+        row[0] = make_float4(w[0], w[1], w[2], w[3]);
+        row[1] = make_float4(w[4], w[5], w[6], w[7]);
         add += __shfl_xor_sync(0xffffffffu, add, 1);
         add += __shfl_xor_sync(0xffffffffu, add, 2);
         l = l * f + add;
@@ -488,23 +510,19 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][j][e] *= f;
       }
-#pragma unroll 1
-      for (int k4 = 0; k4 < PKEYS; k4 += 4) {
-        const float4 a4 = *reinterpret_cast<const float4 *>(P + 2 * ty * pld + k4), b4 = *reinterpret_cast<const float4 *>(P + (2 * ty + 1) * pld + k4);
-        const float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll 2
+      for (int key = 0; key < PKEYS; ++key) {
+        const float a = P[2 * ty * pld + key], b = P[(2 * ty + 1) * pld + key];
+        // (a value that a row does not see may be infinite or NaN: it is left out, not multiplied by zero)
+        const bool first = all_seen || a != 0.f, second = all_seen || b != 0.f;
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          // (a value that a row does not see may be infinite or NaN: it is left out, not multiplied by zero)
-          const bool first = all_seen || a[z] != 0.f, second = all_seen || b[z] != 0.f;
-#pragma unroll
-          for (int j = 0; j < VJ; ++j) {
-            const float4 y = *reinterpret_cast<const float4 *>(V + (k4 + z) * vld + 4 * tx + 32 * j);
-            if (first) {
-              o[0][j][0] = fmaf(a[z], y.x, o[0][j][0]); o[0][j][1] = fmaf(a[z], y.y, o[0][j][1]); o[0][j][2] = fmaf(a[z], y.z, o[0][j][2]); o[0][j][3] = fmaf(a[z], y.w, o[0][j][3]);
-            }
-            if (second) {
-              o[1][j][0] = fmaf(b[z], y.x, o[1][j][0]); o[1][j][1] = fmaf(b[z], y.y, o[1][j][1]); o[1][j][2] = fmaf(b[z], y.z, o[1][j][2]); o[1][j][3] = fmaf(b[z], y.w, o[1][j][3]);
-            }
+        for (int j = 0; j < VJ; ++j) {
+          const float4 y = *reinterpret_cast<const float4 *>(V + key * vld + 4 * tx + 32 * j);
+          if (first) {
+            o[0][j][0] = fmaf(a, y.x, o[0][j][0]); o[0][j][1] = fmaf(a, y.y, o[0][j][1]); o[0][j][2] = fmaf(a, y.z, o[0][j][2]); o[0][j][3] = fmaf(a, y.w, o[0][j][3]);
+          }
+          if (second) {
+            o[1][j][0] = fmaf(b, y.x, o[1][j][0]); o[1][j][1] = fmaf(b, y.y, o[1][j][1]); o[1][j][2] = fmaf(b, y.z, o[1][j][2]); o[1][j][3] = fmaf(b, y.w, o[1][j][3]);
           }
         }
       }
@@ -514,7 +532,7 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
     }
     if ((tid & 3) == 0) {
       sum[tid >> 2] = l;
-      if (!k.whole) p.part_ml[(size_t)k.slot * PROWS + (tid >> 2)] = make_float2(m, l);
+      if (!k.whole && mine < rows) p.part_ml[(size_t)k.slot * p.part_ld + mine] = make_float2(m, l);
     }
     __syncthreads();
 #pragma unroll
@@ -532,7 +550,7 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
           for (int e = 0; e < 4; ++e)
             if (c + e < p.vdim) out[c + e] = rounded<T>(o[i][j][e] * inv);
         } else {
-          *reinterpret_cast<float4 *>(p.part_o + (((size_t)k.slot * ((p.vdim + 3) / 4) + c / 4) * PROWS + r) * 4) = make_float4(o[i][j][0], o[i][j][1], o[i][j][2], o[i][j][3]);
+          *reinterpret_cast<float4 *>(p.part_o + (((size_t)k.slot * ((p.vdim + 3) / 4) + c / 4) * p.part_ld + r) * 4) = make_float4(o[i][j][0], o[i][j][1], o[i][j][2], o[i][j][3]);
         }
       }
     }
@@ -630,21 +648,6 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
 
 // A piece's tile that some rows see in part: keys from `start` on are drafted, those in front of start + n - window are not seen by all.
 __device__ __forceinline__ bool partial(const Params &p, const Seq &x, int j0) { return j0 + TKEYS > x.start || (p.window && x.start + x.n - 1 - j0 >= p.window); }
-// Which of the keys base .. base + 31 token i sees.
-__device__ __forceinline__ uint32_t seen_word(const Params &p, const Seq &x, const uint32_t *seen, int depth, int base) {
-  const int ctx = min(max(x.start - base, 0), 32), low = p.window ? min(max(x.start + depth - p.window + 1 - base, 0), 32) : 0;
-  uint32_t v = ctx == 32 ? 0xffffffffu : (1u << ctx) - 1u;
-  v = low == 32 ? 0u : v & ~((1u << low) - 1u);
-  const int d = base - x.start;      // drafted token of the first key
-  if (d >= 0) {
-    const int k = d >> 5;
-    if (k < WORDS) v |= __funnelshift_r(seen[k], k + 1 < WORDS ? seen[k + 1] : 0u, d & 31);
-  } else if (d > -32) {
-    v |= seen[0] << -d;
-  }
-  return v;
-}
-
 template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
   early_start();
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -1012,7 +1015,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
         const bool store = row < rows;
         const float inv = k.whole ? 1.0f / sum : 1.0f;
         T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + node) * p.out_ld + (size_t)head * p.vdim;
-        if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * TROWS + row] = make_float2(m, sum);
+        if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * p.part_ld + row] = make_float2(m, sum);
 #pragma unroll 1
         for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
           uint32_t v[16];
@@ -1033,9 +1036,9 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
                 for (int b = 0; b < 8; ++b) out[c + z + b] = e[b];
               }
             } else {
-              uint4 *to = reinterpret_cast<uint4 *>(p.part_o + (((size_t)k.slot * (p.vdim / 4) + (c + z) / 4) * TROWS + row) * 4);
+              uint4 *to = reinterpret_cast<uint4 *>(p.part_o + (((size_t)k.slot * (p.vdim / 4) + (c + z) / 4) * p.part_ld + row) * 4);
               to[0] = make_uint4(v[z], v[z + 1], v[z + 2], v[z + 3]);
-              to[TROWS] = make_uint4(v[z + 4], v[z + 5], v[z + 6], v[z + 7]);
+              to[p.part_ld] = make_uint4(v[z + 4], v[z + 5], v[z + 6], v[z + 7]);
             }
           }
         }
@@ -1072,13 +1075,13 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int b = b0; b <= b1; ++b) m = fmaxf(m, p.part_ml[(size_t)(2 * b + (b == b0 ? 1 : 0)) * p.rows_tile + r].x);
+    for (int b = b0; b <= b1; ++b) m = fmaxf(m, p.part_ml[(size_t)(2 * b + (b == b0 ? 1 : 0)) * p.part_ld + r].x);
     if (m == -INFINITY) m = 0.f;
 #pragma unroll 4
     for (int b = b0; b <= b1; ++b) {
       const size_t slot = 2 * b + (b == b0 ? 1 : 0);
-      const float2 ml = p.part_ml[slot * p.rows_tile + r];
-      const float4 w = *reinterpret_cast<const float4 *>(p.part_o + ((slot * v4 + c) * p.rows_tile + r) * 4);
+      const float2 ml = p.part_ml[slot * p.part_ld + r];
+      const float4 w = *reinterpret_cast<const float4 *>(p.part_o + ((slot * v4 + c) * p.part_ld + r) * 4);
       const float f = exp2f(ml.x - m);
       o.x = fmaf(w.x, f, o.x); o.y = fmaf(w.y, f, o.y); o.z = fmaf(w.z, f, o.z); o.w = fmaf(w.w, f, o.w);
       l = fmaf(ml.y, f, l);
@@ -1095,7 +1098,7 @@ template <typename T> __global__ void __launch_bounds__(COMBINE_THREADS) combine
 
 static size_t plan_ints() { return PLAN_HEAD + (size_t)sm_count() * PLAIN_BLOCKS * (sizeof(Start) / 4); }
 // Rows of the parts: two tiles of every block of either kernel.
-static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS, PLAIN_BLOCKS * PROWS); }
+static size_t part_rows() { return (size_t)2 * sm_count() * std::max(TROWS + 8, PLAIN_BLOCKS * (PROWS + 8)); }
 
 template <typename T, int VJ> static int launch_plain(Params &p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
@@ -1137,6 +1140,8 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   int rc;
   const Grid prep(dim3(p.most, p.n_seq + 1));
   if constexpr (std::is_same<T, float>::value) tensor = false;
+  // (an odd number of eights: rows of the same column of parts lie apart by no power of two)
+  p.part_ld = (std::min(tensor ? TROWS : PROWS, p.most * p.qpk) + 7) / 8 * 8 | 8;
   if (tensor) {
     // (A piece beside its tiles costs about as much as two of them: queries in, the last weights and products, the output.)
     p.rows_tile = TROWS; p.keys_tile = TKEYS; p.rows_shift = p.keys_shift = 7; p.extra = 2; p.blocks = sm_count();
