@@ -559,7 +559,7 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 
 // ------------------------------------------------------------------------------------------ tensor cores
 // One block per SM, 128 query rows against tiles of 128 keys.  Queries stay in tensor memory: shared memory is the ring of keys and values, whose depth decides how
-// fast they come (32 KB of queries in two parts cost two of its six slots, and a quarter of the rate behind 60000 positions).  S = Q K^T goes to tensor memory
+// fast they come (32 KB of queries in two parts took two of its six slots: 234 us behind 60000 positions, 222 without).  S = Q K^T goes to tensor memory
 // (lane = row), two softmax threads per row, one for each half of the keys, turn it into weights in place, and O += P V takes those from there and V, keys
 // outermost as the cache has it, from shared memory.  A row's weights would lose 8 or 11 bits' worth when rounded once; as two parts (hi + lo) they keep 15 or
 // more, for a second product with V; rotated queries come in two parts likewise.  Scores have two buffers, so that the products of one tile run beside the
@@ -570,8 +570,10 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 //   warp 10          issues the products; owns the tensor memory: 2 x 128 columns of scores, 128 of output, 2 x 64 of queries.  (All 512 are asked for: they
 //                    begin at 0.)
 // (Twelve warps: an SM quarter's registers are shared by three.)
-// A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads): memory bounds it for up to 128 rows, as long as
-// copies stay in flight.  The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
+// A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads), and 2600 cycles at this SM's share of memory.  Measured
+// are 3700 behind 60000 positions: one warp asks for boxes (700 for a tile of keys or values), one issues products, and each tile's softmax, products and copies
+// hand it on to one another.  Behind some hundred positions a block has one or two tiles, and what bounds it is the way from the plan to the first weights.
+// The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
 // (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
 constexpr int SOFT_WARPS = 8, COPY_WARPS = 2, MMA_WARP = SOFT_WARPS + COPY_WARPS, TENSOR_THREADS = 384, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
 constexpr int RING_BYTES = 192 * 1024, O_COL = 256, Q_COL = 384, Q_LOW = 64;      // columns of output and queries, from there of the queries' second part
@@ -855,7 +857,8 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     const int half = warp >> 2, q = warp & 3, row = q * 32 + lane;
     const uint32_t lanes = (uint32_t)(q * 32) << 16, S = lanes + half * 64, O = lanes + O_COL;
     int pieces = 0, n_s[2] = {0, 0}, n_o = 0;
-    const float a1 = fabsf(p.scale) * kLog2e, a2 = CAP ? 2.0f * a1 / p.softcap : 0.f, b2 = p.softcap * kLog2e;
+    const float a1 = fmaxf(fabsf(p.scale), 1e-30f) * kLog2e, a2 = CAP ? 2.0f * a1 / p.softcap : 0.f, b2 = p.softcap * kLog2e;
+    // (a scale of zero: so small that all scores are equal, but -inf, which marks what is not seen, times it is -inf)
     auto score = [&](float s) { return CAP ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : a1 * s; };      // (grows with s)
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory"); };
     auto meet_partner = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + q) : "memory"); };       // the warp with the same rows
@@ -1202,10 +1205,11 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   PT_REQUIRE(a->q && a->k && a->v && a->pool && a->page_table && a->out, "pt_tree_attn: null pointer argument");
   PT_REQUIRE(a->q_ld >= a->n_head * a->dim && a->out_ld >= a->n_head * a->vdim && a->kv_ld >= a->n_kv * std::max(a->dim, a->vdim),
              "pt_tree_attn: row strides q %d, kv %d, out %d too small", a->q_ld, a->kv_ld, a->out_ld);
-  PT_REQUIRE(a->window >= 0 && a->softcap >= 0.f, "pt_tree_attn: window=%d softcap=%f", a->window, a->softcap);
+  PT_REQUIRE(a->window >= 0 && (a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f)), "pt_tree_attn: window=%d softcap=%g (0, or 1e-20 .. 1e20)", a->window, a->softcap);
   PT_REQUIRE(a->rope_dims >= 0 && a->rope_dims % 2 == 0 && a->rope_dims <= a->dim && (!a->rope_dims || a->rope), "pt_tree_attn: %d rotated dimensions of %d", a->rope_dims, a->dim);
   const long long positions = (long long)a->page_size * a->max_pages;
-  PT_REQUIRE(positions < (1ll << 31) && a->max_len <= positions, "pt_tree_attn: max_len=%d exceeds the %lld positions of the page table", a->max_len, positions);
+  PT_REQUIRE(positions < (1ll << 31) - 1024 && a->max_len <= positions, "pt_tree_attn: max_len=%d exceeds the %lld positions of the page table, or those are 2^31 or nearly", a->max_len,
+             positions);
   ta::Params p{};
   p.n_seq = b.n_seq; p.n_head = a->n_head; p.n_kv = a->n_kv; p.qpk = a->n_head / a->n_kv; p.dim = a->dim; p.vdim = a->vdim;
   p.page = a->page_size; p.max_pages = a->max_pages; p.max_len = a->max_len > 0 ? a->max_len : (int)positions; p.window = a->window;

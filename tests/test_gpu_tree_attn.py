@@ -183,3 +183,44 @@ def test_flags(cuda):
         out = tu.run(s)
         assert s.flag.item() == 14
         tu.check(s, before, out)
+
+
+@pytest.mark.parametrize("dtype,plain", [("bf16", False), ("fp16", False), ("fp16", True), ("fp32", False)])
+def test_a_scale_of_zero_weighs_all_that_is_seen_alike(cuda, dtype, plain):
+    s = tu.batch([20, 7], [150, 700], dtype=DT[dtype], dim=64, seed=13)
+    s.scale = 0.0
+    before = s.cache.pool.clone()
+    tu.check(s, before, tu.run(s, plain=plain))
+    before = s.cache.pool.clone()
+    tu.check(s, before, tu.run(s, softcap=5.0, window=50, plain=plain), softcap=5.0, window=50)
+
+
+def test_two_captured_calls_at_once(cuda):
+    """Graphs on two streams, each with a workspace of its own, many times over: the same bits as one after the other."""
+    from poptransformer_b200 import ops
+    sets = [tu.batch([9, 20], [900, 77], dtype=torch.bfloat16, dim=128, n_kv=2, qpk=4, seed=14, rot=128), tu.batch([31], [2000], dtype=torch.float16, dim=64, n_kv=4, qpk=2, seed=15),
+            tu.batch([12, 3], [300, 40], dtype=torch.float32, dim=80, n_kv=2, qpk=2, seed=16)]
+    want = [tu.run(s).clone() for s in sets]
+    runs = []
+    for s in sets:
+        stream, out = torch.cuda.Stream(), torch.zeros((s.n_tok, s.heads * s.vdim), dtype=s.dtype, device=cuda)
+        ws = ops.tree_attn_workspace(len(s.counts), max(s.counts), s.heads, s.n_kv, s.vdim)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            tu.run(s, out=out, out_ld=out.shape[1], workspace=ws)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                for _ in range(5):
+                    tu.run(s, out=out, out_ld=out.shape[1], workspace=ws)
+        runs.append((stream, graph, out, ws))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for stream, graph, out, _ in runs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for stream, graph, out, _ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (stream, graph, out, _), w, s in zip(runs, want, sets):
+            assert torch.equal(out, w) and s.flag.item() == 0

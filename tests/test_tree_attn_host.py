@@ -40,6 +40,17 @@ def test_tree_attn_refuses(kw, word):
     assert rc == -1 and word in said, said
 
 
+@pytest.mark.parametrize("softcap", [1e-30, 1e30, float("inf"), float("nan")])
+def test_tree_attn_refuses_caps_that_fp32_cannot_divide_by(softcap):
+    rc, said = _attn(softcap=softcap)
+    assert rc == -1 and "softcap" in said, said
+
+
+def test_tree_attn_refuses_positions_that_an_int_cannot_round_up():
+    rc, said = _attn(page_size=(1 << 31) - 512, max_pages=1, max_len=100)
+    assert rc == -1 and "positions" in said, said
+
+
 def _verify(**kw):
     a = _lib.VerifyArgs()
     a.n_seq, a.n_tok, a.dtype, a.vocab, a.logits_ld, a.draft_ld, a.max_path = 2, 8, ops.DT_F32, 100, 100, 100, 4
