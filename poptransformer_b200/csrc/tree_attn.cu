@@ -12,7 +12,8 @@
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
-// Scores, softmax and sums are fp32.
+// Scores, softmax and sums are fp32.  All three in a captured graph: 5 tokens behind 700 positions (32 heads over 8 of 128) 17 us, 16 sequences of 16 tokens behind up to
+// 4000 70 us, 63 tokens behind 60000 182 to 192 us.
 #include <cuda.h>
 
 #include <type_traits>
@@ -387,7 +388,8 @@ __device__ __forceinline__ float tanh_of(float x) {
 // ------------------------------------------------------------------------------------------ any sizes
 // Rows and keys of a tile in shared memory as fp32; thread (ty, tx) has rows 2 ty, 2 ty + 1 and keys tx, tx + 8, .. of the scores, and columns 4 tx + 32 j of
 // the output.  The next keys come in behind the scores, the next values behind the output, four threads a row; fp32 rows of whole 16 bytes by asynchronous copies.
-// What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them.
+// What bounds it: fp32 multiply-adds, six shared loads of 16 bytes for 32 of them; where blocks have two tiles or so, the latency of one warp a scheduler (11 tokens of
+// three sequences behind a window of 512, 16 heads over 4 of 80: 35 us; 73 when rows came in one element after the other).
 constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32, PLAIN_BLOCKS = 2;      // blocks: of an SM
 static size_t plain_smem(int dim, int vdim) { return (size_t)(PROWS + PKEYS) * (dim + 8) * 4 + (size_t)PKEYS * (vdim + 36) * 4 + (size_t)PROWS * (PKEYS + 4) * 4 + PROWS * 8; }
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
