@@ -224,3 +224,12 @@ def test_two_captured_calls_at_once(cuda):
         torch.cuda.synchronize()
         for (stream, graph, out, _), w, s in zip(runs, want, sets):
             assert torch.equal(out, w) and s.flag.item() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("counts,starts", [([63, 40], [40000, 20001]), ([33, 64, 5], [25000, 31000, 70])])
+def test_several_row_tiles_over_the_same_long_cache(cuda, dtype, counts, starts):
+    """Items of several blocks each, two row tiles of tensor cores or eight of fp32 to a kv head."""
+    s = tu.batch(counts, starts, dtype=DT[dtype], dim=64, n_kv=4, qpk=4, rot=64, seed=17)
+    before = s.cache.pool.clone()
+    tu.check(s, before, tu.run(s))
