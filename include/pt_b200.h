@@ -839,7 +839,7 @@ int pt_mlstm(const pt_mlstm_args *args, void *stream);
  *   - sees its ancestors, itself and every cached position, as far as they are less than `window` positions back (0: all; an ancestor
  *     counts by its depth).
  * pool and page_table as in pt_window_attn (grouped heads, key and value widths of their own, at most 256 each); softcap likewise.  A row that
- * no sequence has (from cu[n_seq] on) is neither read nor written.  No slot comes twice in a call, and calls that share a workspace follow one another.  A sequence of more than max_tokens_per_seq tokens (at most 256) sets error_flag to 14,
+ * no sequence has (from cu[n_seq] on) is neither read nor written.  No slot comes twice in a call, and calls that share a workspace follow one another.  A sequence of more than max_tokens_per_seq tokens (at most 256), or of rows that the batch has not, sets error_flag to 14,
  * one whose positions reach max_len to 12: its rows are then left as they were.  A parent that is none sets it to 14 and counts as -1.  Values that a row does
  * not see may be infinite or NaN. */
 typedef struct pt_tree_attn_args {

@@ -12,7 +12,7 @@
 //   tree_plain_kernel     any type, any widths up to 256: fp32 products on the CUDA cores
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
-// Scores, softmax and sums are fp32.  All three in a captured graph: 5 tokens behind 700 positions (32 heads over 8 of 128) 17 us, 16 sequences of 16 tokens behind up to
+// Scores, softmax and sums are fp32.  All three in a captured graph: 5 tokens behind 700 positions (32 heads over 8 of 128) 18 us, 16 sequences of 16 tokens behind up to
 // 4000 70 us, 63 tokens behind 60000 182 to 192 us.
 #include <cuda.h>
 
@@ -37,7 +37,7 @@ template <> __device__ __forceinline__ __half rounded<__half>(float x) { return 
 template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 struct Params {
-  int n_seq, n_head, n_kv, qpk, dim, vdim, page, max_pages, max_len, window, most;
+  int n_seq, n_tok, n_head, n_kv, qpk, dim, vdim, page, max_pages, max_len, window, most;
   int q_ld, kv_ld, out_ld, out_cols, rope_half;
   int rows_tile, keys_tile, extra, blocks; // of an item, of a unit (powers of two); units of an item beside its key tiles; blocks of the attention kernel
   int rows_shift, keys_shift, part_ld;      // part_ld: rows of a part in the workspace
@@ -67,7 +67,7 @@ struct Seq {
 __device__ __forceinline__ Seq sequence(const Params &p, int s) {
   Seq x{p.cu[s], 0, p.start[s]};
   const int n = p.cu[s + 1] - x.row0;
-  if (n > 0 && n <= p.most && x.start >= 0 && x.start <= p.max_len - n) x.n = n;
+  if (n > 0 && n <= p.most && x.row0 >= 0 && x.row0 <= p.n_tok - n && x.start >= 0 && x.start <= p.max_len - n) x.n = n;
   return x;
 }
 struct Span {
@@ -100,7 +100,7 @@ __device__ __noinline__ void write_plan(const Params &p) {
         v = p.n_kv * y.row_tiles * (y.tiles + p.extra);
       } else if (p.error_flag) {
         const int n = p.cu[s + 1] - x.row0;
-        if (n > 0) atomicExch(p.error_flag, n > p.most ? 14 : 12);
+        if (n > 0) atomicExch(p.error_flag, n > p.most || x.row0 < 0 || x.row0 > p.n_tok - n ? 14 : 12);
       }
     }
     int t = v;
@@ -1163,7 +1163,8 @@ template <typename T> static int run(Params &p, bool tensor, cudaStream_t st) {
   // (an odd number of eights: rows of the same column of parts lie apart by no power of two)
   p.part_ld = (std::min(tensor ? TROWS : PROWS, p.most * p.qpk) + 7) / 8 * 8 | 8;
   if (tensor) {
-    // (A piece beside its tiles costs about as much as two of them: queries in, the last weights and products, the output.)
+    // (A piece beside its tiles costs about as much as two of them: queries in, the last weights and products, the output.  19 calls of all sizes, on average: 23.2 us; with
+    // one, three or four 23.4.)
     p.rows_tile = TROWS; p.keys_tile = TKEYS; p.rows_shift = p.keys_shift = 7; p.extra = 2; p.blocks = sm_count();
     if constexpr (!std::is_same<T, float>::value) PT_CUDA(launch_early(tree_prep_kernel<T, true>, prep, PREP_THREADS, 0, st, p));
   } else {
@@ -1213,7 +1214,7 @@ extern "C" int pt_tree_attn(const pt_tree_attn_args *a, void *stream) {
   PT_REQUIRE(positions < (1ll << 31) - 1024 && a->max_len <= positions, "pt_tree_attn: max_len=%d exceeds the %lld positions of the page table, or those are 2^31 or nearly", a->max_len,
              positions);
   ta::Params p{};
-  p.n_seq = b.n_seq; p.n_head = a->n_head; p.n_kv = a->n_kv; p.qpk = a->n_head / a->n_kv; p.dim = a->dim; p.vdim = a->vdim;
+  p.n_seq = b.n_seq; p.n_tok = b.n_tok; p.n_head = a->n_head; p.n_kv = a->n_kv; p.qpk = a->n_head / a->n_kv; p.dim = a->dim; p.vdim = a->vdim;
   p.page = a->page_size; p.max_pages = a->max_pages; p.max_len = a->max_len > 0 ? a->max_len : (int)positions; p.window = a->window;
   p.most = a->max_tokens_per_seq > 0 ? a->max_tokens_per_seq : b.n_tok;
   PT_REQUIRE(p.most <= ta::MAX_NODES, "pt_tree_attn: %d tokens of one sequence (at most %d)", p.most, ta::MAX_NODES);

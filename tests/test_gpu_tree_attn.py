@@ -233,3 +233,16 @@ def test_several_row_tiles_over_the_same_long_cache(cuda, dtype, counts, starts)
     s = tu.batch(counts, starts, dtype=DT[dtype], dim=64, n_kv=4, qpk=4, rot=64, seed=17)
     before = s.cache.pool.clone()
     tu.check(s, before, tu.run(s))
+
+
+@pytest.mark.parametrize("dtype,plain", [("bf16", False), ("fp32", True)])
+def test_rows_that_the_batch_has_not(cuda, dtype, plain):
+    """A sequence that ends behind the batch's rows is left alone, and said."""
+    s = tu.batch([5, 9], [100, 20], dtype=DT[dtype], dim=64, seed=18)
+    before = s.cache.pool.clone()
+    s.cu_d[2] = s.n_tok + 3
+    out = tu.run(s, most=12, plain=plain)
+    assert s.flag.item() == 14 and (out[5:] == 7).all()
+    assert torch.equal(tu._pages(s, s.cache.pool, 1, 29)[0], tu._pages(s, before, 1, 29)[0])
+    ref, tol, _ = tu.reference(s, before)
+    assert ((out.double() - ref).abs()[:5] <= tol[:5]).all()
