@@ -582,7 +582,9 @@ constexpr int RING_BYTES = 192 * 1024, O_COL = 256, Q_COL = 384, Q_LOW = 64;    
 constexpr float RAISE = 8.f;
 
 struct TcShared {
-  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, landed, drained;
+  // landed: by slot, like full.  A slot is sent for again when its products are done, which wait for both copying warps: so both have seen its phase before the next
+  // can begin.  (One barrier for all slots had no such bound: the first warp could go on by two phases while the second was still at a tile.)
+  uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], landed[MAX_SLOTS], s_full[2], p_full[2], o_done[2], q_full, drained;
   uint32_t tmem;               // where the tensor memory begins (at 0: all of it is ours)
   volatile int abort;
   float top[2][2][TROWS], sum[2][2][TROWS];      // of a half of the keys: by tile, by piece (a warp may be one ahead of its partner)
@@ -667,6 +669,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     for (int i = 0; i < slots; ++i) {
       mbar_init(tc::sa(&sm.full[i]), COPY_WARPS * 32);
       mbar_init(tc::sa(&sm.empty[i]), 1);
+      mbar_init(tc::sa(&sm.landed[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tc::sa(&sm.s_full[i]), 1);
@@ -674,7 +677,6 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
       mbar_init(tc::sa(&sm.o_done[i]), 1);
     }
     mbar_init(tc::sa(&sm.q_full), SOFT_WARPS);
-    mbar_init(tc::sa(&sm.landed), 1);
     mbar_init(tc::sa(&sm.drained), 1);
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -693,8 +695,9 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     const int w = warp - SOFT_WARPS;
     const int box = p.box, boxes = box ? TKEYS / box : 0;   // rows of a box, and how many make a tile
     const bool one = tc::elect_one();
-    int slot = 0, phase = 1, e = 0, pieces = 0, fixed = 0;  // where the next tile goes; tiles asked for; tiles of values gone over
-    bool ok = true;
+    int slot = 0, phase = 1, e = 0, pieces = 0;             // where the next tile goes; tiles asked for
+    uint32_t fixed = 0;                                     // by slot: the phase of `landed` that the next tile of values to be gone over has there
+    bool ok = true, flying = false;                         // flying: a tile that was given up has not landed
     for (Piece k = next_piece(p, cursor); k.nt && ok; k = next_piece(p, cursor), ++pieces) {
       const Seq x = k.x;
       const int *table = p.page_table + (size_t)k.table * p.max_pages;
@@ -718,7 +721,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
           const int dims = kv ? p.vdim : p.dim, blocks = kv ? vblocks : kblocks, have = dims / 8, pad = (dims + 15) / 16 * 2;
           const bool look = kv && part;                     // what is seen in part
           if (box) {
-            uint64_t &bar = look ? sm.landed : sm.full[slot];
+            uint64_t &bar = look ? sm.landed[slot] : sm.full[slot];
             if (w == 0) {
               if (tc::elect_one()) mbar_expect_tx(tc::sa(&bar), blocks * TKEYS * 128);
               __syncwarp();
@@ -736,7 +739,8 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
               if (w || !one) mbar_arrive(tc::sa(&bar));
               continue;
             }
-            if (!wait(sm.landed, fixed++ & 1)) { ok = false; break; }
+            if (!wait(sm.landed[slot], fixed >> slot & 1)) { ok = false; flying = true; break; }
+            fixed ^= 1u << slot;
           } else {
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
@@ -787,7 +791,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (w == 0 && box) {
       mbar_wait_ring(tc::sa(&sm.full[0]), e, slots);
-      if (!ok && fixed) mbar_wait_all(tc::sa(&sm.landed), (fixed - 1) & 1);
+      if (flying) mbar_wait_all(tc::sa(&sm.landed[slot]), fixed >> slot & 1);
     }
   } else if (warp == MMA_WARP) {
     // ---- products.  (What they take is the same in all lanes, and the compiler knows it: counters that go up by known steps, in loops whose bounds come
