@@ -13,6 +13,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
   return pred != 0;
 }
+// Every kernel that allocates tensor memory asks for at least TMEM_SHARED bytes of shared memory, of the SM_SHARED that an SM has (BLOCK_SHARED more for each block).  One
+// that lets its successor start before it has its columns asks for so much that no other of these fits beside it: a block of the successor would keep columns while it
+// waits for this kernel, which waits for them.
+constexpr int TMEM_SHARED = 76 * 1024, SM_SHARED = 228 * 1024, BLOCK_SHARED = 1024;
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");

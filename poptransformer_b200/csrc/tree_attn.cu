@@ -1062,7 +1062,8 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TENSOR_THREADS
     tc::tmem_dealloc(sm.tmem, 512);
   }
 }
-static size_t tensor_smem() { return 1024 + RING_BYTES + sizeof(TcShared); }
+constexpr size_t tensor_smem() { return 1024 + RING_BYTES + sizeof(TcShared); }
+static_assert(tensor_smem() + tc::TMEM_SHARED + 2 * tc::BLOCK_SHARED > tc::SM_SHARED, "the next kernel starts before a block has its columns: none that allocates some may fit beside it");
 
 // ------------------------------------------------------------------------------------------ parts of an item
 // Block (x: eight rows of an item, by the most that a sequence can have; y: sequence): adds up the parts in the order of the keys, in one pass with a running
