@@ -73,12 +73,13 @@ __device__ __forceinline__ double widened(float x) {
   return __hiloint2double((b >> 3 & (int)0x8fffffff) + 0x38000000, b << 29);
 }
 // 2^(c x - K) for c x <= K: n = the whole number next to c x - K, r = c x - K - n without a rounding but its own, 2^r by its series up to r^10 (|r| <= 1/2: the
-// next term is below 2^-42).  0 for x <= least, where c x - K is about -1000, which -inf is.  (Fifteen 64-bit operations, of which an SM does 64 a cycle, and no
+// next term is below 2^-42).  0 for x <= least, where c x - K is -1000 or less, which -inf is.  (least is rounded down: floats above it are those above (K - 1000) / c,
+// however near that lies to the largest logit.  Fifteen 64-bit operations, of which an SM does 64 a cycle, and no
 // table: look-ups at random places of shared memory, or by shuffles, cost more than the terms that they save.)
 struct Scale {
   double c, shift;      // 1.5 2^52 - K: the last bit is 1
   float least;
-  __device__ __forceinline__ Scale(double c, double k) : c(c), shift(6755399441055744.0 - k), least((float)((k - 1000.0) / c)) {}
+  __device__ __forceinline__ Scale(double c, double k) : c(c), shift(6755399441055744.0 - k) { least = __double2float_rd((k - 1000.0) / c); }
   __device__ __forceinline__ double operator()(float x) const {
     const double v = widened(x), t = fma(v, c, shift), r = fma(v, c, shift - t);
     double e = fma(r, kSeries[10], kSeries[9]);
@@ -481,8 +482,8 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) verify_kerne
           if (lane >= o) upto += y;
         }
         const unsigned some = __ballot_sync(0xffffffffu, v > 0.0), over_it = __ballot_sync(0xffffffffu, v > 0.0 && from + upto > want);
-        const int pick = over_it ? __ffs(over_it) - 1 : 31 - __clz(some);
-        before = from + __shfl_sync(0xffffffffu, upto - v, max(pick, 0));
+        const int pick = max(over_it ? __ffs(over_it) - 1 : 31 - __clz(some), 0);      // (one in any case: some block has to write)
+        before = from + __shfl_sync(0xffffffffu, upto - v, pick);
         return pick;
       };
       double before, c;

@@ -1,0 +1,26 @@
+"""Verification at temperatures next to 0, random numbers outside [0, 1) and large vocabularies, against the rules in 64 bits (test_gpu_verify)."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_verify import compare, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# A weight is 2^(logit log2(e) / T - K).  From |logit| / T = 1e10 or so neighbouring floats are further apart than all that has weight.
+@pytest.mark.parametrize("t", [1e-6, 1e-8, 1e-9, 1e-10, 1e-11, 3e-12, 1e-13])
+@pytest.mark.parametrize("size", [5.0, 20.0, 30.0, 130.0, 200.0, -5.0, -200.0])
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_temperatures_next_to_zero(cuda, t, size, kind):
+    """All weight is the largest logit's, whatever its size: it is accepted where it is drafted, and drawn."""
+    counts = [5, 9, 1]
+    logits, parents, token, q, u, u_next = inputs(cuda, counts, kind, 1500, torch.float32, 31)
+    logits = logits - logits.amax(-1, keepdim=True) + size
+    logits[1, [7, 1400]] = logits[1].max()            # (two share it)
+    for i in (1, 2, 6):
+        token[i] = int(logits[i - 1].argmax())
+    for draft in (q, None):
+        path, count, said = compare(logits, counts, parents, token, draft, [t] * 3, u, u_next, 9, chain=kind == "chain")
+        assert int(said[2, 0]) == int(logits[14].argmax())
