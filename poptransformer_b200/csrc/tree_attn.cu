@@ -213,7 +213,7 @@ template <> struct Half2<__half> {
     const float2 back = wide(hi);
     lo = pack(a - back.x, b - back.y);
   }
-  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u; }
+  static constexpr uint32_t kExponent = 0x7c00u;
 };
 template <> struct Half2<__nv_bfloat16> {
   static constexpr float kBias = 0.f;
@@ -225,8 +225,17 @@ template <> struct Half2<__nv_bfloat16> {
     hi = __byte_perm(x, y, 0x7632);
     lo = __byte_perm(__float_as_uint(a - __uint_as_float(x & 0xffff0000u)), __float_as_uint(b - __uint_as_float(y & 0xffff0000u)), 0x7632);
   }
-  static __device__ __forceinline__ bool bad(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
+  static constexpr uint32_t kExponent = 0x7f80u;
 };
+// Of a pair: whether a value is infinite or NaN, and the pair with zeros for those.
+template <typename T> __device__ __forceinline__ bool bad(uint32_t v) {
+  constexpr uint32_t e = Half2<T>::kExponent;
+  return (v & e) == e || (v & e << 16) == e << 16;
+}
+template <typename T> __device__ __forceinline__ uint32_t finite(uint32_t v) {
+  constexpr uint32_t e = Half2<T>::kExponent;
+  return ((v & e) == e ? 0u : v & 0xffffu) | ((v & e << 16) == e << 16 ? 0u : v & 0xffff0000u);
+}
 // Eight neighbouring dimensions d .. d + 7 of a head's row, rotated by the angles of `pos`; `own`: their values.
 template <typename T> __device__ __forceinline__ void turn8(const Params &p, const T *src, int d, int pos, const uint4 &own, float2 (&y)[4]) {
   const int h = p.rope_half;
@@ -588,9 +597,8 @@ struct TcShared {
   uint32_t tmem;               // where the tensor memory begins (at 0: all of it is ours)
   volatile int abort;
   float top[2][2][TROWS], sum[2][2][TROWS];      // of a half of the keys: by tile, by piece (a warp may be one ahead of its partner)
-  // Values that are not finite and that not every row sees, by piece: drafted tokens, and positions from the lowest of any row's window on.  They are
-  // zeroed in shared memory (0 * inf would reach rows that do not see them), and the rows that do see them become NaN.
-  uint32_t bad[8][2 * WORDS];
+  // Whether a piece has values that are not finite and that not every row sees: they are zeroed in shared memory (0 * inf would reach rows that do not see them),
+  // and infinite_values gives them back to the rows that do.
   int any_bad[8];
 };
 
@@ -652,6 +660,28 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
   }
 };
 
+// Eight columns c .. c + 7 of a row's output, of keys first .. last - 1: those with an infinite or NaN value that the row sees become the sum of these.  (What the products made of
+// them is none: a weight comes in two parts, of which the second may be 0 or negative, and where not all rows see a value it was 0.)
+template <typename T> __device__ __noinline__ void infinite_values(const Params &p, const int *table, int g, int first, int last, int start, const uint32_t *seen, int c, float (&v)[8]) {
+  float sum[8] = {};
+  for (int j = max(first, 0); j < last; ++j) {
+    const int d = j - start, page = j / p.page;
+    if (d >= 0 && !(seen[d >> 5] >> (d & 31) & 1)) continue;
+    const uint4 w = *reinterpret_cast<const uint4 *>(v_page<T>(p, table[page], g) + (size_t)(j - page * p.page) * p.vdim + c);
+    const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!bad<T>(y[i])) continue;
+      const float2 z = Half2<T>::wide(y[i]);
+      if (!isfinite(z.x)) sum[2 * i] += z.x;
+      if (!isfinite(z.y)) sum[2 * i + 1] += z.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (sum[i] != 0.f) v[i] = sum[i];
+}
+
 // A piece's tile that some rows see in part: keys from `start` on are drafted, those in front of start + n - window are not seen by all.
 __device__ __forceinline__ bool partial(const Params &p, const Seq &x, int j0) { return j0 + TKEYS > x.start || (p.window && x.start + x.n - 1 - j0 >= p.window); }
 // CAP: scores go through cap tanh(score / cap).  As cap (1 - 2 / (e^2x + 1)) alone that is off by cap 2^-21, whatever the score: up to LOW_CAP less than what the weights lose
@@ -686,7 +716,6 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
     sm.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = tid; i < 8 * 2 * WORDS; i += TENSOR_THREADS) (&sm.bad[0][0])[i] = 0;
   if (tid < 8) sm.any_bad[tid] = 0;
   if (warp == MMA_WARP) tc::tmem_alloc(tc::sa(&sm.tmem), 512);
   tc::fence_before();
@@ -763,7 +792,7 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
             asm volatile("cp.async.wait_all;" ::: "memory");
           }
           if (look) {
-            // rows that the sequence has not: zeros; rows that not all see: finite, or noted
+            // rows that the sequence has not: zeros; rows that not all see: made finite, and said
             const int cols = blocks * 8, c = lane % cols, r1 = w * 64 + 64;
             int r = w * 64 + lane / cols;
             if (!p.window) r += max(0, (x.start - j0 - r) / (32 / cols)) * (32 / cols);      // (those in front all see)
@@ -775,16 +804,12 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
               const bool in = key >= lowest && key < last;
               if (in) {
                 const uint4 v = *at;
-                if (!Half2<T>::bad(v.x) && !Half2<T>::bad(v.y) && !Half2<T>::bad(v.z) && !Half2<T>::bad(v.w)) continue;
-                if (d >= 0 || p.window) {
-                  const int bit = d >= 0 ? d : MAX_NODES + b;
-                  atomicOr(&sm.bad[pieces & 7][bit >> 5], 1u << (bit & 31));
-                  sm.any_bad[pieces & 7] = 1;
-                } else {
-                  continue;
-                }
+                if ((!bad<T>(v.x) && !bad<T>(v.y) && !bad<T>(v.z) && !bad<T>(v.w)) || (d < 0 && !p.window)) continue;
+                sm.any_bad[pieces & 7] = 1;
+                *at = make_uint4(finite<T>(v.x), finite<T>(v.y), finite<T>(v.z), finite<T>(v.w));
+              } else {
+                *at = make_uint4(0u, 0u, 0u, 0u);
               }
-              *at = make_uint4(0u, 0u, 0u, 0u);
             }
           }
           tc::fence_operands();
@@ -1011,33 +1036,35 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
       sm.sum[pieces & 1][half][row] = l;
       meet();
       if (tid == 0) sm.any_bad[(pieces + 7) & 7] = 0;       // (of the piece before: everybody is past it)
-      if (tid < 2 * WORDS) sm.bad[(pieces + 7) & 7][tid] = 0;
       output_of(n_o - 1);
       tc::fence_after();
       if (live) {
-        float sum = sm.sum[pieces & 1][0][row] + sm.sum[pieces & 1][1][row];
-        if (sm.any_bad[pieces & 7]) {
-          const uint32_t *bad = sm.bad[pieces & 7];
-          bool hit = false;
-          for (int z = 0; z < WORDS; ++z) hit |= (bad[z] & seen[z]) != 0;
-          if (p.window) {
-            const int low = x.start + depth - p.window + 1 - max(0, x.start - p.window + 1);      // the first of those positions that the token sees
-            for (int z = 0; z < MAX_NODES; ++z) hit |= z >= low && (bad[WORDS + (z >> 5)] >> (z & 31) & 1);
-          }
-          if (hit) sum = NAN;
-        }
-        const bool store = row < rows;
+        const float sum = sm.sum[pieces & 1][0][row] + sm.sum[pieces & 1][1][row];
+        const bool any_bad = sm.any_bad[pieces & 7] != 0, store = row < rows;
         const float inv = k.whole ? 1.0f / sum : 1.0f;
         T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + node) * p.out_ld + (size_t)head * p.vdim;
         if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * p.part_ld + row] = make_float2(m, sum);
 #pragma unroll 1
         for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
           uint32_t v[16];
+          __syncwarp();
           tc::tmem_ld16(O + c, v);
           if (!store) continue;
 #pragma unroll
           for (int z = 0; z < 16; z += 8) {
             if (c + z >= p.vdim) break;
+            bool look = any_bad;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) look |= isnan(__uint_as_float(v[z + b]));
+            if (look && !isnan(sum)) {                      // (where the sum of the weights is NaN all is)
+              float w[8];
+#pragma unroll
+              for (int b = 0; b < 8; ++b) w[b] = __uint_as_float(v[z + b]);
+              const int low = p.window ? x.start + depth - p.window + 1 : 0;
+              infinite_values<T>(p, p.page_table + (size_t)k.table * p.max_pages, k.g, max(k.t0 * TKEYS, low), min((k.t0 + k.nt) * TKEYS, x.start + x.n), x.start, seen, c + z, w);
+#pragma unroll
+              for (int b = 0; b < 8; ++b) v[z + b] = __float_as_uint(w[b]);
+            }
             if (k.whole) {
               uint32_t y[4];
 #pragma unroll
