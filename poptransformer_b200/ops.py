@@ -795,15 +795,23 @@ class PagedKVCache:
 
     def __init__(self, rows, n_kv, head_dim, max_len, page_size=64, device="cuda", page_table=None, extra_pages=0, v_dim=None, dtype=torch.float16,
                  n_pages=None, pool=None):
-        """pool: memory to use, for instance a layer's part of one tensor (its first dimension is the pages)."""
+        """pool: memory to use, for instance a layer's part of one tensor.  Its first dimension is the pages: n_pages of them at least, or as many as the default
+        page table names (which pages a page_table of the caller's names is the caller's to know)."""
         self.rows, self.n_kv, self.head_dim, self.page_size = rows, n_kv, head_dim, page_size
         self.v_dim = head_dim if v_dim is None else v_dim
         self.max_len = max_len
         self.max_pages = (max_len + page_size - 1) // page_size
+        pages_given = n_pages is not None
         n_pages = (rows * self.max_pages if n_pages is None else n_pages) + extra_pages
         shape = (n_pages, 2, n_kv, page_size, head_dim) if self.v_dim == head_dim else (n_pages, n_kv * page_size * (head_dim + self.v_dim))
-        if pool is not None and (pool.dtype != dtype or not pool.is_contiguous() or pool[0].numel() != n_kv * page_size * (head_dim + self.v_dim)):
-            raise PtError(f"PagedKVCache: pool {pool.dtype} {tuple(pool.shape)}, expected contiguous {dtype} pages of {n_kv * page_size * (head_dim + self.v_dim)} elements")
+        if pool is not None:
+            elements, wanted = n_kv * page_size * (head_dim + self.v_dim), torch.device(device)
+            if pool.dtype != dtype or not pool.is_contiguous() or pool.dim() == 0 or pool.numel() != pool.shape[0] * elements:
+                raise PtError(f"PagedKVCache: pool {pool.dtype} {tuple(pool.shape)}, expected contiguous {dtype} pages of {elements} elements")
+            if pool.shape[0] < (n_pages if pages_given or page_table is None else 1):
+                raise PtError(f"PagedKVCache: a pool of {pool.shape[0]} pages, {n_pages} are wanted")
+            if pool.device.type != wanted.type or wanted.index not in (None, pool.device.index) or page_table is not None and page_table.device != pool.device:
+                raise PtError(f"PagedKVCache: pool on {pool.device}, wanted on {wanted}" + ("" if page_table is None else f" with its page table on {page_table.device}"))
         self.pool = torch.zeros(shape, dtype=dtype, device=device) if pool is None else pool
         if page_table is None:
             page_table = torch.arange(rows * self.max_pages, dtype=torch.int32, device=device).reshape(rows, self.max_pages)
