@@ -909,8 +909,8 @@ int pt_verify_drafts(const pt_verify_args *args, void *stream);
  * pt_kv_copy_pages: page dst[i] <- page src[i] of every pool, i < n.  No page is written twice or both read and written in a call, unless it is its
  *   own source.  Pairs with a negative page are left out; a page from n_pages on sets error_flag to 12 and is left out.
  * pt_kv_move_rows: position start[s] + i <- position start[s] + path[s][i], i < count[s] (device arrays, as pt_verify_drafts writes them): the accepted
- *   tokens of a sequence follow its cached positions.  A path that does not increase, or leaves the sequence's new tokens, sets error_flag to 14, positions
- *   outside the table 12; the sequence is then left as it was. */
+ *   tokens of a sequence follow its cached positions.  A path that does not increase, leaves the sequence's new tokens or has more than 512 rows sets error_flag to 14,
+ *   positions outside the table 12; the sequence is then left as it was. */
 typedef struct pt_kv_pool {
   void *pool;
   int n_kv, dim, vdim, elem_bytes;

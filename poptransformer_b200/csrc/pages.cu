@@ -7,7 +7,7 @@
 namespace pt {
 namespace pg {
 
-constexpr int MAX_POOLS = 64, THREADS = 256, MAX_PATH = 256;
+constexpr int MAX_POOLS = 64, THREADS = 256, MAX_PATH = 512;      // (a path: as long as verification makes them)
 
 struct Pools {
   char *pool[MAX_POOLS];
