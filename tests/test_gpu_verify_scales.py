@@ -24,3 +24,17 @@ def test_temperatures_next_to_zero(cuda, t, size, kind):
     for draft in (q, None):
         path, count, said = compare(logits, counts, parents, token, draft, [t] * 3, u, u_next, 9, chain=kind == "chain")
         assert int(said[2, 0]) == int(logits[14].argmax())
+
+
+@pytest.mark.parametrize("vocab", [196000, 256000, 262141, 262144, 262145])
+@pytest.mark.parametrize("mode,dtype", [("drawn", torch.float32), ("chosen", torch.bfloat16), ("greedy", torch.float16)])
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_vocabularies_that_fill_a_cluster(cuda, vocab, mode, dtype, kind):
+    """The weights of sixteen blocks' slices fill their shared memory, or just do not fit any more."""
+    counts = [4, 7, 1]
+    logits, parents, token, q, u, u_next = inputs(cuda, counts, kind, vocab, dtype, 33)
+    token[2] = int(logits[1].argmax())
+    token[5] = vocab - 1
+    logits[4, vocab - 1] = logits[4].max() + 1
+    temps = None if mode == "greedy" else [1.0, 0.7, 1.3]
+    compare(logits, counts, parents, token, q if mode == "drawn" else None, temps, u, u_next, 7, chain=kind == "chain")
