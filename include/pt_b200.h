@@ -886,7 +886,7 @@ int pt_tree_attn(const pt_tree_attn_args *args, void *stream);
  * A path of max_path rows is not followed further.  Logits may be -inf, and NaN counts as that; equal infinities share all the weight.  A
  * row that is -inf everywhere accepts nothing and its token is -1.  Sums, residuals and the drawing are in 64 bits.
  * A token outside the vocabulary, a parent that is none, or a row behind the first 512 of a sequence is never accepted.  A random number of 1 or more
- * draws like the largest below 1. */
+ * draws like the largest below 1, and accepts nothing that has no weight left. */
 typedef struct pt_verify_args {
   int n_seq, n_tok;
   const int32_t *cu;      /* [n_seq + 1]; a sequence without rows has count 0        */

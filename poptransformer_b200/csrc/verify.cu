@@ -408,7 +408,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 2) verify_kerne
         for (int i = 0; i < min(32, kids - k0); ++i) {
           const double pi = __shfl_sync(0xffffffffu, px, i);
           if (__shfl_sync(0xffffffffu, u, i) * Z < pi) { stands = tried = k0 + i; break; }
-          Z -= pi;
+          Z = fmax(Z - pi, 0.0);      // (below 0 by a rounding, a random number of 1 or more would accept what has no weight)
         }
       }
     if (!q && stands < 0) tried = kids;

@@ -38,3 +38,20 @@ def test_vocabularies_that_fill_a_cluster(cuda, vocab, mode, dtype, kind):
     logits[4, vocab - 1] = logits[4].max() + 1
     temps = None if mode == "greedy" else [1.0, 0.7, 1.3]
     compare(logits, counts, parents, token, q if mode == "drawn" else None, temps, u, u_next, 7, chain=kind == "chain")
+
+
+@pytest.mark.parametrize("vocab", [3, 700, 256000])
+def test_random_numbers_of_one_and_more(cuda, vocab):
+    """They accept no token that has no weight left, and draw like the largest below 1."""
+    from poptransformer_b200 import ops
+    logits = torch.full((4, vocab), -math.inf, device=cuda)
+    p = torch.rand(300, generator=torch.Generator().manual_seed(34)).tolist()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)
+    for k in range(0, 300, 2):
+        logits[0, 0], logits[0, 1] = math.log(p[k] + 1e-3), math.log(p[k + 1] + 1e-3)
+        said = []
+        for u in (1.5, 1.0000002, 1.0):                # (the two tokens are all of p; the third has none)
+            _, count, tok, _ = ops.verify_drafts(logits, i32([0, 4]), i32([0, 0, 1, 2]), i32([-1, 0, 0, 0]), max_path=2, temperature=torch.ones(1, device=cuda),
+                                                 uniform=torch.full((4,), u, device=cuda), uniform_next=torch.full((1,), u, device=cuda))
+            said.append((int(count[0]), int(tok[0, 0])))
+        assert all(t in (0, 1) for _, t in said), (k, said)
