@@ -861,7 +861,7 @@ typedef struct pt_tree_attn_args {
   const float *rope;
   void *out;              /* [n_tok, out_ld], columns n_head * vdim .. out_cols - 1 are zeroed (0 = out_ld) */
   int out_ld, out_cols;
-  int max_tokens_per_seq; /* most drafted tokens of one sequence (0 = n_tok)         */
+  int max_tokens_per_seq; /* most drafted tokens of one sequence, up to 256 (0 = n_tok) */
   int plain;              /* 1: the kernel for any sizes, whatever the shape         */
   void *workspace;        /* pt_tree_attn_workspace_bytes, 16-byte aligned; what it holds does not matter */
   size_t workspace_bytes;

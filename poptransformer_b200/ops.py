@@ -481,7 +481,8 @@ def tree_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, parent=None,
               error_flag=None, out_cols=0, plain=False):
     """Attention of drafted tokens, a tree of them behind every sequence of `view`, over a paged cache (see pt_tree_attn).  qkv rows hold [q | k | v] of a
     token; k and v are appended at the rows' own positions, the rotation and the window go by a token's depth.  parent: int32 [n_tok], counted
-    from the first token of a sequence, -1 for those that follow its cached positions (None: every token follows the one before)."""
+    from the first token of a sequence, -1 for those that follow its cached positions (None: every token follows the one before).  max_tokens_per_seq: the most
+    that a sequence has, as the workspace was asked for (0: all of the batch's, or 256, which is the most there may be)."""
     pool, table, dtype = cache.pool, cache.page_table, qkv.dtype
     if pool.dtype != dtype or out.dtype != dtype:
         raise PtError(f"tree_attn: rows {dtype}, cache {pool.dtype}, out {out.dtype}: one type is wanted")
@@ -492,7 +493,7 @@ def tree_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, parent=None,
     k = q + n_head * dim * es
     # (In the order of the structure: setting its fields one by one takes 4 us more.)
     a = TreeAttnArgs(view, dtype_code(dtype), n_head, n_kv, dim, vdim, cache.page_size, table.shape[1], cache.max_len, window, scale, softcap, _ptr(parent), q, qkv_ld, k, k + n_kv * dim * es,
-                     qkv_ld, _ptr(pool), _ptr(table), rope_dims, _ptr(rope), _ptr(out), out_ld, out_cols, max_tokens_per_seq, 1 if plain else 0, _ptr(workspace),
+                     qkv_ld, _ptr(pool), _ptr(table), rope_dims, _ptr(rope), _ptr(out), out_ld, out_cols, max_tokens_per_seq or min(view.n_tok, 256), 1 if plain else 0, _ptr(workspace),
                      0 if workspace is None else workspace.numel(), _ptr(error_flag))
     check(_lib.lib().pt_tree_attn(ctypes.byref(a), _stream()), "pt_tree_attn")
     return out
