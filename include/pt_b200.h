@@ -884,7 +884,8 @@ int pt_tree_attn(const pt_tree_attn_args *args, void *stream);
  * path[s] = the accepted rows (0 = the root, counted from cu[s]), count[s] of them; token[s] = the tokens behind each of them, the last one
  * drawn; logprob[s] (optional) = their log p (temperature 0: of temperature 1).  The rest of a row of max_path entries is -1 (logprob 0).
  * A path of max_path rows is not followed further.  Logits may be -inf, and NaN counts as that; equal infinities share all the weight.  A
- * row that is -inf everywhere accepts nothing and its token is -1.  Sums, residuals and the drawing are in 64 bits.
+ * row that is -inf everywhere accepts nothing and its token is -1.  Sums, residuals and the drawing are in 64 bits, of
+ * weights that are right to 2^-42: a decision can differ from exact arithmetic where a random number lies within about 1e-12 of a border.
  * A token outside the vocabulary, a parent that is none, or a row behind the first 512 of a sequence is never accepted.  A random number of 1 or more
  * draws like the largest below 1, and accepts nothing that has no weight left. */
 typedef struct pt_verify_args {

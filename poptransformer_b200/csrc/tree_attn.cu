@@ -401,6 +401,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 // three sequences behind a window of 512, 16 heads over 4 of 80: 35 us; 73 when rows came in one element after the other).
 constexpr int PLAIN_THREADS = 128, PROWS = 32, PKEYS = 32, PLAIN_BLOCKS = 2;      // blocks: of an SM
 static size_t plain_smem(int dim, int vdim) { return (size_t)(PROWS + PKEYS) * (dim + 8) * 4 + (size_t)PKEYS * (vdim + 36) * 4 + (size_t)PROWS * (PKEYS + 4) * 4 + PROWS * 8; }
+// 16 bytes, zeros where bytes is 0.
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -614,7 +615,7 @@ __device__ __forceinline__ uint32_t product_desc(bool bf16, int n, bool b_by_row
 }
 // Byte of 16-byte unit c of row r of a tile of rows of 128 swizzled bytes (blocks of 128 rows).
 __device__ __forceinline__ uint32_t swizzled(int r, int c) { return (uint32_t)((c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
-// 16 bytes, zeros where bytes is 0.
+// A box of a tensor map into shared memory; its bytes arrive on `bar`.
 __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t &bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(tc::sa(&bar)), "r"(x), "r"(y), "r"(z)
                : "memory");

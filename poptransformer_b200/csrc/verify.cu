@@ -6,7 +6,7 @@
 // number tells a row's whole past.  Without q the tokens that were refused leave p.  The last token is the first whose running sum of r exceeds
 // u Z.  That the tokens follow the target's distribution whatever the draft is the point of these rules, and it holds as far as sums and
 // residuals are exact: p - q cancels, and a step of the running sum can be 1e-6 of Z while a vocabulary of fp32 roundings drifts by 1e-7.
-// They are kept in 64 bits.
+// They are kept in 64 bits, of weights that are right to 2^-42.
 //
 // A cluster of blocks has one sequence and walks down its path: it reads only the rows that the path reaches, each once.  Every block has a slice of the
 // vocabulary, every warp a part of the slice in order, whose weights stay in shared memory in 64 bits.  A part's weights are 2^(z - K), z = logit log2(e) / T and K
@@ -66,7 +66,7 @@ struct Shared {
 };
 
 // ln(2)^n / n!
-__constant__ double kSeries[12] = {1.0, 0.6931471805599453, 0.24022650695910072, 0.05550410866482158, 0.009618129107628477, 0.0013333558146428443, 0.0001540353039338161, 1.5252733804059841e-05, 1.321548679014431e-06, 1.01780860092397e-07, 7.054911620801123e-09, 4.4455382718708116e-10};
+__constant__ double kSeries[11] = {1.0, 0.6931471805599453, 0.24022650695910072, 0.05550410866482158, 0.009618129107628477, 0.0013333558146428443, 0.0001540353039338161, 1.5252733804059841e-05, 1.321548679014431e-06, 1.01780860092397e-07, 7.054911620801123e-09};
 // A finite float as a double, by its bits: conversions are a quarter as fast as additions.  (0 and what is smaller than 2^-126 becomes something below 2^-126.)
 __device__ __forceinline__ double widened(float x) {
   const int b = __float_as_int(x);
