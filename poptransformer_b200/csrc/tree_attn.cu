@@ -662,20 +662,33 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
 };
 
 // Eight columns c .. c + 7 of a row's output, of keys first .. last - 1: those with an infinite or NaN value that the row sees become the sum of these.  (What the products made of
-// them is none: a weight comes in two parts, of which the second may be 0 or negative, and where not all rows see a value it was 0.)
-template <typename T> __device__ __noinline__ void infinite_values(const Params &p, const int *table, int g, int first, int last, int start, const uint32_t *seen, int c, float (&v)[8]) {
+// them is none: a weight comes in two parts, of which the second may be 0 or negative, and where not all rows see a value it was 0.)  all: look at every key, else only at
+// those that not every row sees, which are the first MAX_NODES from the lowest that any row sees, where there is a window, and the drafted ones.  Four keys are asked for at once:
+// others wait meanwhile, with a limit.
+template <typename T> __device__ __noinline__ void infinite_values(const Params &p, const int *table, int g, int first, int last, int start, const uint32_t *seen, int c, bool all, float (&v)[8]) {
   float sum[8] = {};
-  for (int j = max(first, 0); j < last; ++j) {
-    const int d = j - start, page = j / p.page;
-    if (d >= 0 && !(seen[d >> 5] >> (d & 31) & 1)) continue;
-    const uint4 w = *reinterpret_cast<const uint4 *>(v_page<T>(p, table[page], g) + (size_t)(j - page * p.page) * p.vdim + c);
-    const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+  first = max(first, 0);
+  const int skip = all ? last : p.window ? max(first, max(start - p.window + 1, 0) + MAX_NODES) : first;      // from here to `start` all rows see all
+  for (int j0 = first; j0 < last; j0 += 4) {
+    if (j0 >= skip && j0 < start) j0 = start;
+    uint4 w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!bad<T>(y[i])) continue;
-      const float2 z = Half2<T>::wide(y[i]);
-      if (!isfinite(z.x)) sum[2 * i] += z.x;
-      if (!isfinite(z.y)) sum[2 * i + 1] += z.y;
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u, d = j - start, page = j / p.page;
+      w[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (j < last && (d < 0 || (seen[d >> 5] >> (d & 31) & 1)))
+        w[u] = *reinterpret_cast<const uint4 *>(v_page<T>(p, table[page], g) + (size_t)(j - page * p.page) * p.vdim + c);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t y[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!bad<T>(y[i])) continue;
+        const float2 z = Half2<T>::wide(y[i]);
+        if (!isfinite(z.x)) sum[2 * i] += z.x;
+        if (!isfinite(z.y)) sum[2 * i + 1] += z.y;
+      }
     }
   }
 #pragma unroll
@@ -1054,15 +1067,15 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
 #pragma unroll
           for (int z = 0; z < 16; z += 8) {
             if (c + z >= p.vdim) break;
-            bool look = any_bad;
+            bool all = false;                               // (what came out finite holds no such value of a tile that all rows see)
 #pragma unroll
-            for (int b = 0; b < 8; ++b) look |= isnan(__uint_as_float(v[z + b]));
-            if (look && !isnan(sum)) {                      // (where the sum of the weights is NaN all is)
+            for (int b = 0; b < 8; ++b) all |= !isfinite(__uint_as_float(v[z + b]));
+            if ((any_bad || all) && !isnan(sum)) {          // (where the sum of the weights is NaN all is)
               float w[8];
 #pragma unroll
               for (int b = 0; b < 8; ++b) w[b] = __uint_as_float(v[z + b]);
               const int low = p.window ? x.start + depth - p.window + 1 : 0;
-              infinite_values<T>(p, p.page_table + (size_t)k.table * p.max_pages, k.g, max(k.t0 * TKEYS, low), min((k.t0 + k.nt) * TKEYS, x.start + x.n), x.start, seen, c + z, w);
+              infinite_values<T>(p, p.page_table + (size_t)k.table * p.max_pages, k.g, max(k.t0 * TKEYS, low), min((k.t0 + k.nt) * TKEYS, x.start + x.n), x.start, seen, c + z, all, w);
 #pragma unroll
               for (int b = 0; b < 8; ++b) v[z + b] = __float_as_uint(w[b]);
             }

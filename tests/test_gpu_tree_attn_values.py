@@ -182,3 +182,27 @@ def test_a_bad_query_is_its_own(cuda, dtype, plain):
     got = tu.run(s, plain=plain)
     rows = [r for r in range(27) if r != 5]
     assert torch.equal(got[rows], want[rows]) and got[5].isnan().all()
+
+
+@pytest.mark.parametrize("dtype,plain", KERNELS)
+@pytest.mark.parametrize("window,start", [(0, 120), (300, 120), (300, 400), (600, 400), (40, 1000), (5000, 3000)])
+def test_infinite_values_in_cached_and_drafted_positions_meet(cuda, dtype, plain, window, start):
+    """The same columns of cached positions that all rows see, in tiles that they see whole and in tiles with drafted tokens, and of drafted tokens."""
+    s = tu.batch([24, 5], [start, 9], "tree", dtype=DT[dtype], dim=64, n_kv=1, qpk=2, seed=28)
+    s.scale = 0.02
+    for back, c, x in ((1, 3, math.inf), (20, 4, -math.inf), (20, 5, math.nan), (60, 6, math.inf), (119, 7, math.inf), (250, 8, math.inf), (399, 9, -math.inf)):
+        if back <= start:
+            s.cache.pool[s.table[s.slot[0]][(start - back) // s.page], 1, 0, (start - back) % s.page, c] = x
+    for tok, c, x in ((2, 3, -math.inf), (5, 4, -math.inf), (9, 6, math.inf), (4, 8, -math.inf), (7, 9, math.inf), (11, 40, math.nan)):
+        s.qkv[tok, (s.heads + 1) * 64 + c] = x
+    before = s.cache.pool.clone()
+    want = _expected(s, before, window)
+    assert _values(s, tu.run(s, window=window, plain=plain), want) > 0 and s.flag.item() == 0
+
+
+def test_a_long_cache_of_infinite_values_ends_in_time(cuda):
+    """Every column of every row looks at every key again: no wait runs out meanwhile."""
+    s = tu.batch([40], [200000], "chain", dtype=torch.bfloat16, dim=128, n_kv=8, qpk=4, seed=29)
+    s.cache.pool[:, 1, :, 5] = math.inf
+    out = tu.run(s)
+    assert s.flag.item() == 0 and (out == math.inf).all()
