@@ -661,39 +661,46 @@ struct Waits {          // a role's bounded waits: the whole warp goes the same 
   }
 };
 
-// Eight columns c .. c + 7 of a row's output, of keys first .. last - 1: those with an infinite or NaN value that the row sees become the sum of these.  (What the products made of
-// them is none: a weight comes in two parts, of which the second may be 0 or negative, and where not all rows see a value it was 0.)  all: look at every key, else only at
-// those that not every row sees, which are the first MAX_NODES from the lowest that any row sees, where there is a window, and the drafted ones.  Four keys are asked for at once:
-// others wait meanwhile, with a limit.
-template <typename T> __device__ __noinline__ void infinite_values(const Params &p, const int *table, int g, int first, int last, int start, const uint32_t *seen, int c, bool all, float (&v)[8]) {
-  float sum[8] = {};
-  first = max(first, 0);
+// Columns c0 .. c0 + 63 of a row's output, as it was stored: those with an infinite or NaN value that the row sees become the sum of these.  (What the products made of them is
+// none: a weight comes in two parts, of which the second may be 0 or negative, and where not all rows see a value it was 0.)  all: look at every key of the piece, else only at
+// those that not every row sees, which are the first MAX_NODES from the lowest that any row sees, where there is a window, and the drafted ones.  Four keys are asked for at
+// once: others wait meanwhile, with a limit.  (Behind the stores and not in them: there it cost 0.4 us of 16, and 1.4 of 17.4 with a cap.)
+template <typename T> __device__ __noinline__ void infinite_values(const Params &p, const Piece &k, int row, const uint32_t *seen, int depth, int c0, bool all) {
+  const int start = k.x.start, low = p.window ? start + depth - p.window + 1 : 0, first = max(max(k.t0 * TKEYS, low), 0), last = min((k.t0 + k.nt) * TKEYS, start + k.x.n);
   const int skip = all ? last : p.window ? max(first, max(start - p.window + 1, 0) + MAX_NODES) : first;      // from here to `start` all rows see all
-  for (int j0 = first; j0 < last; j0 += 4) {
-    if (j0 >= skip && j0 < start) j0 = start;
-    uint4 w[4];
+  const int *table = p.page_table + (size_t)k.table * p.max_pages;
+  const int at = k.rt * TROWS + row, node = at / p.qpk, head = k.g * p.qpk + at - node * p.qpk;
+  for (int c = c0; c < min(p.vdim, c0 + 64); c += 8) {
+    float sum[8] = {};
+    for (int j0 = first; j0 < last; j0 += 4) {
+      if (j0 >= skip && j0 < start) j0 = start;
+      uint4 w[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = j0 + u, d = j - start, page = j / p.page;
-      w[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (j < last && (d < 0 || (seen[d >> 5] >> (d & 31) & 1)))
-        w[u] = *reinterpret_cast<const uint4 *>(v_page<T>(p, table[page], g) + (size_t)(j - page * p.page) * p.vdim + c);
-    }
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u, d = j - start, page = j / p.page;
+        w[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (j < last && (d < 0 || (seen[d >> 5] >> (d & 31) & 1)))
+          w[u] = *reinterpret_cast<const uint4 *>(v_page<T>(p, table[page], k.g) + (size_t)(j - page * p.page) * p.vdim + c);
+      }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t y[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t y[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!bad<T>(y[i])) continue;
-        const float2 z = Half2<T>::wide(y[i]);
-        if (!isfinite(z.x)) sum[2 * i] += z.x;
-        if (!isfinite(z.y)) sum[2 * i + 1] += z.y;
+        for (int i = 0; i < 4; ++i) {
+          if (!bad<T>(y[i])) continue;
+          const float2 z = Half2<T>::wide(y[i]);
+          if (!isfinite(z.x)) sum[2 * i] += z.x;
+          if (!isfinite(z.y)) sum[2 * i + 1] += z.y;
+        }
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (sum[i] != 0.f) v[i] = sum[i];
+    for (int i = 0; i < 8; ++i) {
+      if (sum[i] == 0.f) continue;
+      if (k.whole) reinterpret_cast<T *>(p.out)[(size_t)(k.x.row0 + node) * p.out_ld + (size_t)head * p.vdim + c + i] = rounded<T>(sum[i]);
+      else p.part_o[(((size_t)k.slot * (p.vdim / 4) + (c + i) / 4) * p.part_ld + row) * 4 + (i & 3)] = sum[i];
+    }
+  }
 }
 
 // A piece's tile that some rows see in part: keys from `start` on are drafted, those in front of start + n - window are not seen by all.
@@ -1054,7 +1061,8 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
       tc::fence_after();
       if (live) {
         const float sum = sm.sum[pieces & 1][0][row] + sm.sum[pieces & 1][1][row];
-        const bool any_bad = sm.any_bad[pieces & 7] != 0, store = row < rows;
+        const bool store = row < rows;
+        float odd = 0.f;                                    // NaN, if something came out infinite or NaN
         const float inv = k.whole ? 1.0f / sum : 1.0f;
         T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + node) * p.out_ld + (size_t)head * p.vdim;
         if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * p.part_ld + row] = make_float2(m, sum);
@@ -1067,18 +1075,8 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
 #pragma unroll
           for (int z = 0; z < 16; z += 8) {
             if (c + z >= p.vdim) break;
-            bool all = false;                               // (what came out finite holds no such value of a tile that all rows see)
 #pragma unroll
-            for (int b = 0; b < 8; ++b) all |= !isfinite(__uint_as_float(v[z + b]));
-            if ((any_bad || all) && !isnan(sum)) {          // (where the sum of the weights is NaN all is)
-              float w[8];
-#pragma unroll
-              for (int b = 0; b < 8; ++b) w[b] = __uint_as_float(v[z + b]);
-              const int low = p.window ? x.start + depth - p.window + 1 : 0;
-              infinite_values<T>(p, p.page_table + (size_t)k.table * p.max_pages, k.g, max(k.t0 * TKEYS, low), min((k.t0 + k.nt) * TKEYS, x.start + x.n), x.start, seen, c + z, all, w);
-#pragma unroll
-              for (int b = 0; b < 8; ++b) v[z + b] = __float_as_uint(w[b]);
-            }
+            for (int b = 0; b < 8; ++b) odd = fmaf(__uint_as_float(v[z + b]), 0.f, odd);
             if (k.whole) {
               uint32_t y[4];
 #pragma unroll
@@ -1097,6 +1095,9 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
             }
           }
         }
+        // (where the sum of the weights is NaN all is; what came out finite holds no infinite value of a tile that all rows see)
+        if (store && (sm.any_bad[pieces & 7] || isnan(odd)) && !isnan(sum)) infinite_values<T>(p, k, row, seen, depth, half * 64, isnan(odd));
+        __syncwarp();
         tc::fence_before();
       }
       k = next;
