@@ -202,9 +202,10 @@ template <typename T> __device__ __forceinline__ float turned(const Params &p, c
 }
 
 // Half: pairs of 16-bit values and fp32
+// Weights are 2^kBias times as large as their row's largest allows, which may be 2^kRaise above (fp16 ends at 2^16).
 template <typename T> struct Half2;
 template <> struct Half2<__half> {
-  static constexpr float kBias = 7.f;      // weights are 2^7 as large
+  static constexpr float kBias = 7.f, kRaise = 8.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
   static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
   // a and b in two parts
@@ -216,7 +217,7 @@ template <> struct Half2<__half> {
   static constexpr uint32_t kExponent = 0x7c00u;
 };
 template <> struct Half2<__nv_bfloat16> {
-  static constexpr float kBias = 0.f;
+  static constexpr float kBias = 0.f, kRaise = 8.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf2(a, b); }
   static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
   // (By cutting off bits, which costs no conversion: the upper half of a float is a bf16.  What is lost is below 2^-15 of the value.)
@@ -585,11 +586,10 @@ template <typename T, int VJ> __global__ void __launch_bounds__(PLAIN_THREADS) t
 // A tile is 64 KB of keys and values for 1536 or, with rotation, 2048 cycles of products (128-wide heads), and 2600 cycles at this SM's share of memory.  Measured
 // are 3700 behind 60000 positions: one warp asks for boxes (700 for a tile of keys or values), one issues products, and each tile's softmax, products and copies
 // hand it on to one another.  Behind some hundred positions a block has one or two tiles, and what bounds it is the way from the plan to the first weights.
-// The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^8: weights stay below 2^8
-// (2^15 in fp16, where they are kept 2^7 times as large, so that small ones keep their bits).
+// The running maximum is only raised, and the output rescaled, when a score exceeds it by 2^kRaise: weights stay below 2^8 (2^15 in fp16, where they are kept 2^7 times
+// as large, so that small ones keep their bits).
 constexpr int SOFT_WARPS = 8, COPY_WARPS = 2, MMA_WARP = SOFT_WARPS + COPY_WARPS, TENSOR_THREADS = 384, TROWS = 128, TKEYS = 128, MAX_SLOTS = 10;
 constexpr int RING_BYTES = 192 * 1024, O_COL = 256, Q_COL = 384, Q_LOW = 64;      // columns of output and queries, from there of the queries' second part
-constexpr float RAISE = 8.f;
 
 struct TcShared {
   // landed: by slot, like full.  A slot is sent for again when its products are done, which wait for both copying warps: so both have seen its phase before the next
@@ -606,6 +606,11 @@ struct TcShared {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t both(float x) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(x));
   return y;
 }
 // Values with the keys outermost: 64 columns (128 bytes) of a key are a swizzled row, eight keys 1024 bytes, 64 columns more a block of 128 rows.
@@ -916,7 +921,8 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
     int pieces = 0, n_s[2] = {0, 0}, n_o = 0;
     const float a1 = fmaxf(fabsf(p.scale), 1e-30f) * kLog2e, a2 = CAP == LOW ? 2.0f * a1 / p.softcap : CAP ? fmaxf(fabsf(p.scale), 1e-30f) / p.softcap : 0.f, b2 = p.softcap * kLog2e;
     // (a scale of zero: so small that all scores are equal, but -inf, which marks what is not seen, times it is -inf)
-    auto score = [&](float s) { return CAP == LOW ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : CAP ? b2 * tanh_of(a2 * s) : a1 * s; };      // (grows with s)
+    auto score = [&](float s) { return CAP == LOW ? b2 * (1.0f - __fdividef(2.0f, ex2(a2 * s) + 1.0f)) : __fmul_rn(b2, tanh_of(a2 * s)); };      // of a cap; grows with s
+    const float unit = CAP ? 1.f : a1;                      // of what the maximum is kept in: capped scores in powers of 2, or scores as the products gave them
     auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory"); };
     auto meet_partner = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + q) : "memory"); };       // the warp with the same rows
     // The output of the block's tile i.  (By turns on two barriers: of either the phase before is done when the scores of tile i are, and the phase behind
@@ -951,7 +957,7 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
       const bool live = q * 32 < rows;                      // (uniform over the warp)
       const int at = min(r0 + row, x.n * p.qpk - 1), node = at / p.qpk, head = k.g * p.qpk + at - node * p.qpk, depth = p.parent ? p.depth[(size_t)k.s * p.most + node] : node;
       const uint32_t *seen = p.seen + ((size_t)k.s * p.most + node) * WORDS;
-      float m = -INFINITY, l = 0.f;                         // m: what the exponents are relative to; l: of this half
+      float m = -INFINITY, l = 0.f;                         // m: the maximum that the exponents are relative to; l: of this half
       // Scores of a tile's half to weights.  (In loops of 32 keys: a block that has a tile or two fetches this code once, and waits for it.  Measured with 64 keys
       // in line and the mask in a copy of it, 5 tokens behind 700: a third of all waiting was for instructions.)
       auto weigh = [&](int t) {
@@ -988,11 +994,11 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
         sm.top[t & 1][half][row] = top;
         meet_partner();
         top = fmaxf(top, sm.top[t & 1][1 - half][row]);
-        top = (top == -INFINITY ? top : score(top)) - Half2<T>::kBias;
+        if (CAP && top != -INFINITY) top = score(top);
         // (keys that went before lie far below, or none was seen: the sums so far are scaled to the new maximum)
-        const bool raise = row < rows && top > m + (m == -INFINITY ? 0.f : RAISE);
+        const bool raise = row < rows && (top - m) * unit > Half2<T>::kRaise;
         if (__any_sync(0xffffffffu, raise) && t > 0) {
-          const float f = raise ? ex2(m - top) : 1.f;        // (m = -inf: 0, of sums that are 0)
+          const float f = raise ? ex2((m - top) * unit) : 1.f;        // (m = -inf: 0, of sums that are 0)
           l *= f;
           output_of(n_o - 1);
           tc::fence_after();
@@ -1006,7 +1012,18 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
           }
         }
         if (raise) m = top;
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float base = m == -INFINITY ? 0.f : m, ref = base - Half2<T>::kBias;
+        // Exponents of two weights.  The maximum is taken off first and as it is: of large scores a product in full lies far beside a rounded one, and floats next to it are further
+        // apart than weights may be.
+        const uint64_t less = both(-base), times = both(a1), plus = both(Half2<T>::kBias);
+        auto exponents = [&](float &y, float &z) {
+          if (CAP) {                                         // (-inf stays what is not seen)
+            if (y != -INFINITY) y = CAP == LOW ? score(y) - ref : (score(y) - base) + Half2<T>::kBias;
+            if (z != -INFINITY) z = CAP == LOW ? score(z) - ref : (score(z) - base) + Half2<T>::kBias;
+          } else {
+            asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tadd.rn.f32x2 t, t, %2;\n\tfma.rn.f32x2 t, t, %3, %4;\n\tmov.b64 {%0, %1}, t;\n\t}" : "+f"(y), "+f"(z) : "l"(less), "l"(times), "l"(plus));
+          }
+        };
         float add[4] = {0.f, 0.f, 0.f, 0.f};
         // 16 keys: eight columns of their weights' first parts, eight of the second
         auto sixteen = [&](const uint32_t (&v)[16], uint32_t to) {
@@ -1014,13 +1031,7 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             float y = __uint_as_float(v[i]), z = __uint_as_float(v[i + 1]);
-            if (CAP) {                                       // (-inf stays what is not seen)
-              y = y == -INFINITY ? y : score(y) - ref;
-              z = z == -INFINITY ? z : score(z) - ref;
-            } else {
-              y = fmaf(y, a1, -ref);
-              z = fmaf(z, a1, -ref);
-            }
+            exponents(y, z);
             y = ex2(y);
             z = ex2(z);
             add[i & 2] += y;
@@ -1065,7 +1076,7 @@ template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS,
         float odd = 0.f;                                    // NaN, if something came out infinite or NaN
         const float inv = k.whole ? 1.0f / sum : 1.0f;
         T *out = reinterpret_cast<T *>(p.out) + (size_t)(x.row0 + node) * p.out_ld + (size_t)head * p.vdim;
-        if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * p.part_ld + row] = make_float2(m, sum);
+        if (!k.whole && half == 0 && store) p.part_ml[(size_t)k.slot * p.part_ld + row] = make_float2(m * unit - Half2<T>::kBias, sum);
 #pragma unroll 1
         for (int c = half * 64; c < min(p.vdim, half * 64 + 64); c += 16) {
           uint32_t v[16];
