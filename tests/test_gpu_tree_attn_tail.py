@@ -1,4 +1,4 @@
-"""Attention of drafted tokens with scores of any size."""
+"""Attention of drafted tokens where one key has by far the highest score and all of the output is the others': they count as exactly as 16-bit weights allow."""
 import math
 
 import pytest
@@ -8,6 +8,43 @@ import tree_util as tu
 
 pytestmark = pytest.mark.gpu
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+# few sequences, whose keys many blocks share, and many, where a block has a sequence's keys to itself
+@pytest.mark.parametrize("n_seq", [1, 60, 200])
+@pytest.mark.parametrize("dtype,plain", [("fp16", False), ("bf16", False), ("fp16", True), ("fp32", False)])
+@pytest.mark.parametrize("below", [8.0, 12.0, 14.5, 17.5, 19.0])
+@pytest.mark.parametrize("where", [3, 1500])
+def test_flat_tail_behind_a_spike(cuda, n_seq, dtype, plain, below, where):
+    """A weight and the output are rounded to 16 bits at most once (bf16: the weights in two parts, 2^-15), the fp32 sums lose 2^-23 a key."""
+    n, C, D = 4, 2000, 64
+    s = tu.batch([n] * n_seq, [C] * n_seq, "tree", dtype=DT[dtype], dim=D, n_kv=2, qpk=2, seed=51)
+    s.scale = 1.0
+    g = torch.Generator(device=cuda).manual_seed(52)
+    pool, cut = s.cache.pool, s.heads * D
+    # scores are exact: q is a unit vector, and the keys' first channel is the score
+    pool[:, 0] = 0
+    pool[:, 0, ..., 0] = -below
+    pool[:, 1] = (torch.rand(pool[:, 1].shape, generator=g, device=cuda) * 250 + 250).to(s.dtype)
+    for i in range(n_seq):
+        page = s.table[s.slot[i]][where // s.page]
+        pool[page, 0, :, where % s.page, 0] = 0
+        pool[page, 1, :, where % s.page] = 0               # all of the output is the tail's
+    s.qkv[:] = 0
+    s.qkv[:, :cut].view(-1, s.heads, D)[:, :, 0] = 1
+    s.qkv[:, cut:cut + s.n_kv * D].view(-1, s.n_kv, D)[:, :, 0] = -below
+    s.qkv[:, cut + s.n_kv * D:] = 300
+    out = tu.run(s, plain=plain).double()
+    half = torch.finfo(s.dtype).eps / 2
+    w = math.exp(-below)
+    for i in range(n_seq):
+        _, V = tu._pages(s, s.cache.pool, i, C)
+        up = torch.tensor([len(a) for a in tu.lines(s.parents[i])], dtype=torch.float64, device=cuda)
+        tail = V.sum(1)[None] + 300 * up[:, None, None]    # [n, n_kv, D]
+        exp = (w * tail / (1 + (C - 1 + up[:, None, None]) * w))[:, :, None].expand(n, 2, 2, D).reshape(n, s.heads * D)
+        bound = exp * (half + max(2.0 ** -11 if s.dtype == torch.float16 else 0.0, 2.0 ** -15) + (C + n) * 2.0 ** -23)
+        worst = float(((out[s.cu[i]:s.cu[i] + n] - exp).abs() / bound).max())
+        assert worst <= 1.0, f"sequence {i}: off by {worst:.2f} of the tolerance"
 
 
 @pytest.mark.parametrize("dtype,plain", [("fp16", False), ("bf16", False), ("fp16", True), ("bf16", True), ("fp32", False)])
