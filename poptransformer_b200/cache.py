@@ -94,7 +94,7 @@ class SequenceSlots:
 
     def truncate(self, slot, n):
         """Keeps the first `n` positions of a sequence (drafted tokens that were refused go this way) and hands the pages behind them back.  Returns the
-        (source, destination) pages that have to be copied before the sequence goes on: its last one, where that is shared and not full."""
+        (source, destination) pages that have to be copied before any sequence goes on: its last one, where that is shared and not full (the other owner may then write to it)."""
         length, n = self.length[slot], int(n)
         if not 0 <= n <= length:
             raise PtError(f"truncate: {n} of {length} positions")

@@ -78,3 +78,34 @@ def test_scores_of_any_size(cuda, dtype, plain, power, sign):
         exp = (w @ V)[:, :, None].expand(-1, n, 2, D).permute(1, 0, 2, 3).reshape(n, -1)
         slack = (half + 2.0 ** -14 + (C + n) * 2.0 ** -23) * (w @ V.abs())[:, :, None].expand(-1, n, 2, D).permute(1, 0, 2, 3).reshape(n, -1)
         assert ((out[s.cu[i]:s.cu[i] + n] - exp).abs() <= slack + 2.0 ** -25).all(), i
+
+
+@pytest.mark.parametrize("dtype,plain", [("fp16", False), ("bf16", False), ("bf16", True), ("fp32", False)])
+@pytest.mark.parametrize("power", [9, 14, 20, 24, 30, 40, 60])
+@pytest.mark.parametrize("times", [0.01, 0.3, 1.0])
+def test_capped_scores_of_any_size(cuda, dtype, plain, power, times):
+    """Caps that the scores come near: the largest has all the weight, or shares it with those that fp32 cannot tell from it."""
+    n, C, D = 7, 900, 64
+    s = tu.batch([n, 3], [C, 70], "tree", dtype=DT[dtype], dim=D, n_kv=2, qpk=2, seed=53)
+    cap = 2.0 ** power
+    s.scale = times * cap
+    pool, cut = s.cache.pool, s.heads * D
+    pool[:, 0, ..., 1:] = 0
+    s.qkv[:, :cut + s.n_kv * D].view(-1, s.heads + s.n_kv, D)[:, :, 1:] = 0
+    s.qkv[:, :cut].view(-1, s.heads, D)[:, :, 0] = 1
+    out = tu.run(s, softcap=cap, plain=plain).double()
+    assert torch.isfinite(out).all() and s.flag.item() == 0
+    for i, (n, C) in enumerate(zip(s.counts, s.starts)):
+        K, V = tu._pages(s, s.cache.pool, i, C + n)
+        seen = torch.zeros((n, C + n), dtype=torch.bool, device=cuda)
+        seen[:, :C] = True
+        for r, up in enumerate(tu.lines(s.parents[i])):
+            seen[r, [C + b for b in up]] = True
+        z = (cap * torch.tanh(K[:, :, 0] * s.scale / cap))[:, None].expand(-1, n, -1).masked_fill(~seen, -math.inf)
+        # capped scores are right to 2^-19 of themselves: the output lies between the smallest and the largest value of those that may have weight
+        top = z.amax(-1, keepdim=True)
+        may = z >= top - top.abs() * 2.0 ** -18 - 40
+        big = V[:, None].masked_fill(~may[..., None], -math.inf).amax(2)[:, :, None].expand(-1, n, 2, D).permute(1, 0, 2, 3).reshape(n, -1)
+        small = V[:, None].masked_fill(~may[..., None], math.inf).amin(2)[:, :, None].expand(-1, n, 2, D).permute(1, 0, 2, 3).reshape(n, -1)
+        got, slack = out[s.cu[i]:s.cu[i] + n], torch.finfo(s.dtype).eps * torch.maximum(big.abs(), small.abs()) + 2.0 ** -12 * V.abs().max()
+        assert ((got <= big + slack) & (got >= small - slack)).all(), i
