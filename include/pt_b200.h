@@ -842,7 +842,7 @@ int pt_mlstm(const pt_mlstm_args *args, void *stream);
  * no sequence has (from cu[n_seq] on) is neither read nor written.  No slot comes twice in a call, and calls that share a workspace follow one another.  A sequence of more than max_tokens_per_seq tokens (at most 256), or of rows that the batch has not, sets error_flag to 14,
  * one whose positions reach max_len to 12: its rows are then left as they were.  A parent that is none sets it to 14 and counts as -1.  Keys and values that a row does
  * not see may be infinite or NaN.  An infinite or NaN value that it sees makes its own column of the row infinite or NaN, as their sum is, and no other (a weight that is 0 in fp32
- * may leave it out, or make it NaN). */
+ * may leave it out, or make it NaN).  A rotated query of 16 bits that its type cannot hold is infinite. */
 typedef struct pt_tree_attn_args {
   pt_batch_view batch;    /* at most 1024 sequences                                  */
   int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16: q, k, v, pool and out */

@@ -13,7 +13,7 @@
 //   tree_tensor_kernel    fp16 and bf16, widths up to 128 in steps of 8: both products on tcgen05
 //   combine_kernel        sums the parts of the items that several blocks shared
 // Scores, softmax and sums are fp32.  All three in a captured graph: 5 tokens behind 700 positions (32 heads over 8 of 128) 18 us, 16 sequences of 16 tokens behind up to
-// 4000 70 us, 63 tokens behind 60000 182 to 192 us.
+// 4000 68 us, 63 tokens behind 60000 187 us.
 #include <cuda.h>
 
 #include <type_traits>
@@ -715,7 +715,7 @@ template <typename T> __device__ __noinline__ void infinite_values(const Params 
 __device__ __forceinline__ bool partial(const Params &p, const Seq &x, int j0) { return j0 + TKEYS > x.start || (p.window && x.start + x.n - 1 - j0 >= p.window); }
 // CAP: scores go through cap tanh(score / cap).  As cap (1 - 2 / (e^2x + 1)) alone that is off by cap 2^-21, whatever the score: up to LOW_CAP less than what the weights lose
 // as two parts and the output by its rounding.  Larger caps, which scores hardly reach, take tanh_of, which is right to 2^-20 of the score and costs twice the time
-// (16 sequences: 69 us without a cap, 85 with a low one, 155; behind 60000 positions 188, 236, 485).
+// (16 sequences: 68 us without a cap, 86 with a low one, 161; behind 60000 positions 187, 237, 508).
 enum Cap { NO_CAP, LOW, ANY };
 constexpr float LOW_CAP = 256.f;
 template <typename T, Cap CAP> __global__ void __launch_bounds__(TENSOR_THREADS, 1) tree_tensor_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
