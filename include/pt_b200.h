@@ -921,6 +921,91 @@ int pt_kv_copy_pages(const pt_kv_pool *pools_host, int n_pools, int page_size, i
 int pt_kv_move_rows(const pt_kv_pool *pools_host, int n_pools, int page_size, int max_pages, const int32_t *page_table, const pt_batch_view *batch,
                     const int32_t *path, int path_ld, const int32_t *count, int32_t *error_flag, void *stream);
 
+/* ---- paged caches of eight bits (csrc/kv8.cu) ----------------------------------------------------------------------------
+ * Keys and values as bytes with a scale for every position and head.  A page of the pool is K [n_kv][page_size][dim] and then V
+ * [n_kv][page_size][vdim], a byte each; its scales are fp32 [2][n_kv][page_size], K's and then V's.  A row x of one position and head is
+ * kept as  byte_i = round(x_i (top / m)),  scale = m / top,  with m = max |x_i|, at least 2^-64, and top 127 (int8, rounded to nearest even) or 448
+ * (E4M3).  A row that has a NaN, an infinity or a magnitude above 2^64 gets the scale NaN and bytes of 0: it reads back as NaN.  E4M3 bytes that are NaN are
+ * never written, and what they read as is not said.  page_table is [slots][max_pages]; dim and vdim are at most 256.
+ * All three calls: rows that no sequence has (from cu[n_seq] on) are neither read nor written; a sequence whose positions reach max_len sets error_flag to 12
+ * and its rows and pages are left as they were, and so are positions whose page is negative. */
+#define PT_KV8_INT8 0
+#define PT_KV8_E4M3 1
+typedef struct pt_kv8_cache {
+  void *pool;
+  float *scales;
+  const int32_t *page_table;
+  int fmt;                /* PT_KV8_*                                                */
+  int n_kv, dim, vdim, page_size, max_pages;
+  int max_len;            /* no position reaches this (0 = page_size * max_pages)    */
+} pt_kv8_cache;
+
+/* pt_rotary: out <- x with the first rope_dims dimensions of every head rotated by the angles of its row's position: pair (i, i + rope_dims / 2), or (2 i,
+ * 2 i + 1) with interleaved, by (cos, sin) = rope[position][i], in 32 bits, rounded once.  inverse: by the negative angles (the gradient of x for
+ * one of out).  out may be x.  A row whose position is outside the table is left as it was and sets error_flag to 12. */
+typedef struct pt_rotary_args {
+  int rows, heads, dim, dtype;   /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16               */
+  const void *x;
+  int x_ld;
+  void *out;
+  int out_ld;
+  const int32_t *position;       /* [rows]                                           */
+  int positions, rope_dims, interleaved, inverse;
+  const float *rope;             /* fp32 [positions, rope_dims / 2, 2]               */
+  int32_t *error_flag;
+} pt_rotary_args;
+int pt_rotary(const pt_rotary_args *args, void *stream);
+
+/* pt_kv8_append: the keys (rotated as in pt_rotary by their positions start[s] + i) and values of the packed tokens go to the cache.  With q_out the
+ * queries go there, rotated, in their own type (q_out may be q).  The rows of q, k and v have one stride. */
+typedef struct pt_kv8_append_args {
+  pt_batch_view batch;
+  pt_kv8_cache cache;
+  int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16: q, k, v and q_out   */
+  int n_head;
+  const void *q, *k, *v;
+  int ld;
+  void *q_out;            /* or NULL: q is not looked at                             */
+  int q_out_ld, rope_dims, interleaved;
+  const float *rope;      /* fp32 [max_len, rope_dims / 2, 2]                        */
+  int32_t *error_flag;
+} pt_kv8_append_args;
+int pt_kv8_append(const pt_kv8_append_args *args, void *stream);
+
+/* pt_kv8_attn: token i of sequence s attends to the cached positions up to its own, start[s] + i (which pt_kv8_append has written): out[h] = sum_j w_j v_j,
+ * w = softmax(c(scale q[h] . k_j)) over the last `window` of them (0: all); softcap c: a score x becomes c tanh(x / c) (0: none).  Meant for few tokens a
+ * sequence: every token reads its history by itself.  A negative page reads as some other page, and sets error_flag to 12. */
+typedef struct pt_kv8_attn_args {
+  pt_batch_view batch;
+  pt_kv8_cache cache;
+  int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16: q and out           */
+  int n_head, window;
+  float scale, softcap;   /* softcap 0 (none) or 1e-20 .. 1e20                       */
+  const void *q;
+  int q_ld;
+  void *out;
+  int out_ld;
+  int plain;              /* 1: the kernel for any sizes, whatever the shape         */
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t *error_flag;
+} pt_kv8_attn_args;
+size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int vdim);
+int pt_kv8_attn(const pt_kv8_attn_args *args, void *stream);
+
+/* pt_kv8_unpack: positions 0 .. start[s] + tokens - 1 of every sequence <- byte * scale, rounded once, in another pool's pages (K [n_kv][into_page_size][dim]
+ * and then V [n_kv][into_page_size][vdim]), which have a table of their own with the same slots: for kernels that read caches of the rows' type. */
+typedef struct pt_kv8_unpack_args {
+  pt_batch_view batch;
+  pt_kv8_cache cache;
+  int dtype;              /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16: into                */
+  void *into;
+  const int32_t *into_table;
+  int into_page_size, into_max_pages, into_max_len;
+  int32_t *error_flag;
+} pt_kv8_unpack_args;
+int pt_kv8_unpack(const pt_kv8_unpack_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -176,6 +176,30 @@ class LlamaStepArgs(ctypes.Structure):
                [("done_flag", c_void_p), ("wait_limit", c_int)]
 
 
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("pool", "scales", "page_table")] + [(n, c_int) for n in ("fmt", "n_kv", "dim", "vdim", "page_size", "max_pages", "max_len")]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("rows", c_int), ("heads", c_int), ("dim", c_int), ("dtype", c_int), ("x", c_void_p), ("x_ld", c_int), ("out", c_void_p), ("out_ld", c_int), ("position", c_void_p),
+                ("positions", c_int), ("rope_dims", c_int), ("interleaved", c_int), ("inverse", c_int), ("rope", c_void_p), ("error_flag", c_void_p)]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    _fields_ = [("batch", BatchView), ("cache", Kv8Cache), ("dtype", c_int), ("n_head", c_int), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("ld", c_int), ("q_out", c_void_p),
+                ("q_out_ld", c_int), ("rope_dims", c_int), ("interleaved", c_int), ("rope", c_void_p), ("error_flag", c_void_p)]
+
+
+class Kv8AttnArgs(ctypes.Structure):
+    _fields_ = [("batch", BatchView), ("cache", Kv8Cache), ("dtype", c_int), ("n_head", c_int), ("window", c_int), ("scale", c_float), ("softcap", c_float), ("q", c_void_p),
+                ("q_ld", c_int), ("out", c_void_p), ("out_ld", c_int), ("plain", c_int), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("error_flag", c_void_p)]
+
+
+class Kv8UnpackArgs(ctypes.Structure):
+    _fields_ = [("batch", BatchView), ("cache", Kv8Cache), ("dtype", c_int), ("into", c_void_p), ("into_table", c_void_p), ("into_page_size", c_int), ("into_max_pages", c_int),
+                ("into_max_len", c_int), ("error_flag", c_void_p)]
+
+
 # name -> (restype, argtypes); mirrors include/pt_b200.h one to one
 SIGNATURES = {
     "pt_last_error": (ctypes.c_char_p, []),
@@ -204,6 +228,11 @@ SIGNATURES = {
     "pt_verify_drafts": (c_int, [ctypes.POINTER(VerifyArgs), c_void_p]),
     "pt_kv_copy_pages": (c_int, [ctypes.POINTER(KvPool), c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "pt_kv_move_rows": (c_int, [ctypes.POINTER(KvPool), c_int, c_int, c_int, c_void_p, ctypes.POINTER(BatchView), c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "pt_rotary": (c_int, [ctypes.POINTER(RotaryArgs), c_void_p]),
+    "pt_kv8_append": (c_int, [ctypes.POINTER(Kv8AppendArgs), c_void_p]),
+    "pt_kv8_attn_workspace_bytes": (c_size_t, [c_int] * 4),
+    "pt_kv8_attn": (c_int, [ctypes.POINTER(Kv8AttnArgs), c_void_p]),
+    "pt_kv8_unpack": (c_int, [ctypes.POINTER(Kv8UnpackArgs), c_void_p]),
     "pt_hyper": (c_int, [ctypes.POINTER(HyperArgs), c_void_p]),
     "pt_window_attn_workspace_bytes": (c_size_t, [c_int] * 7),
     "pt_window_attn": (c_int, [ctypes.POINTER(WindowAttnArgs), c_void_p]),

@@ -1,0 +1,434 @@
+// Paged caches of eight bits: keys and values as bytes (int8 or E4M3), with a scale for every position and head.
+//   pool[page] = K [n_kv][page_size][dim] and then V [n_kv][page_size][vdim], a byte each; scales[page] = fp32 [2][n_kv][page_size], K's and then V's.
+// A row x of one position and head is kept as  byte_i = round(x_i (top / m)),  scale = m / top,  m = max_i |x_i|  (top: 127 or 448).  m is at least 2^-64, so that
+// top / m is finite; a row that has a NaN, an infinity or a magnitude above 2^64 gets the scale NaN and bytes of 0, and reads back as NaN.
+#include "rotate.cuh"
+
+namespace pt {
+namespace kv8 {
+
+constexpr int THREADS = 256;
+constexpr uint32_t SMALL = 0x1f800000u, LARGE = 0x5f800000u;     // 2^-64 and 2^64 as bits
+
+struct Cache {
+  unsigned char *pool;
+  float *scales;
+  const int *page_table;
+  int n_kv, dim, vdim, page, max_pages, max_len;
+  size_t page_bytes;
+};
+struct Batch {
+  int n_seq, n_tok;
+  const int *cu, *start, *slot, *tok_seq;
+};
+
+template <bool E4M3> __device__ __forceinline__ float top_byte() { return E4M3 ? 448.f : 127.f; }
+template <bool E4M3> __device__ __forceinline__ float from_byte(unsigned char b) {
+  if constexpr (E4M3) {
+    __nv_fp8_e4m3 x;
+    x.__x = b;
+    return float(x);
+  }
+  return (float)(signed char)b;
+}
+template <bool E4M3> __device__ __forceinline__ uint32_t to_byte(float x) {
+  if constexpr (E4M3) return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)max(-127, min(127, __float2int_rn(x))) & 0xFFu;
+}
+// Four values as a word.
+template <bool E4M3> __device__ __forceinline__ uint32_t to_word(float a, float b, float c, float d) {
+  if constexpr (E4M3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  }
+  return to_byte<false>(a) | to_byte<false>(b) << 8 | to_byte<false>(c) << 16 | to_byte<false>(d) << 24;
+}
+
+// Whether a sequence's new positions can be there, and the page and place of one.
+__device__ __forceinline__ bool in_table(const Cache &c, int start, int count) { return start >= 0 && count <= c.max_len - start; }
+
+// ------------------------------------------------------------------------------------------ rotation
+struct Rotary {
+  int rows, heads, dim, rot, x_ld, out_ld, positions;
+  const int *position;
+  const float2 *rope;
+  int *error_flag;
+};
+// LANES lanes per head of a row (16 elements each).  blockIdx.x: the row, whose angles a lane reads once; blockIdx.y: a part of its heads.
+// Bound by memory: rows in and out once.
+template <typename T, int LANES, bool WHOLE, bool INVERSE, bool NEIGHBOURS>
+__global__ void __launch_bounds__(THREADS) rotary_kernel(const T *x, T *out, const Rotary p) {
+  early_start();
+  const int row = blockIdx.x, t = threadIdx.x % LANES, pos = p.position[row];
+  if (pos < 0 || pos >= p.positions) {
+    if (threadIdx.x == 0 && blockIdx.y == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    return;
+  }
+  if (16 * t >= p.dim) return;
+  const Turn turn = load_turn(p.rope + (size_t)pos * (p.rot / 2), t, p.rot, INVERSE);
+  for (int h = blockIdx.y * (THREADS / LANES) + threadIdx.x / LANES; h < p.heads; h += gridDim.y * (THREADS / LANES)) {
+    Pairs v = load_pairs<WHOLE>(x + (size_t)row * p.x_ld + (size_t)h * p.dim, t, p.dim, p.rot, NEIGHBOURS);
+    turn_pairs(v, turn, t, p.rot);
+    store_pairs<WHOLE>(out + (size_t)row * p.out_ld + (size_t)h * p.dim, v, t, p.dim, p.rot, NEIGHBOURS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ appending
+struct Append {
+  Batch b;
+  Cache c;
+  int heads, rot, ld, q_out_ld;
+  const float2 *rope;
+  int *error_flag;
+};
+// The rows of a token: its q heads (rotated to q_out), its keys (rotated, kept as bytes), its values (kept as bytes), LANES lanes each.
+template <typename T, int LANES, bool WHOLE, bool NEIGHBOURS, bool E4M3>
+__global__ void __launch_bounds__(THREADS) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
+  early_start();
+  const int tok = blockIdx.x, t = threadIdx.x % LANES;
+  if (tok >= p.b.cu[p.b.n_seq]) return;
+  const int seq = p.b.tok_seq[tok], first = p.b.cu[seq], start = p.b.start[seq];
+  const bool fits = in_table(p.c, start, p.b.cu[seq + 1] - first);
+  const int pos = start + tok - first;
+  const int page = fits ? p.c.page_table[(size_t)p.b.slot[seq] * p.c.max_pages + pos / p.c.page] : -1;
+  if (page < 0) {
+    if (threadIdx.x == 0 && blockIdx.y == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    return;
+  }
+  const Turn turn = load_turn(p.rope + (size_t)pos * (p.rot / 2), t, p.rot, false);
+  const int place = pos % p.c.page, G = p.c.n_kv, all = p.heads + 2 * G;
+  for (int r0 = blockIdx.y * (THREADS / LANES); r0 < all; r0 += gridDim.y * (THREADS / LANES)) {      // (whole warps stay together: the lanes of a row exchange their maxima)
+    const int r = r0 + threadIdx.x / LANES;
+    const bool is_q = r < p.heads, is_v = r >= p.heads + G;
+    const int h = is_q ? r : is_v ? r - p.heads - G : r - p.heads, dim = is_v ? p.c.vdim : p.c.dim, rot = is_v ? 0 : p.rot;
+    const bool in = r < all && 16 * t < dim;
+    Pairs x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.a[j] = x.b[j] = 0.f;
+    if (in) {
+      x = load_pairs<WHOLE>((is_q ? q : is_v ? v : k) + (size_t)tok * p.ld + (size_t)h * dim, t, dim, rot, NEIGHBOURS);
+      turn_pairs(x, turn, t, rot);
+      if (is_q) store_pairs<WHOLE>(q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim, x, t, dim, rot, NEIGHBOURS);
+    }
+    uint32_t m = 0;           // (magnitudes in the order of their bits: NaN is above infinity)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, max(__float_as_uint(x.a[j]) & 0x7fffffffu, __float_as_uint(x.b[j]) & 0x7fffffffu));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!in || is_q) continue;
+    const bool fine = m <= LARGE;
+    const float most = __uint_as_float(max(m, SMALL)), by = fine ? __fdiv_rn(top_byte<E4M3>(), most) : 0.f;
+    const size_t row = (size_t)h * p.c.page + place;
+    if (t == 0) p.c.scales[((size_t)page * 2 * G + (is_v ? G : 0)) * p.c.page + row] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
+    unsigned char *to = p.c.pool + (size_t)page * p.c.page_bytes + (is_v ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x.a[j] = fine ? __fmul_rn(x.a[j], by) : 0.f;
+      x.b[j] = fine ? __fmul_rn(x.b[j], by) : 0.f;
+    }
+    if constexpr (WHOLE) {
+      if (!NEIGHBOURS && 16 * t < rot) {
+        *reinterpret_cast<uint2 *>(to + 8 * t) = make_uint2(to_word<E4M3>(x.a[0], x.a[1], x.a[2], x.a[3]), to_word<E4M3>(x.a[4], x.a[5], x.a[6], x.a[7]));
+        *reinterpret_cast<uint2 *>(to + 8 * t + rot / 2) = make_uint2(to_word<E4M3>(x.b[0], x.b[1], x.b[2], x.b[3]), to_word<E4M3>(x.b[4], x.b[5], x.b[6], x.b[7]));
+      } else {
+        *reinterpret_cast<uint4 *>(to + 16 * t) = make_uint4(to_word<E4M3>(x.a[0], x.b[0], x.a[1], x.b[1]), to_word<E4M3>(x.a[2], x.b[2], x.a[3], x.b[3]),
+                                                              to_word<E4M3>(x.a[4], x.b[4], x.a[5], x.b[5]), to_word<E4M3>(x.a[6], x.b[6], x.a[7], x.b[7]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
+        if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.a[j]);
+        if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.b[j]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ pages in a wider type
+struct Unpack {
+  Batch b;
+  Cache c;
+  const int *into_table;
+  int into_page, into_max_pages, into_max_len;
+  int *error_flag;
+};
+constexpr int UNPACK_ROWS = 64;
+// Block: 64 positions of a sequence, keys or values of one head.  Bound by memory.
+template <typename T, bool WHOLE, bool E4M3> __global__ void __launch_bounds__(THREADS) unpack_kernel(T *into, const Unpack p) {
+  early_start();
+  const int seq = blockIdx.y, G = p.c.n_kv, h = blockIdx.z % G, first = blockIdx.x * UNPACK_ROWS;
+  const bool is_v = blockIdx.z >= G;
+  const int start = p.b.start[seq], count = p.b.cu[seq + 1] - p.b.cu[seq];
+  if (!in_table(p.c, start, count) || count > p.into_max_len - start) {
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    return;
+  }
+  const int rows = min(UNPACK_ROWS, start + count - first), dim = is_v ? p.c.vdim : p.c.dim;
+  if (rows <= 0) return;
+  const int *table = p.c.page_table + (size_t)p.b.slot[seq] * p.c.max_pages, *into_table = p.into_table + (size_t)p.b.slot[seq] * p.into_max_pages;
+  const size_t into_bytes = (size_t)G * p.into_page * (p.c.dim + p.c.vdim);
+  constexpr int UNIT = WHOLE ? 16 : 1;
+  const int units = dim / UNIT;
+  for (int i = threadIdx.x; i < rows * units; i += THREADS) {
+    const int r = i / units, u = i - r * units, pos = first + r;
+    const int page = table[pos / p.c.page], to_page = into_table[pos / p.into_page];
+    if (page < 0 || to_page < 0) {
+      if (p.error_flag) atomicExch(p.error_flag, 12);
+      continue;
+    }
+    const size_t row = (size_t)h * p.c.page + pos % p.c.page;
+    const float scale = p.c.scales[((size_t)page * 2 * G + (is_v ? G : 0)) * p.c.page + row];
+    const unsigned char *from = p.c.pool + (size_t)page * p.c.page_bytes + (is_v ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim + (size_t)u * UNIT;
+    T *to = into + (size_t)to_page * into_bytes + (is_v ? (size_t)G * p.into_page * p.c.dim : 0) + ((size_t)h * p.into_page + pos % p.into_page) * dim + (size_t)u * UNIT;
+    if constexpr (WHOLE) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(from);
+      const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+      float lo[8], hi[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo[j] = from_byte<E4M3>((unsigned char)(word[j >> 2] >> (8 * (j & 3)))) * scale;
+        hi[j] = from_byte<E4M3>((unsigned char)(word[2 + (j >> 2)] >> (8 * (j & 3)))) * scale;
+      }
+      store_run(to, lo);
+      store_run(to + 8, hi);
+    } else {
+      *to = from_f<T>(from_byte<E4M3>(*from) * scale);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ attention
+struct Attn {
+  Batch b;
+  Cache c;
+  int heads, window, q_ld, out_ld;
+  float scale, softcap;
+  int *error_flag;
+};
+// Any sizes: a block per token and head, whose warps take every fourth key each with a running maximum and sum, lanes across the dimensions.
+constexpr int PLAIN_WARPS = 4, MOST_DIM = 256;
+template <typename T, bool E4M3> __global__ void __launch_bounds__(PLAIN_WARPS * 32) attn_plain_kernel(const T *q, T *out, const Attn p) {
+  early_start();
+  __shared__ float top[PLAIN_WARPS], total[PLAIN_WARPS], sums[PLAIN_WARPS][MOST_DIM];
+  const int tok = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.c.n_kv, g = head / (p.heads / G);
+  if (tok >= p.b.cu[p.b.n_seq]) return;
+  const int seq = p.b.tok_seq[tok], first = p.b.cu[seq], start = p.b.start[seq];
+  if (!in_table(p.c, start, p.b.cu[seq + 1] - first)) {
+    if (threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    return;
+  }
+  const int pos = start + tok - first, from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int *table = p.c.page_table + (size_t)p.b.slot[seq] * p.c.max_pages;
+  constexpr int PER = MOST_DIM / 32;
+  float x[PER], o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = lane + 32 * i;
+    x[i] = d < p.c.dim ? to_f(q[(size_t)tok * p.q_ld + (size_t)head * p.c.dim + d]) : 0.f;
+    o[i] = 0.f;
+  }
+  for (int j = from + warp; j <= pos; j += PLAIN_WARPS) {
+    int page = table[j / p.c.page];
+    if (page < 0) {
+      if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+      page = 0;
+    }
+    const size_t row = (size_t)g * p.c.page + j % p.c.page, at = (size_t)page * 2 * G * p.c.page + row;
+    const unsigned char *k = p.c.pool + (size_t)page * p.c.page_bytes + row * p.c.dim, *v = p.c.pool + (size_t)page * p.c.page_bytes + (size_t)G * p.c.page * p.c.dim + row * p.c.vdim;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.c.dim) s = fmaf(x[i], from_byte<E4M3>(k[lane + 32 * i]), s);
+    s = warp_sum(s) * (p.c.scales[at] * p.scale);
+    if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
+    const float t = fmaxf(m, s), was = m == t ? 1.f : expf(m - t), w = expf(s - (t == -INFINITY ? 0.f : t)), wv = w * p.c.scales[at + (size_t)G * p.c.page];
+    m = t;
+    l = l * was + w;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.c.vdim) o[i] = o[i] * was + wv * from_byte<E4M3>(v[lane + 32 * i]);
+  }
+  if (lane == 0) { top[warp] = m; total[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sums[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  float most = top[0], whole = 0.f, share[PLAIN_WARPS];
+#pragma unroll
+  for (int w = 1; w < PLAIN_WARPS; ++w) most = fmaxf(most, top[w]);
+#pragma unroll
+  for (int w = 0; w < PLAIN_WARPS; ++w) {
+    share[w] = total[w] == 0.f ? 0.f : expf(top[w] - most);
+    whole += total[w] * share[w];
+  }
+  for (int d = threadIdx.x; d < p.c.vdim; d += PLAIN_WARPS * 32) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < PLAIN_WARPS; ++w) y += total[w] == 0.f ? 0.f : sums[w][d] * share[w];
+    out[(size_t)tok * p.out_ld + (size_t)head * p.c.vdim + d] = from_f<T>(y / whole);
+  }
+}
+
+static int check_cache(const pt_kv8_cache &c, const char *who) {
+  PT_REQUIRE(c.pool && c.scales && c.page_table, "%s: null pool, scales or page table", who);
+  PT_REQUIRE(c.fmt == PT_KV8_INT8 || c.fmt == PT_KV8_E4M3, "%s: cache format %d (int8 or E4M3)", who, c.fmt);
+  PT_REQUIRE(c.n_kv > 0 && c.dim > 0 && c.dim <= MOST_DIM && c.vdim > 0 && c.vdim <= MOST_DIM, "%s: n_kv=%d, heads of %d and %d (1 .. %d)", who, c.n_kv, c.dim, c.vdim, MOST_DIM);
+  PT_REQUIRE(c.page_size > 0 && c.max_pages > 0 && (long long)c.page_size * c.max_pages < (1ll << 31) && c.max_len >= 0 && c.max_len <= (long long)c.page_size * c.max_pages,
+             "%s: %d pages of %d positions, max_len=%d", who, c.max_pages, c.page_size, c.max_len);
+  PT_REQUIRE(((uintptr_t)c.scales & 3) == 0, "%s: scales on a multiple of 4 bytes", who);
+  return PT_OK;
+}
+static int check_batch(const pt_batch_view &b, const char *who) {
+  PT_REQUIRE(b.n_seq > 0 && b.n_tok >= 0 && b.cu && b.start && b.slot && b.tok_seq, "%s: bad batch (%d sequences, %d tokens)", who, b.n_seq, b.n_tok);
+  return PT_OK;
+}
+static int check_rope(const float *rope, int rope_dims, int dim, const char *who) {
+  PT_REQUIRE(rope_dims >= 0 && rope_dims % 2 == 0 && rope_dims <= dim, "%s: %d rotated dimensions of %d (an even number)", who, rope_dims, dim);
+  PT_REQUIRE(rope_dims == 0 || (rope && aligned_to(rope, 8)), "%s: %d rotated dimensions want a table (on a multiple of 8 bytes)", who, rope_dims);
+  return PT_OK;
+}
+static Cache cache_of(const pt_kv8_cache &c) {
+  return {(unsigned char *)c.pool, c.scales, c.page_table, c.n_kv, c.dim, c.vdim, c.page_size, c.max_pages, c.max_len ? c.max_len : c.page_size * c.max_pages,
+          (size_t)c.n_kv * c.page_size * (c.dim + c.vdim)};
+}
+static Batch batch_of(const pt_batch_view &b) { return {b.n_seq, b.n_tok, b.cu, b.start, b.slot, b.tok_seq}; }
+static int elem_bytes(int dtype) { return dtype == PT_DT_F32 ? 4 : 2; }
+static int lanes_of(int dim) { return dim <= 64 ? 4 : dim <= 128 ? 8 : 16; }
+// Parts of a row's heads for blocks of their own: few rows have to fill the GPU, many do without reading the angles again.
+static int head_parts(int rows, int heads, int per_block) { return std::max(1, std::min(ceil_div(heads, per_block), ceil_div(sm_count() * 4, std::max(1, rows)))); }
+
+template <typename T, int LANES, bool WHOLE> static cudaError_t launch_rotary(const pt_rotary_args &a, const Rotary &p, dim3 grid, cudaStream_t st) {
+  const T *x = (const T *)a.x;
+  T *out = (T *)a.out;
+  const auto kernel = a.inverse ? (a.interleaved ? rotary_kernel<T, LANES, WHOLE, true, true> : rotary_kernel<T, LANES, WHOLE, true, false>)
+                                : (a.interleaved ? rotary_kernel<T, LANES, WHOLE, false, true> : rotary_kernel<T, LANES, WHOLE, false, false>);
+  return launch_early(kernel, Grid(grid), THREADS, 0, st, x, out, p);
+}
+template <typename T> static cudaError_t launch_rotary(const pt_rotary_args &a, const Rotary &p, bool whole, cudaStream_t st) {
+  const int lanes = lanes_of(a.dim);
+  const dim3 grid(a.rows, head_parts(a.rows, a.heads, THREADS / lanes));
+  if (lanes == 4) return whole ? launch_rotary<T, 4, true>(a, p, grid, st) : launch_rotary<T, 4, false>(a, p, grid, st);
+  if (lanes == 8) return whole ? launch_rotary<T, 8, true>(a, p, grid, st) : launch_rotary<T, 8, false>(a, p, grid, st);
+  return whole ? launch_rotary<T, 16, true>(a, p, grid, st) : launch_rotary<T, 16, false>(a, p, grid, st);
+}
+
+template <typename T, int LANES, bool WHOLE> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, dim3 grid, cudaStream_t st) {
+  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3;
+  const auto kernel = e4m3 ? (a.interleaved ? append_kernel<T, LANES, WHOLE, true, true> : append_kernel<T, LANES, WHOLE, false, true>)
+                           : (a.interleaved ? append_kernel<T, LANES, WHOLE, true, false> : append_kernel<T, LANES, WHOLE, false, false>);
+  return launch_early(kernel, Grid(grid), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
+}
+template <typename T> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, bool whole, cudaStream_t st) {
+  const int lanes = lanes_of(std::max(a.cache.dim, a.cache.vdim));
+  const dim3 grid(a.batch.n_tok, head_parts(a.batch.n_tok, p.heads + 2 * a.cache.n_kv, THREADS / lanes));
+  if (lanes == 4) return whole ? launch_append<T, 4, true>(a, p, grid, st) : launch_append<T, 4, false>(a, p, grid, st);
+  if (lanes == 8) return whole ? launch_append<T, 8, true>(a, p, grid, st) : launch_append<T, 8, false>(a, p, grid, st);
+  return whole ? launch_append<T, 16, true>(a, p, grid, st) : launch_append<T, 16, false>(a, p, grid, st);
+}
+
+template <typename T> static cudaError_t launch_unpack(const pt_kv8_unpack_args &a, const Unpack &p, bool whole, cudaStream_t st) {
+  const dim3 grid(ceil_div(std::min(p.c.max_len, p.into_max_len), UNPACK_ROWS), a.batch.n_seq, 2 * a.cache.n_kv);
+  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3;
+  const auto kernel = whole ? (e4m3 ? unpack_kernel<T, true, true> : unpack_kernel<T, true, false>) : (e4m3 ? unpack_kernel<T, false, true> : unpack_kernel<T, false, false>);
+  return launch_early(kernel, Grid(grid), THREADS, 0, st, (T *)a.into, p);
+}
+
+template <typename T> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, cudaStream_t st) {
+  const auto kernel = a.cache.fmt == PT_KV8_E4M3 ? attn_plain_kernel<T, true> : attn_plain_kernel<T, false>;
+  return launch_early(kernel, Grid(dim3(a.batch.n_tok, a.n_head)), PLAIN_WARPS * 32, 0, st, (const T *)a.q, (T *)a.out, p);
+}
+
+}  // namespace kv8
+}  // namespace pt
+
+using namespace pt;
+
+extern "C" int pt_rotary(const pt_rotary_args *a, void *stream) {
+  PT_REQUIRE(a, "pt_rotary: null args");
+  PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_rotary: type %d", a->dtype);
+  PT_REQUIRE(a->rows >= 0 && a->heads > 0 && a->heads <= 65535 && a->dim > 0 && a->dim <= kv8::MOST_DIM, "pt_rotary: %d rows of %d heads of %d (heads of 1 .. %d)", a->rows, a->heads, a->dim,
+             kv8::MOST_DIM);
+  PT_REQUIRE(a->x && a->out && a->position, "pt_rotary: null pointer argument");
+  PT_REQUIRE(a->x_ld >= (long long)a->heads * a->dim && a->out_ld >= (long long)a->heads * a->dim, "pt_rotary: rows of %d and %d elements, %d heads of %d", a->x_ld, a->out_ld, a->heads, a->dim);
+  PT_REQUIRE(a->x != a->out || a->x_ld == a->out_ld, "pt_rotary: rows that are rotated in place have one stride, got %d and %d", a->x_ld, a->out_ld);
+  PT_REQUIRE(a->positions > 0 && a->rope_dims > 0, "pt_rotary: %d rotated dimensions, a table of %d positions", a->rope_dims, a->positions);
+  if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->dim, "pt_rotary")) return rc;
+  if (a->rows == 0) return PT_OK;
+  const int es = kv8::elem_bytes(a->dtype);
+  const bool whole = a->dim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->x, 16) && aligned_to(a->out, 16) && (long long)a->x_ld * es % 16 == 0 && (long long)a->out_ld * es % 16 == 0;
+  const kv8::Rotary p{a->rows, a->heads, a->dim, a->rope_dims, a->x_ld, a->out_ld, a->positions, a->position, (const float2 *)a->rope, a->error_flag};
+  const cudaStream_t st = as_stream(stream);
+  PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_rotary<float>(*a, p, whole, st)
+          : a->dtype == PT_DT_F16 ? kv8::launch_rotary<__half>(*a, p, whole, st)
+                                  : kv8::launch_rotary<__nv_bfloat16>(*a, p, whole, st));
+  PT_LAUNCH_CHECK("pt_rotary");
+  return PT_OK;
+}
+
+extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
+  PT_REQUIRE(a, "pt_kv8_append: null args");
+  PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_append: type %d", a->dtype);
+  if (int rc = kv8::check_batch(a->batch, "pt_kv8_append")) return rc;
+  if (int rc = kv8::check_cache(a->cache, "pt_kv8_append")) return rc;
+  if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->cache.dim, "pt_kv8_append")) return rc;
+  PT_REQUIRE(a->k && a->v && a->ld > 0, "pt_kv8_append: null pointer argument, or rows of %d elements", a->ld);
+  PT_REQUIRE(!a->q_out || (a->q && a->n_head > 0 && a->q_out_ld >= (long long)a->n_head * a->cache.dim), "pt_kv8_append: q_out wants q and rows of %d heads of %d, got %d elements", a->n_head,
+             a->cache.dim, a->q_out_ld);
+  PT_REQUIRE(!a->q_out || a->q != a->q_out || a->ld == a->q_out_ld, "pt_kv8_append: queries that are rotated in place have one stride, got %d and %d", a->ld, a->q_out_ld);
+  if (a->batch.n_tok == 0) return PT_OK;
+  const kv8::Append p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->q_out ? a->n_head : 0, a->rope_dims, a->ld, a->q_out_ld, (const float2 *)a->rope, a->error_flag};
+  const int es = kv8::elem_bytes(a->dtype);
+  const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->cache.pool, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
+                     (long long)a->ld * es % 16 == 0 && (!a->q_out || (aligned_to(a->q, 16) && aligned_to(a->q_out, 16) && (long long)a->q_out_ld * es % 16 == 0));
+  const cudaStream_t st = as_stream(stream);
+  PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_append<float>(*a, p, whole, st)
+          : a->dtype == PT_DT_F16 ? kv8::launch_append<__half>(*a, p, whole, st)
+                                  : kv8::launch_append<__nv_bfloat16>(*a, p, whole, st));
+  PT_LAUNCH_CHECK("pt_kv8_append");
+  return PT_OK;
+}
+
+extern "C" int pt_kv8_unpack(const pt_kv8_unpack_args *a, void *stream) {
+  PT_REQUIRE(a, "pt_kv8_unpack: null args");
+  PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_unpack: type %d", a->dtype);
+  if (int rc = kv8::check_batch(a->batch, "pt_kv8_unpack")) return rc;
+  if (int rc = kv8::check_cache(a->cache, "pt_kv8_unpack")) return rc;
+  PT_REQUIRE(a->into && a->into_table && a->into_page_size > 0 && a->into_max_pages > 0 && (long long)a->into_page_size * a->into_max_pages < (1ll << 31),
+             "pt_kv8_unpack: null pointer argument, or %d pages of %d positions", a->into_max_pages, a->into_page_size);
+  PT_REQUIRE(a->into_max_len >= 0 && a->into_max_len <= (long long)a->into_page_size * a->into_max_pages, "pt_kv8_unpack: %d pages of %d positions, max_len=%d", a->into_max_pages,
+             a->into_page_size, a->into_max_len);
+  PT_REQUIRE(a->batch.n_seq <= 65535 && a->cache.n_kv <= 32767, "pt_kv8_unpack: %d sequences (65535 at most), %d heads (32767)", a->batch.n_seq, a->cache.n_kv);
+  const kv8::Unpack p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->into_table, a->into_page_size, a->into_max_pages,
+                      a->into_max_len ? a->into_max_len : a->into_page_size * a->into_max_pages, a->error_flag};
+  const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && aligned_to(a->cache.pool, 16) && aligned_to(a->into, 16);
+  const cudaStream_t st = as_stream(stream);
+  PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_unpack<float>(*a, p, whole, st)
+          : a->dtype == PT_DT_F16 ? kv8::launch_unpack<__half>(*a, p, whole, st)
+                                  : kv8::launch_unpack<__nv_bfloat16>(*a, p, whole, st));
+  PT_LAUNCH_CHECK("pt_kv8_unpack");
+  return PT_OK;
+}
+
+extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int vdim) { return 0; }
+
+extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
+  PT_REQUIRE(a, "pt_kv8_attn: null args");
+  PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_attn: type %d", a->dtype);
+  if (int rc = kv8::check_batch(a->batch, "pt_kv8_attn")) return rc;
+  if (int rc = kv8::check_cache(a->cache, "pt_kv8_attn")) return rc;
+  PT_REQUIRE(a->q && a->out, "pt_kv8_attn: null pointer argument");
+  PT_REQUIRE(a->n_head > 0 && a->n_head <= 65535 && a->n_head % a->cache.n_kv == 0, "pt_kv8_attn: %d heads over %d", a->n_head, a->cache.n_kv);
+  PT_REQUIRE(a->q_ld >= (long long)a->n_head * a->cache.dim && a->out_ld >= (long long)a->n_head * a->cache.vdim, "pt_kv8_attn: rows of %d and %d elements, %d heads of %d and %d", a->q_ld,
+             a->out_ld, a->n_head, a->cache.dim, a->cache.vdim);
+  PT_REQUIRE(a->window >= 0, "pt_kv8_attn: window=%d", a->window);
+  PT_REQUIRE(a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f), "pt_kv8_attn: softcap=%g (0, or 1e-20 .. 1e20)", (double)a->softcap);
+  PT_REQUIRE(a->scale - a->scale == 0.f, "pt_kv8_attn: scale=%g", (double)a->scale);
+  if (a->batch.n_tok == 0) return PT_OK;
+  const kv8::Attn p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->n_head, a->window, a->q_ld, a->out_ld, a->scale, a->softcap, a->error_flag};
+  const cudaStream_t st = as_stream(stream);
+  PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_attn<float>(*a, p, st)
+          : a->dtype == PT_DT_F16 ? kv8::launch_attn<__half>(*a, p, st)
+                                  : kv8::launch_attn<__nv_bfloat16>(*a, p, st));
+  PT_LAUNCH_CHECK("pt_kv8_attn");
+  return PT_OK;
+}

@@ -13,15 +13,17 @@ Reference op            -> function here
   BeamSearch            -> beam_search
   Remap                 -> remap_tensor        (layout hint on IPU; identity here)
 plus the fused decode stages that replace chains of reference ops: PackedLinear / linear,
-rms_norm, kv_append_attn, topk, embedding, step_containers, wkv.
+rms_norm, kv_append_attn, topk, embedding, step_containers, wkv; and caches of eight bits (rotary,
+kv8_append, kv8_attn, kv8_unpack).
 """
 import ctypes
+import math
 
 import torch
 
 from . import _lib
-from ._lib import (AttnArgs, BatchView, ContextRows, DenseExt, GemmArgs, HyperArgs, LatentAttnArgs, LatentContextArgs, LatentPrepArgs, LinearArgs, MlstmArgs,
-                   MoeRouteArgs, PostNormArgs, PtError, ShiftNormArgs, SsmArgs, TreeAttnArgs, VerifyArgs, WindowAttnArgs, check)
+from ._lib import (AttnArgs, BatchView, ContextRows, DenseExt, GemmArgs, HyperArgs, Kv8AppendArgs, Kv8AttnArgs, Kv8Cache, Kv8UnpackArgs, LatentAttnArgs, LatentContextArgs, LatentPrepArgs,
+                   LinearArgs, MlstmArgs, MoeRouteArgs, PostNormArgs, PtError, RotaryArgs, ShiftNormArgs, SsmArgs, TreeAttnArgs, VerifyArgs, WindowAttnArgs, check)
 
 W_INT4, W_FP16, W_FP8, W_BF16 = 0, 1, 2, 3
 DT_F16, DT_F32, DT_BF16 = 0, 1, 2
@@ -31,6 +33,7 @@ GLU_CLAMPED, GLU_SILU, GLU_GELU = 0, 1, 2
 MOE_SOFTMAX, MOE_SIGMOID, MOE_SOFTMAX_ALL = 0, 1, 2
 ROPE_NONE, ROPE_LLAMA, ROPE_CHATGLM2 = 0, 1, 2
 SOFTMAX_F32, SOFTMAX_F16 = 0, 1
+KV8_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 def _stream():
@@ -449,6 +452,7 @@ def window_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, window=0, 
     (a layer that reads another layer's cache).  q_norm, k_norm, rope: per-head norm and rotation of q and k; q is then rewritten.  gate: rows
     whose sigmoid multiplies the output (a view that starts at its first column).  context: an object with k, v, shared, ld, shared_dim
     and cu that names rows of the whole context as keys and values of a prompt, in place of the cache's pages (see pt_context_rows)."""
+    _wide(cache, "window_attn")
     a = WindowAttnArgs()
     a.batch, a.dtype = view, dtype_code(qkv.dtype)
     a.n_head, a.n_kv, a.dim, a.vdim = n_head, cache.n_kv, cache.head_dim, cache.v_dim
@@ -789,15 +793,24 @@ def kv_cache_pipeline(state, step, updater):
 
 
 # ------------------------------------------------------------------------------------------ paged cache + attention
+def _wide(cache, who):
+    """For what reads or writes a cache in the rows' type."""
+    if cache.scales is not None:
+        raise PtError(f"{who}: a cache of {cache.pool.dtype} is written by kv8_append and read by kv8_attn and kv8_unpack")
+
+
 class PagedKVCache:
     """Page pool of one layer plus the (shared) page table.  pool[page][2][n_kv][page_size][head_dim]; with a value width of its own
     (v_dim) a page is K [n_kv][page_size][head_dim] followed by V [n_kv][page_size][v_dim].  n_pages: size of the pool where pages
-    are handed out on demand (cache.SequenceSlots) instead of max_len tokens per row."""
+    are handed out on demand (cache.SequenceSlots) instead of max_len tokens per row.
+
+    dtype torch.int8 or torch.float8_e4m3fn: a cache of eight bits, with fp32 `scales` [pages, 2, n_kv, page_size] of every position and head (K's and
+    V's), which kv8_append writes and kv8_attn and kv8_unpack read; PagePools serves both kinds, the other kernels want caches of the rows' type."""
 
     def __init__(self, rows, n_kv, head_dim, max_len, page_size=64, device="cuda", page_table=None, extra_pages=0, v_dim=None, dtype=torch.float16,
-                 n_pages=None, pool=None):
+                 n_pages=None, pool=None, scales=None):
         """pool: memory to use, for instance a layer's part of one tensor.  Its first dimension is the pages: n_pages of them at least, or as many as the default
-        page table names (which pages a page_table of the caller's names is the caller's to know)."""
+        page table names (which pages a page_table of the caller's names is the caller's to know).  scales: the same for a pool of eight bits."""
         self.rows, self.n_kv, self.head_dim, self.page_size = rows, n_kv, head_dim, page_size
         self.v_dim = head_dim if v_dim is None else v_dim
         self.max_len = max_len
@@ -814,12 +827,25 @@ class PagedKVCache:
             if pool.device.type != wanted.type or wanted.index not in (None, pool.device.index) or page_table is not None and page_table.device != pool.device:
                 raise PtError(f"PagedKVCache: pool on {pool.device}, wanted on {wanted}" + ("" if page_table is None else f" with its page table on {page_table.device}"))
         self.pool = torch.zeros(shape, dtype=dtype, device=device) if pool is None else pool
+        self.scales = None
+        if dtype in KV8_FORMATS:
+            if not 1 <= min(head_dim, self.v_dim) <= max(head_dim, self.v_dim) <= 256:
+                raise PtError(f"PagedKVCache: eight bits want heads of 1 to 256 dimensions, got {head_dim} and {self.v_dim}")
+            if (scales is None) != (pool is None):
+                raise PtError("PagedKVCache: a pool of eight bits and its scales are given together")
+            shape = (self.pool.shape[0], 2, n_kv, page_size)
+            if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != shape or not scales.is_contiguous() or scales.device != self.pool.device):
+                raise PtError(f"PagedKVCache: scales {scales.dtype} {tuple(scales.shape)} on {scales.device}, expected contiguous float32 {shape} on {self.pool.device}")
+            self.scales = torch.zeros(shape, dtype=torch.float32, device=device) if scales is None else scales
+        elif scales is not None:
+            raise PtError(f"PagedKVCache: a pool of {dtype} has no scales")
         if page_table is None:
             page_table = torch.arange(rows * self.max_pages, dtype=torch.int32, device=device).reshape(rows, self.max_pages)
         self.page_table = page_table
 
     def export(self, step, max_len):
         """Reference-layout view [2, rows, n_kv, max_len, head_dim], newest first, zeros beyond step."""
+        _wide(self, "export")
         out = torch.empty((2, self.rows, self.n_kv, max_len, self.head_dim), dtype=torch.float16, device=self.pool.device)
         check(_lib.lib().pt_kv_export(_ptr(self.pool), _ptr(self.page_table), _ptr(step), self.rows, self.n_kv, self.head_dim,
                                       self.page_size, self.max_pages, max_len, _ptr(out), _stream()), "pt_kv_export")
@@ -838,16 +864,20 @@ class PagePools:
             if c.page_size != first.page_size or c.page_table is not first.page_table and (c.page_table.data_ptr(), c.page_table.shape) != (first.page_table.data_ptr(), first.page_table.shape):
                 raise PtError("PagePools: the caches share neither page size nor page table")
         self.pools = [c.pool for c in caches]      # (keeps them alive)
+        self.scales = [c.scales for c in caches if c.scales is not None]
         self.page_size, self.page_table = first.page_size, first.page_table
         self.n_pages = min(t.shape[0] for t in self.pools)
-        self._pools = (_lib.KvPool * len(caches))(*[_lib.KvPool(_ptr(c.pool), c.n_kv, c.head_dim, c.v_dim, c.pool.element_size()) for c in caches])
+        pools = [_lib.KvPool(_ptr(c.pool), c.n_kv, c.head_dim, c.v_dim, c.pool.element_size()) for c in caches]
+        # Scales are pools of one fp32 value a position.  They have a launch of their own: the pools of a launch are copied in the unit that divides the rows of all of them.
+        small = [_lib.KvPool(_ptr(c.scales), c.n_kv, 1, 1, 4) for c in caches if c.scales is not None]
+        self._pools = [(_lib.KvPool * len(p))(*p) for p in (pools, small) if p]
 
     def copy_pages(self, src, dst, error_flag=None):
         """Page dst[i] <- page src[i] in every layer (int32 on the device; see pt_kv_copy_pages)."""
         if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.numel() != dst.numel():
             raise PtError(f"copy_pages: int32 pages, as many sources as destinations, got {src.dtype} {src.numel()} and {dst.dtype} {dst.numel()}")
-        check(_lib.lib().pt_kv_copy_pages(self._pools, len(self._pools), self.page_size, self.n_pages, _ptr(src), _ptr(dst), src.numel(), _ptr(error_flag), _stream()),
-              "pt_kv_copy_pages")
+        for pools in self._pools:
+            check(_lib.lib().pt_kv_copy_pages(pools, len(pools), self.page_size, self.n_pages, _ptr(src), _ptr(dst), src.numel(), _ptr(error_flag), _stream()), "pt_kv_copy_pages")
 
     def copy(self, pairs):
         """The same for a list of (source, destination), as SequenceSlots returns it."""
@@ -860,8 +890,157 @@ class PagePools:
         returns them (see pt_kv_move_rows)."""
         if path.dtype != torch.int32 or count.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != view.n_seq or count.numel() != view.n_seq:
             raise PtError(f"move_rows: int32 path [{view.n_seq}, max_path] and count [{view.n_seq}], got {path.dtype} {tuple(path.shape)}, {count.dtype} {tuple(count.shape)}")
-        check(_lib.lib().pt_kv_move_rows(self._pools, len(self._pools), self.page_size, self.page_table.shape[1], _ptr(self.page_table), ctypes.byref(view), _ptr(path), path.shape[1],
-                                         _ptr(count), _ptr(error_flag), _stream()), "pt_kv_move_rows")
+        for pools in self._pools:
+            check(_lib.lib().pt_kv_move_rows(pools, len(pools), self.page_size, self.page_table.shape[1], _ptr(self.page_table), ctypes.byref(view), _ptr(path), path.shape[1],
+                                             _ptr(count), _ptr(error_flag), _stream()), "pt_kv_move_rows")
+
+
+# ------------------------------------------------------------------------------------------ rotation, caches of eight bits
+def rope_table(positions, dims, base=10000.0, scaling=None, device="cuda"):
+    """fp32 [positions, dims / 2, 2]: (cos, sin) of pair i at every position, from angles in 64 bits.  Pair i turns by base ** (-2 i / dims) a position.  scaling, for contexts beyond the
+    `original` one that a model was trained with: a dict whose "kind" is
+      "linear": positions are divided by `factor`;
+      "base":   the base is multiplied by factor ** (dims / (dims - 2)), so that the slowest pair turns `factor` times slower and the fastest as before;
+      "ramp":   pairs that turn less than `slow` times (default 1) over `original` positions are divided by `factor`, those that turn more than `fast` times (32) are
+                left, in proportion to their index between; (cos, sin) are multiplied by `magnitude` (default 0.1 ln(factor) + 1);
+      "bands":  pairs that turn less than `low` times over `original` are divided by `factor`, those that turn more than `high` times are left, in proportion to their turns between."""
+    if dims <= 0 or dims % 2 or positions <= 0:
+        raise PtError(f"rope_table: {positions} positions of {dims} dimensions (an even number)")
+    kind, s, magnitude = (scaling or {}).get("kind"), dict(scaling or {}), 1.0
+    i = torch.arange(dims // 2, dtype=torch.float64, device=device)
+    try:
+        if kind == "base":
+            if dims == 2:
+                raise PtError("rope_table: one pair has no slower one")
+            base = base * float(s["factor"]) ** (dims / (dims - 2))
+        f = float(base) ** (-2.0 * i / dims)
+        if kind == "linear":
+            f = f / float(s["factor"])
+        elif kind == "ramp":
+            factor, original = float(s["factor"]), float(s["original"])
+            pair = lambda turns: dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+            lo, hi = max(math.floor(pair(float(s.get("fast", 32)))), 0), min(math.ceil(pair(float(s.get("slow", 1)))), dims - 1)
+            kept = 1.0 - ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+            f = f / factor * (1.0 - kept) + f * kept
+            magnitude = float(s.get("magnitude", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+        elif kind == "bands":
+            turns = float(s["original"]) * f / (2 * math.pi)
+            kept = ((turns - float(s["low"])) / (float(s["high"]) - float(s["low"]))).clamp(0, 1)
+            f = f / float(s["factor"]) * (1.0 - kept) + f * kept
+        elif kind != "base" and scaling:
+            raise PtError(f"rope_table: unknown scaling {kind!r}")
+    except KeyError as e:
+        raise PtError(f"rope_table: {kind!r} wants {e.args[0]}") from None
+    a = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * f
+    return (torch.stack([a.cos(), a.sin()], -1) * magnitude).float().contiguous()
+
+
+def _here(who, *tensors):
+    """Launches go to the current device: tensors of another one are refused."""
+    now = torch._C._cuda_getDevice() if any(t is not None and t.is_cuda for t in tensors) else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != now):
+            raise PtError(f"{who}: a tensor on {t.device}, the current device is " + (f"cuda:{now}" if now >= 0 else "another (libpt_b200 ops need CUDA tensors)"))
+
+
+def _rope_ok(who, rope, rope_dims, positions):
+    if rope_dims and (rope is None or rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[0] < positions or rope.shape[1] * 2 != rope_dims or rope.shape[2] != 2):
+        raise PtError(f"{who}: {rope_dims} rotated dimensions want float32 rope [{positions} positions or more, {rope_dims // 2}, 2], got "
+                      f"{None if rope is None else (rope.dtype, tuple(rope.shape))}")
+
+
+def _row_ld(who, name, t, rows, width):
+    """Row stride of a 2-D tensor whose rows lie together."""
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or t.shape[1] > 1 and t.stride(1) != 1:
+        raise PtError(f"{who}: {name} wants {rows} rows of {width} neighbouring elements or more, got {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rotary(x, heads, dim, rope, positions, out=None, rope_dims=None, interleaved=False, inverse=False, error_flag=None):
+    """Rows of heads rotated by their positions (see pt_rotary): x [rows, heads * dim or more], whose rows may lie apart (a part of wider rows), positions int32 [rows], rope as rope_table makes
+    it.  out: None rotates x itself.  rope_dims: rotated dimensions at the front of a head (None: the table's).  interleaved: pairs are neighbours.  inverse: by
+    the negative angles, which takes the gradient of the output to that of x."""
+    rows = x.shape[0]
+    out = x if out is None else out
+    rope_dims = rope.shape[1] * 2 if rope_dims is None else rope_dims
+    _here("rotary", x, out, positions, rope, error_flag)
+    _rope_ok("rotary", rope, rope_dims, 1)
+    x_ld, out_ld = _row_ld("rotary", "x", x, rows, heads * dim), _row_ld("rotary", "out", out, rows, heads * dim)
+    if out.dtype != x.dtype or out.shape[0] != rows or positions.dtype != torch.int32 or positions.numel() != rows:
+        raise PtError(f"rotary: {rows} rows of {x.dtype} want out of that and int32 positions of each, got {out.dtype} {tuple(out.shape)}, {positions.dtype} {tuple(positions.shape)}")
+    if not rows:
+        return out
+    a = RotaryArgs(rows, heads, dim, dtype_code(x.dtype), x.data_ptr(), x_ld, out.data_ptr(), out_ld, _ptr(positions), rope.shape[0], rope_dims, 1 if interleaved else 0, 1 if inverse else 0,
+                   _ptr(rope), _ptr(error_flag))
+    check(_lib.lib().pt_rotary(ctypes.byref(a), _stream()), "pt_rotary")
+    return out
+
+
+def _kv8(cache, who):
+    fmt = KV8_FORMATS.get(cache.pool.dtype)
+    if fmt is None:
+        raise PtError(f"{who}: a cache of {cache.pool.dtype}; int8 or float8_e4m3fn is wanted")
+    table = cache.page_table
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] * cache.page_size < cache.max_len:
+        raise PtError(f"{who}: the page table is int32 [slots, pages of {cache.max_len} positions], got {table.dtype} {tuple(table.shape)}")
+    return Kv8Cache(_ptr(cache.pool), _ptr(cache.scales), _ptr(table), fmt, cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len)
+
+
+def _rows_fit(who, name, t, rows, width, ld):
+    if rows and (ld < width or t.numel() < (rows - 1) * ld + width):
+        raise PtError(f"{who}: {name} has {t.numel()} elements, {rows} rows of {width} at a stride of {ld} are wanted")
+
+
+def kv8_append(view, rows, ld, cache, n_head=0, rope=None, rope_dims=0, interleaved=False, q_out=None, q_out_ld=0, error_flag=None):
+    """Keys (rotated) and values of the packed tokens of `view` go to a cache of eight bits (see pt_kv8_append).  Rows hold [q | k | v] of n_head query heads, or [k | v] with n_head = 0.  q_out: where
+    the rotated queries go, rows of q_out_ld (`rows` itself rotates them in place).  rope: as rope_table makes it, of cache.max_len positions or more."""
+    n_tok, n_kv, dim, vdim, es = view.n_tok, cache.n_kv, cache.head_dim, cache.v_dim, rows.element_size()
+    _here("kv8_append", rows, cache.pool, rope, q_out, error_flag)
+    _rope_ok("kv8_append", rope, rope_dims, cache.max_len)
+    _rows_fit("kv8_append", "rows", rows, n_tok, (n_head + n_kv) * dim + n_kv * vdim, ld)
+    if q_out is not None:
+        if q_out.dtype != rows.dtype or n_head < 1:
+            raise PtError(f"kv8_append: {n_head} query heads of {rows.dtype} to q_out of {q_out.dtype}")
+        _rows_fit("kv8_append", "q_out", q_out, n_tok, n_head * dim, q_out_ld)
+    q = _ptr(rows)
+    k = q + n_head * dim * es
+    a = Kv8AppendArgs(view, _kv8(cache, "kv8_append"), dtype_code(rows.dtype), n_head, q, k, k + n_kv * dim * es, ld, _ptr(q_out), q_out_ld, rope_dims, 1 if interleaved else 0, _ptr(rope),
+                      _ptr(error_flag))
+    check(_lib.lib().pt_kv8_append(ctypes.byref(a), _stream()), "pt_kv8_append")
+
+
+def kv8_attn_workspace(n_tok, n_head, n_kv, vdim, device="cuda"):
+    """Workspace of kv8_attn calls of up to n_tok tokens that follow one another on a stream (any number of layers); zeroed once."""
+    return torch.zeros(_lib.lib().pt_kv8_attn_workspace_bytes(n_tok, n_head, n_kv, vdim), dtype=torch.uint8, device=device)
+
+
+def kv8_attn(view, q, q_ld, cache, out, out_ld, n_head, scale, window=0, softcap=0.0, workspace=None, error_flag=None, plain=False):
+    """Attention of new tokens (one a sequence, or a few) over a cache of eight bits that has their keys and values already (see pt_kv8_attn).  q rows begin with n_head rotated
+    queries, out rows with n_head * v_dim outputs."""
+    n_tok = view.n_tok
+    if out.dtype != q.dtype:
+        raise PtError(f"kv8_attn: q {q.dtype}, out {out.dtype}: one type is wanted")
+    _here("kv8_attn", q, out, cache.pool, workspace, error_flag)
+    _rows_fit("kv8_attn", "q", q, n_tok, n_head * cache.head_dim, q_ld)
+    _rows_fit("kv8_attn", "out", out, n_tok, n_head * cache.v_dim, out_ld)
+    a = Kv8AttnArgs(view, _kv8(cache, "kv8_attn"), dtype_code(q.dtype), n_head, window, scale, softcap, _ptr(q), q_ld, _ptr(out), out_ld, 1 if plain else 0, _ptr(workspace),
+                    0 if workspace is None else workspace.numel(), _ptr(error_flag))
+    check(_lib.lib().pt_kv8_attn(ctypes.byref(a), _stream()), "pt_kv8_attn")
+    return out
+
+
+def kv8_unpack(view, cache, into, error_flag=None):
+    """All positions of the sequences of `view`, the cached and the new ones, from a cache of eight bits into the pages of one of 16 or 32 bits (`into`: same heads, its own table with the same slots), for
+    the kernels that read those: a prompt's window_attn(append=False), for instance (see pt_kv8_unpack)."""
+    _wide(into, "kv8_unpack (into)")
+    table = into.page_table
+    if (into.n_kv, into.head_dim, into.v_dim) != (cache.n_kv, cache.head_dim, cache.v_dim):
+        raise PtError(f"kv8_unpack: {cache.n_kv} heads of {cache.head_dim} and {cache.v_dim} into {into.n_kv} of {into.head_dim} and {into.v_dim}")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < cache.page_table.shape[0] or table.shape[1] * into.page_size < into.max_len:
+        raise PtError(f"kv8_unpack: a table of int32 [{cache.page_table.shape[0]} slots or more, pages of {into.max_len} positions], got {table.dtype} {tuple(table.shape)}")
+    _here("kv8_unpack", cache.pool, into.pool, table, error_flag)
+    a = Kv8UnpackArgs(view, _kv8(cache, "kv8_unpack"), dtype_code(into.pool.dtype), _ptr(into.pool), _ptr(table), into.page_size, table.shape[1], into.max_len, _ptr(error_flag))
+    check(_lib.lib().pt_kv8_unpack(ctypes.byref(a), _stream()), "pt_kv8_unpack")
 
 
 def attn_workspace(batch, n_head, head_dim, max_pages, device="cuda"):
@@ -871,6 +1050,7 @@ def attn_workspace(batch, n_head, head_dim, max_pages, device="cuda"):
 
 def attn_args(qkv, step, cache, out, n_head, rope_mode, softmax_mode, score_scale, rope_sin, rope_cos, workspace, error_flag, pdl=0,
               out_fp8=None, out_fp8_scale=0.0):
+    _wide(cache, "kv_append_attn")
     a = AttnArgs()
     a.batch, a.n_head, a.n_kv, a.head_dim = qkv.shape[0], n_head, cache.n_kv, cache.head_dim
     a.page_size, a.max_pages, a.rope_mode, a.softmax_mode = cache.page_size, cache.max_pages, rope_mode, softmax_mode
@@ -901,6 +1081,7 @@ def prefill_attn(qkv, cache, batch, n_tokens, start, n_head, score_scale, rope_s
     """Causal attention over a whole prompt chunk (the reference's sequence_length != 1 attention, llama2/attention.py:64-114):
     qkv fp16 [batch * n_tokens, 3 * n_head * H], row b * n_tokens + t = position start + t of sequence b.  Rotates q in place,
     appends rotated k and v to the paged cache and returns softmax(q K^T * scale + causal mask) V, [batch * n_tokens, n_head * H]."""
+    _wide(cache, "prefill_attn")
     if qkv.shape != (batch * n_tokens, 3 * n_head * cache.head_dim) or cache.n_kv != n_head:
         raise PtError(f"prefill_attn: qkv {tuple(qkv.shape)} does not match batch={batch} n_tokens={n_tokens} n_head={n_head} (no grouped KV heads)")
     if out is None:
