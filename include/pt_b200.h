@@ -986,11 +986,11 @@ typedef struct pt_kv8_attn_args {
   void *out;
   int out_ld;
   int plain;              /* 1: the kernel for any sizes, whatever the shape         */
-  void *workspace;
+  void *workspace;        /* pt_kv8_attn_workspace_bytes, 16-byte aligned, zeroed once (the kernel for any sizes needs none); calls that share one follow one another */
   size_t workspace_bytes;
   int32_t *error_flag;
 } pt_kv8_attn_args;
-size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int vdim);
+size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width); /* width: the wider of a head's key and value */
 int pt_kv8_attn(const pt_kv8_attn_args *args, void *stream);
 
 /* pt_kv8_unpack: positions 0 .. start[s] + tokens - 1 of every sequence <- byte * scale, rounded once, in another pool's pages (K [n_kv][into_page_size][dim]

@@ -206,6 +206,11 @@ struct Attn {
   float scale, softcap;
   int *error_flag;
 };
+}  // namespace kv8
+}  // namespace pt
+#include "kv8_attn.cuh"
+namespace pt {
+namespace kv8 {
 // Any sizes: a block per token and head, whose warps take every fourth key each with a running maximum and sum, lanes across the dimensions.
 constexpr int PLAIN_WARPS = 4, MOST_DIM = 256;
 template <typename T, bool E4M3> __global__ void __launch_bounds__(PLAIN_WARPS * 32) attn_plain_kernel(const T *q, T *out, const Attn p) {
@@ -333,9 +338,20 @@ template <typename T> static cudaError_t launch_unpack(const pt_kv8_unpack_args 
   return launch_early(kernel, Grid(grid), THREADS, 0, st, (T *)a.into, p);
 }
 
-template <typename T> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, cudaStream_t st) {
+template <typename T> static cudaError_t launch_plain(const pt_kv8_attn_args &a, const Attn &p, cudaStream_t st) {
   const auto kernel = a.cache.fmt == PT_KV8_E4M3 ? attn_plain_kernel<T, true> : attn_plain_kernel<T, false>;
   return launch_early(kernel, Grid(dim3(a.batch.n_tok, a.n_head)), PLAIN_WARPS * 32, 0, st, (const T *)a.q, (T *)a.out, p);
+}
+static int launch_blocks(int width) { return sm_count() * (width > 128 ? 2 : BLOCKS_PER_SM); }
+static size_t part_bytes(int width) { return sizeof(float) * (width > 128 ? Shape<256>::PART : width > 64 ? Shape<128>::PART : Shape<64>::PART); }
+template <int SIZE> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
+  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype == PT_DT_F32;
+  const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, true, 2> : attn_kernel<SIZE, true, 1>) : (wide ? attn_kernel<SIZE, false, 2> : attn_kernel<SIZE, false, 1>);
+  static std::atomic<uint64_t> allowed[4];
+  constexpr int FIXED = NW * Shape<SIZE>::STAGES * Shape<SIZE>::STAGE + Shape<SIZE>::JOIN;
+  const cudaError_t e = allow_smem(kernel, FIXED + (3 * MAX_TOKENS + 1) * (int)sizeof(int), allowed[2 * e4m3 + wide]);
+  if (e != cudaSuccess) return e;
+  return launch_early(kernel, Grid(sp.grid), NW * 32, FIXED + (3 * sp.tokens + 1) * sizeof(int), st, p, sp);
 }
 
 }  // namespace kv8
@@ -409,7 +425,10 @@ extern "C" int pt_kv8_unpack(const pt_kv8_unpack_args *a, void *stream) {
   return PT_OK;
 }
 
-extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int vdim) { return 0; }
+extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width) {
+  if (n_tok < 1 || n_kv < 1 || n_head < n_kv) return 0;
+  return kv8::COUNTERS * sizeof(int) + (size_t)kv8::launch_blocks(width) * 2 * kv8::part_bytes(width);
+}
 
 extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   PT_REQUIRE(a, "pt_kv8_attn: null args");
@@ -426,9 +445,34 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Attn p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->n_head, a->window, a->q_ld, a->out_ld, a->scale, a->softcap, a->error_flag};
   const cudaStream_t st = as_stream(stream);
-  PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_attn<float>(*a, p, st)
-          : a->dtype == PT_DT_F16 ? kv8::launch_attn<__half>(*a, p, st)
-                                  : kv8::launch_attn<__nv_bfloat16>(*a, p, st));
-  PT_LAUNCH_CHECK("pt_kv8_attn");
+  const int width = std::max(a->cache.dim, a->cache.vdim);
+  // (16 bytes of a row a lane, 16 positions of a page a group)
+  if (a->plain || a->cache.dim % 16 || a->cache.vdim % 16 || a->cache.page_size % 16 || !aligned_to(a->cache.pool, 16)) {
+    PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_plain<float>(*a, p, st)
+            : a->dtype == PT_DT_F16 ? kv8::launch_plain<__half>(*a, p, st)
+                                    : kv8::launch_plain<__nv_bfloat16>(*a, p, st));
+    PT_LAUNCH_CHECK("pt_kv8_attn");
+    return PT_OK;
+  }
+  const size_t need = pt_kv8_attn_workspace_bytes(a->batch.n_tok, a->n_head, a->cache.n_kv, width);
+  PT_REQUIRE(a->workspace && aligned_to(a->workspace, 16) && a->workspace_bytes >= need, "pt_kv8_attn: %zu workspace bytes (on a multiple of 16) are wanted, got %zu", need,
+             a->workspace ? a->workspace_bytes : 0);
+  const int es = kv8::elem_bytes(a->dtype);
+  kv8::Split sp{};
+  sp.chunks = ceil_div(a->n_head / a->cache.n_kv, kv8::HEADS);
+  sp.dtype = a->dtype;
+  sp.q_whole = aligned_to(a->q, 16) && (long long)a->q_ld * es % 16 == 0;
+  sp.out_whole = aligned_to(a->out, 16) && (long long)a->out_ld * es % 16 == 0;
+  sp.counters = (int *)a->workspace;
+  sp.parts = (float *)(sp.counters + kv8::COUNTERS);
+  sp.q = a->q;
+  sp.out = a->out;
+  sp.grid = kv8::launch_blocks(width);
+  const int most = std::min(kv8::MAX_TOKENS, kv8::COUNTERS / (a->cache.n_kv * sp.chunks));
+  for (; sp.tok0 < a->batch.n_tok; sp.tok0 += most) {
+    sp.tokens = std::min(a->batch.n_tok - sp.tok0, most);
+    PT_CUDA(width > 128 ? kv8::launch_attn<256>(*a, p, sp, st) : width > 64 ? kv8::launch_attn<128>(*a, p, sp, st) : kv8::launch_attn<64>(*a, p, sp, st));
+    PT_LAUNCH_CHECK("pt_kv8_attn");
+  }
   return PT_OK;
 }

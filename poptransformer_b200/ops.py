@@ -1009,9 +1009,9 @@ def kv8_append(view, rows, ld, cache, n_head=0, rope=None, rope_dims=0, interlea
     check(_lib.lib().pt_kv8_append(ctypes.byref(a), _stream()), "pt_kv8_append")
 
 
-def kv8_attn_workspace(n_tok, n_head, n_kv, vdim, device="cuda"):
-    """Workspace of kv8_attn calls of up to n_tok tokens that follow one another on a stream (any number of layers); zeroed once."""
-    return torch.zeros(_lib.lib().pt_kv8_attn_workspace_bytes(n_tok, n_head, n_kv, vdim), dtype=torch.uint8, device=device)
+def kv8_attn_workspace(n_tok, n_head, n_kv, width, device="cuda"):
+    """Workspace of kv8_attn calls of up to n_tok tokens that follow one another on a stream (any number of layers); zeroed once.  width: the wider of a head's key and value."""
+    return torch.zeros(_lib.lib().pt_kv8_attn_workspace_bytes(n_tok, n_head, n_kv, width), dtype=torch.uint8, device=device)
 
 
 def kv8_attn(view, q, q_ld, cache, out, out_ld, n_head, scale, window=0, softcap=0.0, workspace=None, error_flag=None, plain=False):

@@ -163,7 +163,7 @@ def attend(s, q, window=0, softcap=0.0, out=None, plain=False, workspace=None):
     n = s.view.n_tok
     out = torch.empty((n, s.heads * s.vdim), dtype=s.dtype, device=s.device) if out is None else out
     if workspace is None and not plain:
-        workspace = ops.kv8_attn_workspace(n, s.heads, s.n_kv, s.vdim, s.device)
+        workspace = ops.kv8_attn_workspace(n, s.heads, s.n_kv, max(s.dim, s.vdim), s.device)
     return ops.kv8_attn(s.view, q, q.shape[1], s.cache, out, out.shape[1], s.heads, s.scale, window=window, softcap=softcap, workspace=workspace, error_flag=s.flag, plain=plain)
 
 
