@@ -280,6 +280,7 @@ static int check_cache(const pt_kv8_cache &c, const char *who) {
   PT_REQUIRE(c.n_kv > 0 && c.dim > 0 && c.dim <= MOST_DIM && c.vdim > 0 && c.vdim <= MOST_DIM, "%s: n_kv=%d, heads of %d and %d (1 .. %d)", who, c.n_kv, c.dim, c.vdim, MOST_DIM);
   PT_REQUIRE(c.page_size > 0 && c.max_pages > 0 && (long long)c.page_size * c.max_pages < (1ll << 31) && c.max_len >= 0 && c.max_len <= (long long)c.page_size * c.max_pages,
              "%s: %d pages of %d positions, max_len=%d", who, c.max_pages, c.page_size, c.max_len);
+  PT_REQUIRE((long long)c.n_kv * c.page_size * (c.dim + c.vdim) < (1ll << 31), "%s: a page of 2 GB or more", who);
   PT_REQUIRE(((uintptr_t)c.scales & 3) == 0, "%s: scales on a multiple of 4 bytes", who);
   return PT_OK;
 }
@@ -342,16 +343,23 @@ template <typename T> static cudaError_t launch_plain(const pt_kv8_attn_args &a,
   const auto kernel = a.cache.fmt == PT_KV8_E4M3 ? attn_plain_kernel<T, true> : attn_plain_kernel<T, false>;
   return launch_early(kernel, Grid(dim3(a.batch.n_tok, a.n_head)), PLAIN_WARPS * 32, 0, st, (const T *)a.q, (T *)a.out, p);
 }
-static int launch_blocks(int width) { return sm_count() * (width > 128 ? 2 : BLOCKS_PER_SM); }
-static size_t part_bytes(int width) { return sizeof(float) * (width > 128 ? Shape<256>::PART : width > 64 ? Shape<128>::PART : Shape<64>::PART); }
-template <int SIZE> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
+// A workspace: counters, then (by the width of the heads) pieces of every block.
+static size_t workspace_bytes(int width) {
+  const size_t pieces = width > 128 ? (Shape<256>::WARPS + 2) * Shape<256>::PIECE : width > 64 ? (Shape<128>::WARPS + 2) * Shape<128>::PIECE : (Shape<64>::WARPS + 2) * Shape<64>::PIECE;
+  return sizeof(int) * COUNTERS + sizeof(float) * sm_count() * pieces;
+}
+template <int SIZE, bool FULL> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
   const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype == PT_DT_F32;
-  const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, true, 2> : attn_kernel<SIZE, true, 1>) : (wide ? attn_kernel<SIZE, false, 2> : attn_kernel<SIZE, false, 1>);
+  const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, FULL, true, 2> : attn_kernel<SIZE, FULL, true, 1>) : (wide ? attn_kernel<SIZE, FULL, false, 2> : attn_kernel<SIZE, FULL, false, 1>);
   static std::atomic<uint64_t> allowed[4];
-  constexpr int FIXED = NW * Shape<SIZE>::STAGES * Shape<SIZE>::STAGE + Shape<SIZE>::JOIN;
+  constexpr int WARPS = Shape<SIZE>::WARPS, FIXED = WARPS * Shape<SIZE>::RING;
   const cudaError_t e = allow_smem(kernel, FIXED + (3 * MAX_TOKENS + 1) * (int)sizeof(int), allowed[2 * e4m3 + wide]);
   if (e != cudaSuccess) return e;
-  return launch_early(kernel, Grid(sp.grid), NW * 32, FIXED + (3 * sp.tokens + 1) * sizeof(int), st, p, sp);
+  return launch_early(kernel, Grid(sp.grid), WARPS * 32, FIXED + (3 * sp.tokens + 1) * sizeof(int), st, p, sp);
+}
+template <int SIZE> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, Split sp, cudaStream_t st) {
+  sp.parts = sp.heads + (size_t)sp.grid * Shape<SIZE>::WARPS * Shape<SIZE>::PIECE;
+  return p.c.dim == SIZE && p.c.vdim == SIZE ? launch_attn<SIZE, true>(a, p, sp, st) : launch_attn<SIZE, false>(a, p, sp, st);
 }
 
 }  // namespace kv8
@@ -425,10 +433,7 @@ extern "C" int pt_kv8_unpack(const pt_kv8_unpack_args *a, void *stream) {
   return PT_OK;
 }
 
-extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width) {
-  if (n_tok < 1 || n_kv < 1 || n_head < n_kv) return 0;
-  return kv8::COUNTERS * sizeof(int) + (size_t)kv8::launch_blocks(width) * 2 * kv8::part_bytes(width);
-}
+extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width) { return n_tok < 1 || n_kv < 1 || n_head < n_kv ? 0 : kv8::workspace_bytes(width); }
 
 extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   PT_REQUIRE(a, "pt_kv8_attn: null args");
@@ -464,11 +469,14 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   sp.q_whole = aligned_to(a->q, 16) && (long long)a->q_ld * es % 16 == 0;
   sp.out_whole = aligned_to(a->out, 16) && (long long)a->out_ld * es % 16 == 0;
   sp.counters = (int *)a->workspace;
-  sp.parts = (float *)(sp.counters + kv8::COUNTERS);
+  sp.heads = (float *)(sp.counters + kv8::COUNTERS);
   sp.q = a->q;
   sp.out = a->out;
-  sp.grid = kv8::launch_blocks(width);
-  const int most = std::min(kv8::MAX_TOKENS, kv8::COUNTERS / (a->cache.n_kv * sp.chunks));
+  sp.grid = sm_count();
+  // Tokens of a launch: what its blocks plan in shared memory, a counter for every segment, and tiles that an int counts.
+  const long long segs = (long long)a->cache.n_kv * sp.chunks, tiles = segs * (ceil_div(p.c.max_len, 16) + 1);
+  PT_REQUIRE(tiles < 1ll << 30, "pt_kv8_attn: %lld heads of a history of %d positions", segs, p.c.max_len);
+  const int most = (int)std::min<long long>({kv8::MAX_TOKENS, kv8::COUNTERS / segs, (1ll << 30) / tiles});
   for (; sp.tok0 < a->batch.n_tok; sp.tok0 += most) {
     sp.tokens = std::min(a->batch.n_tok - sp.tok0, most);
     PT_CUDA(width > 128 ? kv8::launch_attn<256>(*a, p, sp, st) : width > 64 ? kv8::launch_attn<128>(*a, p, sp, st) : kv8::launch_attn<64>(*a, p, sp, st));

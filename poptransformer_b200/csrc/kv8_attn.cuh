@@ -1,15 +1,17 @@
 // Attention of new tokens over a cache of eight bits, on tensor cores (included by kv8.cu).
 //
 // A segment is one token, one kv head and up to eight of its query heads; its keys are tiles of KT positions.  All tiles of a launch lie in one row, segment
-// after segment, and every block takes an equal run of them, so that unequal histories cost nobody a wait; the warps of a block take every NW-th tile of its run.
+// after segment; every block takes an equal run of them, and every warp an equal run of its block's, so that unequal histories cost nobody a wait and warps meet
+// once, at their end.  A segment that lies in one warp's run leaves from there; the pieces of others are added up by the block that has all of them, or by the last of the blocks that
+// have some to come (in the order of the pieces, so that the sum does not depend on who was last).
 //   scores [16 keys x 8 heads] = K . q^T,   out^T [16 dims x 8 heads] += V^T . W^T      (mma m16n8k16, fp16 operands, fp32 sums)
 // A lane copies to shared memory (cp.async) exactly what it reads back, so the ring of a warp needs no barrier and no swizzle: 16 bytes of two key rows (row of the fragment), 16
 // bytes of four value rows (its keys).  Which dimension of the head is which k of an instruction does not matter as long as K and q agree: a lane's k are the dimensions of
 // its bytes.  Bytes become fp16 exactly: int8 b as (1024 + 128 + b) - 1152, E4M3 by its bits (times 2^-8, which the scales take back).
 //
 // Numbers.  q comes in fp16 times a power of two that brings its row's largest element to [1, 2): what is lost lies below 2^-25 of that; queries of 32 bits have a second fp16 part.
-// With x = score log2(e), v_j = bytes times vs_j, and e_j the exponent of vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
-// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, at most 2^15: rounded to fp16 once (2^-11; two parts for rows of 32 bits), whole down to 2^-29 of the largest and then off by
+// With x = score log2(e), v_j = bytes times vs_j, and e_j about log2 vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
+// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once (2^-11; two parts for rows of 32 bits), whole down to 2^-29 of the largest and then off by
 // 2^-40 of it, however far the scales of the values lie apart.
 #pragma once
 #include <type_traits>
@@ -19,20 +21,20 @@
 namespace pt {
 namespace kv8 {
 
-constexpr int NW = 4, HEADS = 8, MAX_TOKENS = 1024;
+constexpr int HEADS = 8, MAX_TOKENS = 1024;
 constexpr int COUNTERS = 1 << 16;      // of a workspace, always in front: whichever calls share one, nothing else is written there
 
 // SIZE: the widest head, 64, 128 or 256.
 template <int SIZE> struct Shape {
+  static constexpr int WARPS = SIZE == 256 ? 8 : 12;    // one block to an SM: 168 registers a thread (254), 16.5 KB of shared memory a warp
   static constexpr int KT = SIZE == 256 ? 16 : 32, GROUPS = KT / 16, STAGES = SIZE == 64 ? 4 : 2;   // 8 KB of a warp's ring are on their way while 8 KB are in use
   static constexpr int NK = SIZE / 64;                  // 16-byte runs of a key row per lane
   static constexpr int VB = SIZE == 64 ? 8 : 16, NV = SIZE == 256 ? 2 : 1;   // bytes of a run of a value row, runs per lane
   static constexpr int MT = SIZE / 16;                  // tiles of 16 output dimensions
-  static constexpr int K_BYTES = GROUPS * 2 * NK * 512, V_BYTES = GROUPS * 4 * NV * VB * 32, STAGE = K_BYTES + V_BYTES + GROUPS * 128;
-  static constexpr int JOIN = MT * 4 * 32 * 4;          // a warp's sums
-  static constexpr int PART = JOIN / 4 + 2 * HEADS;     // ... with maxima and totals, in floats
+  static constexpr int K_BYTES = GROUPS * 2 * NK * 512, V_BYTES = GROUPS * 4 * NV * VB * 32, STAGE = K_BYTES + V_BYTES + GROUPS * 128, RING = STAGES * STAGE;
+  static constexpr int PIECE = MT * 4 * 32 + 2 * HEADS; // floats of a piece of a segment: a warp's sums, maxima and totals
+  static_assert(PIECE * 4 <= RING, "a warp's last piece takes the place of its keys and values");
 };
-constexpr int BLOCKS_PER_SM = 3;
 
 struct Plan {     // of a launch, in the shared memory of every block
   int *cum, *pos, *slot;      // [tokens + 1] tiles before, [tokens] position (of the token), [tokens]
@@ -41,15 +43,20 @@ struct Split {
   int tok0, tokens, chunks;   // the launch's tokens; parts of a kv head's query heads
   int grid, dtype, q_whole, out_whole;
   int *counters;              // [COUNTERS], zero between launches; [token][segment]
-  float *parts;               // [grid][2][PART]
+  float *heads;               // [grid][WARPS][PIECE]: the pieces that warps begin with and do not end with
+  float *parts;               // [grid][2][PIECE]: what blocks have of segments that are not theirs alone, in front and at their end
   const void *q;
   void *out;
 };
 
-__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes, bool in) {
-  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-  else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(in ? 8 : 0) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+// Asynchronous copies of B bytes; zeros where !in (the source is then not read).
+template <int B> __device__ __forceinline__ void copy_whole(uint32_t dst, const void *src) {
+  if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(B) : "memory");
+}
+template <int B> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool in) {
+  if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(in ? B : 0) : "memory");
 }
 template <int N> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -132,6 +139,12 @@ template <int N> __device__ __forceinline__ void store_n(void *out, size_t at, i
   else run((__nv_bfloat16 *)out);
 }
 
+__device__ __forceinline__ void store_one(void *out, size_t at, int dtype, float v) {
+  if (dtype == PT_DT_F32) ((float *)out)[at] = v;
+  else if (dtype == PT_DT_F16) ((__half *)out)[at] = from_f<__half>(v);
+  else ((__nv_bfloat16 *)out)[at] = from_f<__nv_bfloat16>(v);
+}
+
 // Where a run of tiles has come to: token, segment of it, tile of that.
 struct Walk {
   int tok, seg, tile, tiles;
@@ -147,20 +160,67 @@ __device__ __forceinline__ void settle(Walk &w, const Plan &pl, int segs, int to
     }
   }
 }
+__device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, int tokens) {
+  Walk w;
+  const int x = at / segs;
+  int lo = 0, hi = tokens - 1;       // the last token whose tiles begin at or before x: it has some
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (pl.cum[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  w.tok = lo;
+  w.tiles = pl.cum[lo + 1] - pl.cum[lo];
+  const int rest = at - pl.cum[lo] * segs;
+  w.seg = rest / w.tiles;
+  w.tile = rest - w.seg * w.tiles;
+  return w;
+}
 
-template <int SIZE, bool E4M3, int PARTS>
-__global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn_kernel(const Attn p, const Split sp) {
+// Pieces of one segment added up, unit j (four floats of every lane) of each: the sum, and l and R of heads 2 tg and 2 tg + 1.
+struct Joined { float4 o; float L[2], R[2]; };
+// OTHERS: other blocks have written them; else they may lie in shared memory.
+template <int SIZE, bool OTHERS, typename At> __device__ __forceinline__ Joined add_pieces(int from, int to, int j, int lane, const At &at) {
+  constexpr int SUMS = Shape<SIZE>::PIECE - 2 * HEADS;
+  auto load = [](const float *p, int i) { return OTHERS ? __ldcg(reinterpret_cast<const float4 *>(p) + i) : reinterpret_cast<const float4 *>(p)[i]; };
+  Joined r;
+  r.o = make_float4(0.f, 0.f, 0.f, 0.f);
+  r.R[0] = r.R[1] = -INFINITY;
+  r.L[0] = r.L[1] = 0.f;
+#pragma unroll 4
+  for (int i = from; i < to; ++i) {
+    const float *p = at(i);
+    if (!p) continue;
+    const float4 ml = load(p + SUMS, lane & 3);
+    r.R[0] = fmaxf(r.R[0], ml.x);
+    r.R[1] = fmaxf(r.R[1], ml.z);
+  }
+#pragma unroll 4
+  for (int i = from; i < to; ++i) {
+    const float *p = at(i);
+    if (!p) continue;
+    const float4 ml = load(p + SUMS, lane & 3), o = load(p, j * 32 + lane);
+    const float f0 = ml.x == r.R[0] ? 1.f : exp2_fast(ml.x - r.R[0]), f1 = ml.z == r.R[1] ? 1.f : exp2_fast(ml.z - r.R[1]);
+    r.L[0] += ml.y * f0;
+    r.L[1] += ml.w * f1;
+    r.o.x += o.x * f0; r.o.y += o.y * f1; r.o.z += o.z * f0; r.o.w += o.w * f1;
+  }
+  return r;
+}
+
+// FULL: keys and values are as wide as SIZE.
+template <int SIZE, bool FULL, bool E4M3, int PARTS>
+__global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const Attn p, const Split sp) {
   early_start();
   using S = Shape<SIZE>;
-  constexpr int KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
+  constexpr int NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float join_ml[2 * HEADS];
-  __shared__ int scan[NW];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tg = lane & 3;
+  __shared__ int scan[NW], piece[2 * NW], last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, tg = lane & 3;
+  const int dim = FULL ? SIZE : p.c.dim, vdim = FULL ? SIZE : p.c.vdim;
   const int G = p.c.n_kv, qpk = p.heads / G, segs = G * sp.chunks, tokens = sp.tokens;
-  float *join = reinterpret_cast<float *>(smem + NW * STAGES * S::STAGE);
   Plan pl;
-  pl.cum = reinterpret_cast<int *>(smem + NW * STAGES * S::STAGE + S::JOIN);
+  pl.cum = reinterpret_cast<int *>(smem + NW * S::RING);
   pl.pos = pl.cum + tokens + 1;
   pl.slot = pl.pos + tokens;
 
@@ -202,142 +262,131 @@ __global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn
     __syncthreads();
   }
   if (tid == 0) pl.cum[0] = 0;
+  if (tid < 2 * NW) piece[tid] = -1;
   __syncthreads();
-  const long long all = (long long)before * segs, per = max((long long)NW, (all + sp.grid - 1) / sp.grid), run0 = blockIdx.x * per, run1 = min(all, run0 + per);
-  if (run0 >= run1) return;
+  const int all = before * segs, per = max(NW, (all + sp.grid - 1) / sp.grid), block0 = blockIdx.x * per, block_n = min(per, all - block0);
+  if (block_n <= 0) return;
 
-  // ---- the segment that the run begins in, and where this warp begins
-  Walk from;
-  {
-    const int x = (int)(run0 / segs);
-    int lo = 0, hi = tokens - 1;       // the last token whose tiles begin at or before x, and which has some
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (pl.cum[mid] <= x) lo = mid;
-      else hi = mid - 1;
-    }
-    from.tok = lo;
-    from.tiles = pl.cum[lo + 1] - pl.cum[lo];
-    const long long rest = run0 - (long long)pl.cum[lo] * segs;
-    from.seg = (int)(rest / from.tiles);
-    from.tile = (int)(rest - (long long)from.seg * from.tiles);
-  }
-  const int count = (int)(run1 - run0);
-  unsigned char *ring = smem + warp * STAGES * S::STAGE;
-  const uint32_t ring_s = smem_addr(ring);
-
-  // ---- copies: a tile a call, STAGES - 1 ahead of what is used
-  Walk ahead = from;
-  ahead.tile += warp;
-  settle(ahead, pl, segs, tokens);
-  int ahead_at = warp, stage_in = 0, listed_tok = -1, listed_seg = -1, listed_tile = 0, page_l = 0, row_l = 0;
-  auto fetch = [&]() {
-    if (ahead_at < count) {
-      const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
-      // (pages of the next tiles of this warp in this segment, one group of 16 positions a lane)
-      if (ahead.tok != listed_tok || ahead.seg != listed_seg || ahead.tile - listed_tile >= 32 / GROUPS * NW) {
-        listed_tok = ahead.tok; listed_seg = ahead.seg; listed_tile = ahead.tile;
-        const int at = (first + ahead.tile + lane / GROUPS * NW) * KT + lane % GROUPS * 16;
-        const int pg = at <= pos ? at / p.c.page : 0;
-        page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
-        row_l = at - pg * p.c.page;
-        if (page_l < 0) {
-          if (p.error_flag) atomicExch(p.error_flag, 12);
-          page_l = 0;
+  // ---- this warp's run
+  const int run0 = block0 + block_n * warp / NW, count = block0 + block_n * (warp + 1) / NW - run0;
+  unsigned char *ring = smem + warp * S::RING;
+  if (count > 0) {
+    Walk w = walk_to(run0, pl, segs, tokens), ahead = w;
+    const uint32_t ring_s = smem_addr(ring) + lane * 16;
+    // copies: a tile a call, STAGES - 1 ahead of what is used.  A lane knows the page and the row in it of one of the next 32 groups of 16 positions.
+    int ahead_at = 0, stage_in = 0, listed = 0, list_end = 0, page_l = 0, row_l = 0, kvh_in = 0;
+    auto fetch = [&]() {
+      if (ahead_at < count) {
+        if (ahead_at >= list_end) {      // (a segment's first tile, or the list has been used up)
+          const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
+          const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? at / p.c.page : 0;
+          row_l = at <= pos ? at - pg * p.c.page : -1;      // (-1: behind the last position)
+          page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
+          if (page_l < 0) {
+            if (p.error_flag) atomicExch(p.error_flag, 12);
+            page_l = 0;
+          }
+          listed = ahead_at;
+          list_end = ahead_at + min(32 / GROUPS, ahead.tiles - ahead.tile);
+          kvh_in = ahead.seg / sp.chunks;
         }
-      }
-      const int kvh = ahead.seg / sp.chunks, in_list = (ahead.tile - listed_tile) / NW * GROUPS;
-      const uint32_t st = ring_s + stage_in * S::STAGE;
+        const uint32_t st = ring_s + stage_in * S::STAGE;
 #pragma unroll
-      for (int u = 0; u < GROUPS; ++u) {
-        const int page = __shfl_sync(0xffffffffu, page_l, in_list + u), row = __shfl_sync(0xffffffffu, row_l, in_list + u);
-        const bool in = (first + ahead.tile) * KT + 16 * u <= pos;
-        const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes;
-        const unsigned char *k = base + ((size_t)kvh * p.c.page + (in ? row : 0) + g) * p.c.dim + 16 * tg;
-        const unsigned char *v = base + (size_t)G * p.c.page * p.c.dim + ((size_t)kvh * p.c.page + (in ? row : 0) + 2 * tg) * p.c.vdim + VB * g;
+        for (int u = 0; u < GROUPS; ++u) {
+          const int page = __shfl_sync(0xffffffffu, page_l, (ahead_at - listed) * GROUPS + u), row = __shfl_sync(0xffffffffu, row_l, (ahead_at - listed) * GROUPS + u);
+          const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes;
+          const unsigned char *k = base + (kvh_in * p.c.page + row + g) * dim + 16 * tg;
+          const unsigned char *v = base + (G * p.c.page) * dim + (kvh_in * p.c.page + row + 2 * tg) * vdim + VB * g;
+          const float *sc = p.c.scales + (size_t)page * (2 * G * p.c.page) + ((lane >> 4) * G + kvh_in) * p.c.page + row + (lane & 15);
+          const uint32_t st_v = st + S::K_BYTES + u * (4 * NV * VB * 32) - (VB == 8 ? lane * 8 : 0), st_s = st + S::K_BYTES + S::V_BYTES + u * 128 - lane * 12;
+          if (FULL && row >= 0) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            const bool here = in && 16 * tg + 64 * i < p.c.dim;
-            copy_async(st + ((u * 2 + r) * NK + i) * 512 + lane * 16, here ? k + (size_t)(8 * r) * p.c.dim + 64 * i : base, 16, here);
+              for (int i = 0; i < NK; ++i) copy_whole<16>(st + ((u * 2 + r) * NK + i) * 512, k + 8 * r * SIZE + 64 * i);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int i = 0; i < NV; ++i) copy_whole<VB>(st_v + (r * NV + i) * (VB * 32), v + ((r & 1) + 8 * (r >> 1)) * SIZE + 128 * i);
+            copy_whole<4>(st_s, sc);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < NK; ++i) {
+                const bool here = row >= 0 && 16 * tg + 64 * i < dim;
+                copy_async<16>(st + ((u * 2 + r) * NK + i) * 512, here ? k + 8 * r * dim + 64 * i : base, here);
+              }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int i = 0; i < NV; ++i) {
+                const bool here = row >= 0 && VB * g + 128 * i < vdim;
+                copy_async<VB>(st_v + (r * NV + i) * (VB * 32), here ? v + ((r & 1) + 8 * (r >> 1)) * vdim + 128 * i : base, here);
+              }
+            copy_async<4>(st_s, row >= 0 ? sc : p.c.scales, row >= 0);
           }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int i = 0; i < NV; ++i) {
-            const bool here = in && VB * g + 128 * i < p.c.vdim;
-            copy_async(st + S::K_BYTES + ((u * 4 + r) * NV + i) * (VB * 32) + lane * VB, here ? v + (size_t)((r & 1) + 8 * (r >> 1)) * p.c.vdim + 128 * i : base, VB, here);
-          }
-        copy_async(st + S::K_BYTES + S::V_BYTES + u * 128 + lane * 4,
-                   p.c.scales + (((size_t)page * 2 + (lane >> 4)) * G + kvh) * p.c.page + (in ? row : 0) + (lane & 15), 4, in);
+        }
+        ++ahead_at;
+        ++ahead.tile;
+        settle(ahead, pl, segs, tokens);
+        if (++stage_in == STAGES) stage_in = 0;
       }
-      ahead_at += NW;
-      ahead.tile += NW;
-      settle(ahead, pl, segs, tokens);
-      if (++stage_in == STAGES) stage_in = 0;
-    }
-    copies_end();       // (the groups are counted)
-  };
+      copies_end();       // (the groups are counted)
+    };
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) fetch();
+    for (int s = 0; s < STAGES - 1; ++s) fetch();
 
-  // ---- segment after segment
-  Walk w = from;
-  int done = 0, mine = warp, stage = 0;       // tiles of the run that lie behind; this warp's next
-  while (done < count) {
-    const int here = min(count - done, w.tiles - w.tile), tok = w.tok;      // tiles of this segment that are the block's
-    const int kvh = w.seg / sp.chunks, chunk = w.seg - kvh * sp.chunks, head0 = kvh * qpk + chunk * HEADS, heads = min(HEADS, qpk - chunk * HEADS);
-    const int pos = pl.pos[tok], begin = p.window > 0 ? max(0, pos - p.window + 1) : 0, first = begin / KT;
-    float O[MT][4], R[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+    int done = 0, stage = 0;
+    while (done < count) {      // segment after segment
+      const int here = min(count - done, w.tiles - w.tile), tok = w.tok;      // tiles of this segment that are the warp's
+      const int kvh = w.seg / sp.chunks, chunk = w.seg - kvh * sp.chunks, head0 = kvh * qpk + chunk * HEADS, heads = min(HEADS, qpk - chunk * HEADS);
+      const int pos = pl.pos[tok], begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      float O[MT][4], R[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < MT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
-    if (mine < done + here) {
+      for (int j = 0; j < MT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
       // q as B operand: lane (g, tg) holds head g's dimensions 64 i + 16 tg + 4 c + {0, 2} and {1, 3} of k step 4 i + c
       uint32_t qf[PARTS][NK * 4][2];
-      float unit;
+      float by[2];          // factors of the scores of heads 2 tg and 2 tg + 1
       {
         float x[NK][16], most = 0.f;
-        const size_t at = (size_t)(sp.tok0 + tok) * p.q_ld + (size_t)(head0 + g) * p.c.dim + 16 * tg;
+        const size_t at = (size_t)(sp.tok0 + tok) * p.q_ld + (size_t)(head0 + g) * dim + 16 * tg;
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          load16(sp.q, at + 64 * i, sp.dtype, sp.q_whole, g < heads ? p.c.dim - 64 * i - 16 * tg : 0, x[i]);
+        for (int i = 0; i < NK; ++i) load16(sp.q, at + 64 * i, sp.dtype, sp.q_whole, g < heads ? dim - 64 * i - 16 * tg : 0, x[i]);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(x[i][j]));
-        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // the power of two at or below the largest element (1 for a row of zeros or infinities; 2^-120 at least, so that its reciprocal is a number)
-        const uint32_t e = __float_as_uint(most) >> 23;
-        const uint32_t f = e == 0 ? (most == 0.f ? 127u : 7u) : e == 255 ? 127u : min(max(e, 7u), 247u);
-        const float by = __uint_as_float((254u - f) << 23);
-        unit = __uint_as_float(f << 23);
+        // the power of two at or below the largest element (1 for a row of zeros or infinities; within 2^-120 .. 2^120, so that its reciprocal is a number)
+        const uint32_t e = __float_as_uint(most) >> 23, f = most == 0.f || e == 255 ? 127u : min(max(e, 7u), 247u);
+        const float turn = __uint_as_float((254u - f) << 23), unit = __uint_as_float(f << 23);
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-              const float a = x[i][4 * c + o] * by, b = x[i][4 * c + o + 2] * by;
+              const float a = x[i][4 * c + o] * turn, b = x[i][4 * c + o + 2] * turn;
               qf[0][4 * i + c][o] = pack2(a, b);
               if constexpr (PARTS == 2) {
                 const float2 h = unpack2(qf[0][4 * i + c][o]);
                 qf[PARTS - 1][4 * i + c][o] = pack2(a - h.x, b - h.y);
               }
             }
-      }
-      // factors of the scores of heads 2 tg and 2 tg + 1, whose q rows lanes 8 tg and 8 tg + 4 have
-      float by[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) by[h] = __shfl_sync(0xffffffffu, unit, 8 * tg + 4 * h) * (p.scale * byte_unit<E4M3>());
+        for (int h = 0; h < 2; ++h) by[h] = __shfl_sync(0xffffffffu, unit, 8 * tg + 4 * h) * (p.scale * byte_unit<E4M3>());     // (lanes 8 tg and 8 tg + 4 have their rows)
+      }
       const float log2e = 1.4426950408889634f;
-      for (; mine < done + here; mine += NW) {
+      if (!(p.softcap > 0.f)) { by[0] *= log2e; by[1] *= log2e; }
+      int key0 = (begin / KT + w.tile) * KT;
+      for (int t = 0; t < here; ++t, key0 += KT) {
         fetch();
         copies_left<STAGES - 1>();
         __syncwarp();
         const unsigned char *st = ring + stage * S::STAGE;
         const float *sc = reinterpret_cast<const float *>(st + S::K_BYTES + S::V_BYTES);
-        const int key0 = (first + w.tile + mine - done) * KT;
         float x[GROUPS][4];
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
@@ -363,26 +412,30 @@ __global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn
 #pragma unroll
           for (int u = 0; u < GROUPS; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[u][e] = p.softcap * tanhf(x[u][e] / p.softcap);
+            for (int e = 0; e < 4; ++e) x[u][e] = p.softcap * tanhf(x[u][e] / p.softcap) * log2e;
         }
-        const bool border = key0 < begin || key0 + KT > pos + 1;
+        // about log2 of the value scales: exponent and mantissa as one number (at most 0.09 below; no less than -80: appended scales are above that)
         float vs[GROUPS][2], ev[GROUPS][2];
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             vs[u][r] = sc[u * 32 + 16 + 8 * r + g];
-            ev[u][r] = (float)(min(max((int)(__float_as_uint(vs[u][r]) >> 23 & 255u), 47), 191) - 127);      // (2^-80 .. 2^64: appended scales are within)
+            ev[u][r] = fmaxf(fmaf((float)__float_as_int(vs[u][r]), 1.f / (1 << 23), -127.f), -80.f);
+          }
+        if (key0 < begin || key0 + KT > pos + 1) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              x[u][2 * r + h] *= log2e;
-              if (border) {
-                const int key = key0 + 16 * u + 8 * r + g;
-                if (key < begin || key > pos) x[u][2 * r + h] = -INFINITY;
+          for (int u = 0; u < GROUPS; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int key = key0 + 16 * u + 8 * r + g;
+              if (key < begin || key > pos) {
+                x[u][2 * r] = x[u][2 * r + 1] = -INFINITY;
+                vs[u][r] = 0.f;
+                ev[u][r] = 0.f;
               }
             }
-            if (border && (key0 + 16 * u + 8 * r + g < begin || key0 + 16 * u + 8 * r + g > pos)) vs[u][r] = 0.f;
-          }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float m = R[h];
@@ -390,9 +443,9 @@ __global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn
           for (int u = 0; u < GROUPS; ++u) m = fmaxf(m, fmaxf(x[u][h] + ev[u][0], x[u][2 + h] + ev[u][1]));
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const float was = R[h] == m ? 1.f : exp2_fast(R[h] - m);
-          R[h] = m;
-          if (__any_sync(0xffffffffu, was != 1.f)) {
+          if (__any_sync(0xffffffffu, R[h] != m)) {
+            const float was = R[h] == m ? 1.f : exp2_fast(R[h] - m);
+            R[h] = m;
             L[h] *= was;
 #pragma unroll
             for (int j = 0; j < MT; ++j) { O[j][h] *= was; O[j][2 + h] *= was; }
@@ -402,9 +455,9 @@ __global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn
           for (int u = 0; u < GROUPS; ++u)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const float t = exp2_fast(x[u][2 * r + h] - ref);
-              L[h] += t;
-              x[u][2 * r + h] = t * vs[u][r];
+              const float e = exp2_fast(x[u][2 * r + h] - ref);
+              L[h] += e;
+              x[u][2 * r + h] = e * vs[u][r];
             }
         }
 #pragma unroll
@@ -452,109 +505,95 @@ __global__ void __launch_bounds__(NW * 32, SIZE == 256 ? 2 : BLOCKS_PER_SM) attn
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) L[h] += __shfl_xor_sync(0xffffffffu, L[h], o);
-    }
 
-    // ---- the warps' sums come together in warp 0, one after the other
-    for (int j0 = 0; j0 < min(here, NW); ++j0) {
-      const int who = (int)((done + j0) % NW);       // (the warps that have tiles of it)
-      if (who == 0) continue;
-      __syncthreads();
-      if (warp == who) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j) reinterpret_cast<float4 *>(join)[j * 32 + lane] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
-        if (g == 0) {
-          join_ml[4 * tg] = R[0]; join_ml[4 * tg + 1] = L[0];
-          join_ml[4 * tg + 2] = R[1]; join_ml[4 * tg + 3] = L[1];
-        }
-      }
-      __syncthreads();
-      if (warp == 0) {
-        float mine_by[2], its_by[2];
+      done += here;
+      if (here == w.tiles) {          // a whole segment leaves
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float r = join_ml[4 * tg + 2 * h], l = join_ml[4 * tg + 2 * h + 1], m = fmaxf(R[h], r);
-          mine_by[h] = R[h] == m ? 1.f : exp2_fast(R[h] - m);
-          its_by[h] = r == m ? 1.f : exp2_fast(r - m);
-          R[h] = m;
-          L[h] = L[h] * mine_by[h] + l * its_by[h];
-        }
+          if (2 * tg + h >= heads) continue;
+          const float f = byte_unit<E4M3>() / L[h];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const float4 o = reinterpret_cast<const float4 *>(join)[j * 32 + lane];
-          O[j][0] = O[j][0] * mine_by[0] + o.x * its_by[0]; O[j][1] = O[j][1] * mine_by[1] + o.y * its_by[1];
-          O[j][2] = O[j][2] * mine_by[0] + o.z * its_by[0]; O[j][3] = O[j][3] * mine_by[1] + o.w * its_by[1];
-        }
-      }
-    }
-
-    // ---- a whole segment leaves; of a part the last block to come finds the others'
-    const long long seg_tile0 = run0 + done - w.tile, seg_tile1 = seg_tile0 + w.tiles;
-    const int b0 = (int)(seg_tile0 / per), b1 = (int)((seg_tile1 - 1) / per);
-    bool write = warp == 0;
-    if (b1 > b0) {
-      constexpr int PART = S::PART;
-      const int id = tok * segs + w.seg;
-      if (warp == 0) {
-        float *to = sp.parts + ((size_t)blockIdx.x * 2 + (seg_tile0 > run0 ? 1 : 0)) * PART;
+          for (int i = 0; i < NV; ++i) {
+            if (VB * g + 128 * i >= vdim) continue;
+            float y[VB];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) __stcg(reinterpret_cast<float4 *>(to) + j * 32 + lane, make_float4(O[j][0], O[j][1], O[j][2], O[j][3]));
-        if (g == 0) __stcg(reinterpret_cast<float4 *>(to + S::JOIN / 4) + tg, make_float4(R[0], L[0], R[1], L[1]));
-        __threadfence();
-        __syncwarp();
-        int last = lane == 0 ? atomicAdd(sp.counters + id, 1) == b1 - b0 : 0;
-        write = __shfl_sync(0xffffffffu, last, 0);
-      }
-      if (write) {
-        __threadfence();
-        if (lane == 0) sp.counters[id] = 0;
-        auto part_of = [&](int b) { return sp.parts + ((size_t)b * 2 + (seg_tile0 > b * per ? 1 : 0)) * PART; };
-        R[0] = R[1] = -INFINITY;
-        L[0] = L[1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < MT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
-        for (int b = b0; b <= b1; ++b) {
-          const float4 ml = __ldcg(reinterpret_cast<const float4 *>(part_of(b) + S::JOIN / 4) + tg);
-          R[0] = fmaxf(R[0], ml.x);
-          R[1] = fmaxf(R[1], ml.z);
-        }
-        for (int b = b0; b <= b1; ++b) {
-          const float *from_part = part_of(b);
-          const float4 ml = __ldcg(reinterpret_cast<const float4 *>(from_part + S::JOIN / 4) + tg);
-          const float f0 = ml.x == R[0] ? 1.f : exp2_fast(ml.x - R[0]), f1 = ml.z == R[1] ? 1.f : exp2_fast(ml.z - R[1]);
-          L[0] += ml.y * f0;
-          L[1] += ml.w * f1;
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            const float4 o = __ldcg(reinterpret_cast<const float4 *>(from_part) + j * 32 + lane);
-            O[j][0] += o.x * f0; O[j][1] += o.y * f1; O[j][2] += o.z * f0; O[j][3] += o.w * f1;
+            for (int j = 0; j < VB / 2; ++j) {
+              y[2 * j] = O[i * 8 + j][h] * f;
+              y[2 * j + 1] = O[i * 8 + j][2 + h] * f;
+            }
+            store_n<VB>(sp.out, (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(head0 + 2 * tg + h) * vdim + VB * g + 128 * i, sp.dtype, sp.out_whole, y);
           }
         }
-      }
-    }
-    if (write) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (2 * tg + h >= heads) continue;
-        const float by = byte_unit<E4M3>() / L[h];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          constexpr int N = VB;            // dimensions VB g + 128 i .. of this lane
-          if (VB * g + 128 * i >= p.c.vdim) continue;
-          float y[N];
-#pragma unroll
-          for (int j = 0; j < N / 2; ++j) {
-            y[2 * j] = O[i * 8 + j][h] * by;
-            y[2 * j + 1] = O[i * 8 + j][2 + h] * by;
-          }
-          store_n<N>(sp.out, (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(head0 + 2 * tg + h) * p.c.vdim + VB * g + 128 * i, sp.dtype, sp.out_whole, y);
+      } else {                        // a piece stays: the last one in shared memory, where no tile is needed any more
+        const bool end = done == count;
+        float *to = end ? reinterpret_cast<float *>(ring) : sp.heads + ((size_t)blockIdx.x * NW + warp) * S::PIECE;
+        if (end) {
+          copies_left<0>();
+          __syncwarp();
         }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) reinterpret_cast<float4 *>(to)[j * 32 + lane] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
+        if (g == 0) reinterpret_cast<float4 *>(to + MT * 128)[tg] = make_float4(R[0], L[0], R[1], L[1]);
+        if (lane == 0) piece[2 * warp + end] = tok * segs + w.seg;
       }
+      w.tile += here;
+      settle(w, pl, segs, tokens);
     }
-    done += here;
-    w.tile += here;
-    settle(w, pl, segs, tokens);
+    copies_left<0>();
   }
-  copies_left<0>();
+  __syncthreads();
+
+  // ---- pieces of a segment come together
+  auto leave = [&](const Joined &r, int id, int j) {
+    const int tok = id / segs, seg = id - tok * segs, kvh = seg / sp.chunks, chunk = seg - kvh * sp.chunks, heads = min(HEADS, qpk - chunk * HEADS);
+    const int d = VB * g + 128 * (j / 8) + 2 * (j % 8);
+    const float o[2][2] = {{r.o.x, r.o.z}, {r.o.y, r.o.w}};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (2 * tg + h >= heads || d >= vdim) continue;
+      const float f = byte_unit<E4M3>() / r.L[h];
+      const size_t at = (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(kvh * qpk + chunk * HEADS + 2 * tg + h) * vdim + d;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) store_one(sp.out, at + e, sp.dtype, o[h][e] * f);
+    }
+  };
+  for (int i0 = 0; i0 < 2 * NW;) {
+    const int id = piece[i0];
+    int i1 = i0 + 1;
+    if (id >= 0) {
+      while (i1 < 2 * NW && (piece[i1] == id || piece[i1] < 0)) ++i1;
+      auto mine = [&](int i) -> const float * {
+        return piece[i] < 0 ? nullptr : i & 1 ? reinterpret_cast<const float *>(smem + (i >> 1) * S::RING) : sp.heads + ((size_t)blockIdx.x * NW + (i >> 1)) * S::PIECE;
+      };
+      const int tok = id / segs, tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per, b1 = (tile0 + tiles - 1) / per;
+      float *part = sp.parts + ((size_t)blockIdx.x * 2 + (tile0 > block0)) * S::PIECE;
+      for (int j = warp; j < MT; j += NW) {
+        const Joined r = add_pieces<SIZE, false>(i0, i1, j, lane, mine);
+        if (b0 == b1) {
+          leave(r, id, j);
+        } else {
+          __stcg(reinterpret_cast<float4 *>(part) + j * 32 + lane, r.o);
+          if (j == 0 && g == 0) __stcg(reinterpret_cast<float4 *>(part + MT * 128) + tg, make_float4(r.R[0], r.L[0], r.R[1], r.L[1]));
+        }
+      }
+      if (b0 != b1) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          last = atomicAdd(sp.counters + id, 1) == b1 - b0;
+          if (last) sp.counters[id] = 0;
+          __threadfence();
+        }
+        __syncthreads();
+        if (last) {
+          auto theirs = [&](int b) -> const float * { return sp.parts + ((size_t)b * 2 + (tile0 > b * per)) * S::PIECE; };
+          for (int j = warp; j < MT; j += NW) leave(add_pieces<SIZE, true>(b0, b1 + 1, j, lane, theirs), id, j);
+        }
+        __syncthreads();
+      }
+    }
+    i0 = i1;
+  }
 }
 
 }  // namespace kv8
