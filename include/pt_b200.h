@@ -926,7 +926,7 @@ int pt_kv_move_rows(const pt_kv_pool *pools_host, int n_pools, int page_size, in
  * [n_kv][page_size][vdim], a byte each; its scales are fp32 [2][n_kv][page_size], K's and then V's.  A row x of one position and head is
  * kept as  byte_i = round(x_i (top / m)),  scale = m / top,  with m = max |x_i|, at least 2^-64, and top 127 (int8, rounded to nearest even) or 448
  * (E4M3).  A row that has a NaN, an infinity or a magnitude above 2^64 gets the scale NaN and bytes of 0: it reads back as NaN.  E4M3 bytes that are NaN are
- * never written, and what they read as is not said.  page_table is [slots][max_pages]; dim and vdim are at most 256.
+ * never written, and read as NaN.  page_table is [slots][max_pages]; dim and vdim are at most 256.
  * All three calls: rows that no sequence has (from cu[n_seq] on) are neither read nor written; a sequence whose positions reach max_len sets error_flag to 12
  * and its rows and pages are left as they were, and so are positions whose page is negative. */
 #define PT_KV8_INT8 0

@@ -473,6 +473,11 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   sp.q = a->q;
   sp.out = a->out;
   sp.grid = sm_count();
+  sp.segs = a->cache.n_kv * sp.chunks;
+  sp.by_segs = kv8::Divide::by(sp.segs);
+  sp.by_chunks = kv8::Divide::by(sp.chunks);
+  sp.by_page = kv8::Divide::by(p.c.page);
+  sp.by_grid = kv8::Divide::by(sp.grid);
   // Tokens of a launch: what its blocks plan in shared memory, a counter for every segment, and tiles that an int counts.
   const long long segs = (long long)a->cache.n_kv * sp.chunks, tiles = segs * (ceil_div(p.c.max_len, 16) + 1);
   PT_REQUIRE(tiles < 1ll << 30, "pt_kv8_attn: %lld heads of a history of %d positions", segs, p.c.max_len);

@@ -5,11 +5,14 @@
 // once, at their end.  A segment that lies in one warp's run leaves from there; the pieces of others are added up by the block that has all of them, or by the last of the blocks that
 // have some to come (in the order of the pieces, so that the sum does not depend on who was last).
 //   scores [16 keys x 8 heads] = K . q^T,   out^T [16 dims x 8 heads] += V^T . W^T      (mma m16n8k16, fp16 operands, fp32 sums)
-// A lane copies to shared memory (cp.async) exactly what it reads back, so the ring of a warp needs no barrier and no swizzle: 16 bytes of two key rows (row of the fragment), 16
+// Rows come to a warp's ring by asynchronous copies of 512 bytes that lie together (16 a lane; copies in the order of the fragments, four or eight rows each, reached 4.8 TB/s alone,
+// these 6.5), and are read as fragments: a lane has 16 bytes of two key rows (row of the fragment), 16
 // bytes of four value rows (its keys).  Which dimension of the head is which k of an instruction does not matter as long as K and q agree: a lane's k are the dimensions of
-// its bytes.  Bytes become fp16 exactly: int8 b as (1024 + 128 + b) - 1152, E4M3 by its bits (times 2^-8, which the scales take back).
+// its bytes.  Keys of int8 are multiplied as they are, with q in three parts of 8 bits (m16n8k32, whole numbers); all other bytes become fp16, exactly: E4M3 by conversion, int8 b as
+// (1024 + 128 + b) - 1152.  (Both at fp16 a tile of 32 keys took 270 cycles of an SM, 350 is what its bytes take to come.)
 //
-// Numbers.  q comes in fp16 times a power of two that brings its row's largest element to [1, 2): what is lost lies below 2^-25 of that; queries of 32 bits have a second fp16 part.
+// Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), with a second part of what is
+// left for queries of 32 bits: what is lost lies below 2^-25 of the largest.
 // With x = score log2(e), v_j = bytes times vs_j, and e_j about log2 vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
 // w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once (2^-11; two parts for rows of 32 bits), whole down to 2^-29 of the largest and then off by
 // 2^-40 of it, however far the scales of the values lie apart.
@@ -22,6 +25,10 @@ namespace pt {
 namespace kv8 {
 
 constexpr int HEADS = 8, MAX_TOKENS = 1024;
+#ifndef KV8_SHORT
+#define KV8_SHORT 4
+#endif
+constexpr int SHORT = KV8_SHORT;
 constexpr int COUNTERS = 1 << 16;      // of a workspace, always in front: whichever calls share one, nothing else is written there
 
 // SIZE: the widest head, 64, 128 or 256.
@@ -31,9 +38,22 @@ template <int SIZE> struct Shape {
   static constexpr int NK = SIZE / 64;                  // 16-byte runs of a key row per lane
   static constexpr int VB = SIZE == 64 ? 8 : 16, NV = SIZE == 256 ? 2 : 1;   // bytes of a run of a value row, runs per lane
   static constexpr int MT = SIZE / 16;                  // tiles of 16 output dimensions
-  static constexpr int K_BYTES = GROUPS * 2 * NK * 512, V_BYTES = GROUPS * 4 * NV * VB * 32, STAGE = K_BYTES + V_BYTES + GROUPS * 128, RING = STAGES * STAGE;
+  static constexpr int COPIES = SIZE / 32;              // of 512 bytes, 16 a lane, for 16 rows
+  static constexpr int ROWS = KT * SIZE, STAGE = 2 * ROWS + GROUPS * 128, RING = STAGES * STAGE;      // keys, values, scales
   static constexpr int PIECE = MT * 4 * 32 + 2 * HEADS; // floats of a piece of a segment: a warp's sums, maxima and totals
   static_assert(PIECE * 4 <= RING, "a warp's last piece takes the place of its keys and values");
+};
+
+// Division by what a launch has but once: n / d = (n + high word of n mul) >> shift for 0 <= n < 2^31, mul = ceil(2^32 (2^shift - d) / d), 2^shift the power of two at or above d.
+struct Divide {
+  uint32_t d, mul, shift;
+  __host__ static Divide by(uint32_t d) {
+    Divide r{d, 0, 0};
+    while ((1ull << r.shift) < d) ++r.shift;
+    r.mul = (uint32_t)((((1ull << r.shift) - d) << 32) / d + 1);
+    return r;
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
 };
 
 struct Plan {     // of a launch, in the shared memory of every block
@@ -41,7 +61,8 @@ struct Plan {     // of a launch, in the shared memory of every block
 };
 struct Split {
   int tok0, tokens, chunks;   // the launch's tokens; parts of a kv head's query heads
-  int grid, dtype, q_whole, out_whole;
+  int segs, grid, dtype, q_whole, out_whole;
+  Divide by_segs, by_chunks, by_page, by_grid;
   int *counters;              // [COUNTERS], zero between launches; [token][segment]
   float *heads;               // [grid][WARPS][PIECE]: the pieces that warps begin with and do not end with
   float *parts;               // [grid][2][PIECE]: what blocks have of segments that are not theirs alone, in front and at their end
@@ -61,22 +82,25 @@ template <int B> __device__ __forceinline__ void copy_async(uint32_t dst, const 
 template <int N> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// Bytes 0 and 2, and 1 and 3, of a word as fp16 pairs.
-template <bool E4M3> __device__ __forceinline__ void widen(uint32_t w, uint32_t &even, uint32_t &odd) {
+// Bytes of two words as fp16 pairs: (byte 2 half of x, of y) and (byte 2 half + 1 of x, of y).
+template <bool E4M3> __device__ __forceinline__ void widen(uint32_t x, uint32_t y, int half, uint32_t &first, uint32_t &second) {
   if constexpr (E4M3) {
-    const uint32_t w8 = w << 8;
-    odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
-    even = ((w8 >> 1) & 0x3f803f80u) | (w8 & 0x80008000u);
+    const uint32_t w = __byte_perm(x, y, half ? 0x7362 : 0x5140);
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(first), "=r"(second) : "r"(w));
   } else {
+    const uint32_t w = __byte_perm(x, y, half ? 0x7632 : 0x5410);
     const __half2 off = __float2half2_rn(1152.f);
-    uint32_t e = (w & 0x00ff00ffu) ^ 0x64806480u, o = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
-    const __half2 he = __hsub2(*reinterpret_cast<__half2 *>(&e), off), ho = __hsub2(*reinterpret_cast<__half2 *>(&o), off);
-    even = *reinterpret_cast<const uint32_t *>(&he);
-    odd = *reinterpret_cast<const uint32_t *>(&ho);
+    uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;     // 1024 + 128 + byte
+    const __half2 ha = __hsub2(*reinterpret_cast<__half2 *>(&a), off), hb = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+    first = *reinterpret_cast<const uint32_t *>(&ha);
+    second = *reinterpret_cast<const uint32_t *>(&hb);
   }
 }
-template <bool E4M3> __device__ __forceinline__ float byte_unit() { return E4M3 ? 256.f : 1.f; }
-
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -160,9 +184,9 @@ __device__ __forceinline__ void settle(Walk &w, const Plan &pl, int segs, int to
     }
   }
 }
-__device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, int tokens) {
+__device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, const Divide &by_segs, int tokens) {
   Walk w;
-  const int x = at / segs;
+  const int x = by_segs(at);
   int lo = 0, hi = tokens - 1;       // the last token whose tiles begin at or before x: it has some
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -177,48 +201,20 @@ __device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, int to
   return w;
 }
 
-// Pieces of one segment added up, unit j (four floats of every lane) of each: the sum, and l and R of heads 2 tg and 2 tg + 1.
-struct Joined { float4 o; float L[2], R[2]; };
-// OTHERS: other blocks have written them; else they may lie in shared memory.
-template <int SIZE, bool OTHERS, typename At> __device__ __forceinline__ Joined add_pieces(int from, int to, int j, int lane, const At &at) {
-  constexpr int SUMS = Shape<SIZE>::PIECE - 2 * HEADS;
-  auto load = [](const float *p, int i) { return OTHERS ? __ldcg(reinterpret_cast<const float4 *>(p) + i) : reinterpret_cast<const float4 *>(p)[i]; };
-  Joined r;
-  r.o = make_float4(0.f, 0.f, 0.f, 0.f);
-  r.R[0] = r.R[1] = -INFINITY;
-  r.L[0] = r.L[1] = 0.f;
-#pragma unroll 4
-  for (int i = from; i < to; ++i) {
-    const float *p = at(i);
-    if (!p) continue;
-    const float4 ml = load(p + SUMS, lane & 3);
-    r.R[0] = fmaxf(r.R[0], ml.x);
-    r.R[1] = fmaxf(r.R[1], ml.z);
-  }
-#pragma unroll 4
-  for (int i = from; i < to; ++i) {
-    const float *p = at(i);
-    if (!p) continue;
-    const float4 ml = load(p + SUMS, lane & 3), o = load(p, j * 32 + lane);
-    const float f0 = ml.x == r.R[0] ? 1.f : exp2_fast(ml.x - r.R[0]), f1 = ml.z == r.R[1] ? 1.f : exp2_fast(ml.z - r.R[1]);
-    r.L[0] += ml.y * f0;
-    r.L[1] += ml.w * f1;
-    r.o.x += o.x * f0; r.o.y += o.y * f1; r.o.z += o.z * f0; r.o.w += o.w * f1;
-  }
-  return r;
-}
-
 // FULL: keys and values are as wide as SIZE.
 template <int SIZE, bool FULL, bool E4M3, int PARTS>
 __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const Attn p, const Split sp) {
   early_start();
   using S = Shape<SIZE>;
-  constexpr int NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
+  constexpr int QPARTS = E4M3 ? PARTS : 3, QREGS = E4M3 ? 2 : 1, NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int scan[NW], piece[2 * NW], last;
+  // The pieces of segments that warps begin and end with: which segments, and (R, l) of heads 2 tg and 2 tg + 1.
+  __shared__ int scan[NW], widest[NW], front[NW], rear[NW], last[2];
+  __shared__ float4 front_ml[NW][4], rear_ml[NW][4];
+  __shared__ float2 whole_ml[HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, tg = lane & 3;
   const int dim = FULL ? SIZE : p.c.dim, vdim = FULL ? SIZE : p.c.vdim;
-  const int G = p.c.n_kv, qpk = p.heads / G, segs = G * sp.chunks, tokens = sp.tokens;
+  const int G = p.c.n_kv, qpk = p.heads / G, segs = sp.segs, tokens = sp.tokens;
   Plan pl;
   pl.cum = reinterpret_cast<int *>(smem + NW * S::RING);
   pl.pos = pl.cum + tokens + 1;
@@ -226,16 +222,24 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
 
   // ---- how many tiles every token has, and the sums in front of it
   const int used = p.b.cu[p.b.n_seq];
-  int before = 0;
+  int before = 0, most = 0;
   for (int t0 = 0; t0 < tokens; t0 += NW * 32) {
     const int t = t0 + tid, tok = sp.tok0 + t;
     int n = 0;
     if (t < tokens) {
       int pos = -1, slot = 0;
+      // (of a batch of one token a sequence these are asked for together; a row that no sequence has may name any)
+      const int guess = min(tok, p.b.n_seq - 1), seq = p.b.tok_seq[tok];
+      int first = p.b.cu[guess], end = p.b.cu[guess + 1], start = p.b.start[guess];
+      slot = p.b.slot[guess];
       if (tok < used) {
-        const int seq = p.b.tok_seq[tok], first = p.b.cu[seq], start = p.b.start[seq];
-        slot = p.b.slot[seq];
-        if (in_table(p.c, start, p.b.cu[seq + 1] - first)) {
+        if (seq != guess) {
+          first = p.b.cu[seq];
+          end = p.b.cu[seq + 1];
+          start = p.b.start[seq];
+          slot = p.b.slot[seq];
+        }
+        if (in_table(p.c, start, end - first)) {
           pos = start + tok - first;
           n = pos / KT - (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT + 1;
         } else if (blockIdx.x == 0 && p.error_flag) {
@@ -252,34 +256,57 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       if (lane >= o) sum += up;
     }
     if (lane == 31) scan[warp] = sum;
+    const int w_most = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+    if (lane == 0) widest[warp] = w_most;
     __syncthreads();
     int base = before;
+#pragma unroll
     for (int w = 0; w < NW; ++w) {
       if (w < warp) base += scan[w];
       before += scan[w];
+      most = max(most, widest[w]);
     }
     if (t < tokens) pl.cum[t + 1] = base + sum;
     __syncthreads();
   }
   if (tid == 0) pl.cum[0] = 0;
-  if (tid < 2 * NW) piece[tid] = -1;
+  if (tid < NW) front[tid] = rear[tid] = -1;
   __syncthreads();
-  const int all = before * segs, per = max(NW, (all + sp.grid - 1) / sp.grid), block0 = blockIdx.x * per, block_n = min(per, all - block0);
+  const int all = before * segs, per = max(NW, sp.by_grid(all + sp.grid - 1));
+  int block0 = blockIdx.x * per, block_n = min(per, all - block0);
+  Walk w;
+  // (Few short segments: a block each, so that blocks need not wait for one another's sums.)
+  const bool one_each = tokens * segs <= sp.grid && most <= SHORT * NW;
+  if (one_each) {
+    w.tok = sp.by_segs(blockIdx.x);
+    w.seg = blockIdx.x - w.tok * segs;
+    w.tiles = block_n = w.tok < tokens ? pl.cum[w.tok + 1] - pl.cum[w.tok] : 0;
+    if (block_n) block0 = pl.cum[w.tok] * segs + w.seg * block_n;
+  }
   if (block_n <= 0) return;
 
   // ---- this warp's run
   const int run0 = block0 + block_n * warp / NW, count = block0 + block_n * (warp + 1) / NW - run0;
   unsigned char *ring = smem + warp * S::RING;
   if (count > 0) {
-    Walk w = walk_to(run0, pl, segs, tokens), ahead = w;
-    const uint32_t ring_s = smem_addr(ring) + lane * 16;
-    // copies: a tile a call, STAGES - 1 ahead of what is used.  A lane knows the page and the row in it of one of the next 32 groups of 16 positions.
+    if (one_each) w.tile = run0 - block0;
+    else w = walk_to(run0, pl, segs, sp.by_segs, tokens);
+    Walk ahead = w;
+    // Rows of SIZE bytes; the 16-byte runs of a row are exchanged so that the lanes that read together hit different banks: run c of key row r lies at c ^ 4 (r & 1), of value row
+    // r at c ^ (r & 6) (rows of 64 bytes: keys as they are, values at c ^ (r / 2 & 3)).  A copy's 32 lanes have neighbouring runs of ROW_LANES each: 512 bytes that lie together.
+    constexpr int ROW_LANES = SIZE / 16;
+    const int row_in = lane / ROW_LANES, run_in = lane % ROW_LANES;
+    const uint32_t ring_s = smem_addr(ring), k_in = row_in * SIZE + ((run_in ^ (SIZE == 64 ? 0 : (row_in & 1) << 2)) << 4),
+                   v_in = row_in * SIZE + ((run_in ^ (SIZE == 64 ? row_in >> 1 & 3 : row_in & 6)) << 4);
+    const int k_at0 = g * SIZE + ((tg ^ (SIZE == 64 ? 0 : (g & 1) << 2)) << 4);
+    const int v_at0 = 2 * tg * SIZE + (SIZE == 64 ? (((g >> 1) ^ tg) << 4) + (g & 1) * 8 : (g ^ 2 * tg) << 4);
+    // copies: a tile a call, STAGES of them before the first is used and then one behind each.  A lane knows the page and the row in it of one of the next 32 groups of 16 positions.
     int ahead_at = 0, stage_in = 0, listed = 0, list_end = 0, page_l = 0, row_l = 0, kvh_in = 0;
     auto fetch = [&]() {
       if (ahead_at < count) {
         if (ahead_at >= list_end) {      // (a segment's first tile, or the list has been used up)
           const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
-          const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? at / p.c.page : 0;
+          const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? sp.by_page(at) : 0;
           row_l = at <= pos ? at - pg * p.c.page : -1;      // (-1: behind the last position)
           page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
           if (page_l < 0) {
@@ -288,42 +315,31 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
           }
           listed = ahead_at;
           list_end = ahead_at + min(32 / GROUPS, ahead.tiles - ahead.tile);
-          kvh_in = ahead.seg / sp.chunks;
+          kvh_in = sp.by_chunks(ahead.seg);
         }
         const uint32_t st = ring_s + stage_in * S::STAGE;
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
           const int page = __shfl_sync(0xffffffffu, page_l, (ahead_at - listed) * GROUPS + u), row = __shfl_sync(0xffffffffu, row_l, (ahead_at - listed) * GROUPS + u);
           const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes;
-          const unsigned char *k = base + (kvh_in * p.c.page + row + g) * dim + 16 * tg;
-          const unsigned char *v = base + (G * p.c.page) * dim + (kvh_in * p.c.page + row + 2 * tg) * vdim + VB * g;
+          const unsigned char *k = base + (kvh_in * p.c.page + row + row_in) * dim + 16 * run_in;
+          const unsigned char *v = base + (G * p.c.page) * dim + (kvh_in * p.c.page + row + row_in) * vdim + 16 * run_in;
           const float *sc = p.c.scales + (size_t)page * (2 * G * p.c.page) + ((lane >> 4) * G + kvh_in) * p.c.page + row + (lane & 15);
-          const uint32_t st_v = st + S::K_BYTES + u * (4 * NV * VB * 32) - (VB == 8 ? lane * 8 : 0), st_s = st + S::K_BYTES + S::V_BYTES + u * 128 - lane * 12;
+          const uint32_t st_k = st + u * (16 * SIZE) + k_in, st_v = st + S::ROWS + u * (16 * SIZE) + v_in, st_s = st + 2 * S::ROWS + u * 128 + lane * 4;
+          auto v_to = [&](int j) { return (SIZE == 128 ? st_v ^ (j & 1) << 6 : SIZE == 256 ? st_v ^ (2 * j & 6) << 4 : st_v) + j * 512; };
           if (FULL && row >= 0) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int j = 0; j < S::COPIES; ++j) copy_whole<16>(st_k + j * 512, k + j * 512);
 #pragma unroll
-              for (int i = 0; i < NK; ++i) copy_whole<16>(st + ((u * 2 + r) * NK + i) * 512, k + 8 * r * SIZE + 64 * i);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int i = 0; i < NV; ++i) copy_whole<VB>(st_v + (r * NV + i) * (VB * 32), v + ((r & 1) + 8 * (r >> 1)) * SIZE + 128 * i);
+            for (int j = 0; j < S::COPIES; ++j) copy_whole<16>(v_to(j), v + j * 512);
             copy_whole<4>(st_s, sc);
           } else {
+            const bool k_here = row >= 0 && 16 * run_in < dim, v_here = row >= 0 && 16 * run_in < vdim;
+            constexpr int AT_ONCE = 512 / SIZE;      // rows of a copy
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int j = 0; j < S::COPIES; ++j) copy_async<16>(st_k + j * 512, k_here ? k + j * AT_ONCE * dim : base, k_here);
 #pragma unroll
-              for (int i = 0; i < NK; ++i) {
-                const bool here = row >= 0 && 16 * tg + 64 * i < dim;
-                copy_async<16>(st + ((u * 2 + r) * NK + i) * 512, here ? k + 8 * r * dim + 64 * i : base, here);
-              }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int i = 0; i < NV; ++i) {
-                const bool here = row >= 0 && VB * g + 128 * i < vdim;
-                copy_async<VB>(st_v + (r * NV + i) * (VB * 32), here ? v + ((r & 1) + 8 * (r >> 1)) * vdim + 128 * i : base, here);
-              }
+            for (int j = 0; j < S::COPIES; ++j) copy_async<16>(v_to(j), v_here ? v + j * AT_ONCE * vdim : base, v_here);
             copy_async<4>(st_s, row >= 0 ? sc : p.c.scales, row >= 0);
           }
         }
@@ -335,78 +351,113 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       copies_end();       // (the groups are counted)
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch();
+    for (int s = 0; s < STAGES; ++s) fetch();
 
     int done = 0, stage = 0;
     while (done < count) {      // segment after segment
       const int here = min(count - done, w.tiles - w.tile), tok = w.tok;      // tiles of this segment that are the warp's
-      const int kvh = w.seg / sp.chunks, chunk = w.seg - kvh * sp.chunks, head0 = kvh * qpk + chunk * HEADS, heads = min(HEADS, qpk - chunk * HEADS);
+      const int kvh = sp.by_chunks(w.seg), chunk = w.seg - kvh * sp.chunks, head0 = kvh * qpk + chunk * HEADS, heads = min(HEADS, qpk - chunk * HEADS);
       const int pos = pl.pos[tok], begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;
       float O[MT][4], R[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < MT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
-      // q as B operand: lane (g, tg) holds head g's dimensions 64 i + 16 tg + 4 c + {0, 2} and {1, 3} of k step 4 i + c
-      uint32_t qf[PARTS][NK * 4][2];
+      // q as B operand: lane (g, tg) holds head g's dimensions 64 i + 16 tg + .. of the byte runs that it reads of the keys.  int8: three parts of 8 bits of (127 2^14 / the row's largest) q;
+      // E4M3: fp16, after a power of two, in PARTS parts.
+      uint32_t qf[QPARTS][NK * 4][QREGS];
       float by[2];          // factors of the scores of heads 2 tg and 2 tg + 1
       {
-        float x[NK][16], most = 0.f;
+        float x[NK][16];
+        uint32_t most = 0;           // (in the order of bits: NaN above infinity)
         const size_t at = (size_t)(sp.tok0 + tok) * p.q_ld + (size_t)(head0 + g) * dim + 16 * tg;
 #pragma unroll
         for (int i = 0; i < NK; ++i) load16(sp.q, at + 64 * i, sp.dtype, sp.q_whole, g < heads ? dim - 64 * i - 16 * tg : 0, x[i]);
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(x[i][j]));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // the power of two at or below the largest element (1 for a row of zeros or infinities; within 2^-120 .. 2^120, so that its reciprocal is a number)
-        const uint32_t e = __float_as_uint(most) >> 23, f = most == 0.f || e == 255 ? 127u : min(max(e, 7u), 247u);
-        const float turn = __uint_as_float((254u - f) << 23), unit = __uint_as_float(f << 23);
+          for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        float unit;
+        if constexpr (E4M3) {
+          // the power of two at or below the largest element (1 for a row of zeros, infinities or NaN; within 2^-120 .. 2^120, so that its reciprocal is a number)
+          const uint32_t e = most >> 23, f = most == 0 || e == 255 ? 127u : min(max(e, 7u), 247u);
+          const float turn = __uint_as_float((254u - f) << 23);
+          unit = __uint_as_float(f << 23);
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+          for (int i = 0; i < NK; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-              const float a = x[i][4 * c + o] * turn, b = x[i][4 * c + o + 2] * turn;
-              qf[0][4 * i + c][o] = pack2(a, b);
-              if constexpr (PARTS == 2) {
-                const float2 h = unpack2(qf[0][4 * i + c][o]);
-                qf[PARTS - 1][4 * i + c][o] = pack2(a - h.x, b - h.y);
+              for (int o = 0; o < 2; ++o) {
+                const float a = x[i][4 * c + 2 * o] * turn, b = x[i][4 * c + 2 * o + 1] * turn;
+                qf[0][4 * i + c][o % QREGS] = pack2(a, b);
+                if constexpr (PARTS == 2) {
+                  const float2 h = unpack2(qf[0][4 * i + c][o % QREGS]);
+                  qf[QPARTS - 1][4 * i + c][o % QREGS] = pack2(a - h.x, b - h.y);
+                }
               }
-            }
+        } else {
+          const float top = fmaxf(__uint_as_float(most), 0x1p-100f), turn = 127.f * 16384.f / top;
+          unit = __uint_as_float(most) == 0.f ? 0.f : most > 0x7f800000u ? __uint_as_float(most) : top / (127.f * 16384.f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) by[h] = __shfl_sync(0xffffffffu, unit, 8 * tg + 4 * h) * (p.scale * byte_unit<E4M3>());     // (lanes 8 tg and 8 tg + 4 have their rows)
+          for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t part[3] = {0, 0, 0};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int v = __float2int_rn(x[i][4 * c + e] * turn), hi = (v + 8192) >> 14, rest = v - (hi << 14), mid = (rest + 64) >> 7, lo = rest - (mid << 7);
+                part[0] |= (uint32_t)(hi & 255) << (8 * e);
+                part[1] |= (uint32_t)(mid & 255) << (8 * e);
+                part[2] |= (uint32_t)(lo & 255) << (8 * e);
+              }
+#pragma unroll
+              for (int q = 0; q < QPARTS; ++q) qf[q][4 * i + c][0] = part[q];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) by[h] = __shfl_sync(0xffffffffu, unit, 8 * tg + 4 * h) * p.scale;     // (lanes 8 tg and 8 tg + 4 have their rows)
       }
       const float log2e = 1.4426950408889634f;
       if (!(p.softcap > 0.f)) { by[0] *= log2e; by[1] *= log2e; }
       int key0 = (begin / KT + w.tile) * KT;
       for (int t = 0; t < here; ++t, key0 += KT) {
-        fetch();
         copies_left<STAGES - 1>();
         __syncwarp();
         const unsigned char *st = ring + stage * S::STAGE;
-        const float *sc = reinterpret_cast<const float *>(st + S::K_BYTES + S::V_BYTES);
+        const float *sc = reinterpret_cast<const float *>(st + 2 * S::ROWS);
         float x[GROUPS][4];
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
           float c[2][4] = {};
+          int n[3][4] = {};
 #pragma unroll
           for (int i = 0; i < NK; ++i) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(st + ((u * 2 + 0) * NK + i) * 512 + lane * 16), b = *reinterpret_cast<const uint4 *>(st + ((u * 2 + 1) * NK + i) * 512 + lane * 16);
+            const unsigned char *at = st + u * (16 * SIZE) + (k_at0 ^ (i & 1) << 6) + (i >> 1) * 128;
+            const uint4 a = *reinterpret_cast<const uint4 *>(at), b = *reinterpret_cast<const uint4 *>(at + 8 * SIZE);
             const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+            if constexpr (E4M3) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t a0, a1, a2, a3;
-              widen<E4M3>(wa[k], a0, a2);
-              widen<E4M3>(wb[k], a1, a3);
+              for (int k = 0; k < 4; ++k) {
+                uint32_t a0, a1, a2, a3;
+                asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(a0), "=r"(a2) : "r"(wa[k]));
+                asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(a1), "=r"(a3) : "r"(wb[k]));
 #pragma unroll
-              for (int q = 0; q < PARTS; ++q) mma(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][1]);
+                for (int q = 0; q < QPARTS; ++q) mma(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; k += 2)
+#pragma unroll
+                for (int q = 0; q < QPARTS; ++q) mma_s8(n[q % 3], wa[k], wb[k], wa[k + 1], wb[k + 1], qf[q][4 * i + k][0], qf[q][4 * i + k + 1][0]);
             }
           }
           const float ks[2] = {sc[u * 32 + g], sc[u * 32 + 8 + g]};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][e] = (c[0][e] + c[1][e]) * (ks[e >> 1] * by[e & 1]);
+          for (int e = 0; e < 4; ++e) {
+            const float s = E4M3 ? c[0][e] + c[1][e] : fmaf((float)n[0][e], 16384.f, fmaf((float)n[1][e], 128.f, (float)n[2][e]));
+            x[u][e] = s * (ks[e >> 1] * by[e & 1]);
+          }
         }
         if (p.softcap > 0.f) {
 #pragma unroll
@@ -423,7 +474,8 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
             vs[u][r] = sc[u * 32 + 16 + 8 * r + g];
             ev[u][r] = fmaxf(fmaf((float)__float_as_int(vs[u][r]), 1.f / (1 << 23), -127.f), -80.f);
           }
-        if (key0 < begin || key0 + KT > pos + 1) {
+        const bool border = key0 < begin || key0 + KT > pos + 1;
+        if (border) {
 #pragma unroll
           for (int u = 0; u < GROUPS; ++u)
 #pragma unroll
@@ -477,7 +529,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
             uint32_t v[4][VB / 4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const unsigned char *at = st + S::K_BYTES + ((u * 4 + r) * NV + i) * (VB * 32) + lane * VB;
+              const unsigned char *at = st + S::ROWS + (u * 16 + (r & 1) + 8 * (r >> 1)) * SIZE + v_at0 + i * 128;
               if constexpr (VB == 16) {
                 const uint4 y = *reinterpret_cast<const uint4 *>(at);
                 v[r][0] = y.x; v[r][1] = y.y; v[r][VB / 4 - 2] = y.z; v[r][VB / 4 - 1] = y.w;
@@ -485,14 +537,19 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
                 const uint2 y = *reinterpret_cast<const uint2 *>(at);
                 v[r][0] = y.x; v[r][1] = y.y;
               }
+              const int key = key0 + 16 * u + 2 * tg + (r & 1) + 8 * (r >> 1);
+              if (E4M3 && border && (key < begin || key > pos)) {      // (whatever lies there may be NaN)
+#pragma unroll
+                for (int k = 0; k < VB / 4; ++k) v[r][k] = 0;
+              }
             }
 #pragma unroll
             for (int k = 0; k < VB / 4; ++k)
 #pragma unroll
               for (int half = 0; half < 2; ++half) {     // dimensions 4 k + 2 half and the next, of keys (0, 1) and (2, 3)
                 uint32_t a0, a1, a2, a3;
-                widen<E4M3>(__byte_perm(v[0][k], v[1][k], half ? 0x7632 : 0x5410), a0, a1);
-                widen<E4M3>(__byte_perm(v[2][k], v[3][k], half ? 0x7632 : 0x5410), a2, a3);
+                widen<E4M3>(v[0][k], v[1][k], half, a0, a1);
+                widen<E4M3>(v[2][k], v[3][k], half, a2, a3);
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) mma(O[i * 8 + 2 * k + half], a0, a1, a2, a3, wf[q][0], wf[q][1]);
               }
@@ -500,6 +557,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         }
         __syncwarp();      // the scales have been read by all lanes
         if (++stage == STAGES) stage = 0;
+        fetch();           // (to the stage that was used)
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -511,7 +569,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (2 * tg + h >= heads) continue;
-          const float f = byte_unit<E4M3>() / L[h];
+          const float f = 1.f / L[h];
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
             if (VB * g + 128 * i >= vdim) continue;
@@ -533,8 +591,8 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j) reinterpret_cast<float4 *>(to)[j * 32 + lane] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
-        if (g == 0) reinterpret_cast<float4 *>(to + MT * 128)[tg] = make_float4(R[0], L[0], R[1], L[1]);
-        if (lane == 0) piece[2 * warp + end] = tok * segs + w.seg;
+        if (g == 0) (end ? rear_ml : front_ml)[warp][tg] = make_float4(R[0], L[0], R[1], L[1]);
+        if (lane == 0) (end ? rear : front)[warp] = tok * segs + w.seg;
       }
       w.tile += here;
       settle(w, pl, segs, tokens);
@@ -543,56 +601,111 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   }
   __syncthreads();
 
-  // ---- pieces of a segment come together
-  auto leave = [&](const Joined &r, int id, int j) {
-    const int tok = id / segs, seg = id - tok * segs, kvh = seg / sp.chunks, chunk = seg - kvh * sp.chunks, heads = min(HEADS, qpk - chunk * HEADS);
+  // ---- pieces of a segment come together: the ends of some warps and the front of the next, a unit of four floats a lane at a time, dealt out to the warps.  What is
+  // not the block's alone goes where the others find it.
+  auto leave = [&](const float4 &o, float l0, float l1, int id, int j) {       // (l of heads 2 tg and 2 tg + 1)
+    const int tok = sp.by_segs(id), seg = id - tok * segs, kvh = sp.by_chunks(seg), chunk = seg - kvh * sp.chunks, heads = min(HEADS, qpk - chunk * HEADS);
     const int d = VB * g + 128 * (j / 8) + 2 * (j % 8);
-    const float o[2][2] = {{r.o.x, r.o.z}, {r.o.y, r.o.w}};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (2 * tg + h >= heads || d >= vdim) continue;
-      const float f = byte_unit<E4M3>() / r.L[h];
-      const size_t at = (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(kvh * qpk + chunk * HEADS + 2 * tg + h) * vdim + d;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) store_one(sp.out, at + e, sp.dtype, o[h][e] * f);
+    const size_t at = (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(kvh * qpk + chunk * HEADS + 2 * tg) * vdim + d;
+    const float f0 = 1.f / l0, f1 = 1.f / l1;
+    if (2 * tg < heads && d < vdim) {
+      store_one(sp.out, at, sp.dtype, o.x * f0);
+      store_one(sp.out, at + 1, sp.dtype, o.z * f0);
+    }
+    if (2 * tg + 1 < heads && d < vdim) {
+      store_one(sp.out, at + vdim, sp.dtype, o.y * f1);
+      store_one(sp.out, at + vdim + 1, sp.dtype, o.w * f1);
     }
   };
-  for (int i0 = 0; i0 < 2 * NW;) {
-    const int id = piece[i0];
-    int i1 = i0 + 1;
-    if (id >= 0) {
-      while (i1 < 2 * NW && (piece[i1] == id || piece[i1] < 0)) ++i1;
-      auto mine = [&](int i) -> const float * {
-        return piece[i] < 0 ? nullptr : i & 1 ? reinterpret_cast<const float *>(smem + (i >> 1) * S::RING) : sp.heads + ((size_t)blockIdx.x * NW + (i >> 1)) * S::PIECE;
-      };
-      const int tok = id / segs, tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per, b1 = (tile0 + tiles - 1) / per;
-      float *part = sp.parts + ((size_t)blockIdx.x * 2 + (tile0 > block0)) * S::PIECE;
-      for (int j = warp; j < MT; j += NW) {
-        const Joined r = add_pieces<SIZE, false>(i0, i1, j, lane, mine);
-        if (b0 == b1) {
-          leave(r, id, j);
-        } else {
-          __stcg(reinterpret_cast<float4 *>(part) + j * 32 + lane, r.o);
-          if (j == 0 && g == 0) __stcg(reinterpret_cast<float4 *>(part + MT * 128) + tg, make_float4(r.R[0], r.L[0], r.R[1], r.L[1]));
-        }
+  const int rear_l = lane < NW ? rear[lane] : -1, front_l = lane < NW ? front[lane] : -1;
+  const uint32_t any_front = __ballot_sync(0xffffffffu, front_l >= 0);
+  int unit = 0, open0 = -1, open1 = -1;       // the segments that begin before the block's run, and that end behind it
+  for (int w0 = any_front ? -1 : 0; w0 < NW;) {      // (-1: what began before the block and ends in its first warp that has tiles; every other front belongs to the rears before it)
+    const int id = __shfl_sync(0xffffffffu, w0 < 0 ? front_l : rear_l, w0 < 0 ? __ffs(any_front) - 1 : w0);
+    const uint32_t rears = __ballot_sync(0xffffffffu, rear_l == id), fronts = __ballot_sync(0xffffffffu, front_l == id);
+    if (id < 0 || (w0 < 0 && rears)) { ++w0; continue; }
+    const int tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles;
+    const bool alone = tile0 >= block0 && tile0 + tiles <= block0 + block_n;
+    const int side = tile0 >= block0;
+    if (!alone) (side ? open1 : open0) = id;
+    float *part = sp.parts + ((size_t)blockIdx.x * 2 + side) * S::PIECE;
+    for (int j = 0; j < MT; ++j, ++unit) {
+      if (unit % NW != warp) continue;
+      float4 ml[NW + 1], o[NW + 1];       // (all of them asked for at once)
+      const int fw = fronts ? __ffs(fronts) - 1 : 0;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        ml[k] = rear_ml[k][tg];
+        o[k] = reinterpret_cast<const float4 *>(smem + k * S::RING)[j * 32 + lane];
       }
-      if (b0 != b1) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          last = atomicAdd(sp.counters + id, 1) == b1 - b0;
-          if (last) sp.counters[id] = 0;
-          __threadfence();
+      ml[NW] = front_ml[fw][tg];
+      o[NW] = fronts ? __ldcg(reinterpret_cast<const float4 *>(sp.heads + ((size_t)blockIdx.x * NW + fw) * S::PIECE) + j * 32 + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k <= NW; ++k)
+        if (k < NW ? rears >> k & 1 : fronts != 0) { m0 = fmaxf(m0, ml[k].x); m1 = fmaxf(m1, ml[k].z); }
+#pragma unroll
+      for (int k = 0; k <= NW; ++k)
+        if (k < NW ? rears >> k & 1 : fronts != 0) {
+          const float f0 = ml[k].x == m0 ? 1.f : exp2_fast(ml[k].x - m0), f1 = ml[k].z == m1 ? 1.f : exp2_fast(ml[k].z - m1);
+          l0 += ml[k].y * f0; l1 += ml[k].w * f1;
+          r.x += o[k].x * f0; r.y += o[k].y * f1; r.z += o[k].z * f0; r.w += o[k].w * f1;
         }
-        __syncthreads();
-        if (last) {
-          auto theirs = [&](int b) -> const float * { return sp.parts + ((size_t)b * 2 + (tile0 > b * per)) * S::PIECE; };
-          for (int j = warp; j < MT; j += NW) leave(add_pieces<SIZE, true>(b0, b1 + 1, j, lane, theirs), id, j);
-        }
-        __syncthreads();
+      if (alone) {
+        leave(r, l0, l1, id, j);
+      } else {
+        __stcg(reinterpret_cast<float4 *>(part) + j * 32 + lane, r);
+        if (j == 0 && g == 0) __stcg(reinterpret_cast<float4 *>(part + MT * 128) + tg, make_float4(m0, l0, m1, l1));
       }
     }
-    i0 = i1;
+    w0 = w0 < 0 ? 0 : 32 - __clz(rears);
+  }
+  if (open0 < 0 && open1 < 0) return;
+  // ---- ... and the last block of a segment to come adds them up, in their order
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    const int id = tid ? open1 : open0;
+    last[tid] = 0;
+    if (id >= 0) {
+      const int tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles;
+      last[tid] = atomicAdd(sp.counters + id, 1) == (tile0 + tiles - 1) / per - tile0 / per;
+      if (last[tid]) sp.counters[id] = 0;
+    }
+    __threadfence();
+  }
+  __syncthreads();
+  float *others = reinterpret_cast<float *>(smem);      // [block][head]: factors (the pieces in shared memory have been used)
+  for (int side = 0; side < 2; ++side) {
+    if (!last[side]) continue;
+    const int id = side ? open1 : open0, tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per, n = (tile0 + tiles - 1) / per - b0 + 1;
+    auto part_of = [&](int i) { return sp.parts + ((size_t)(b0 + i) * 2 + (tile0 >= (b0 + i) * per)) * S::PIECE; };
+    if (warp < HEADS) {       // a warp per head
+      float m = -INFINITY, l = 0.f;
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part_of(i) + MT * 128) + warp).x);
+      m = warp_max(m);
+      for (int i = lane; i < n; i += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(i) + MT * 128) + warp);
+        const float f = ml.x == m ? 1.f : exp2_fast(ml.x - m);
+        others[i * HEADS + warp] = f;
+        l += ml.y * f;
+      }
+      l = warp_sum(l);
+      if (lane == 0) whole_ml[warp] = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int j = warp; j < MT; j += NW) {
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float4 o = __ldcg(reinterpret_cast<const float4 *>(part_of(i)) + j * 32 + lane);
+        const float2 f = *reinterpret_cast<const float2 *>(&others[i * HEADS + 2 * tg]);
+        r.x += o.x * f.x; r.y += o.y * f.y; r.z += o.z * f.x; r.w += o.w * f.y;
+      }
+      leave(r, whole_ml[2 * tg].y, whole_ml[2 * tg + 1].y, id, j);
+    }
+    __syncthreads();
   }
 }
 
