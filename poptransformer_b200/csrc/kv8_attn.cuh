@@ -211,7 +211,6 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   // The pieces of segments that warps begin and end with: which segments, and (R, l) of heads 2 tg and 2 tg + 1.
   __shared__ int scan[NW], widest[NW], front[NW], rear[NW], last[2];
   __shared__ float4 front_ml[NW][4], rear_ml[NW][4];
-  __shared__ float2 whole_ml[HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, tg = lane & 3;
   const int dim = FULL ? SIZE : p.c.dim, vdim = FULL ? SIZE : p.c.vdim;
   const int G = p.c.n_kv, qpk = p.heads / G, segs = sp.segs, tokens = sp.tokens;
@@ -350,8 +349,6 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       }
       copies_end();       // (the groups are counted)
     };
-#pragma unroll
-    for (int s = 0; s < STAGES; ++s) fetch();
 
     int done = 0, stage = 0;
     while (done < count) {      // segment after segment
@@ -371,6 +368,10 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         const size_t at = (size_t)(sp.tok0 + tok) * p.q_ld + (size_t)(head0 + g) * dim + 16 * tg;
 #pragma unroll
         for (int i = 0; i < NK; ++i) load16(sp.q, at + 64 * i, sp.dtype, sp.q_whole, g < heads ? dim - 64 * i - 16 * tg : 0, x[i]);
+        if (done == 0) {        // (the first segment's queries are asked for before all tiles: they would come behind them)
+#pragma unroll
+          for (int s = 0; s < STAGES; ++s) fetch();
+        }
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
@@ -676,36 +677,35 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
     __threadfence();
   }
   __syncthreads();
-  float *others = reinterpret_cast<float *>(smem);      // [block][head]: factors (the pieces in shared memory have been used)
-  for (int side = 0; side < 2; ++side) {
+  for (int unit = warp; unit < 2 * MT; unit += NW) {
+    const int side = unit >= MT, j = unit - side * MT;
     if (!last[side]) continue;
-    const int id = side ? open1 : open0, tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per, n = (tile0 + tiles - 1) / per - b0 + 1;
-    auto part_of = [&](int i) { return sp.parts + ((size_t)(b0 + i) * 2 + (tile0 >= (b0 + i) * per)) * S::PIECE; };
-    if (warp < HEADS) {       // a warp per head
-      float m = -INFINITY, l = 0.f;
-      for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part_of(i) + MT * 128) + warp).x);
-      m = warp_max(m);
-      for (int i = lane; i < n; i += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(i) + MT * 128) + warp);
-        const float f = ml.x == m ? 1.f : exp2_fast(ml.x - m);
-        others[i * HEADS + warp] = f;
-        l += ml.y * f;
+    const int id = side ? open1 : open0, tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per,
+              n = (tile0 + tiles - 1) / per - b0 + 1;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int AHEAD = 4;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+      float4 ml[AHEAD], o[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int b = b0 + min(i0 + k, n - 1);
+        const float *from = sp.parts + ((size_t)b * 2 + (tile0 >= b * per)) * S::PIECE;
+        ml[k] = __ldcg(reinterpret_cast<const float4 *>(from + MT * 128) + tg);
+        o[k] = __ldcg(reinterpret_cast<const float4 *>(from) + j * 32 + lane);
       }
-      l = warp_sum(l);
-      if (lane == 0) whole_ml[warp] = make_float2(m, l);
-    }
-    __syncthreads();
-    for (int j = warp; j < MT; j += NW) {
-      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float4 o = __ldcg(reinterpret_cast<const float4 *>(part_of(i)) + j * 32 + lane);
-        const float2 f = *reinterpret_cast<const float2 *>(&others[i * HEADS + 2 * tg]);
-        r.x += o.x * f.x; r.y += o.y * f.y; r.z += o.z * f.x; r.w += o.w * f.y;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (i0 + k >= n) continue;
+        const float a0 = fmaxf(m0, ml[k].x), a1 = fmaxf(m1, ml[k].z);
+        const float w0 = m0 == a0 ? 1.f : exp2_fast(m0 - a0), w1 = m1 == a1 ? 1.f : exp2_fast(m1 - a1), f0 = ml[k].x == a0 ? 1.f : exp2_fast(ml[k].x - a0),
+                    f1 = ml[k].z == a1 ? 1.f : exp2_fast(ml[k].z - a1);
+        m0 = a0; m1 = a1;
+        l0 = l0 * w0 + ml[k].y * f0; l1 = l1 * w1 + ml[k].w * f1;
+        r.x = r.x * w0 + o[k].x * f0; r.y = r.y * w1 + o[k].y * f1; r.z = r.z * w0 + o[k].z * f0; r.w = r.w * w1 + o[k].w * f1;
       }
-      leave(r, whole_ml[2 * tg].y, whole_ml[2 * tg + 1].y, id, j);
     }
-    __syncthreads();
+    leave(r, l0, l1, id, j);
   }
 }
 
