@@ -163,10 +163,17 @@ template <int N> __device__ __forceinline__ void store_n(void *out, size_t at, i
   else run((__nv_bfloat16 *)out);
 }
 
-__device__ __forceinline__ void store_one(void *out, size_t at, int dtype, float v) {
-  if (dtype == PT_DT_F32) ((float *)out)[at] = v;
-  else if (dtype == PT_DT_F16) ((__half *)out)[at] = from_f<__half>(v);
-  else ((__nv_bfloat16 *)out)[at] = from_f<__nv_bfloat16>(v);
+// Two neighbouring dimensions of up to two heads, the sums o over l.
+static __device__ __noinline__ void store_sums(void *out, size_t at, int vdim, int dtype, int heads, float4 o, float l0, float l1) {
+  const float y[4] = {__fdividef(o.x, l0), __fdividef(o.z, l0), __fdividef(o.y, l1), __fdividef(o.w, l1)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i / 2 >= heads) return;
+    const size_t to = at + (i & 1) + (i / 2) * vdim;
+    if (dtype == PT_DT_F32) ((float *)out)[to] = y[i];
+    else if (dtype == PT_DT_F16) ((__half *)out)[to] = from_f<__half>(y[i]);
+    else ((__nv_bfloat16 *)out)[to] = from_f<__nv_bfloat16>(y[i]);
+  }
 }
 
 // Where a run of tiles has come to: token, segment of it, tile of that.
@@ -208,9 +215,11 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   using S = Shape<SIZE>;
   constexpr int QPARTS = E4M3 ? PARTS : 3, QREGS = E4M3 ? 2 : 1, NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
   extern __shared__ __align__(128) unsigned char smem[];
-  // The pieces of segments that warps begin and end with: which segments, and (R, l) of heads 2 tg and 2 tg + 1.
-  __shared__ int scan[NW], widest[NW], front[NW], rear[NW], last[2];
-  __shared__ float4 front_ml[NW][4], rear_ml[NW][4];
+  // The pieces of segments that warps begin and end with: which segments, and (R, l) of every head.
+  __shared__ int scan[NW], widest[NW], front[NW], rear[NW], first_block[2], parts[2];
+  __shared__ float2 ml[2 * NW][HEADS];      // rears, fronts
+  __shared__ __align__(16) float2 share[2 * NW][HEADS];      // factors that bring the pieces of a segment to one R, and l times those
+  __shared__ float top[2 * NW][HEADS];      // that R
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, tg = lane & 3;
   const int dim = FULL ? SIZE : p.c.dim, vdim = FULL ? SIZE : p.c.vdim;
   const int G = p.c.n_kv, qpk = p.heads / G, segs = sp.segs, tokens = sp.tokens;
@@ -222,8 +231,9 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   // ---- how many tiles every token has, and the sums in front of it
   const int used = p.b.cu[p.b.n_seq];
   int before = 0, most = 0;
-  for (int t0 = 0; t0 < tokens; t0 += NW * 32) {
-    const int t = t0 + tid, tok = sp.tok0 + t;
+  const bool few = tokens <= 32;      // (every warp counts them by itself)
+  for (int t0 = 0; t0 < tokens; t0 += few ? 32 : NW * 32) {
+    const int t = few ? lane : t0 + tid, tok = sp.tok0 + t;
     int n = 0;
     if (t < tokens) {
       int pos = -1, slot = 0;
@@ -241,12 +251,14 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         if (in_table(p.c, start, end - first)) {
           pos = start + tok - first;
           n = pos / KT - (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT + 1;
-        } else if (blockIdx.x == 0 && p.error_flag) {
+        } else if (blockIdx.x == 0 && (!few || warp == 0) && p.error_flag) {
           atomicExch(p.error_flag, 12);
         }
       }
-      pl.pos[t] = pos;
-      pl.slot[t] = slot;
+      if (!few || warp == 0) {
+        pl.pos[t] = pos;
+        pl.slot[t] = slot;
+      }
     }
     int sum = n;
 #pragma unroll
@@ -254,8 +266,14 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       const int up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    if (lane == 31) scan[warp] = sum;
     const int w_most = (int)__reduce_max_sync(0xffffffffu, (unsigned)n);
+    if (few) {
+      before = __shfl_sync(0xffffffffu, sum, 31);
+      most = w_most;
+      if (warp == 0 && t < tokens) pl.cum[t + 1] = sum;
+      break;
+    }
+    if (lane == 31) scan[warp] = sum;
     if (lane == 0) widest[warp] = w_most;
     __syncthreads();
     int base = before;
@@ -285,7 +303,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   if (block_n <= 0) return;
 
   // ---- this warp's run
-  const int run0 = block0 + block_n * warp / NW, count = block0 + block_n * (warp + 1) / NW - run0;
+  const int each = block_n / NW, more = block_n - each * NW, run0 = block0 + each * warp + min(warp, more), count = each + (warp < more);      // (warps without tiles are the last)
   unsigned char *ring = smem + warp * S::RING;
   if (count > 0) {
     if (one_each) w.tile = run0 - block0;
@@ -398,22 +416,24 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
                 }
               }
         } else {
+          // v = round((127 2^14 / top) x) as digits 2^14 hi + 2^7 mid + lo, mid and lo in -64 .. 63: those of v + 64 + 64 2^7, less 64.  (1.5 2^23 is added in fp32: the sum's lowest bits are v.)
           const float top = fmaxf(__uint_as_float(most), 0x1p-100f), turn = 127.f * 16384.f / top;
-          unit = __uint_as_float(most) == 0.f ? 0.f : most > 0x7f800000u ? __uint_as_float(most) : top / (127.f * 16384.f);
+          unit = __uint_as_float(most) == 0.f ? 0.f : most >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : top / (127.f * 16384.f);
 #pragma unroll
           for (int i = 0; i < NK; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              uint32_t part[3] = {0, 0, 0};
+              uint32_t v[4], part[3];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int v = __float2int_rn(x[i][4 * c + e] * turn), hi = (v + 8192) >> 14, rest = v - (hi << 14), mid = (rest + 64) >> 7, lo = rest - (mid << 7);
-                part[0] |= (uint32_t)(hi & 255) << (8 * e);
-                part[1] |= (uint32_t)(mid & 255) << (8 * e);
-                part[2] |= (uint32_t)(lo & 255) << (8 * e);
+              for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[i][4 * c + e], turn, 12582912.f)) + (64u + (64u << 7) - 0x4B400000u);
+#pragma unroll
+              for (int q = 0; q < 3; ++q) {       // bits 0 .. 6, 7 .. 13 and 14 .. 21 as byte 0, 1 and 2
+                const uint32_t sel = q == 0 ? 0x0040u : q == 1 ? 0x0051u : 0x0062u, sh = q;
+                part[q] = __byte_perm(__byte_perm(v[0] << sh, v[1] << sh, sel), __byte_perm(v[2] << sh, v[3] << sh, sel), 0x5410);
               }
+              qf[0][4 * i + c][0] = part[2];
 #pragma unroll
-              for (int q = 0; q < QPARTS; ++q) qf[q][4 * i + c][0] = part[q];
+              for (int q = 1; q < QPARTS; ++q) qf[q][4 * i + c][0] = (((part[2 - q] & 0x7f7f7f7fu) | 0x80808080u) - 0x40404040u) ^ 0x80808080u;
             }
         }
 #pragma unroll
@@ -592,7 +612,10 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j) reinterpret_cast<float4 *>(to)[j * 32 + lane] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
-        if (g == 0) (end ? rear_ml : front_ml)[warp][tg] = make_float4(R[0], L[0], R[1], L[1]);
+        if (g == 0) {
+          ml[end ? warp : NW + warp][2 * tg] = make_float2(R[0], L[0]);
+          ml[end ? warp : NW + warp][2 * tg + 1] = make_float2(R[1], L[1]);
+        }
         if (lane == 0) (end ? rear : front)[warp] = tok * segs + w.seg;
       }
       w.tile += here;
@@ -602,62 +625,63 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   }
   __syncthreads();
 
-  // ---- pieces of a segment come together: the ends of some warps and the front of the next, a unit of four floats a lane at a time, dealt out to the warps.  What is
-  // not the block's alone goes where the others find it.
-  auto leave = [&](const float4 &o, float l0, float l1, int id, int j) {       // (l of heads 2 tg and 2 tg + 1)
+  // ---- pieces of a segment come together: the rears of some warps and the front of the next.  (Whoever has the block's last tile, the others wait for this: few instructions one after
+  // the other.)  First their shares, a warp per head and a lane per piece ...
+  static_assert(2 * NW <= 32 && NW >= HEADS, "a lane per piece, a warp per head");
+  if (warp < HEADS) {
+    const int id = lane < NW ? rear[lane] : lane < 2 * NW ? front[lane - NW] : -1;
+    const float2 x = ml[min(lane, 2 * NW - 1)][warp];
+    const int key = __float_as_int(x.x), most_key = __reduce_max_sync(__match_any_sync(0xffffffffu, id), key ^ (key >> 31 & 0x7fffffff));      // (floats in the order of whole numbers)
+    const float r = __int_as_float(most_key ^ (most_key >> 31 & 0x7fffffff)), f = x.x == r ? 1.f : exp2_fast(x.x - r);
+    if (lane < 2 * NW) {
+      share[lane][warp] = make_float2(f, x.y * f);
+      top[lane][warp] = r;
+    }
+  }
+  __syncthreads();
+  // ... then the sums, a unit of four floats a lane at a time, dealt out to the warps.  What is not the block's alone goes where the others find it.
+  auto leave = [&](const float4 &o, float l0, float l1, int id, int j) {
     const int tok = sp.by_segs(id), seg = id - tok * segs, kvh = sp.by_chunks(seg), chunk = seg - kvh * sp.chunks, heads = min(HEADS, qpk - chunk * HEADS);
     const int d = VB * g + 128 * (j / 8) + 2 * (j % 8);
     const size_t at = (size_t)(sp.tok0 + tok) * p.out_ld + (size_t)(kvh * qpk + chunk * HEADS + 2 * tg) * vdim + d;
-    const float f0 = 1.f / l0, f1 = 1.f / l1;
-    if (2 * tg < heads && d < vdim) {
-      store_one(sp.out, at, sp.dtype, o.x * f0);
-      store_one(sp.out, at + 1, sp.dtype, o.z * f0);
-    }
-    if (2 * tg + 1 < heads && d < vdim) {
-      store_one(sp.out, at + vdim, sp.dtype, o.y * f1);
-      store_one(sp.out, at + vdim + 1, sp.dtype, o.w * f1);
-    }
+    if (d < vdim) store_sums(sp.out, at, vdim, sp.dtype, heads - 2 * tg, o, l0, l1);
   };
   const int rear_l = lane < NW ? rear[lane] : -1, front_l = lane < NW ? front[lane] : -1;
-  const uint32_t any_front = __ballot_sync(0xffffffffu, front_l >= 0);
   int unit = 0, open0 = -1, open1 = -1;       // the segments that begin before the block's run, and that end behind it
-  for (int w0 = any_front ? -1 : 0; w0 < NW;) {      // (-1: what began before the block and ends in its first warp that has tiles; every other front belongs to the rears before it)
-    const int id = __shfl_sync(0xffffffffu, w0 < 0 ? front_l : rear_l, w0 < 0 ? __ffs(any_front) - 1 : w0);
-    const uint32_t rears = __ballot_sync(0xffffffffu, rear_l == id), fronts = __ballot_sync(0xffffffffu, front_l == id);
-    if (id < 0 || (w0 < 0 && rears)) { ++w0; continue; }
+  for (int w0 = -1; w0 < NW;) {               // (-1: what began before the block and ends in its first warp; every other front belongs to the rears before it)
+    const int id = __shfl_sync(0xffffffffu, w0 < 0 ? front_l : rear_l, max(w0, 0));
+    const uint32_t rears = __ballot_sync(0xffffffffu, rear_l == id), fronts = __ballot_sync(0xffffffffu, front_l == id);      // (rears of one segment are neighbours)
+    if (id < 0) { ++w0; continue; }
     const int tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles;
     const bool alone = tile0 >= block0 && tile0 + tiles <= block0 + block_n;
     const int side = tile0 >= block0;
     if (!alone) (side ? open1 : open0) = id;
     float *part = sp.parts + ((size_t)blockIdx.x * 2 + side) * S::PIECE;
+    const int fw = __ffs(fronts) - 1, r0 = rears ? __ffs(rears) - 1 : 0, r1 = 32 - __clz(rears);
+#pragma unroll 1
     for (int j = 0; j < MT; ++j, ++unit) {
       if (unit % NW != warp) continue;
-      float4 ml[NW + 1], o[NW + 1];       // (all of them asked for at once)
-      const int fw = fronts ? __ffs(fronts) - 1 : 0;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        ml[k] = rear_ml[k][tg];
-        o[k] = reinterpret_cast<const float4 *>(smem + k * S::RING)[j * 32 + lane];
-      }
-      ml[NW] = front_ml[fw][tg];
-      o[NW] = fronts ? __ldcg(reinterpret_cast<const float4 *>(sp.heads + ((size_t)blockIdx.x * NW + fw) * S::PIECE) + j * 32 + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
       float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k <= NW; ++k)
-        if (k < NW ? rears >> k & 1 : fronts != 0) { m0 = fmaxf(m0, ml[k].x); m1 = fmaxf(m1, ml[k].z); }
-#pragma unroll
-      for (int k = 0; k <= NW; ++k)
-        if (k < NW ? rears >> k & 1 : fronts != 0) {
-          const float f0 = ml[k].x == m0 ? 1.f : exp2_fast(ml[k].x - m0), f1 = ml[k].z == m1 ? 1.f : exp2_fast(ml[k].z - m1);
-          l0 += ml[k].y * f0; l1 += ml[k].w * f1;
-          r.x += o[k].x * f0; r.y += o[k].y * f1; r.z += o[k].z * f0; r.w += o[k].w * f1;
-        }
+      float l0 = 0.f, l1 = 0.f;
+      if (fw >= 0) {
+        const float4 o = __ldcg(reinterpret_cast<const float4 *>(sp.heads + ((size_t)blockIdx.x * NW + fw) * S::PIECE) + j * 32 + lane), f = *reinterpret_cast<const float4 *>(&share[NW + fw][2 * tg]);
+        r = make_float4(o.x * f.x, o.y * f.z, o.z * f.x, o.w * f.z);
+        l0 = f.y; l1 = f.w;
+      }
+#pragma unroll 2
+      for (int k = r0; k < r1; ++k) {
+        const float4 o = reinterpret_cast<const float4 *>(smem + k * S::RING)[j * 32 + lane], f = *reinterpret_cast<const float4 *>(&share[k][2 * tg]);
+        r.x += o.x * f.x; r.y += o.y * f.z; r.z += o.z * f.x; r.w += o.w * f.z;
+        l0 += f.y; l1 += f.w;
+      }
       if (alone) {
         leave(r, l0, l1, id, j);
       } else {
         __stcg(reinterpret_cast<float4 *>(part) + j * 32 + lane, r);
-        if (j == 0 && g == 0) __stcg(reinterpret_cast<float4 *>(part + MT * 128) + tg, make_float4(m0, l0, m1, l1));
+        if (j == 0 && g == 0) {
+          const int any = rears ? __ffs(rears) - 1 : NW + fw;
+          __stcg(reinterpret_cast<float4 *>(part + MT * 128) + tg, make_float4(top[any][2 * tg], l0, top[any][2 * tg + 1], l1));
+        }
       }
     }
     w0 = w0 < 0 ? 0 : 32 - __clz(rears);
@@ -668,44 +692,52 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   __syncthreads();
   if (tid < 2) {
     const int id = tid ? open1 : open0;
-    last[tid] = 0;
+    parts[tid] = 0;
     if (id >= 0) {
-      const int tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles;
-      last[tid] = atomicAdd(sp.counters + id, 1) == (tile0 + tiles - 1) / per - tile0 / per;
-      if (last[tid]) sp.counters[id] = 0;
+      const int tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per, n = (tile0 + tiles - 1) / per - b0 + 1;
+      if (atomicAdd(sp.counters + id, 1) == n - 1) {
+        sp.counters[id] = 0;
+        first_block[tid] = b0;
+        parts[tid] = n;
+      }
     }
     __threadfence();
   }
   __syncthreads();
-  for (int unit = warp; unit < 2 * MT; unit += NW) {
-    const int side = unit >= MT, j = unit - side * MT;
-    if (!last[side]) continue;
-    const int id = side ? open1 : open0, tok = sp.by_segs(id), tiles = pl.cum[tok + 1] - pl.cum[tok], tile0 = pl.cum[tok] * segs + (id - tok * segs) * tiles, b0 = tile0 / per,
-              n = (tile0 + tiles - 1) / per - b0 + 1;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int AHEAD = 4;
-    for (int i0 = 0; i0 < n; i0 += AHEAD) {
-      float4 ml[AHEAD], o[AHEAD];
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int b = b0 + min(i0 + k, n - 1);
-        const float *from = sp.parts + ((size_t)b * 2 + (tile0 >= b * per)) * S::PIECE;
-        ml[k] = __ldcg(reinterpret_cast<const float4 *>(from + MT * 128) + tg);
-        o[k] = __ldcg(reinterpret_cast<const float4 *>(from) + j * 32 + lane);
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (i0 + k >= n) continue;
-        const float a0 = fmaxf(m0, ml[k].x), a1 = fmaxf(m1, ml[k].z);
-        const float w0 = m0 == a0 ? 1.f : exp2_fast(m0 - a0), w1 = m1 == a1 ? 1.f : exp2_fast(m1 - a1), f0 = ml[k].x == a0 ? 1.f : exp2_fast(ml[k].x - a0),
-                    f1 = ml[k].z == a1 ? 1.f : exp2_fast(ml[k].z - a1);
-        m0 = a0; m1 = a1;
-        l0 = l0 * w0 + ml[k].y * f0; l1 = l1 * w1 + ml[k].w * f1;
-        r.x = r.x * w0 + o[k].x * f0; r.y = r.y * w1 + o[k].y * f1; r.z = r.z * w0 + o[k].z * f0; r.w = r.w * w1 + o[k].w * f1;
+  // (Of both segments at once.  Shares first, a warp per head and a lane per part.)
+  if (!parts[0] && !parts[1]) return;
+  auto part_of = [&](int side, int i) { return sp.parts + ((size_t)(first_block[side] + i) * 2 + (i == 0)) * S::PIECE; };     // (a segment begins in its first block)
+  float2 *shares = reinterpret_cast<float2 *>(smem);      // [side][grid][head]: the pieces in shared memory have been used
+  if (warp < HEADS) {
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+      const int n = parts[side];
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(reinterpret_cast<const float2 *>(part_of(side, i) + MT * 128) + warp).x);
+      m = warp_max(m);
+#pragma unroll 1
+      for (int i = lane; i < n; i += 32) {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part_of(side, i) + MT * 128) + warp);
+        const float f = x.x == m ? 1.f : exp2_fast(x.x - m);
+        shares[(side * sp.grid + i) * HEADS + warp] = make_float2(f, x.y * f);
       }
     }
-    leave(r, l0, l1, id, j);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int n = warp; n < 2 * MT; n += NW) {
+    const int side = n >= MT, j = n - side * MT;
+    if (!parts[side]) continue;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l0 = 0.f, l1 = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < parts[side]; ++i) {
+      const float4 o = __ldcg(reinterpret_cast<const float4 *>(part_of(side, i)) + j * 32 + lane), f = *reinterpret_cast<const float4 *>(&shares[(side * sp.grid + i) * HEADS + 2 * tg]);
+      r.x += o.x * f.x; r.y += o.y * f.z; r.z += o.z * f.x; r.w += o.w * f.z;
+      l0 += f.y; l1 += f.w;
+    }
+    leave(r, l0, l1, side ? open1 : open0, j);
   }
 }
 
