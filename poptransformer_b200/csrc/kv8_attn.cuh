@@ -44,18 +44,6 @@ template <int SIZE> struct Shape {
   static_assert(PIECE * 4 <= RING, "a warp's last piece takes the place of its keys and values");
 };
 
-// Division by what a launch has but once: n / d = (n + high word of n mul) >> shift for 0 <= n < 2^31, mul = ceil(2^32 (2^shift - d) / d), 2^shift the power of two at or above d.
-struct Divide {
-  uint32_t d, mul, shift;
-  __host__ static Divide by(uint32_t d) {
-    Divide r{d, 0, 0};
-    while ((1ull << r.shift) < d) ++r.shift;
-    r.mul = (uint32_t)((((1ull << r.shift) - d) << 32) / d + 1);
-    return r;
-  }
-  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-};
-
 struct Plan {     // of a launch, in the shared memory of every block
   int *cum, *pos, *slot;      // [tokens + 1] tiles before, [tokens] position (of the token), [tokens]
 };

@@ -1,4 +1,4 @@
-// Rotation of rows by their positions, a lane at a time: what the rotation, appending and rounding kernels share.
+// Rotation of rows by their positions, a lane at a time: what the rotation and appending kernels share.
 //
 // A lane has eight pairs of a row: pairs 8 t .. 8 t + 7 of item t.  Pair p < rot / 2 is elements (p, p + rot / 2), or (2 p, 2 p + 1) where neighbours
 // turn together; behind the rotated part it is (2 p, 2 p + 1).  So a lane holds both elements of each of its pairs (a row can be rotated where it lies), and
@@ -12,6 +12,8 @@ __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
 struct Pairs { float a[8], b[8]; };
+// What a lane reads of a row, as it lies there (two runs of eight): asked for before it is known how far the row turns.
+template <typename T> struct Runs { uint4 v[sizeof(T) / 2 * 2]; };
 
 // Eight values that lie together, from or to a multiple of 16 bytes.
 __device__ __forceinline__ void load_run(const float *p, float (&v)[8]) {
@@ -40,29 +42,41 @@ template <typename T> __device__ __forceinline__ void store_run(T *p, const floa
 // Elements of pair p of a row.
 __device__ __forceinline__ int2 pair_at(int p, int rot, bool neighbours) { return p < rot / 2 && !neighbours ? make_int2(p, p + rot / 2) : make_int2(2 * p, 2 * p + 1); }
 
-// WHOLE: rows lie on multiples of 16 bytes, dim is a multiple of 16, and so is rot: every item is two whole runs.  apart: the runs are rot / 2 apart.
-template <bool WHOLE, typename T> __device__ __forceinline__ Pairs load_pairs(const T *x, int t, int dim, int rot, bool neighbours) {
+// Of rows that lie on multiples of 16 bytes, with dim and rot multiples of 16: every item is two whole runs, rot / 2 apart or one behind the other.
+template <typename T> __device__ __forceinline__ Runs<T> load_runs(const T *x, int t, int rot, bool neighbours) {
+  constexpr int N = sizeof(T) / 2;
+  const bool apart = !neighbours && 16 * t < rot;
+  const uint4 *lo = reinterpret_cast<const uint4 *>(x + (apart ? 8 * t : 16 * t)), *hi = reinterpret_cast<const uint4 *>(x + (apart ? 8 * t + rot / 2 : 16 * t + 8));
+  Runs<T> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) { r.v[i] = lo[i]; r.v[N + i] = hi[i]; }
+  return r;
+}
+template <typename T> __device__ __forceinline__ Pairs pairs_of(const Runs<T> &r, int t, int rot, bool neighbours) {
+  const bool apart = !neighbours && 16 * t < rot;
+  T e[16];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4 *>(e)[i] = r.v[i];
   Pairs v;
-  if constexpr (WHOLE) {
-    const bool apart = !neighbours && 16 * t < rot;
-    float lo[8], hi[8];
-    load_run(x + (apart ? 8 * t : 16 * t), lo);
-    load_run(x + (apart ? 8 * t + rot / 2 : 16 * t + 8), hi);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v.a[j] = apart ? lo[j] : j < 4 ? lo[2 * (j & 3)] : hi[2 * (j & 3)];
-      v.b[j] = apart ? hi[j] : j < 4 ? lo[2 * (j & 3) + 1] : hi[2 * (j & 3) + 1];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int2 e = pair_at(8 * t + j, rot, neighbours);
-      v.a[j] = e.x < dim ? to_f(x[e.x]) : 0.f;
-      v.b[j] = e.y < dim ? to_f(x[e.y]) : 0.f;
-    }
+  for (int j = 0; j < 8; ++j) {
+    v.a[j] = to_f(apart ? e[j] : e[2 * j]);
+    v.b[j] = to_f(apart ? e[8 + j] : e[2 * j + 1]);
   }
   return v;
 }
+// Of any rows.
+template <typename T> __device__ __forceinline__ Pairs load_pairs(const T *x, int t, int dim, int rot, bool neighbours) {
+  Pairs v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int2 e = pair_at(8 * t + j, rot, neighbours);
+    v.a[j] = e.x < dim ? to_f(x[e.x]) : 0.f;
+    v.b[j] = e.y < dim ? to_f(x[e.y]) : 0.f;
+  }
+  return v;
+}
+// WHOLE: as load_runs wants them.
 template <bool WHOLE, typename T> __device__ __forceinline__ void store_pairs(T *x, const Pairs &v, int t, int dim, int rot, bool neighbours) {
   if constexpr (WHOLE) {
     const bool apart = !neighbours && 16 * t < rot;
@@ -84,15 +98,24 @@ template <bool WHOLE, typename T> __device__ __forceinline__ void store_pairs(T 
   }
 }
 
-// (cos, sin) of an item's pairs; (1, 0) behind the rotated part.
+// (cos, sin) of an item's pairs; (1, 0) behind the rotated part.  WHOLE: a row of the table lies on a multiple of 16 bytes, and an item is rotated as a whole or not at all.
 struct Turn { float c[8], s[8]; };
-__device__ __forceinline__ Turn load_turn(const float2 *row, int t, int rot, bool inverse) {
+template <bool WHOLE> __device__ __forceinline__ Turn load_turn(const float2 *row, int t, int rot, bool inverse) {
   Turn r;
+  if constexpr (WHOLE) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float2 cs = 8 * t + j < rot / 2 ? __ldg(row + 8 * t + j) : make_float2(1.f, 0.f);
-    r.c[j] = cs.x;
-    r.s[j] = inverse ? -cs.y : cs.y;
+    for (int j = 0; j < 4; ++j) {
+      const float4 cs = 16 * t < rot ? __ldg(reinterpret_cast<const float4 *>(row + 8 * t) + j) : make_float4(1.f, 0.f, 1.f, 0.f);
+      r.c[2 * j] = cs.x; r.c[2 * j + 1] = cs.z;
+      r.s[2 * j] = inverse ? -cs.y : cs.y; r.s[2 * j + 1] = inverse ? -cs.w : cs.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 cs = 8 * t + j < rot / 2 ? __ldg(row + 8 * t + j) : make_float2(1.f, 0.f);
+      r.c[j] = cs.x;
+      r.s[j] = inverse ? -cs.y : cs.y;
+    }
   }
   return r;
 }

@@ -827,7 +827,7 @@ class PagedKVCache:
             if pool.device.type != wanted.type or wanted.index not in (None, pool.device.index) or page_table is not None and page_table.device != pool.device:
                 raise PtError(f"PagedKVCache: pool on {pool.device}, wanted on {wanted}" + ("" if page_table is None else f" with its page table on {page_table.device}"))
         self.pool = torch.zeros(shape, dtype=dtype, device=device) if pool is None else pool
-        self.scales = None
+        self.scales = self.kv8 = None
         if dtype in KV8_FORMATS:
             if not 1 <= min(head_dim, self.v_dim) <= max(head_dim, self.v_dim) <= 256:
                 raise PtError(f"PagedKVCache: eight bits want heads of 1 to 256 dimensions, got {head_dim} and {self.v_dim}")
@@ -951,39 +951,54 @@ def _rope_ok(who, rope, rope_dims, positions):
 
 def _row_ld(who, name, t, rows, width):
     """Row stride of a 2-D tensor whose rows lie together."""
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or t.shape[1] > 1 and t.stride(1) != 1:
-        raise PtError(f"{who}: {name} wants {rows} rows of {width} neighbouring elements or more, got {tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] < rows or shape[1] < width or shape[1] > 1 and stride[1] != 1:
+        raise PtError(f"{who}: {name} wants {rows} rows of {width} neighbouring elements or more, got {tuple(shape)} with strides {stride}")
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def rotary(x, heads, dim, rope, positions, out=None, rope_dims=None, interleaved=False, inverse=False, error_flag=None):
     """Rows of heads rotated by their positions (see pt_rotary): x [rows, heads * dim or more], whose rows may lie apart (a part of wider rows), positions int32 [rows], rope as rope_table makes
     it.  out: None rotates x itself.  rope_dims: rotated dimensions at the front of a head (None: the table's).  interleaved: pairs are neighbours.  inverse: by
     the negative angles, which takes the gradient of the output to that of x."""
-    rows = x.shape[0]
+    rows, table, dtype = x.shape[0], rope.shape, x.dtype
     out = x if out is None else out
-    rope_dims = rope.shape[1] * 2 if rope_dims is None else rope_dims
-    _here("rotary", x, out, positions, rope, error_flag)
-    _rope_ok("rotary", rope, rope_dims, 1)
-    x_ld, out_ld = _row_ld("rotary", "x", x, rows, heads * dim), _row_ld("rotary", "out", out, rows, heads * dim)
-    if out.dtype != x.dtype or out.shape[0] != rows or positions.dtype != torch.int32 or positions.numel() != rows:
-        raise PtError(f"rotary: {rows} rows of {x.dtype} want out of that and int32 positions of each, got {out.dtype} {tuple(out.shape)}, {positions.dtype} {tuple(positions.shape)}")
+    rope_dims = table[1] * 2 if rope_dims is None else rope_dims
+    now = torch._C._cuda_getDevice() if x.is_cuda else -1
+    # (One look at what is right, the same again with words where it is not: a launch takes less time than the checks one by one.)
+    if not (x.get_device() == out.get_device() == positions.get_device() == rope.get_device() == now >= 0 and (error_flag is None or error_flag.get_device() == now)):
+        _here("rotary", x, out, positions, rope, error_flag)
+    if rope.dtype is not torch.float32 or len(table) != 3 or table[1] * 2 != rope_dims or table[2] != 2:
+        _rope_ok("rotary", rope, rope_dims, 1)
+    x_ld = _row_ld("rotary", "x", x, rows, heads * dim)
+    out_ld = x_ld if out is x else _row_ld("rotary", "out", out, rows, heads * dim)
+    if out.dtype is not dtype or out.shape[0] != rows or positions.dtype is not torch.int32 or positions.numel() != rows:
+        raise PtError(f"rotary: {rows} rows of {dtype} want out of that and int32 positions of each, got {out.dtype} {tuple(out.shape)}, {positions.dtype} {tuple(positions.shape)}")
     if not rows:
         return out
-    a = RotaryArgs(rows, heads, dim, dtype_code(x.dtype), x.data_ptr(), x_ld, out.data_ptr(), out_ld, _ptr(positions), rope.shape[0], rope_dims, 1 if interleaved else 0, 1 if inverse else 0,
-                   _ptr(rope), _ptr(error_flag))
-    check(_lib.lib().pt_rotary(ctypes.byref(a), _stream()), "pt_rotary")
+    a = RotaryArgs(rows, heads, dim, dtype_code(dtype), x.data_ptr(), x_ld, out.data_ptr(), out_ld, _ptr(positions), table[0], rope_dims, 1 if interleaved else 0, 1 if inverse else 0,
+                   _ptr(rope), None if error_flag is None else _ptr(error_flag))
+    rc = _lib.lib().pt_rotary(ctypes.byref(a), _stream())
+    if rc:
+        check(rc, "pt_rotary")
     return out
 
 
 def _kv8(cache, who):
-    fmt = KV8_FORMATS.get(cache.pool.dtype)
+    """The structure of a cache of eight bits.  (Made once: its tensors are the same from call to call.)"""
+    pool, scales, table, made = cache.pool, cache.scales, cache.page_table, cache.kv8
+    if made is not None and made[0] is pool and made[1] is scales and made[2] is table:
+        return made[3]
+    fmt = KV8_FORMATS.get(pool.dtype)
     if fmt is None:
-        raise PtError(f"{who}: a cache of {cache.pool.dtype}; int8 or float8_e4m3fn is wanted")
-    table = cache.page_table
+        raise PtError(f"{who}: a cache of {pool.dtype}; int8 or float8_e4m3fn is wanted")
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] * cache.page_size < cache.max_len:
         raise PtError(f"{who}: the page table is int32 [slots, pages of {cache.max_len} positions], got {table.dtype} {tuple(table.shape)}")
-    return Kv8Cache(_ptr(cache.pool), _ptr(cache.scales), _ptr(table), fmt, cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len)
+    if not pool.get_device() == scales.get_device() == table.get_device():
+        raise PtError(f"{who}: pool on {pool.device}, scales on {scales.device}, page table on {table.device}")
+    made = Kv8Cache(_ptr(pool), _ptr(scales), _ptr(table), fmt, cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len)
+    cache.kv8 = (pool, scales, table, made)
+    return made
 
 
 def _rows_fit(who, name, t, rows, width, ld):
@@ -994,19 +1009,27 @@ def _rows_fit(who, name, t, rows, width, ld):
 def kv8_append(view, rows, ld, cache, n_head=0, rope=None, rope_dims=0, interleaved=False, q_out=None, q_out_ld=0, error_flag=None):
     """Keys (rotated) and values of the packed tokens of `view` go to a cache of eight bits (see pt_kv8_append).  Rows hold [q | k | v] of n_head query heads, or [k | v] with n_head = 0.  q_out: where
     the rotated queries go, rows of q_out_ld (`rows` itself rotates them in place).  rope: as rope_table makes it, of cache.max_len positions or more."""
-    n_tok, n_kv, dim, vdim, es = view.n_tok, cache.n_kv, cache.head_dim, cache.v_dim, rows.element_size()
-    _here("kv8_append", rows, cache.pool, rope, q_out, error_flag)
-    _rope_ok("kv8_append", rope, rope_dims, cache.max_len)
+    n_tok, n_kv, dim, vdim, es, dtype = view.n_tok, cache.n_kv, cache.head_dim, cache.v_dim, rows.element_size(), rows.dtype
+    now = torch._C._cuda_getDevice() if rows.is_cuda else -1
+    if not (rows.get_device() == cache.pool.get_device() == view.keep[0].get_device() == now >= 0 and (rope is None or rope.get_device() == now) and (q_out is None or q_out.get_device() == now)
+            and (error_flag is None or error_flag.get_device() == now)):
+        _here("kv8_append", rows, cache.pool, *view.keep, rope, q_out, error_flag)
+    if rope_dims:
+        _rope_ok("kv8_append", rope, rope_dims, cache.max_len)
     _rows_fit("kv8_append", "rows", rows, n_tok, (n_head + n_kv) * dim + n_kv * vdim, ld)
+    to = None
     if q_out is not None:
-        if q_out.dtype != rows.dtype or n_head < 1:
-            raise PtError(f"kv8_append: {n_head} query heads of {rows.dtype} to q_out of {q_out.dtype}")
+        if q_out.dtype is not dtype or n_head < 1:
+            raise PtError(f"kv8_append: {n_head} query heads of {dtype} to q_out of {q_out.dtype}")
         _rows_fit("kv8_append", "q_out", q_out, n_tok, n_head * dim, q_out_ld)
+        to = _ptr(q_out)
     q = _ptr(rows)
     k = q + n_head * dim * es
-    a = Kv8AppendArgs(view, _kv8(cache, "kv8_append"), dtype_code(rows.dtype), n_head, q, k, k + n_kv * dim * es, ld, _ptr(q_out), q_out_ld, rope_dims, 1 if interleaved else 0, _ptr(rope),
-                      _ptr(error_flag))
-    check(_lib.lib().pt_kv8_append(ctypes.byref(a), _stream()), "pt_kv8_append")
+    a = Kv8AppendArgs(view, _kv8(cache, "kv8_append"), dtype_code(dtype), n_head, q, k, k + n_kv * dim * es, ld, to, q_out_ld, rope_dims, 1 if interleaved else 0, None if rope is None else _ptr(rope),
+                      None if error_flag is None else _ptr(error_flag))
+    rc = _lib.lib().pt_kv8_append(ctypes.byref(a), _stream())
+    if rc:
+        check(rc, "pt_kv8_append")
 
 
 def kv8_attn_workspace(n_tok, n_head, n_kv, width, device="cuda"):
@@ -1017,15 +1040,20 @@ def kv8_attn_workspace(n_tok, n_head, n_kv, width, device="cuda"):
 def kv8_attn(view, q, q_ld, cache, out, out_ld, n_head, scale, window=0, softcap=0.0, workspace=None, error_flag=None, plain=False):
     """Attention of new tokens (one a sequence, or a few) over a cache of eight bits that has their keys and values already (see pt_kv8_attn).  q rows begin with n_head rotated
     queries, out rows with n_head * v_dim outputs."""
-    n_tok = view.n_tok
-    if out.dtype != q.dtype:
-        raise PtError(f"kv8_attn: q {q.dtype}, out {out.dtype}: one type is wanted")
-    _here("kv8_attn", q, out, cache.pool, workspace, error_flag)
+    n_tok, dtype = view.n_tok, q.dtype
+    if out.dtype is not dtype:
+        raise PtError(f"kv8_attn: q {dtype}, out {out.dtype}: one type is wanted")
+    now = torch._C._cuda_getDevice() if q.is_cuda else -1
+    if not (q.get_device() == out.get_device() == cache.pool.get_device() == view.keep[0].get_device() == now >= 0 and (workspace is None or workspace.get_device() == now)
+            and (error_flag is None or error_flag.get_device() == now)):
+        _here("kv8_attn", q, out, cache.pool, *view.keep, workspace, error_flag)
     _rows_fit("kv8_attn", "q", q, n_tok, n_head * cache.head_dim, q_ld)
     _rows_fit("kv8_attn", "out", out, n_tok, n_head * cache.v_dim, out_ld)
-    a = Kv8AttnArgs(view, _kv8(cache, "kv8_attn"), dtype_code(q.dtype), n_head, window, scale, softcap, _ptr(q), q_ld, _ptr(out), out_ld, 1 if plain else 0, _ptr(workspace),
-                    0 if workspace is None else workspace.numel(), _ptr(error_flag))
-    check(_lib.lib().pt_kv8_attn(ctypes.byref(a), _stream()), "pt_kv8_attn")
+    a = Kv8AttnArgs(view, _kv8(cache, "kv8_attn"), dtype_code(dtype), n_head, window, scale, softcap, _ptr(q), q_ld, _ptr(out), out_ld, 1 if plain else 0,
+                    None if workspace is None else _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), None if error_flag is None else _ptr(error_flag))
+    rc = _lib.lib().pt_kv8_attn(ctypes.byref(a), _stream())
+    if rc:
+        check(rc, "pt_kv8_attn")
     return out
 
 
@@ -1033,14 +1061,20 @@ def kv8_unpack(view, cache, into, error_flag=None):
     """All positions of the sequences of `view`, the cached and the new ones, from a cache of eight bits into the pages of one of 16 or 32 bits (`into`: same heads, its own table with the same slots), for
     the kernels that read those: a prompt's window_attn(append=False), for instance (see pt_kv8_unpack)."""
     _wide(into, "kv8_unpack (into)")
-    table = into.page_table
-    if (into.n_kv, into.head_dim, into.v_dim) != (cache.n_kv, cache.head_dim, cache.v_dim):
+    pool, table = into.pool, into.page_table
+    if into.n_kv != cache.n_kv or into.head_dim != cache.head_dim or into.v_dim != cache.v_dim:
         raise PtError(f"kv8_unpack: {cache.n_kv} heads of {cache.head_dim} and {cache.v_dim} into {into.n_kv} of {into.head_dim} and {into.v_dim}")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < cache.page_table.shape[0] or table.shape[1] * into.page_size < into.max_len:
-        raise PtError(f"kv8_unpack: a table of int32 [{cache.page_table.shape[0]} slots or more, pages of {into.max_len} positions], got {table.dtype} {tuple(table.shape)}")
-    _here("kv8_unpack", cache.pool, into.pool, table, error_flag)
-    a = Kv8UnpackArgs(view, _kv8(cache, "kv8_unpack"), dtype_code(into.pool.dtype), _ptr(into.pool), _ptr(table), into.page_size, table.shape[1], into.max_len, _ptr(error_flag))
-    check(_lib.lib().pt_kv8_unpack(ctypes.byref(a), _stream()), "pt_kv8_unpack")
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != 2 or shape[0] < cache.page_table.shape[0] or shape[1] * into.page_size < into.max_len:
+        raise PtError(f"kv8_unpack: a table of int32 [{cache.page_table.shape[0]} slots or more, pages of {into.max_len} positions], got {table.dtype} {tuple(shape)}")
+    now = torch._C._cuda_getDevice() if pool.is_cuda else -1
+    if not (cache.pool.get_device() == view.keep[0].get_device() == pool.get_device() == table.get_device() == now >= 0 and (error_flag is None or error_flag.get_device() == now)):
+        _here("kv8_unpack", cache.pool, pool, *view.keep, table, error_flag)
+    a = Kv8UnpackArgs(view, _kv8(cache, "kv8_unpack"), dtype_code(pool.dtype), _ptr(pool), _ptr(table), into.page_size, shape[1], into.max_len,
+                      None if error_flag is None else _ptr(error_flag))
+    rc = _lib.lib().pt_kv8_unpack(ctypes.byref(a), _stream())
+    if rc:
+        check(rc, "pt_kv8_unpack")
 
 
 def attn_workspace(batch, n_head, head_dim, max_pages, device="cuda"):

@@ -41,7 +41,9 @@ def test_other_kernels_refuse_it():
 def test_tensors_that_are_not_on_the_device_are_refused():
     """Launches go to the current device; what lies elsewhere is said, not read."""
     c = cache()
+    i = torch.zeros(2, dtype=torch.int32)
     view = _lib.BatchView(1, 1)
+    view.keep = (i, i, i, i)
     x = torch.zeros((1, 6 * 64), dtype=torch.float16)
     for call in (lambda: ops.kv8_append(view, x, 384, c, 2), lambda: ops.kv8_attn(view, x, 384, c, x, 384, 2, 1.0), lambda: ops.rotary(x, 6, 64, torch.zeros((4, 32, 2)), torch.zeros(1, dtype=torch.int32)),
                  lambda: ops.kv8_unpack(view, c, cache(torch.float16))):
