@@ -2,6 +2,8 @@
 //   pool[page] = K [n_kv][page_size][dim] and then V [n_kv][page_size][vdim], a byte each; scales[page] = fp32 [2][n_kv][page_size], K's and then V's.
 // A row x of one position and head is kept as  byte_i = round(x_i (top / m)),  scale = m / top,  m = max_i |x_i|  (top: 127 or 448).  m is at least 2^-64, so that
 // top / m is finite; a row that has a NaN, an infinity or a magnitude above 2^64 gets the scale NaN and bytes of 0, and reads back as NaN.
+#include <type_traits>
+
 #include "rotate.cuh"
 
 namespace pt {
@@ -53,7 +55,9 @@ template <bool E4M3> __device__ __forceinline__ uint32_t to_word(float a, float 
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   }
-  return to_byte<false>(a) | to_byte<false>(b) << 8 | to_byte<false>(c) << 16 | to_byte<false>(d) << 24;
+  // (|x| is at most 127 (1 + 2^-23): behind 1.5 2^23 the nearest whole number, ties to even, is in the lowest byte)
+  const uint32_t w = __float_as_uint(__fadd_rn(a, 12582912.f)), x = __float_as_uint(__fadd_rn(b, 12582912.f)), y = __float_as_uint(__fadd_rn(c, 12582912.f)), z = __float_as_uint(__fadd_rn(d, 12582912.f));
+  return __byte_perm(__byte_perm(w, x, 0x0040), __byte_perm(y, z, 0x0040), 0x5410);
 }
 
 // Whether a sequence's new positions can be there, and the page and place of one.
@@ -75,19 +79,27 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const T *x, T *out, 
   const int item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES, row = p.by_heads(item), h = item - row * p.heads;
   if (row >= p.rows || 16 * t >= p.dim) return;
   const T *from = x + (size_t)row * p.x_ld + (size_t)h * p.dim;
-  Runs<T> runs;
-  if constexpr (WHOLE) runs = load_runs(from, t, p.rot, NEIGHBOURS);
+  T *to = out + (size_t)row * p.out_ld + (size_t)h * p.dim;
+  const Runs runs = runs_of(t, p.dim, p.rot, NEIGHBOURS);
+  Raw<T> raw;
+  if constexpr (WHOLE) raw = load_raw(from, runs);
   const int pos = p.position[row];
   if (pos < 0 || pos >= p.positions) {
     if (h == 0 && t == 0 && p.error_flag) atomicExch(p.error_flag, 12);
     return;
   }
-  const Turn turn = load_turn<WHOLE>(p.rope + (size_t)pos * (p.rot / 2), t, p.rot, INVERSE);
-  Pairs v;
-  if constexpr (WHOLE) v = pairs_of<T>(runs, t, p.rot, NEIGHBOURS);
-  else v = load_pairs(from, t, p.dim, p.rot, NEIGHBOURS);
-  turn_pairs(v, turn, t, p.rot);
-  store_pairs<WHOLE>(out + (size_t)row * p.out_ld + (size_t)h * p.dim, v, t, p.dim, p.rot, NEIGHBOURS);
+  const float2 *angles = p.rope + (size_t)pos * (p.rot / 2);
+  const float sign = INVERSE ? -1.f : 1.f;
+  if constexpr (WHOLE) {
+    Item v = item_of<T>(raw);
+    turn_item(v, angles, runs, NEIGHBOURS, sign);
+    store_run(to + runs.lo, v.lo);
+    store_run(to + runs.hi, v.hi);
+  } else {
+    Item v = load_pairs(from, t, p.dim, p.rot, NEIGHBOURS);
+    turn_pairs(v, angles, t, p.rot, sign);
+    store_pairs(to, v, t, p.dim, p.rot, NEIGHBOURS);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ appending
@@ -111,9 +123,10 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T 
   const T *from = (is_q ? q : is_v ? v : k) + (size_t)tok * p.ld + (size_t)h * dim;
   bool in = tok < p.b.n_tok && 16 * t < dim;          // (whole warps stay together: the lanes of a row exchange their maxima)
   const int used = p.b.cu[p.b.n_seq], seq = tok < p.b.n_tok ? p.b.tok_seq[tok] : 0;
-  Runs<T> runs;
+  const Runs runs = runs_of(t, dim, rot, NEIGHBOURS);
+  Raw<T> raw{};
   if constexpr (WHOLE) {
-    if (in) runs = load_runs(from, t, rot, NEIGHBOURS);
+    if (in) raw = load_raw(from, runs);
   }
   in = in && tok < used;
   int pos = -1, page = -1;
@@ -129,46 +142,52 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T 
     }
   }
   const int place = pos - p.by_page(max(pos, 0)) * p.c.page;
-  Pairs x;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x.a[j] = x.b[j] = 0.f;
+  Item x{};
   if (in) {
-    const Turn turn = load_turn<WHOLE>(p.rope + (size_t)pos * (p.rot / 2), t, rot, false);
-    if constexpr (WHOLE) x = pairs_of<T>(runs, t, rot, NEIGHBOURS);
-    else x = load_pairs(from, t, dim, rot, NEIGHBOURS);
-    turn_pairs(x, turn, t, rot);
-    if (is_q) store_pairs<WHOLE>(q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim, x, t, dim, rot, NEIGHBOURS);
+    const float2 *angles = p.rope + (size_t)pos * (rot / 2);
+    if constexpr (WHOLE) {
+      x = item_of<T>(raw);
+      turn_item(x, angles, runs, NEIGHBOURS, 1.f);
+    } else {
+      x = load_pairs(from, t, dim, rot, NEIGHBOURS);
+      turn_pairs(x, angles, t, rot, 1.f);
+    }
+    if (is_q) {
+      T *to = q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim;
+      if constexpr (WHOLE) {
+        store_run(to + runs.lo, x.lo);
+        store_run(to + runs.hi, x.hi);
+      } else {
+        store_pairs(to, x, t, dim, rot, NEIGHBOURS);
+      }
+    }
   }
+  if (__all_sync(0xffffffffu, !in || is_q)) return;
   uint32_t m = 0;           // (magnitudes in the order of their bits: NaN is above infinity)
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, max(__float_as_uint(x.a[j]) & 0x7fffffffu, __float_as_uint(x.b[j]) & 0x7fffffffu));
+  for (int j = 0; j < 8; ++j) m = max(m, max(__float_as_uint(x.lo[j]) & 0x7fffffffu, __float_as_uint(x.hi[j]) & 0x7fffffffu));
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (!in || is_q) return;
   const bool fine = m <= LARGE;
-  const float most = __uint_as_float(max(m, SMALL)), by = fine ? __fdiv_rn(top_byte<E4M3>(), most) : 0.f;
+  const float most = __uint_as_float(max(m, SMALL)), by = __fdiv_rn(top_byte<E4M3>(), most);
   const size_t row = (size_t)h * p.c.page + place;
   if (t == 0) p.c.scales[((size_t)page * 2 * G + (is_v ? G : 0)) * p.c.page + row] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
   unsigned char *to = p.c.pool + (size_t)page * p.c.page_bytes + (is_v ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    x.a[j] = fine ? __fmul_rn(x.a[j], by) : 0.f;
-    x.b[j] = fine ? __fmul_rn(x.b[j], by) : 0.f;
+    x.lo[j] = fine ? __fmul_rn(x.lo[j], by) : 0.f;
+    x.hi[j] = fine ? __fmul_rn(x.hi[j], by) : 0.f;
   }
   if constexpr (WHOLE) {
-    if (!NEIGHBOURS && 16 * t < rot) {
-      *reinterpret_cast<uint2 *>(to + 8 * t) = make_uint2(to_word<E4M3>(x.a[0], x.a[1], x.a[2], x.a[3]), to_word<E4M3>(x.a[4], x.a[5], x.a[6], x.a[7]));
-      *reinterpret_cast<uint2 *>(to + 8 * t + rot / 2) = make_uint2(to_word<E4M3>(x.b[0], x.b[1], x.b[2], x.b[3]), to_word<E4M3>(x.b[4], x.b[5], x.b[6], x.b[7]));
-    } else {
-      *reinterpret_cast<uint4 *>(to + 16 * t) = make_uint4(to_word<E4M3>(x.a[0], x.b[0], x.a[1], x.b[1]), to_word<E4M3>(x.a[2], x.b[2], x.a[3], x.b[3]),
-                                                            to_word<E4M3>(x.a[4], x.b[4], x.a[5], x.b[5]), to_word<E4M3>(x.a[6], x.b[6], x.a[7], x.b[7]));
-    }
+    *reinterpret_cast<uint2 *>(to + runs.lo) = make_uint2(to_word<E4M3>(x.lo[0], x.lo[1], x.lo[2], x.lo[3]), to_word<E4M3>(x.lo[4], x.lo[5], x.lo[6], x.lo[7]));
+    *reinterpret_cast<uint2 *>(to + runs.hi) = make_uint2(to_word<E4M3>(x.hi[0], x.hi[1], x.hi[2], x.hi[3]), to_word<E4M3>(x.hi[4], x.hi[5], x.hi[6], x.hi[7]));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
-      if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.a[j]);
-      if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.b[j]);
+      if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.lo[j]);
+      if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.hi[j]);
     }
   }
 }
@@ -178,11 +197,10 @@ struct Unpack {
   Batch b;
   Cache c;
   const int *into_table;
-  int into_page, into_max_pages, into_max_len, heads_each;
+  int into_page, into_max_pages, into_max_len, rows_each, heads_each;
   int *error_flag;
   Divide by_page, by_into_page;
 };
-constexpr int UNPACK_ROWS = 64;
 template <bool E4M3> __device__ __forceinline__ void from_word(uint32_t w, float scale, float *v) {
   if constexpr (E4M3) {
     const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3))), b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
@@ -192,23 +210,24 @@ template <bool E4M3> __device__ __forceinline__ void from_word(uint32_t w, float
     for (int j = 0; j < 4; ++j) v[j] = (float)(signed char)(w >> (8 * j)) * scale;
   }
 }
-// Block: 64 positions of a sequence, keys or values of heads_each heads.  Bound by memory: a thread finds its places once and asks for four heads' bytes together (a block a head, which found
+// Block: rows_each positions of a sequence, keys or values of heads_each heads.  Bound by memory: a thread finds its places once and asks for four heads' bytes together (a block a head, which found
 // them again: 4 sequences of 16500 positions, 8 heads of 128, 63.4 us).
 template <typename T, bool WHOLE, bool E4M3> __global__ void __launch_bounds__(THREADS) unpack_kernel(T *into, const Unpack p) {
   early_start();
   const int parts = gridDim.z / 2;
   const bool is_v = blockIdx.z >= parts;
-  const int seq = blockIdx.y, G = p.c.n_kv, h0 = (blockIdx.z - (is_v ? parts : 0)) * p.heads_each, h1 = min(G, h0 + p.heads_each), first = blockIdx.x * UNPACK_ROWS;
+  const int seq = blockIdx.y, G = p.c.n_kv, h0 = (blockIdx.z - (is_v ? parts : 0)) * p.heads_each, h1 = min(G, h0 + p.heads_each), first = blockIdx.x * p.rows_each;
   const int start = p.b.start[seq], count = p.b.cu[seq + 1] - p.b.cu[seq], slot = p.b.slot[seq];
   if (!in_table(p.c, start, count) || count > p.into_max_len - start) {
     if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 12);
     return;
   }
-  const int rows = min(UNPACK_ROWS, start + count - first), dim = is_v ? p.c.vdim : p.c.dim;
+  const int rows = min(p.rows_each, start + count - first), dim = is_v ? p.c.vdim : p.c.dim;
   if (rows <= 0) return;
   const int *table = p.c.page_table + (size_t)slot * p.c.max_pages, *into_table = p.into_table + (size_t)slot * p.into_max_pages;
   const size_t into_page_elements = (size_t)G * p.into_page * (p.c.dim + p.c.vdim);
-  constexpr int UNIT = WHOLE ? 16 : 1, TOGETHER = 4;
+  constexpr int UNIT = WHOLE ? 16 / (int)sizeof(T) : 1, TOGETHER = 4;      // (16 bytes of the wider type: the warps' stores are whole)
+  using Bytes = std::conditional_t<UNIT == 4, uint32_t, uint2>;
   const int units = dim / UNIT;
   for (int i = threadIdx.x; i < rows * units; i += THREADS) {
     const int r = i / units, u = i - r * units, pos = first + r, pg = p.by_page(pos), to_pg = p.by_into_page(pos);
@@ -223,23 +242,27 @@ template <typename T, bool WHOLE, bool E4M3> __global__ void __launch_bounds__(T
     T *to = into + (size_t)to_page * into_page_elements + (is_v ? (size_t)G * p.into_page * p.c.dim : 0) + (size_t)(pos - to_pg * p.into_page) * dim + (size_t)u * UNIT;
     if constexpr (WHOLE) {
       for (int h = h0; h < h1; h += TOGETHER) {
-        uint4 w[TOGETHER];
+        Bytes w[TOGETHER];
         float s[TOGETHER];
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k)
           if (h + k < h1) {
-            w[k] = *reinterpret_cast<const uint4 *>(from + (size_t)(h + k) * p.c.page * dim);
+            w[k] = *reinterpret_cast<const Bytes *>(from + (size_t)(h + k) * p.c.page * dim);
             s[k] = scale[(size_t)(h + k) * p.c.page];
           }
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k)
           if (h + k < h1) {
-            float lo[8], hi[8];
-            from_word<E4M3>(w[k].x, s[k], lo); from_word<E4M3>(w[k].y, s[k], lo + 4);
-            from_word<E4M3>(w[k].z, s[k], hi); from_word<E4M3>(w[k].w, s[k], hi + 4);
             T *at = to + (size_t)(h + k) * p.into_page * dim;
-            store_run(at, lo);
-            store_run(at + 8, hi);
+            if constexpr (UNIT == 4) {
+              float v[4];
+              from_word<E4M3>(w[k], s[k], v);
+              *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+              float v[8];
+              from_word<E4M3>(w[k].x, s[k], v); from_word<E4M3>(w[k].y, s[k], v + 4);
+              store_run(at, v);
+            }
           }
       }
     } else {
@@ -382,7 +405,8 @@ template <typename T> static cudaError_t launch_append(const pt_kv8_append_args 
 
 template <typename T> static cudaError_t launch_unpack(const pt_kv8_unpack_args &a, Unpack p, bool whole, cudaStream_t st) {
   // Heads of a block: all, unless the longest histories that there may be would not fill the GPU then.
-  const int chunks = ceil_div(std::min(p.c.max_len, p.into_max_len), UNPACK_ROWS);
+  p.rows_each = std::max(1, THREADS / std::max(1, std::min(p.c.dim, p.c.vdim) / (whole ? 16 / (int)sizeof(T) : 1)));      // (a thread has one place)
+  const int chunks = ceil_div(std::min(p.c.max_len, p.into_max_len), p.rows_each);
   p.heads_each = p.c.n_kv;
   while (p.heads_each > 1 && (long long)chunks * a.batch.n_seq * 2 * ceil_div(p.c.n_kv, p.heads_each) < 8ll * sm_count()) p.heads_each = (p.heads_each + 1) / 2;
   const dim3 grid(chunks, a.batch.n_seq, 2 * ceil_div(p.c.n_kv, p.heads_each));
@@ -479,7 +503,7 @@ extern "C" int pt_kv8_unpack(const pt_kv8_unpack_args *a, void *stream) {
              a->into_page_size, a->into_max_len);
   PT_REQUIRE(a->batch.n_seq <= 65535 && a->cache.n_kv <= 32767, "pt_kv8_unpack: %d sequences (65535 at most), %d heads (32767)", a->batch.n_seq, a->cache.n_kv);
   const kv8::Unpack p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->into_table, a->into_page_size, a->into_max_pages,
-                      a->into_max_len ? a->into_max_len : a->into_page_size * a->into_max_pages, 1, a->error_flag, kv8::Divide::by(a->cache.page_size), kv8::Divide::by(a->into_page_size)};
+                      a->into_max_len ? a->into_max_len : a->into_page_size * a->into_max_pages, 1, 1, a->error_flag, kv8::Divide::by(a->cache.page_size), kv8::Divide::by(a->into_page_size)};
   const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && aligned_to(a->cache.pool, 16) && aligned_to(a->into, 16);
   const cudaStream_t st = as_stream(stream);
   PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_unpack<float>(*a, p, whole, st)

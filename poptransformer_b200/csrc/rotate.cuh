@@ -1,8 +1,7 @@
 // Rotation of rows by their positions, a lane at a time: what the rotation and appending kernels share.
 //
-// A lane has eight pairs of a row: pairs 8 t .. 8 t + 7 of item t.  Pair p < rot / 2 is elements (p, p + rot / 2), or (2 p, 2 p + 1) where neighbours
-// turn together; behind the rotated part it is (2 p, 2 p + 1).  So a lane holds both elements of each of its pairs (a row can be rotated where it lies), and
-// sixteen elements that are one run of 16 or two runs of 8.
+// Pair p < rot / 2 of a row is elements (p, p + rot / 2), or (2 p, 2 p + 1) where neighbours turn together.  A lane has sixteen elements, both of every pair that it has any of, so
+// that a row can be rotated where it lies.
 #pragma once
 #include "elem.cuh"
 
@@ -10,10 +9,6 @@ namespace pt {
 
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-
-struct Pairs { float a[8], b[8]; };
-// What a lane reads of a row, as it lies there (two runs of eight): asked for before it is known how far the row turns.
-template <typename T> struct Runs { uint4 v[sizeof(T) / 2 * 2]; };
 
 // Eight values that lie together, from or to a multiple of 16 bytes.
 __device__ __forceinline__ void load_run(const float *p, float (&v)[8]) {
@@ -39,95 +34,90 @@ template <typename T> __device__ __forceinline__ void store_run(T *p, const floa
   *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
 }
 
-// Elements of pair p of a row.
-__device__ __forceinline__ int2 pair_at(int p, int rot, bool neighbours) { return p < rot / 2 && !neighbours ? make_int2(p, p + rot / 2) : make_int2(2 * p, 2 * p + 1); }
-
-// Of rows that lie on multiples of 16 bytes, with dim and rot multiples of 16: every item is two whole runs, rot / 2 apart or one behind the other.
-template <typename T> __device__ __forceinline__ Runs<T> load_runs(const T *x, int t, int rot, bool neighbours) {
-  constexpr int N = sizeof(T) / 2;
-  const bool apart = !neighbours && 16 * t < rot;
-  const uint4 *lo = reinterpret_cast<const uint4 *>(x + (apart ? 8 * t : 16 * t)), *hi = reinterpret_cast<const uint4 *>(x + (apart ? 8 * t + rot / 2 : 16 * t + 8));
-  Runs<T> r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) { r.v[i] = lo[i]; r.v[N + i] = hi[i]; }
-  return r;
+// Three roundings, as written: what is cached does not depend on which products a compiler joins.
+__device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
+  const float a = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+  y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+  x = a;
 }
-template <typename T> __device__ __forceinline__ Pairs pairs_of(const Runs<T> &r, int t, int rot, bool neighbours) {
-  const bool apart = !neighbours && 16 * t < rot;
+
+// ---- rows on multiples of 16 bytes, dim and rot multiples of 16: lane t has two runs of eight, and neighbouring lanes neighbouring runs
+struct Item { float lo[8], hi[8]; };
+struct Runs { int lo, hi; bool turns_lo, turns_hi; };
+__device__ __forceinline__ Runs runs_of(int t, int dim, int rot, bool neighbours) {
+  if (neighbours) return {8 * t, 8 * t + dim / 2, 8 * t < rot, 8 * t + dim / 2 < rot};
+  if (16 * t < rot) return {8 * t, 8 * t + rot / 2, true, true};
+  return {rot / 2 + 8 * t, rot / 2 + 8 * t + (dim - rot) / 2, false, false};      // (behind the rotated part, from element rot on)
+}
+// As they lie there: asked for before it is known how far the row turns.
+template <typename T> struct Raw { uint4 v[sizeof(T)]; };
+template <typename T> __device__ __forceinline__ Raw<T> load_raw(const T *x, const Runs &r) {
+  constexpr int N = sizeof(T) / 2;
+  Raw<T> w;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w.v[i] = reinterpret_cast<const uint4 *>(x + r.lo)[i];
+    w.v[N + i] = reinterpret_cast<const uint4 *>(x + r.hi)[i];
+  }
+  return w;
+}
+template <typename T> __device__ __forceinline__ Item item_of(const Raw<T> &w) {
   T e[16];
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4 *>(e)[i] = r.v[i];
-  Pairs v;
+  for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4 *>(e)[i] = w.v[i];
+  Item v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v.a[j] = to_f(apart ? e[j] : e[2 * j]);
-    v.b[j] = to_f(apart ? e[8 + j] : e[2 * j + 1]);
-  }
+  for (int j = 0; j < 8; ++j) { v.lo[j] = to_f(e[j]); v.hi[j] = to_f(e[8 + j]); }
   return v;
 }
-// Of any rows.
-template <typename T> __device__ __forceinline__ Pairs load_pairs(const T *x, int t, int dim, int rot, bool neighbours) {
-  Pairs v;
+// row: (cos, sin) of the position's pairs, on a multiple of 16 bytes.
+__device__ __forceinline__ void turn_item(Item &v, const float2 *row, const Runs &r, bool neighbours, float sign) {
+  const float4 *cs = reinterpret_cast<const float4 *>(row);
+  if (neighbours) {
+    float4 a[2], b[2];
+    if (r.turns_lo) { a[0] = __ldg(cs + r.lo / 4); a[1] = __ldg(cs + r.lo / 4 + 1); }
+    if (r.turns_hi) { b[0] = __ldg(cs + r.hi / 4); b[1] = __ldg(cs + r.hi / 4 + 1); }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (r.turns_lo) { turn(v.lo[4 * j], v.lo[4 * j + 1], a[j].x, sign * a[j].y); turn(v.lo[4 * j + 2], v.lo[4 * j + 3], a[j].z, sign * a[j].w); }
+      if (r.turns_hi) { turn(v.hi[4 * j], v.hi[4 * j + 1], b[j].x, sign * b[j].y); turn(v.hi[4 * j + 2], v.hi[4 * j + 3], b[j].z, sign * b[j].w); }
+    }
+  } else if (r.turns_lo) {
+    float4 a[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = __ldg(cs + r.lo / 2 + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { turn(v.lo[2 * j], v.hi[2 * j], a[j].x, sign * a[j].y); turn(v.lo[2 * j + 1], v.hi[2 * j + 1], a[j].z, sign * a[j].w); }
+  }
+}
+
+// ---- any rows: lane t has pairs 8 t .. 8 t + 7, those behind the rotated part being (2 p, 2 p + 1)
+__device__ __forceinline__ int2 pair_at(int p, int rot, bool neighbours) { return p < rot / 2 && !neighbours ? make_int2(p, p + rot / 2) : make_int2(2 * p, 2 * p + 1); }
+template <typename T> __device__ __forceinline__ Item load_pairs(const T *x, int t, int dim, int rot, bool neighbours) {
+  Item v;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int2 e = pair_at(8 * t + j, rot, neighbours);
-    v.a[j] = e.x < dim ? to_f(x[e.x]) : 0.f;
-    v.b[j] = e.y < dim ? to_f(x[e.y]) : 0.f;
+    v.lo[j] = e.x < dim ? to_f(x[e.x]) : 0.f;
+    v.hi[j] = e.y < dim ? to_f(x[e.y]) : 0.f;
   }
   return v;
 }
-// WHOLE: as load_runs wants them.
-template <bool WHOLE, typename T> __device__ __forceinline__ void store_pairs(T *x, const Pairs &v, int t, int dim, int rot, bool neighbours) {
-  if constexpr (WHOLE) {
-    const bool apart = !neighbours && 16 * t < rot;
-    float lo[8], hi[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo[j] = apart ? v.a[j] : j & 1 ? v.b[j >> 1] : v.a[j >> 1];
-      hi[j] = apart ? v.b[j] : j & 1 ? v.b[4 + (j >> 1)] : v.a[4 + (j >> 1)];
-    }
-    store_run(x + (apart ? 8 * t : 16 * t), lo);
-    store_run(x + (apart ? 8 * t + rot / 2 : 16 * t + 8), hi);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int2 e = pair_at(8 * t + j, rot, neighbours);
-      if (e.x < dim) x[e.x] = from_f<T>(v.a[j]);
-      if (e.y < dim) x[e.y] = from_f<T>(v.b[j]);
-    }
-  }
-}
-
-// (cos, sin) of an item's pairs; (1, 0) behind the rotated part.  WHOLE: a row of the table lies on a multiple of 16 bytes, and an item is rotated as a whole or not at all.
-struct Turn { float c[8], s[8]; };
-template <bool WHOLE> __device__ __forceinline__ Turn load_turn(const float2 *row, int t, int rot, bool inverse) {
-  Turn r;
-  if constexpr (WHOLE) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 cs = 16 * t < rot ? __ldg(reinterpret_cast<const float4 *>(row + 8 * t) + j) : make_float4(1.f, 0.f, 1.f, 0.f);
-      r.c[2 * j] = cs.x; r.c[2 * j + 1] = cs.z;
-      r.s[2 * j] = inverse ? -cs.y : cs.y; r.s[2 * j + 1] = inverse ? -cs.w : cs.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 cs = 8 * t + j < rot / 2 ? __ldg(row + 8 * t + j) : make_float2(1.f, 0.f);
-      r.c[j] = cs.x;
-      r.s[j] = inverse ? -cs.y : cs.y;
-    }
-  }
-  return r;
-}
-// Three roundings, as written: what is cached does not depend on which products a compiler joins.
-__device__ __forceinline__ void turn_pairs(Pairs &v, const Turn &r, int t, int rot) {
+template <typename T> __device__ __forceinline__ void store_pairs(T *x, const Item &v, int t, int dim, int rot, bool neighbours) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    if (8 * t + j >= rot / 2) continue;
-    const float x = v.a[j], y = v.b[j];
-    v.a[j] = __fsub_rn(__fmul_rn(x, r.c[j]), __fmul_rn(y, r.s[j]));
-    v.b[j] = __fadd_rn(__fmul_rn(y, r.c[j]), __fmul_rn(x, r.s[j]));
+    const int2 e = pair_at(8 * t + j, rot, neighbours);
+    if (e.x < dim) x[e.x] = from_f<T>(v.lo[j]);
+    if (e.y < dim) x[e.y] = from_f<T>(v.hi[j]);
   }
+}
+__device__ __forceinline__ void turn_pairs(Item &v, const float2 *row, int t, int rot, float sign) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (8 * t + j < rot / 2) {
+      const float2 cs = __ldg(row + 8 * t + j);
+      turn(v.lo[j], v.hi[j], cs.x, sign * cs.y);
+    }
 }
 
 }  // namespace pt
