@@ -10,7 +10,7 @@ namespace pt {
 namespace kv8 {
 
 constexpr int THREADS = 256;
-constexpr uint32_t SMALL = 0x1f800000u, LARGE = 0x5f800000u;     // 2^-64 and 2^64 as bits
+constexpr float SMALL = 0x1p-64f, LARGE = 0x1p64f;
 
 // Division by what a launch has but once: n / d = (n + high word of n mul) >> shift for 0 <= n < 2^31, mul = ceil(2^32 (2^shift - d) / d), 2^shift the power of two at or above d.
 struct Divide {
@@ -48,6 +48,12 @@ template <bool E4M3> __device__ __forceinline__ float from_byte(unsigned char b)
 template <bool E4M3> __device__ __forceinline__ uint32_t to_byte(float x) {
   if constexpr (E4M3) return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
   return (uint32_t)max(-127, min(127, __float2int_rn(x))) & 0xFFu;
+}
+// The largest magnitude of three values; NaN if one of them is.
+__device__ __forceinline__ float larger(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
 }
 // Four values as a word.
 template <bool E4M3> __device__ __forceinline__ uint32_t to_word(float a, float b, float c, float d) {
@@ -92,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const T *x, T *out, 
   const float sign = INVERSE ? -1.f : 1.f;
   if constexpr (WHOLE) {
     Item v = item_of<T>(raw);
-    turn_item(v, angles, runs, NEIGHBOURS, sign);
+    turn_item(v, load_angles(angles, runs, NEIGHBOURS), runs, NEIGHBOURS, sign);
     store_run(to + runs.lo, v.lo);
     store_run(to + runs.hi, v.hi);
   } else {
@@ -109,85 +115,97 @@ struct Append {
   int heads, rot, ld, q_out_ld;
   const float2 *rope;
   int *error_flag;
-  Divide by_rows, by_page;
+  int items;                  // of a token: its rows in groups of ROWS
+  Divide by_items, by_page;
 };
-// The rows of a token: its q heads (rotated to q_out), its keys (rotated, kept as bytes), its values (kept as bytes); LANES lanes each, a thread has one.  Bound by memory, and before that by the
-// way to a row's place (sequence, position, page): rows are asked for first.
-template <typename T, int LANES, bool WHOLE, bool NEIGHBOURS, bool E4M3>
+// The rows of a token: its q heads (rotated to q_out), its keys (rotated, kept as bytes), its values (kept as bytes).  LANES lanes have the same sixteenth elements of ROWS neighbouring rows.
+// Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  (A row a lane:
+// 11,000 tokens of 32 + 8 + 8 heads of 128 69.7 us; where there is less than a wave of rows one is faster, a token in 2.5 us so.)
+template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
   early_start();
   const int G = p.c.n_kv, all = p.heads + 2 * G;
-  const int item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES, tok = p.by_rows(item), r = item - tok * all;
-  const bool is_q = r < p.heads, is_v = r >= p.heads + G;
-  const int h = is_q ? r : is_v ? r - p.heads - G : r - p.heads, dim = is_v ? p.c.vdim : p.c.dim, rot = is_v ? 0 : p.rot;
-  const T *from = (is_q ? q : is_v ? v : k) + (size_t)tok * p.ld + (size_t)h * dim;
-  bool in = tok < p.b.n_tok && 16 * t < dim;          // (whole warps stay together: the lanes of a row exchange their maxima)
-  const int used = p.b.cu[p.b.n_seq], seq = tok < p.b.n_tok ? p.b.tok_seq[tok] : 0;
-  const Runs runs = runs_of(t, dim, rot, NEIGHBOURS);
-  Raw<T> raw{};
+  const int item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES, tok = p.by_items(item), r0 = (item - tok * p.items) * ROWS;
+  const bool there = tok < p.b.n_tok;
+  // Row r0 + i of the token: what it is, its head, its width and where it lies.
+  auto is_q = [&](int i) { return r0 + i < p.heads; };
+  auto is_v = [&](int i) { return r0 + i >= p.heads + G; };
+  auto head = [&](int i) { return is_q(i) ? r0 + i : is_v(i) ? r0 + i - p.heads - G : r0 + i - p.heads; };
+  auto width = [&](int i) { return is_v(i) ? p.c.vdim : p.c.dim; };
+  auto has = [&](int i) { return there && r0 + i < all && 16 * t < width(i); };
+  auto from = [&](int i) { return (is_q(i) ? q : is_v(i) ? v : k) + (size_t)tok * p.ld + (size_t)head(i) * width(i); };
+  const int used = p.b.cu[p.b.n_seq], seq = there ? p.b.tok_seq[tok] : 0;
+  Raw<T> raw[ROWS];
   if constexpr (WHOLE) {
-    if (in) raw = load_raw(from, runs);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      if (has(i)) raw[i] = load_raw(from(i), runs_of(t, width(i), is_v(i) ? 0 : p.rot, NEIGHBOURS));
   }
-  in = in && tok < used;
   int pos = -1, page = -1;
-  if (in) {
+  if (there && tok < used) {
     const int first = p.b.cu[seq], start = p.b.start[seq];
     if (in_table(p.c, start, p.b.cu[seq + 1] - first)) {
       pos = start + tok - first;
       page = p.c.page_table[(size_t)p.b.slot[seq] * p.c.max_pages + p.by_page(pos)];
     }
-    if (page < 0) {
-      in = false;
-      if (r == 0 && t == 0 && p.error_flag) atomicExch(p.error_flag, 12);
-    }
+    if (page < 0 && r0 == 0 && t == 0 && p.error_flag) atomicExch(p.error_flag, 12);
   }
   const int place = pos - p.by_page(max(pos, 0)) * p.c.page;
-  Item x{};
-  if (in) {
-    const float2 *angles = p.rope + (size_t)pos * (rot / 2);
-    if constexpr (WHOLE) {
-      x = item_of<T>(raw);
-      turn_item(x, angles, runs, NEIGHBOURS, 1.f);
-    } else {
-      x = load_pairs(from, t, dim, rot, NEIGHBOURS);
-      turn_pairs(x, angles, t, rot, 1.f);
-    }
-    if (is_q) {
-      T *to = q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim;
+  const float2 *angles = p.rope + (size_t)max(pos, 0) * (p.rot / 2);
+  Angles turned{};
+  if (WHOLE && page >= 0 && !is_v(0) && 16 * t < p.c.dim) turned = load_angles(angles, runs_of(t, p.c.dim, p.rot, NEIGHBOURS), NEIGHBOURS);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {      // (whole warps stay together: the lanes of a row exchange their maxima)
+    const int dim = width(i), rot = is_v(i) ? 0 : p.rot, h = head(i);
+    const bool in = page >= 0 && has(i);
+    const Runs runs = runs_of(t, dim, rot, NEIGHBOURS);
+    Item x{};
+    if (in) {
       if constexpr (WHOLE) {
-        store_run(to + runs.lo, x.lo);
-        store_run(to + runs.hi, x.hi);
+        x = item_of<T>(raw[i]);
+        turn_item(x, turned, runs, NEIGHBOURS, 1.f);
       } else {
-        store_pairs(to, x, t, dim, rot, NEIGHBOURS);
+        x = load_pairs(from(i), t, dim, rot, NEIGHBOURS);
+        turn_pairs(x, angles, t, rot, 1.f);
+      }
+      if (is_q(i)) {
+        T *to = q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim;
+        if constexpr (WHOLE) {
+          store_run(to + runs.lo, x.lo);
+          store_run(to + runs.hi, x.hi);
+        } else {
+          store_pairs(to, x, t, dim, rot, NEIGHBOURS);
+        }
       }
     }
-  }
-  if (__all_sync(0xffffffffu, !in || is_q)) return;
-  uint32_t m = 0;           // (magnitudes in the order of their bits: NaN is above infinity)
+    if (__all_sync(0xffffffffu, !in || is_q(i))) continue;
+    float m = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, max(__float_as_uint(x.lo[j]) & 0x7fffffffu, __float_as_uint(x.hi[j]) & 0x7fffffffu));
+    for (int j = 0; j < 8; ++j) m = larger(m, x.lo[j], x.hi[j]);
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (!in || is_q) return;
-  const bool fine = m <= LARGE;
-  const float most = __uint_as_float(max(m, SMALL)), by = __fdiv_rn(top_byte<E4M3>(), most);
-  const size_t row = (size_t)h * p.c.page + place;
-  if (t == 0) p.c.scales[((size_t)page * 2 * G + (is_v ? G : 0)) * p.c.page + row] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
-  unsigned char *to = p.c.pool + (size_t)page * p.c.page_bytes + (is_v ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x.lo[j] = fine ? __fmul_rn(x.lo[j], by) : 0.f;
-    x.hi[j] = fine ? __fmul_rn(x.hi[j], by) : 0.f;
-  }
-  if constexpr (WHOLE) {
-    *reinterpret_cast<uint2 *>(to + runs.lo) = make_uint2(to_word<E4M3>(x.lo[0], x.lo[1], x.lo[2], x.lo[3]), to_word<E4M3>(x.lo[4], x.lo[5], x.lo[6], x.lo[7]));
-    *reinterpret_cast<uint2 *>(to + runs.hi) = make_uint2(to_word<E4M3>(x.hi[0], x.hi[1], x.hi[2], x.hi[3]), to_word<E4M3>(x.hi[4], x.hi[5], x.hi[6], x.hi[7]));
-  } else {
+    for (int o = LANES / 2; o > 0; o >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o), 0.f);
+    if (!in || is_q(i)) continue;
+    const bool fine = m <= LARGE;
+    const float most = fmaxf(m, SMALL), by = __fdiv_rn(top_byte<E4M3>(), most);
+    const size_t row = (size_t)h * p.c.page + place;
+    if (t == 0) p.c.scales[((size_t)page * 2 * G + (is_v(i) ? G : 0)) * p.c.page + row] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
+    unsigned char *to = p.c.pool + (size_t)page * p.c.page_bytes + (is_v(i) ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
-      if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.lo[j]);
-      if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.hi[j]);
+      x.lo[j] = __fmul_rn(x.lo[j], by);
+      x.hi[j] = __fmul_rn(x.hi[j], by);
+    }
+    if (!fine) x = Item{};
+    if constexpr (WHOLE) {
+      *reinterpret_cast<uint2 *>(to + runs.lo) = make_uint2(to_word<E4M3>(x.lo[0], x.lo[1], x.lo[2], x.lo[3]), to_word<E4M3>(x.lo[4], x.lo[5], x.lo[6], x.lo[7]));
+      *reinterpret_cast<uint2 *>(to + runs.hi) = make_uint2(to_word<E4M3>(x.hi[0], x.hi[1], x.hi[2], x.hi[3]), to_word<E4M3>(x.hi[4], x.hi[5], x.hi[6], x.hi[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
+        if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.lo[j]);
+        if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.hi[j]);
+      }
     }
   }
 }
@@ -389,18 +407,23 @@ template <typename T> static cudaError_t launch_rotary(const pt_rotary_args &a, 
   return whole ? launch_rotary<T, 16, true>(a, p, grid, st) : launch_rotary<T, 16, false>(a, p, grid, st);
 }
 
-template <typename T, int LANES, bool WHOLE> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, dim3 grid, cudaStream_t st) {
+template <typename T, int LANES, int ROWS, bool WHOLE> static cudaError_t launch_append(const pt_kv8_append_args &a, Append p, cudaStream_t st) {
+  p.items = ceil_div(p.heads + 2 * p.c.n_kv, ROWS);
+  p.by_items = Divide::by(p.items);
   const bool e4m3 = a.cache.fmt == PT_KV8_E4M3;
-  const auto kernel = e4m3 ? (a.interleaved ? append_kernel<T, LANES, WHOLE, true, true> : append_kernel<T, LANES, WHOLE, false, true>)
-                           : (a.interleaved ? append_kernel<T, LANES, WHOLE, true, false> : append_kernel<T, LANES, WHOLE, false, false>);
-  return launch_early(kernel, Grid(grid), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
+  const auto kernel = e4m3 ? (a.interleaved ? append_kernel<T, LANES, ROWS, WHOLE, true, true> : append_kernel<T, LANES, ROWS, WHOLE, false, true>)
+                           : (a.interleaved ? append_kernel<T, LANES, ROWS, WHOLE, true, false> : append_kernel<T, LANES, ROWS, WHOLE, false, false>);
+  return launch_early(kernel, Grid(ceil_div(a.batch.n_tok * p.items, THREADS / LANES)), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
+}
+template <typename T, int LANES> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, bool whole, cudaStream_t st) {
+  constexpr int MANY = 2;      // rows of a lane, where there are more than a wave of rows one by one (four: fewer warps, 61.6 us)
+  const bool many = (long long)a.batch.n_tok * (p.heads + 2 * p.c.n_kv) * LANES > 1024ll * sm_count();
+  if (!whole) return launch_append<T, LANES, 1, false>(a, p, st);
+  return many ? launch_append<T, LANES, MANY, true>(a, p, st) : launch_append<T, LANES, 1, true>(a, p, st);
 }
 template <typename T> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, bool whole, cudaStream_t st) {
   const int lanes = lanes_of(std::max(a.cache.dim, a.cache.vdim));
-  const dim3 grid(ceil_div(a.batch.n_tok * (p.heads + 2 * a.cache.n_kv), THREADS / lanes));
-  if (lanes == 4) return whole ? launch_append<T, 4, true>(a, p, grid, st) : launch_append<T, 4, false>(a, p, grid, st);
-  if (lanes == 8) return whole ? launch_append<T, 8, true>(a, p, grid, st) : launch_append<T, 8, false>(a, p, grid, st);
-  return whole ? launch_append<T, 16, true>(a, p, grid, st) : launch_append<T, 16, false>(a, p, grid, st);
+  return lanes == 4 ? launch_append<T, 4>(a, p, whole, st) : lanes == 8 ? launch_append<T, 8>(a, p, whole, st) : launch_append<T, 16>(a, p, whole, st);
 }
 
 template <typename T> static cudaError_t launch_unpack(const pt_kv8_unpack_args &a, Unpack p, bool whole, cudaStream_t st) {
@@ -480,7 +503,7 @@ extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
              a->cache.n_kv);
   if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Append p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->q_out ? a->n_head : 0, a->rope_dims, a->ld, a->q_out_ld, (const float2 *)a->rope, a->error_flag,
-                      kv8::Divide::by((a->q_out ? a->n_head : 0) + 2 * a->cache.n_kv), kv8::Divide::by(a->cache.page_size)};
+                      0, {}, kv8::Divide::by(a->cache.page_size)};
   const int es = kv8::elem_bytes(a->dtype);
   const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->cache.pool, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
                      (long long)a->ld * es % 16 == 0 && (!a->q_out || (aligned_to(a->q, 16) && aligned_to(a->q_out, 16) && (long long)a->q_out_ld * es % 16 == 0));

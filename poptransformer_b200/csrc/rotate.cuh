@@ -70,24 +70,31 @@ template <typename T> __device__ __forceinline__ Item item_of(const Raw<T> &w) {
   for (int j = 0; j < 8; ++j) { v.lo[j] = to_f(e[j]); v.hi[j] = to_f(e[8 + j]); }
   return v;
 }
-// row: (cos, sin) of the position's pairs, on a multiple of 16 bytes.
-__device__ __forceinline__ void turn_item(Item &v, const float2 *row, const Runs &r, bool neighbours, float sign) {
+// (cos, sin) of a lane's pairs; row: those of the position, on a multiple of 16 bytes.
+struct Angles { float4 v[4]; };
+__device__ __forceinline__ Angles load_angles(const float2 *row, const Runs &r, bool neighbours) {
   const float4 *cs = reinterpret_cast<const float4 *>(row);
-  if (neighbours) {
-    float4 a[2], b[2];
-    if (r.turns_lo) { a[0] = __ldg(cs + r.lo / 4); a[1] = __ldg(cs + r.lo / 4 + 1); }
-    if (r.turns_hi) { b[0] = __ldg(cs + r.hi / 4); b[1] = __ldg(cs + r.hi / 4 + 1); }
+  Angles a{};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (r.turns_lo) { turn(v.lo[4 * j], v.lo[4 * j + 1], a[j].x, sign * a[j].y); turn(v.lo[4 * j + 2], v.lo[4 * j + 3], a[j].z, sign * a[j].w); }
-      if (r.turns_hi) { turn(v.hi[4 * j], v.hi[4 * j + 1], b[j].x, sign * b[j].y); turn(v.hi[4 * j + 2], v.hi[4 * j + 3], b[j].z, sign * b[j].w); }
+  for (int j = 0; j < 4; ++j) {
+    if (neighbours ? (j < 2 ? r.turns_lo : r.turns_hi) : r.turns_lo) a.v[j] = __ldg(cs + (neighbours ? (j < 2 ? r.lo / 4 + j : r.hi / 4 + j - 2) : r.lo / 2 + j));
+  }
+  return a;
+}
+__device__ __forceinline__ void turn_item(Item &v, const Angles &a, const Runs &r, bool neighbours, float sign) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 cs = make_float4(a.v[j].x, sign * a.v[j].y, a.v[j].z, sign * a.v[j].w);
+    if (neighbours) {
+      float(&run)[8] = j < 2 ? v.lo : v.hi;
+      if (j < 2 ? r.turns_lo : r.turns_hi) {
+        turn(run[4 * (j & 1)], run[4 * (j & 1) + 1], cs.x, cs.y);
+        turn(run[4 * (j & 1) + 2], run[4 * (j & 1) + 3], cs.z, cs.w);
+      }
+    } else if (r.turns_lo) {
+      turn(v.lo[2 * j], v.hi[2 * j], cs.x, cs.y);
+      turn(v.lo[2 * j + 1], v.hi[2 * j + 1], cs.z, cs.w);
     }
-  } else if (r.turns_lo) {
-    float4 a[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = __ldg(cs + r.lo / 2 + j);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { turn(v.lo[2 * j], v.hi[2 * j], a[j].x, sign * a[j].y); turn(v.lo[2 * j + 1], v.hi[2 * j + 1], a[j].z, sign * a[j].w); }
   }
 }
 
