@@ -25,10 +25,7 @@ namespace pt {
 namespace kv8 {
 
 constexpr int HEADS = 8, MAX_TOKENS = 1024;
-#ifndef KV8_SHORT
-#define KV8_SHORT 4
-#endif
-constexpr int SHORT = KV8_SHORT;
+constexpr int SHORT = 3;      // tiles of a warp up to which a segment stays in one block (32 query over 8 kv heads of 128, one token: 700 positions 10.2 us so, 13.0 dealt out; 1300 13.7 either way)
 constexpr int COUNTERS = 1 << 16;      // of a workspace, always in front: whichever calls share one, nothing else is written there
 
 // SIZE: the widest head, 64, 128 or 256.
@@ -110,25 +107,40 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ void load16(const void *q, size_t at, int dtype, bool whole, int n, float (&v)[16]) {
+// Sixteen elements of a query, as they lie there (`whole`: on a multiple of 16 bytes) or, of any other rows, as fp32; asked for before the tiles, used behind them.
+__device__ __forceinline__ void load16(const void *q, size_t at, int dtype, bool whole, int n, uint32_t (&v)[16]) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = 0.f;
+  for (int j = 0; j < 16; ++j) v[j] = 0;
   if (n <= 0) return;
-  auto run = [&](auto *p) {
-    if (whole) {
-      float lo[8], hi[8];
-      load_run(p + at, lo);
-      load_run(p + at + 8, hi);
+  if (whole) {
+    const uint4 *p = reinterpret_cast<const uint4 *>((const char *)q + at * (dtype == PT_DT_F32 ? 4 : 2));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { v[j] = lo[j]; v[8 + j] = hi[j]; }
-    } else {
+    for (int i = 0; i < 4; ++i)
+      if (i < 2 || dtype == PT_DT_F32) {
+        const uint4 w = p[i];
+        v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
+      }
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t x = __float_as_uint(dtype == PT_DT_F32 ? ((const float *)q)[at + j] : dtype == PT_DT_F16 ? __half2float(((const __half *)q)[at + j]) : __bfloat162float(((const __nv_bfloat16 *)q)[at + j]));
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = to_f(p[at + j]);
+      for (int k = 0; k < 16; ++k) v[k] = k == j ? x : v[k];
     }
-  };
-  if (dtype == PT_DT_F32) run((const float *)q);
-  else if (dtype == PT_DT_F16) run((const __half *)q);
-  else run((const __nv_bfloat16 *)q);
+  }
+}
+__device__ __forceinline__ void floats16(uint32_t (&v)[16], int dtype, bool whole) {
+  if (!whole || dtype == PT_DT_F32) return;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    const uint32_t w = v[j];
+    if (dtype == PT_DT_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+      v[2 * j] = __float_as_uint(f.x); v[2 * j + 1] = __float_as_uint(f.y);
+    } else {
+      v[2 * j] = w << 16; v[2 * j + 1] = w & 0xffff0000u;
+    }
+  }
 }
 template <int N> __device__ __forceinline__ void store_n(void *out, size_t at, int dtype, bool whole, const float (&v)[N]) {     // 8 or 16 of them
   auto run = [&](auto *p) {
@@ -307,25 +319,28 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
     const int v_at0 = 2 * tg * SIZE + (SIZE == 64 ? (((g >> 1) ^ tg) << 4) + (g & 1) * 8 : (g ^ 2 * tg) << 4);
     // copies: a tile a call, STAGES of them before the first is used and then one behind each.  A lane knows the page and the row in it of one of the next 32 groups of 16 positions.
     int ahead_at = 0, stage_in = 0, listed = 0, list_end = 0, page_l = 0, row_l = 0, kvh_in = 0;
+    auto list = [&]() {
+      const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
+      const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? sp.by_page(at) : 0;
+      row_l = at <= pos ? at - pg * p.c.page : -1;      // (-1: behind the last position)
+      page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
+      listed = ahead_at;       // (nothing waits for the page yet: the queries are asked for behind it)
+      list_end = ahead_at + min(32 / GROUPS, ahead.tiles - ahead.tile);
+      kvh_in = sp.by_chunks(ahead.seg);
+    };
+    list();
     auto fetch = [&]() {
       if (ahead_at < count) {
-        if (ahead_at >= list_end) {      // (a segment's first tile, or the list has been used up)
-          const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
-          const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? sp.by_page(at) : 0;
-          row_l = at <= pos ? at - pg * p.c.page : -1;      // (-1: behind the last position)
-          page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
-          if (page_l < 0) {
-            if (p.error_flag) atomicExch(p.error_flag, 12);
-            page_l = 0;
-          }
-          listed = ahead_at;
-          list_end = ahead_at + min(32 / GROUPS, ahead.tiles - ahead.tile);
-          kvh_in = sp.by_chunks(ahead.seg);
-        }
+        if (ahead_at >= list_end) list();      // (a segment's first tile, or the list has been used up)
         const uint32_t st = ring_s + stage_in * S::STAGE;
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
-          const int page = __shfl_sync(0xffffffffu, page_l, (ahead_at - listed) * GROUPS + u), row = __shfl_sync(0xffffffffu, row_l, (ahead_at - listed) * GROUPS + u);
+          int page = __shfl_sync(0xffffffffu, page_l, (ahead_at - listed) * GROUPS + u);
+          if (page < 0) {
+            if (p.error_flag) atomicExch(p.error_flag, 12);
+            page = 0;
+          }
+          const int row = __shfl_sync(0xffffffffu, row_l, (ahead_at - listed) * GROUPS + u);
           const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes;
           const unsigned char *k = base + (kvh_in * p.c.page + row + row_in) * dim + 16 * run_in;
           const unsigned char *v = base + (G * p.c.page) * dim + (kvh_in * p.c.page + row + row_in) * vdim + 16 * run_in;
@@ -369,19 +384,20 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       uint32_t qf[QPARTS][NK * 4][QREGS];
       float by[2];          // factors of the scores of heads 2 tg and 2 tg + 1
       {
-        float x[NK][16];
-        uint32_t most = 0;           // (in the order of bits: NaN above infinity)
+        uint32_t x[NK][16], most = 0;           // (in the order of bits: NaN above infinity)
         const size_t at = (size_t)(sp.tok0 + tok) * p.q_ld + (size_t)(head0 + g) * dim + 16 * tg;
 #pragma unroll
         for (int i = 0; i < NK; ++i) load16(sp.q, at + 64 * i, sp.dtype, sp.q_whole, g < heads ? dim - 64 * i - 16 * tg : 0, x[i]);
         if (done == 0) {        // (the first segment's queries are asked for before all tiles: they would come behind them)
-#pragma unroll
+#pragma unroll 1
           for (int s = 0; s < STAGES; ++s) fetch();
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int i = 0; i < NK; ++i) {
+          floats16(x[i], sp.dtype, sp.q_whole);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+          for (int j = 0; j < 16; ++j) most = max(most, x[i][j] & 0x7fffffffu);
+        }
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
         float unit;
@@ -396,7 +412,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int o = 0; o < 2; ++o) {
-                const float a = x[i][4 * c + 2 * o] * turn, b = x[i][4 * c + 2 * o + 1] * turn;
+                const float a = __uint_as_float(x[i][4 * c + 2 * o]) * turn, b = __uint_as_float(x[i][4 * c + 2 * o + 1]) * turn;
                 qf[0][4 * i + c][o % QREGS] = pack2(a, b);
                 if constexpr (PARTS == 2) {
                   const float2 h = unpack2(qf[0][4 * i + c][o % QREGS]);
@@ -413,7 +429,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
             for (int c = 0; c < 4; ++c) {
               uint32_t v[4], part[3];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(x[i][4 * c + e], turn, 12582912.f)) + (64u + (64u << 7) - 0x4B400000u);
+              for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(fmaf(__uint_as_float(x[i][4 * c + e]), turn, 12582912.f)) + (64u + (64u << 7) - 0x4B400000u);
 #pragma unroll
               for (int q = 0; q < 3; ++q) {       // bits 0 .. 6, 7 .. 13 and 14 .. 21 as byte 0, 1 and 2
                 const uint32_t sel = q == 0 ? 0x0040u : q == 1 ? 0x0051u : 0x0062u, sh = q;
