@@ -81,6 +81,17 @@ template <bool E4M3> __device__ __forceinline__ void widen(uint32_t x, uint32_t 
     second = *reinterpret_cast<const uint32_t *>(&hb);
   }
 }
+// The first product of a sum.
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -318,7 +329,8 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
     const int k_at0 = g * SIZE + ((tg ^ (SIZE == 64 ? 0 : (g & 1) << 2)) << 4);
     const int v_at0 = 2 * tg * SIZE + (SIZE == 64 ? (((g >> 1) ^ tg) << 4) + (g & 1) * 8 : (g ^ 2 * tg) << 4);
     // copies: a tile a call, STAGES of them before the first is used and then one behind each.  A lane knows the page and the row in it of one of the next 32 groups of 16 positions.
-    int ahead_at = 0, stage_in = 0, listed = 0, list_end = 0, page_l = 0, row_l = 0, kvh_in = 0;
+    int ahead_at = 0, stage_in = 0, listed = 0, list_end = 0, page_l = 0, row_l = 0, k_l = 0, v_l = 0, s_l = 0;
+    uint32_t whole_l = 0;        // groups that are there as a whole
     auto list = [&]() {
       const int pos = pl.pos[ahead.tok], first = (p.window > 0 ? max(0, pos - p.window + 1) : 0) / KT;
       const int at = (first + ahead.tile) * KT + lane * 16, pg = at <= pos ? sp.by_page(at) : 0;
@@ -326,41 +338,50 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
       page_l = at <= pos ? p.c.page_table[(size_t)pl.slot[ahead.tok] * p.c.max_pages + pg] : 0;
       listed = ahead_at;       // (nothing waits for the page yet: the queries are asked for behind it)
       list_end = ahead_at + min(32 / GROUPS, ahead.tiles - ahead.tile);
-      kvh_in = sp.by_chunks(ahead.seg);
+      const int kvh = sp.by_chunks(ahead.seg);       // this lane's first bytes and scale of a page, but for the row
+      k_l = (kvh * p.c.page + row_in) * dim + 16 * run_in;
+      v_l = G * p.c.page * dim + (kvh * p.c.page + row_in) * vdim + 16 * run_in;
+      s_l = ((lane >> 4) * G + kvh) * p.c.page + (lane & 15);
     };
     list();
     auto fetch = [&]() {
       if (ahead_at < count) {
         if (ahead_at >= list_end) list();      // (a segment's first tile, or the list has been used up)
+        const int at = (ahead_at - listed) * GROUPS;
+        if (at == 0) whole_l = __ballot_sync(0xffffffffu, FULL && row_l >= 0 && page_l >= 0);
+        const bool whole = (whole_l >> at & ((1 << GROUPS) - 1)) == (1 << GROUPS) - 1;
         const uint32_t st = ring_s + stage_in * S::STAGE;
+        auto v_to = [&](uint32_t st_v, int j) { return (SIZE == 128 ? st_v ^ (j & 1) << 6 : SIZE == 256 ? st_v ^ (2 * j & 6) << 4 : st_v) + j * 512; };
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < GROUPS; ++u) {
-          int page = __shfl_sync(0xffffffffu, page_l, (ahead_at - listed) * GROUPS + u);
-          if (page < 0) {
-            if (p.error_flag) atomicExch(p.error_flag, 12);
-            page = 0;
-          }
-          const int row = __shfl_sync(0xffffffffu, row_l, (ahead_at - listed) * GROUPS + u);
-          const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes;
-          const unsigned char *k = base + (kvh_in * p.c.page + row + row_in) * dim + 16 * run_in;
-          const unsigned char *v = base + (G * p.c.page) * dim + (kvh_in * p.c.page + row + row_in) * vdim + 16 * run_in;
-          const float *sc = p.c.scales + (size_t)page * (2 * G * p.c.page) + ((lane >> 4) * G + kvh_in) * p.c.page + row + (lane & 15);
-          const uint32_t st_k = st + u * (16 * SIZE) + k_in, st_v = st + S::ROWS + u * (16 * SIZE) + v_in, st_s = st + 2 * S::ROWS + u * 128 + lane * 4;
-          auto v_to = [&](int j) { return (SIZE == 128 ? st_v ^ (j & 1) << 6 : SIZE == 256 ? st_v ^ (2 * j & 6) << 4 : st_v) + j * 512; };
-          if (FULL && row >= 0) {
+          for (int u = 0; u < GROUPS; ++u) {
+            const int page = __shfl_sync(0xffffffffu, page_l, at + u), row = __shfl_sync(0xffffffffu, row_l, at + u);
+            const unsigned char *base = p.c.pool + (size_t)(uint32_t)page * p.c.page_bytes, *k = base + (k_l + row * SIZE), *v = base + (v_l + row * SIZE);
+            const uint32_t st_k = st + u * (16 * SIZE) + k_in, st_v = st + S::ROWS + u * (16 * SIZE) + v_in;
 #pragma unroll
             for (int j = 0; j < S::COPIES; ++j) copy_whole<16>(st_k + j * 512, k + j * 512);
 #pragma unroll
-            for (int j = 0; j < S::COPIES; ++j) copy_whole<16>(v_to(j), v + j * 512);
-            copy_whole<4>(st_s, sc);
-          } else {
+            for (int j = 0; j < S::COPIES; ++j) copy_whole<16>(v_to(st_v, j), v + j * 512);
+            copy_whole<4>(st + 2 * S::ROWS + u * 128 + lane * 4, p.c.scales + (size_t)(uint32_t)page * (2 * G * p.c.page) + (s_l + row));
+          }
+        } else {
+#pragma unroll 1
+          for (int u = 0; u < GROUPS; ++u) {
+            int page = __shfl_sync(0xffffffffu, page_l, at + u);
+            const int row = __shfl_sync(0xffffffffu, row_l, at + u);
+            if (page < 0) {
+              if (p.error_flag) atomicExch(p.error_flag, 12);
+              page = 0;
+            }
+            const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes, *k = base + (k_l + row * dim), *v = base + (v_l + row * vdim);
+            const uint32_t st_k = st + u * (16 * SIZE) + k_in, st_v = st + S::ROWS + u * (16 * SIZE) + v_in;
             const bool k_here = row >= 0 && 16 * run_in < dim, v_here = row >= 0 && 16 * run_in < vdim;
             constexpr int AT_ONCE = 512 / SIZE;      // rows of a copy
 #pragma unroll
             for (int j = 0; j < S::COPIES; ++j) copy_async<16>(st_k + j * 512, k_here ? k + j * AT_ONCE * dim : base, k_here);
 #pragma unroll
-            for (int j = 0; j < S::COPIES; ++j) copy_async<16>(v_to(j), v_here ? v + j * AT_ONCE * vdim : base, v_here);
-            copy_async<4>(st_s, row >= 0 ? sc : p.c.scales, row >= 0);
+            for (int j = 0; j < S::COPIES; ++j) copy_async<16>(v_to(st_v, j), v_here ? v + j * AT_ONCE * vdim : base, v_here);
+            copy_async<4>(st + 2 * S::ROWS + u * 128 + lane * 4, row >= 0 ? p.c.scales + (size_t)page * (2 * G * p.c.page) + (s_l + row) : p.c.scales, row >= 0);
           }
         }
         ++ahead_at;
@@ -454,8 +475,8 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         float x[GROUPS][4];
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
-          float c[2][4] = {};
-          int n[3][4] = {};
+          float c[2][4];
+          int n[3][4];
 #pragma unroll
           for (int i = 0; i < NK; ++i) {
             const unsigned char *at = st + u * (16 * SIZE) + (k_at0 ^ (i & 1) << 6) + (i >> 1) * 128;
@@ -468,13 +489,19 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
                 asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(a0), "=r"(a2) : "r"(wa[k]));
                 asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(a1), "=r"(a3) : "r"(wb[k]));
 #pragma unroll
-                for (int q = 0; q < QPARTS; ++q) mma(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
+                for (int q = 0; q < QPARTS; ++q) {
+                  if (i == 0 && k < 2 && q == 0) mma_first(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
+                  else mma(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
+                }
               }
             } else {
 #pragma unroll
               for (int k = 0; k < 4; k += 2)
 #pragma unroll
-                for (int q = 0; q < QPARTS; ++q) mma_s8(n[q % 3], wa[k], wb[k], wa[k + 1], wb[k + 1], qf[q][4 * i + k][0], qf[q][4 * i + k + 1][0]);
+                for (int q = 0; q < QPARTS; ++q) {
+                  if (i == 0 && k == 0) mma_s8_first(n[q % 3], wa[k], wb[k], wa[k + 1], wb[k + 1], qf[q][4 * i + k][0], qf[q][4 * i + k + 1][0]);
+                  else mma_s8(n[q % 3], wa[k], wb[k], wa[k + 1], wb[k + 1], qf[q][4 * i + k][0], qf[q][4 * i + k + 1][0]);
+                }
             }
           }
           const float ks[2] = {sc[u * 32 + g], sc[u * 32 + 8 + g]};
