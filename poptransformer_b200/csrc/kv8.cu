@@ -115,31 +115,25 @@ struct Append {
   int heads, rot, ld, q_out_ld;
   const float2 *rope;
   int *error_flag;
-  int items;                  // of a token: its rows in groups of ROWS
-  Divide by_items, by_page;
+  Divide by_page, by_q, by_kv;      // a page's positions; a token's query heads and its kv heads in groups of ROWS
+  int q_blocks, kv_blocks;          // blocks of query heads, of keys (and as many of values)
 };
-// The rows of a token: its q heads (rotated to q_out), its keys (rotated, kept as bytes), its values (kept as bytes).  LANES lanes have the same sixteenth elements of ROWS neighbouring rows.
-// Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  (A row a lane:
-// 11,000 tokens of 32 + 8 + 8 heads of 128 69.7 us; where there is less than a wave of rows one is faster, a token in 2.5 us so.)
-template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3>
-__global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
-  early_start();
-  const int G = p.c.n_kv, all = p.heads + 2 * G;
-  const int item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES, tok = p.by_items(item), r0 = (item - tok * p.items) * ROWS;
-  const bool there = tok < p.b.n_tok;
-  // Row r0 + i of the token: what it is, its head, its width and where it lies.
-  auto is_q = [&](int i) { return r0 + i < p.heads; };
-  auto is_v = [&](int i) { return r0 + i >= p.heads + G; };
-  auto head = [&](int i) { return is_q(i) ? r0 + i : is_v(i) ? r0 + i - p.heads - G : r0 + i - p.heads; };
-  auto width = [&](int i) { return is_v(i) ? p.c.vdim : p.c.dim; };
-  auto has = [&](int i) { return there && r0 + i < all && 16 * t < width(i); };
-  auto from = [&](int i) { return (is_q(i) ? q : is_v(i) ? v : k) + (size_t)tok * p.ld + (size_t)head(i) * width(i); };
+enum Kind { QUERY, KEY, VALUE };
+// LANES lanes have the same sixteenth elements of ROWS neighbouring heads of a token: of queries, which are rotated, of keys, rotated and kept as bytes, or of values, kept as bytes.
+template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3, Kind KIND>
+__device__ __forceinline__ void append_rows(const T *src, T *q_out, const Append &p, int block) {
+  const int heads = KIND == QUERY ? p.heads : p.c.n_kv, dim = KIND == VALUE ? p.c.vdim : p.c.dim, rot = KIND == VALUE ? 0 : p.rot;
+  const Divide &by = KIND == QUERY ? p.by_q : p.by_kv;
+  const int item = block * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES, tok = by(item), h0 = (item - tok * (int)by.d) * ROWS;
+  const bool there = tok < p.b.n_tok, mine = there && 16 * t < dim;
+  const Runs runs = runs_of(t, dim, rot, NEIGHBOURS);
+  const T *from = src + (size_t)tok * p.ld + h0 * dim;
   const int used = p.b.cu[p.b.n_seq], seq = there ? p.b.tok_seq[tok] : 0;
   Raw<T> raw[ROWS];
   if constexpr (WHOLE) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
-      if (has(i)) raw[i] = load_raw(from(i), runs_of(t, width(i), is_v(i) ? 0 : p.rot, NEIGHBOURS));
+      if (mine && h0 + i < heads) raw[i] = load_raw(from + i * dim, runs);
   }
   int pos = -1, page = -1;
   if (there && tok < used) {
@@ -148,66 +142,77 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T 
       pos = start + tok - first;
       page = p.c.page_table[(size_t)p.b.slot[seq] * p.c.max_pages + p.by_page(pos)];
     }
-    if (page < 0 && r0 == 0 && t == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    if (page < 0 && h0 == 0 && t == 0 && p.error_flag) atomicExch(p.error_flag, 12);
   }
+  const bool fits = mine && page >= 0;
+  const float2 *row = p.rope + (size_t)max(pos, 0) * (rot / 2);
+  Angles angles{};
+  if (WHOLE && KIND != VALUE && fits) angles = load_angles(row, runs, NEIGHBOURS);
   const int place = pos - p.by_page(max(pos, 0)) * p.c.page;
-  const float2 *angles = p.rope + (size_t)max(pos, 0) * (p.rot / 2);
-  Angles turned{};
-  if (WHOLE && page >= 0 && !is_v(0) && 16 * t < p.c.dim) turned = load_angles(angles, runs_of(t, p.c.dim, p.rot, NEIGHBOURS), NEIGHBOURS);
+  unsigned char *to = p.c.pool + (size_t)max(page, 0) * p.c.page_bytes + (KIND == VALUE ? (size_t)p.c.n_kv * p.c.page * p.c.dim : 0) + ((size_t)h0 * p.c.page + place) * dim;
+  float *scale = p.c.scales + ((size_t)max(page, 0) * 2 + (KIND == VALUE)) * p.c.n_kv * p.c.page + h0 * p.c.page + place;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {      // (whole warps stay together: the lanes of a row exchange their maxima)
-    const int dim = width(i), rot = is_v(i) ? 0 : p.rot, h = head(i);
-    const bool in = page >= 0 && has(i);
-    const Runs runs = runs_of(t, dim, rot, NEIGHBOURS);
+    const bool in = fits && h0 + i < heads;
     Item x{};
     if (in) {
       if constexpr (WHOLE) {
         x = item_of<T>(raw[i]);
-        turn_item(x, turned, runs, NEIGHBOURS, 1.f);
+        if (KIND != VALUE) turn_item(x, angles, runs, NEIGHBOURS, 1.f);
       } else {
-        x = load_pairs(from(i), t, dim, rot, NEIGHBOURS);
-        turn_pairs(x, angles, t, rot, 1.f);
+        x = load_pairs(from + i * dim, t, dim, rot, NEIGHBOURS);
+        if (KIND != VALUE) turn_pairs(x, row, t, rot, 1.f);
       }
-      if (is_q(i)) {
-        T *to = q_out + (size_t)tok * p.q_out_ld + (size_t)h * dim;
-        if constexpr (WHOLE) {
-          store_run(to + runs.lo, x.lo);
-          store_run(to + runs.hi, x.hi);
-        } else {
-          store_pairs(to, x, t, dim, rot, NEIGHBOURS);
+    }
+    if constexpr (KIND == QUERY) {
+      T *out = q_out + (size_t)tok * p.q_out_ld + (h0 + i) * dim;
+      if (!in) continue;
+      if constexpr (WHOLE) {
+        store_run(out + runs.lo, x.lo);
+        store_run(out + runs.hi, x.hi);
+      } else {
+        store_pairs(out, x, t, dim, rot, NEIGHBOURS);
+      }
+    } else {
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = larger(m, x.lo[j], x.hi[j]);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o), 0.f);
+      if (!in) continue;
+      const bool fine = m <= LARGE;
+      const float most = fmaxf(m, SMALL), times = __fdiv_rn(top_byte<E4M3>(), most);
+      if (t == 0) scale[i * p.c.page] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x.lo[j] = __fmul_rn(x.lo[j], times);
+        x.hi[j] = __fmul_rn(x.hi[j], times);
+      }
+      if (!fine) x = Item{};
+      unsigned char *bytes = to + (size_t)i * p.c.page * dim;
+      if constexpr (WHOLE) {
+        *reinterpret_cast<uint2 *>(bytes + runs.lo) = make_uint2(to_word<E4M3>(x.lo[0], x.lo[1], x.lo[2], x.lo[3]), to_word<E4M3>(x.lo[4], x.lo[5], x.lo[6], x.lo[7]));
+        *reinterpret_cast<uint2 *>(bytes + runs.hi) = make_uint2(to_word<E4M3>(x.hi[0], x.hi[1], x.hi[2], x.hi[3]), to_word<E4M3>(x.hi[4], x.hi[5], x.hi[6], x.hi[7]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
+          if (e.x < dim) bytes[e.x] = (unsigned char)to_byte<E4M3>(x.lo[j]);
+          if (e.y < dim) bytes[e.y] = (unsigned char)to_byte<E4M3>(x.hi[j]);
         }
       }
     }
-    if (__all_sync(0xffffffffu, !in || is_q(i))) continue;
-    float m = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = larger(m, x.lo[j], x.hi[j]);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o), 0.f);
-    if (!in || is_q(i)) continue;
-    const bool fine = m <= LARGE;
-    const float most = fmaxf(m, SMALL), by = __fdiv_rn(top_byte<E4M3>(), most);
-    const size_t row = (size_t)h * p.c.page + place;
-    if (t == 0) p.c.scales[((size_t)page * 2 * G + (is_v(i) ? G : 0)) * p.c.page + row] = fine ? __fdiv_rn(most, top_byte<E4M3>()) : __uint_as_float(0x7fffffffu);
-    unsigned char *to = p.c.pool + (size_t)page * p.c.page_bytes + (is_v(i) ? (size_t)G * p.c.page * p.c.dim : 0) + row * dim;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x.lo[j] = __fmul_rn(x.lo[j], by);
-      x.hi[j] = __fmul_rn(x.hi[j], by);
-    }
-    if (!fine) x = Item{};
-    if constexpr (WHOLE) {
-      *reinterpret_cast<uint2 *>(to + runs.lo) = make_uint2(to_word<E4M3>(x.lo[0], x.lo[1], x.lo[2], x.lo[3]), to_word<E4M3>(x.lo[4], x.lo[5], x.lo[6], x.lo[7]));
-      *reinterpret_cast<uint2 *>(to + runs.hi) = make_uint2(to_word<E4M3>(x.hi[0], x.hi[1], x.hi[2], x.hi[3]), to_word<E4M3>(x.hi[4], x.hi[5], x.hi[6], x.hi[7]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int2 e = pair_at(8 * t + j, rot, NEIGHBOURS);
-        if (e.x < dim) to[e.x] = (unsigned char)to_byte<E4M3>(x.lo[j]);
-        if (e.y < dim) to[e.y] = (unsigned char)to_byte<E4M3>(x.hi[j]);
-      }
-    }
   }
+}
+// Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  (A row a lane:
+// 11,000 tokens of 32 + 8 + 8 heads of 128 69.7 us, two 59.0; where there is less than a wave of rows one is faster, a token in 2.5 us so.)
+template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3>
+__global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
+  early_start();
+  const int block = blockIdx.x;
+  if (block < p.kv_blocks) append_rows<T, LANES, ROWS, WHOLE, NEIGHBOURS, E4M3, KEY>(k, nullptr, p, block);
+  else if (block < 2 * p.kv_blocks) append_rows<T, LANES, ROWS, WHOLE, NEIGHBOURS, E4M3, VALUE>(v, nullptr, p, block - p.kv_blocks);
+  else append_rows<T, LANES, ROWS, WHOLE, NEIGHBOURS, E4M3, QUERY>(q, q_out, p, block - 2 * p.kv_blocks);
 }
 
 // ------------------------------------------------------------------------------------------ pages in a wider type
@@ -408,12 +413,14 @@ template <typename T> static cudaError_t launch_rotary(const pt_rotary_args &a, 
 }
 
 template <typename T, int LANES, int ROWS, bool WHOLE> static cudaError_t launch_append(const pt_kv8_append_args &a, Append p, cudaStream_t st) {
-  p.items = ceil_div(p.heads + 2 * p.c.n_kv, ROWS);
-  p.by_items = Divide::by(p.items);
+  p.by_q = Divide::by(std::max(1, ceil_div(p.heads, ROWS)));
+  p.by_kv = Divide::by(ceil_div(p.c.n_kv, ROWS));
+  p.q_blocks = p.heads ? ceil_div(a.batch.n_tok * (int)p.by_q.d, THREADS / LANES) : 0;
+  p.kv_blocks = ceil_div(a.batch.n_tok * (int)p.by_kv.d, THREADS / LANES);
   const bool e4m3 = a.cache.fmt == PT_KV8_E4M3;
   const auto kernel = e4m3 ? (a.interleaved ? append_kernel<T, LANES, ROWS, WHOLE, true, true> : append_kernel<T, LANES, ROWS, WHOLE, false, true>)
                            : (a.interleaved ? append_kernel<T, LANES, ROWS, WHOLE, true, false> : append_kernel<T, LANES, ROWS, WHOLE, false, false>);
-  return launch_early(kernel, Grid(ceil_div(a.batch.n_tok * p.items, THREADS / LANES)), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
+  return launch_early(kernel, Grid(p.q_blocks + 2 * p.kv_blocks), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
 }
 template <typename T, int LANES> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, bool whole, cudaStream_t st) {
   constexpr int MANY = 2;      // rows of a lane, where there are more than a wave of rows one by one (four: fewer warps, 61.6 us)
@@ -503,7 +510,7 @@ extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
              a->cache.n_kv);
   if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Append p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->q_out ? a->n_head : 0, a->rope_dims, a->ld, a->q_out_ld, (const float2 *)a->rope, a->error_flag,
-                      0, {}, kv8::Divide::by(a->cache.page_size)};
+                      kv8::Divide::by(a->cache.page_size), {}, {}, 0, 0};
   const int es = kv8::elem_bytes(a->dtype);
   const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->cache.pool, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
                      (long long)a->ld * es % 16 == 0 && (!a->q_out || (aligned_to(a->q, 16) && aligned_to(a->q_out, 16) && (long long)a->q_out_ld * es % 16 == 0));
