@@ -455,7 +455,7 @@ static size_t workspace_bytes(int width) {
   return sizeof(int) * COUNTERS + sizeof(float) * sm_count() * pieces;
 }
 template <int SIZE, bool FULL> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
-  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype == PT_DT_F32;
+  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype != PT_DT_BF16;      // (weights in two fp16 parts: one would double the error of an fp16 output)
   const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, FULL, true, 2> : attn_kernel<SIZE, FULL, true, 1>) : (wide ? attn_kernel<SIZE, FULL, false, 2> : attn_kernel<SIZE, FULL, false, 1>);
   static std::atomic<uint64_t> allowed[4];
   constexpr int WARPS = Shape<SIZE>::WARPS, FIXED = WARPS * Shape<SIZE>::RING;

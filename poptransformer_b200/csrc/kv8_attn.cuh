@@ -11,10 +11,10 @@
 // its bytes.  Keys of int8 are multiplied as they are, with q in three parts of 8 bits (m16n8k32, whole numbers); all other bytes become fp16, exactly: E4M3 by conversion, int8 b as
 // (1024 + 128 + b) - 1152.  (Both at fp16 a tile of 32 keys took 270 cycles of an SM, 350 is what its bytes take to come.)
 //
-// Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), with a second part of what is
-// left for queries of 32 bits: what is lost lies below 2^-25 of the largest.
+// Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), with PARTS = 2 a second part of what is
+// left: what is lost lies below 2^-25 of the largest.
 // With x = score log2(e), v_j = bytes times vs_j, and e_j about log2 vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
-// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once (2^-11; two parts for rows of 32 bits), whole down to 2^-29 of the largest and then off by
+// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once for rows of bf16 (2^-11, an eighth of what their output is rounded by) and to two parts for others (2^-21), whole down to 2^-29 of the largest and then off by
 // 2^-40 of it, however far the scales of the values lie apart.
 #pragma once
 #include <type_traits>
@@ -219,7 +219,7 @@ __device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, const 
   return w;
 }
 
-// FULL: keys and values are as wide as SIZE.
+// FULL: keys and values are as wide as SIZE.  PARTS: fp16 parts of the weights (and of the queries that are fp16): 1 for rows of bf16, 2 for others.
 template <int SIZE, bool FULL, bool E4M3, int PARTS>
 __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const Attn p, const Split sp) {
   early_start();

@@ -126,13 +126,13 @@ def reference(s, q, window=0, softcap=0.0):
 
     A score is a sum of dim products in 32 bits, each exact but for the query (kept to 2^-22 of its row's largest element, or exactly), times two factors: off by at most
     e = (dim + 8) 2^-24 sum |q_i k_i| scale, and with a softcap a few units of its result more.  exp and its argument in powers of two add 2^-20 at scores below 2^10 (their own
-    rounding is in e).  A weight is rounded once, to fp16 (half a step: 2^-11) for rows of 16 bits and to two fp16 parts (2^-21) for 32 bits, and below 2^-29 of the largest it is off by 2^-40 of
+    rounding is in e).  A weight is rounded once, to fp16 (half a step: 2^-11) for rows of bf16 and to two fp16 parts (2^-21) for others, and below 2^-29 of the largest it is off by 2^-40 of
     that.  The sums of the weighted values are sums in 32 bits of n terms in runs, 2^-22 of the sum of magnitudes.  So an output is off by at most
     (2 e + 2^-20 + weight) sum p |v| + n 2^-40 max |v|, and half a step of its type."""
     H, G = s.heads, s.n_kv
     out = torch.zeros((s.n_tok, H, s.vdim), dtype=torch.float64, device=s.device)
     tol = torch.zeros_like(out)
-    weight = 2.0 ** -21 if s.dtype == torch.float32 else 2.0 ** -11
+    weight = 2.0 ** -11 if s.dtype == torch.bfloat16 else 2.0 ** -21
     half = torch.finfo(s.dtype).eps / 2
     for i, n in enumerate(s.counts):
         if not n:
