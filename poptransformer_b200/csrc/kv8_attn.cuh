@@ -26,6 +26,7 @@ namespace kv8 {
 
 constexpr int HEADS = 8, MAX_TOKENS = 1024;
 constexpr int SHORT = 3;      // tiles of a warp up to which a segment stays in one block (32 query over 8 kv heads of 128, one token: 700 positions 10.2 us so, 13.0 dealt out; 1300 13.7 either way)
+constexpr int ALIGNED = 6;    // ... and up to which a block has whole segments (64 sequences of 300 positions 21.0 us dealt out evenly, so 18.6; of 2000 48.5 and 45.7; from 9 on the blocks' loads differ too much)
 constexpr int COUNTERS = 1 << 16;      // of a workspace, always in front: whichever calls share one, nothing else is written there
 
 // SIZE: the widest head, 64, 128 or 256.
@@ -95,11 +96,6 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
@@ -311,6 +307,17 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
     w.tiles = block_n = w.tok < tokens ? pl.cum[w.tok + 1] - pl.cum[w.tok] : 0;
     if (block_n) block0 = pl.cum[w.tok] * segs + w.seg * block_n;
   }
+  // (Many short ones: whole segments to a block, those that begin in its run, for the same reason; not where most blocks would have none.)
+  if (!one_each && most <= ALIGNED * NW && most <= 2 * per) {
+    const int at = block0 + (lane & 1) * per;
+    int begin = min(at, all);
+    if (at < all) {
+      const Walk x = walk_to(at, pl, segs, sp.by_segs, tokens);
+      if (x.tile) begin = at + x.tiles - x.tile;
+    }
+    block0 = __shfl_sync(0xffffffffu, begin, 0);
+    block_n = __shfl_sync(0xffffffffu, begin, 1) - block0;
+  }
   if (block_n <= 0) return;
 
   // ---- this warp's run
@@ -491,7 +498,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
 #pragma unroll
                 for (int q = 0; q < QPARTS; ++q) {
                   if (i == 0 && k < 2 && q == 0) mma_first(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
-                  else mma(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
+                  else mma16816(c[k & 1], a0, a1, a2, a3, qf[q][4 * i + k][0], qf[q][4 * i + k][QREGS - 1]);
                 }
               }
             } else {
@@ -603,7 +610,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
                 widen<E4M3>(v[0][k], v[1][k], half, a0, a1);
                 widen<E4M3>(v[2][k], v[3][k], half, a2, a3);
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) mma(O[i * 8 + 2 * k + half], a0, a1, a2, a3, wf[q][0], wf[q][1]);
+                for (int q = 0; q < PARTS; ++q) mma16816(O[i * 8 + 2 * k + half], a0, a1, a2, a3, wf[q][0], wf[q][1]);
               }
           }
         }

@@ -10,19 +10,7 @@ namespace pt {
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
-// Eight values that lie together, from or to a multiple of 16 bytes.
-__device__ __forceinline__ void load_run(const float *p, float (&v)[8]) {
-  const float4 x = reinterpret_cast<const float4 *>(p)[0], y = reinterpret_cast<const float4 *>(p)[1];
-  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-}
-template <typename T> __device__ __forceinline__ void load_run(const T *p, float (&v)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4 *>(p);
-  T h[8];
-  *reinterpret_cast<uint4 *>(h) = r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_f(h[j]);
-}
+// Eight values that lie together, to a multiple of 16 bytes.
 __device__ __forceinline__ void store_run(float *p, const float (&v)[8]) {
   reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
