@@ -942,7 +942,7 @@ typedef struct pt_kv8_cache {
 
 /* pt_rotary: out <- x with the first rope_dims dimensions of every head rotated by the angles of its row's position: pair (i, i + rope_dims / 2), or (2 i,
  * 2 i + 1) with interleaved, by (cos, sin) = rope[position][i], in 32 bits, rounded once.  inverse: by the negative angles (the gradient of x for
- * one of out).  out may be x.  A row whose position is outside the table is left as it was and sets error_flag to 12. */
+ * one of out).  out may be x itself, or lies apart from it.  A row whose position is outside the table is left as it was and sets error_flag to 12. */
 typedef struct pt_rotary_args {
   int rows, heads, dim, dtype;   /* PT_DT_F16, PT_DT_F32 or PT_DT_BF16               */
   const void *x;
@@ -957,7 +957,7 @@ typedef struct pt_rotary_args {
 int pt_rotary(const pt_rotary_args *args, void *stream);
 
 /* pt_kv8_append: the keys (rotated as in pt_rotary by their positions start[s] + i) and values of the packed tokens go to the cache.  With q_out the
- * queries go there, rotated, in their own type (q_out may be q).  The rows of q, k and v have one stride. */
+ * queries go there, rotated, in their own type (q_out may be q itself, or lies apart from the rows).  The rows of q, k and v have one stride. */
 typedef struct pt_kv8_append_args {
   pt_batch_view batch;
   pt_kv8_cache cache;
@@ -973,7 +973,7 @@ typedef struct pt_kv8_append_args {
 int pt_kv8_append(const pt_kv8_append_args *args, void *stream);
 
 /* pt_kv8_attn: token i of sequence s attends to the cached positions up to its own, start[s] + i (which pt_kv8_append has written): out[h] = sum_j w_j v_j,
- * w = softmax(c(scale q[h] . k_j)) over the last `window` of them (0: all); softcap c: a score x becomes c tanh(x / c) (0: none).  Meant for few tokens a
+ * w = softmax(c(scale q[h] . k_j)) over the last `window` of them (0: all); softcap c: a score x becomes c tanh(x / c) (0: none).  out may be q itself where keys and values are equally wide.  Meant for few tokens a
  * sequence: every token reads its history by itself.  A negative page reads as some other page, and sets error_flag to 12. */
 typedef struct pt_kv8_attn_args {
   pt_batch_view batch;

@@ -78,7 +78,8 @@ struct Rotary {
   Divide by_heads;
 };
 // LANES lanes (16 elements each) for a head of a row; a thread has one.  Bound by memory: rows in and out once.  So nothing waits for the position before the row has been asked for, and no lane
-// loops (a block a row, whose lanes went through its heads in turn with the angles in registers: 4000 rows of 34 heads 16.1 us).
+// loops (4000 rows of 34 heads of 128, half of each turned: 13.3 us, 5.3 TB/s; a block a row, whose lanes went
+// through its heads in turn with the angles in registers, 16.1).
 template <typename T, int LANES, bool WHOLE, bool INVERSE, bool NEIGHBOURS>
 __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const T *x, T *out, const Rotary p) {
   early_start();
@@ -204,8 +205,9 @@ __device__ __forceinline__ void append_rows(const T *src, T *q_out, const Append
     }
   }
 }
-// Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  (A row a lane:
-// 11,000 tokens of 32 + 8 + 8 heads of 128 69.7 us, two 59.0; where there is less than a wave of rows one is faster, a token in 2.5 us so.)
+// Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  11,000 tokens
+// of 32 + 8 + 8 heads of 128, 250 MB: 46.0 us, 5.4 TB/s; a row a lane 69.7, two rows of any kind 59.0 (selects and addresses of three kinds).  Where there is less than a wave of rows one is
+// faster: a token 2.4 us.
 template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
   early_start();
@@ -233,8 +235,8 @@ template <bool E4M3> __device__ __forceinline__ void from_word(uint32_t w, float
     for (int j = 0; j < 4; ++j) v[j] = (float)(signed char)(w >> (8 * j)) * scale;
   }
 }
-// Block: rows_each positions of a sequence, keys or values of heads_each heads.  Bound by memory: a thread finds its places once and asks for four heads' bytes together (a block a head, which found
-// them again: 4 sequences of 16500 positions, 8 heads of 128, 63.4 us).
+// Block: rows_each positions of a sequence, keys or values of heads_each heads.  Bound by memory: a thread finds its places once and asks for four heads' bytes together, and a warp's stores are whole
+// sectors.  4 sequences of up to 16500 positions, 8 heads of 128, E4M3 to fp16, 299 MB: 49.7 us, 6.0 TB/s (a block a head, which found its places again, 63.4; stores of half sectors 60.4).
 template <typename T, bool WHOLE, bool E4M3> __global__ void __launch_bounds__(THREADS) unpack_kernel(T *into, const Unpack p) {
   early_start();
   const int parts = gridDim.z / 2;
@@ -307,7 +309,7 @@ struct Attn {
 #include "kv8_attn.cuh"
 namespace pt {
 namespace kv8 {
-// Any sizes: a block per token and head, whose warps take every fourth key each with a running maximum and sum, lanes across the dimensions.
+// Any sizes (and 54 times the time of the tensor cores' on 48 sequences of up to 8000 positions): a block per token and head, whose warps take every fourth key each with a running maximum and sum, lanes across the dimensions.
 constexpr int PLAIN_WARPS = 4, MOST_DIM = 256;
 template <typename T, bool E4M3> __global__ void __launch_bounds__(PLAIN_WARPS * 32) attn_plain_kernel(const T *q, T *out, const Attn p) {
   early_start();
@@ -381,13 +383,21 @@ static int check_cache(const pt_kv8_cache &c, const char *who) {
   return PT_OK;
 }
 static int check_batch(const pt_batch_view &b, const char *who) {
-  PT_REQUIRE(b.n_seq > 0 && b.n_tok >= 0 && b.cu && b.start && b.slot && b.tok_seq, "%s: bad batch (%d sequences, %d tokens)", who, b.n_seq, b.n_tok);
+  PT_REQUIRE(b.n_seq > 0 && b.n_tok >= 0 && b.cu && b.start && b.slot && (b.tok_seq || b.n_tok == 0), "%s: bad batch (%d sequences, %d tokens)", who, b.n_seq, b.n_tok);
   return PT_OK;
 }
 static int check_rope(const float *rope, int rope_dims, int dim, const char *who) {
   PT_REQUIRE(rope_dims >= 0 && rope_dims % 2 == 0 && rope_dims <= dim, "%s: %d rotated dimensions of %d (an even number)", who, rope_dims, dim);
   PT_REQUIRE(rope_dims == 0 || (rope && aligned_to(rope, 8)), "%s: %d rotated dimensions want a table (on a multiple of 8 bytes)", who, rope_dims);
   return PT_OK;
+}
+// Whether rows of `width` that are read and rows of `to_width` that are written while others are still read have no element in common.
+static bool apart(const void *x, long long ld, long long width, const void *to, long long to_ld, long long to_width, long long rows, int es) {
+  const char *a = (const char *)x, *b = (const char *)to;
+  if (rows <= 0 || a + ((rows - 1) * ld + width) * es <= b || b + ((rows - 1) * to_ld + to_width) * es <= a) return true;
+  if (ld != to_ld || (b - a) % es != 0) return false;
+  const long long d = (((b - a) / es) % ld + ld) % ld;      // columns of the same wider rows
+  return d >= width && d + to_width <= ld;
 }
 static Cache cache_of(const pt_kv8_cache &c) {
   return {(unsigned char *)c.pool, c.scales, c.page_table, c.n_kv, c.dim, c.vdim, c.page_size, c.max_pages, c.max_len ? c.max_len : c.page_size * c.max_pages,
@@ -423,7 +433,7 @@ template <typename T, int LANES, int ROWS, bool WHOLE> static cudaError_t launch
   return launch_early(kernel, Grid(p.q_blocks + 2 * p.kv_blocks), THREADS, 0, st, (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.q_out, p);
 }
 template <typename T, int LANES> static cudaError_t launch_append(const pt_kv8_append_args &a, const Append &p, bool whole, cudaStream_t st) {
-  constexpr int MANY = 2;      // rows of a lane, where there are more than a wave of rows one by one (four: fewer warps, 61.6 us)
+  constexpr int MANY = 2;      // rows of a lane, where there are more than a wave of rows one by one (four: fewer warps, 61.6 us where two took 59.0)
   const bool many = (long long)a.batch.n_tok * (p.heads + 2 * p.c.n_kv) * LANES > 1024ll * sm_count();
   if (!whole) return launch_append<T, LANES, 1, false>(a, p, st);
   return many ? launch_append<T, LANES, MANY, true>(a, p, st) : launch_append<T, LANES, 1, true>(a, p, st);
@@ -480,11 +490,13 @@ extern "C" int pt_rotary(const pt_rotary_args *a, void *stream) {
              kv8::MOST_DIM);
   PT_REQUIRE(a->x && a->out && a->position, "pt_rotary: null pointer argument");
   PT_REQUIRE(a->x_ld >= (long long)a->heads * a->dim && a->out_ld >= (long long)a->heads * a->dim, "pt_rotary: rows of %d and %d elements, %d heads of %d", a->x_ld, a->out_ld, a->heads, a->dim);
-  PT_REQUIRE(a->x != a->out || a->x_ld == a->out_ld, "pt_rotary: rows that are rotated in place have one stride, got %d and %d", a->x_ld, a->out_ld);
+  const int es = kv8::elem_bytes(a->dtype);
+  const long long width = (long long)a->heads * a->dim;
+  PT_REQUIRE((a->x == a->out && a->x_ld == a->out_ld) || kv8::apart(a->x, a->x_ld, width, a->out, a->out_ld, width, a->rows, es), "pt_rotary: out is x itself (with its stride, %d, not %d) or apart from it",
+             a->x_ld, a->out_ld);
   PT_REQUIRE(a->positions > 0 && a->rope_dims > 0, "pt_rotary: %d rotated dimensions, a table of %d positions", a->rope_dims, a->positions);
   if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->dim, "pt_rotary")) return rc;
   if (a->rows == 0) return PT_OK;
-  const int es = kv8::elem_bytes(a->dtype);
   PT_REQUIRE((long long)a->rows * a->heads < (1ll << 30), "pt_rotary: %d rows of %d heads", a->rows, a->heads);
   const bool whole = a->dim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->x, 16) && aligned_to(a->out, 16) && (long long)a->x_ld * es % 16 == 0 && (long long)a->out_ld * es % 16 == 0;
   const kv8::Rotary p{a->rows, a->heads, a->dim, a->rope_dims, a->x_ld, a->out_ld, a->positions, a->position, (const float2 *)a->rope, a->error_flag, kv8::Divide::by(a->heads)};
@@ -501,17 +513,22 @@ extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
   PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_append: type %d", a->dtype);
   if (int rc = kv8::check_batch(a->batch, "pt_kv8_append")) return rc;
   if (int rc = kv8::check_cache(a->cache, "pt_kv8_append")) return rc;
-  if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->cache.dim, "pt_kv8_append")) return rc;
   PT_REQUIRE(a->k && a->v && a->ld > 0, "pt_kv8_append: null pointer argument, or rows of %d elements", a->ld);
   PT_REQUIRE(!a->q_out || (a->q && a->n_head > 0 && a->q_out_ld >= (long long)a->n_head * a->cache.dim), "pt_kv8_append: q_out wants q and rows of %d heads of %d, got %d elements", a->n_head,
              a->cache.dim, a->q_out_ld);
-  PT_REQUIRE(!a->q_out || a->q != a->q_out || a->ld == a->q_out_ld, "pt_kv8_append: queries that are rotated in place have one stride, got %d and %d", a->ld, a->q_out_ld);
+  const int es = kv8::elem_bytes(a->dtype);
+  if (a->q_out) {
+    const long long n = a->batch.n_tok, width = (long long)a->n_head * a->cache.dim, kv = a->cache.n_kv;
+    PT_REQUIRE(((a->q == a->q_out && a->ld == a->q_out_ld) || kv8::apart(a->q, a->ld, width, a->q_out, a->q_out_ld, width, n, es)) &&
+                   kv8::apart(a->k, a->ld, kv * a->cache.dim, a->q_out, a->q_out_ld, width, n, es) && kv8::apart(a->v, a->ld, kv * a->cache.vdim, a->q_out, a->q_out_ld, width, n, es),
+               "pt_kv8_append: q_out is q itself (with its stride, %d, not %d) or apart from the rows", a->ld, a->q_out_ld);
+  }
+  if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->cache.dim, "pt_kv8_append")) return rc;
   PT_REQUIRE((long long)a->batch.n_tok * ((a->q_out ? a->n_head : 0) + 2ll * a->cache.n_kv) < (1ll << 30), "pt_kv8_append: %d tokens of %d and %d heads", a->batch.n_tok, a->n_head,
              a->cache.n_kv);
   if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Append p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->q_out ? a->n_head : 0, a->rope_dims, a->ld, a->q_out_ld, (const float2 *)a->rope, a->error_flag,
                       kv8::Divide::by(a->cache.page_size), {}, {}, 0, 0};
-  const int es = kv8::elem_bytes(a->dtype);
   const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->cache.pool, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
                      (long long)a->ld * es % 16 == 0 && (!a->q_out || (aligned_to(a->q, 16) && aligned_to(a->q_out, 16) && (long long)a->q_out_ld * es % 16 == 0));
   const cudaStream_t st = as_stream(stream);
@@ -554,6 +571,10 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   PT_REQUIRE(a->n_head > 0 && a->n_head <= 65535 && a->n_head % a->cache.n_kv == 0, "pt_kv8_attn: %d heads over %d", a->n_head, a->cache.n_kv);
   PT_REQUIRE(a->q_ld >= (long long)a->n_head * a->cache.dim && a->out_ld >= (long long)a->n_head * a->cache.vdim, "pt_kv8_attn: rows of %d and %d elements, %d heads of %d and %d", a->q_ld,
              a->out_ld, a->n_head, a->cache.dim, a->cache.vdim);
+  const int es = kv8::elem_bytes(a->dtype);
+  PT_REQUIRE((a->q == a->out && a->q_ld == a->out_ld && a->cache.dim == a->cache.vdim) || kv8::apart(a->q, a->q_ld, (long long)a->n_head * a->cache.dim, a->out, a->out_ld, (long long)a->n_head * a->cache.vdim,
+                                                                                                      a->batch.n_tok, es),
+             "pt_kv8_attn: out is q itself (with its stride and width) or apart from it");
   PT_REQUIRE(a->window >= 0, "pt_kv8_attn: window=%d", a->window);
   PT_REQUIRE(a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f), "pt_kv8_attn: softcap=%g (0, or 1e-20 .. 1e20)", (double)a->softcap);
   PT_REQUIRE(a->scale - a->scale == 0.f, "pt_kv8_attn: scale=%g", (double)a->scale);
@@ -572,7 +593,6 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   const size_t need = pt_kv8_attn_workspace_bytes(a->batch.n_tok, a->n_head, a->cache.n_kv, width);
   PT_REQUIRE(a->workspace && aligned_to(a->workspace, 16) && a->workspace_bytes >= need, "pt_kv8_attn: %zu workspace bytes (on a multiple of 16) are wanted, got %zu", need,
              a->workspace ? a->workspace_bytes : 0);
-  const int es = kv8::elem_bytes(a->dtype);
   kv8::Split sp{};
   sp.chunks = ceil_div(a->n_head / a->cache.n_kv, kv8::HEADS);
   sp.dtype = a->dtype;

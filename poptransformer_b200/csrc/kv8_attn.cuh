@@ -9,7 +9,9 @@
 // these 6.5), and are read as fragments: a lane has 16 bytes of two key rows (row of the fragment), 16
 // bytes of four value rows (its keys).  Which dimension of the head is which k of an instruction does not matter as long as K and q agree: a lane's k are the dimensions of
 // its bytes.  Keys of int8 are multiplied as they are, with q in three parts of 8 bits (m16n8k32, whole numbers); all other bytes become fp16, exactly: E4M3 by conversion, int8 b as
-// (1024 + 128 + b) - 1152.  (Both at fp16 a tile of 32 keys took 270 cycles of an SM, 350 is what its bytes take to come.)
+// (1024 + 128 + b) - 1152.
+// Bound by memory: 48 sequences of up to 8000 positions, 32 query over 8 kv heads of 128, 519 MB, 98 us, 5.3 TB/s; 7 TB/s from a block's first tile to its last, 780 instructions a tile of 32
+// positions, which is half of the issue slots.  Two sequences of 100,000, E4M3: 78 us.  One of 700: 10.3 us, latency.
 //
 // Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), with PARTS = 2 a second part of what is
 // left: what is lost lies below 2^-25 of the largest.

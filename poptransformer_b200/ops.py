@@ -906,6 +906,8 @@ def rope_table(positions, dims, base=10000.0, scaling=None, device="cuda"):
       "bands":  pairs that turn less than `low` times over `original` are divided by `factor`, those that turn more than `high` times are left, in proportion to their turns between."""
     if dims <= 0 or dims % 2 or positions <= 0:
         raise PtError(f"rope_table: {positions} positions of {dims} dimensions (an even number)")
+    if base <= 0 or any(not float(v) > 0 for k, v in (scaling or {}).items() if k != "kind"):
+        raise PtError(f"rope_table: base {base} and scaling {scaling} are positive")
     kind, s, magnitude = (scaling or {}).get("kind"), dict(scaling or {}), 1.0
     i = torch.arange(dims // 2, dtype=torch.float64, device=device)
     try:
@@ -987,7 +989,7 @@ def rotary(x, heads, dim, rope, positions, out=None, rope_dims=None, interleaved
 def _kv8(cache, who):
     """The structure of a cache of eight bits.  (Made once: its tensors are the same from call to call.)"""
     pool, scales, table, made = cache.pool, cache.scales, cache.page_table, cache.kv8
-    if made is not None and made[0] is pool and made[1] is scales and made[2] is table:
+    if made is not None and made[0] is pool and made[1] is scales and made[2] is table and made[4] == (pool.data_ptr(), scales.data_ptr(), table.data_ptr()):
         return made[3]
     fmt = KV8_FORMATS.get(pool.dtype)
     if fmt is None:
@@ -997,7 +999,7 @@ def _kv8(cache, who):
     if not pool.get_device() == scales.get_device() == table.get_device():
         raise PtError(f"{who}: pool on {pool.device}, scales on {scales.device}, page table on {table.device}")
     made = Kv8Cache(_ptr(pool), _ptr(scales), _ptr(table), fmt, cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len)
-    cache.kv8 = (pool, scales, table, made)
+    cache.kv8 = (pool, scales, table, made, (made.pool, made.scales, made.page_table))
     return made
 
 

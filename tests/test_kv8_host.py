@@ -116,6 +116,34 @@ def test_bad_arguments():
         assert "pt_rotary" in refused(L.pt_rotary, make(**kw)), kw
 
 
+def test_outputs_that_others_still_read_are_refused():
+    """An output is the input itself, columns of the same wider rows that are none of the input's, or memory of its own."""
+    L = _lib.lib()
+    d = dict(rows=5, heads=2, dim=64, dtype=0, x=1 << 20, x_ld=400, out=1 << 20, out_ld=400, position=4096, positions=10, rope_dims=64, interleaved=0, inverse=0, rope=4096, error_flag=None)
+    make = lambda **kw: _lib.RotaryArgs(*[{**d, **kw}[n] for n, _ in _lib.RotaryArgs._fields_])
+    for off, ld in ((2, 400), (254, 400), (2 * 300, 400), (-2, 400), (1, 400), (0, 404), (2 * 128, 401), (2 * 800 + 2, 400)):
+        assert "apart" in refused(L.pt_rotary, make(out=(1 << 20) + off, out_ld=ld)), (off, ld)
+    for off, ld in ((0, 400), (256, 400), (2 * 272, 400), (-256, 400), (2 * (4 * 400 + 128), 500), (-2 * (4 * 130 + 128), 130)):      # (these pass, and the next check refuses them: nothing is launched)
+        assert "0 positions" in refused(L.pt_rotary, make(out=(1 << 20) + off, out_ld=ld, positions=0)), (off, ld)
+    at = 1 << 20                                    # q | k | v: 2, 2 and 2 heads of 64 in rows of 384
+    rows = dict(of=view(n_tok=3), q=at, k=at + 256, v=at + 512, ld=384, q_out_ld=384)
+    for off in (2, 256, 512, 700, -2):
+        assert "apart" in refused(L.pt_kv8_append, append_args(**rows, q_out=at + off)), off
+    assert "apart" in refused(L.pt_kv8_append, append_args(**{**rows, "q_out_ld": 200}, q_out=at))
+    for kw in (dict(q_out=at), dict(q_out=at + 2 * 3 * 384), dict(q_out=at - 2 * 3 * 384)):
+        assert "rotated dimensions" in refused(L.pt_kv8_append, append_args(**{**rows, **kw}, rope_dims=3)), kw
+    assert "apart" in refused(L.pt_kv8_attn, attn_args(of=view(n_tok=3), q=at, out=at + 2))
+    assert "apart" in refused(L.pt_kv8_attn, attn_args(at=kv8(vdim=32), of=view(n_tok=3), q=at, out=at))
+    assert "workspace" in refused(L.pt_kv8_attn, attn_args(of=view(n_tok=3), q=at, out=at))
+
+
+def test_batches_without_tokens():
+    L = _lib.lib()
+    empty = view(n_tok=0, tok_seq=None)
+    for fn, args in ((L.pt_kv8_append, append_args(of=empty)), (L.pt_kv8_attn, attn_args(of=empty, q=4096, out=8192))):
+        assert fn(ctypes.byref(args), None) == 0
+
+
 # ------------------------------------------------------------------------------------------ tables of angles
 def test_rope_table():
     t = ops.rope_table(1000, 64, device="cpu")
@@ -156,7 +184,8 @@ def test_bands_are_those_of_the_decoders():
 
 
 def test_tables_that_are_refused():
-    for args, kw in (((0, 8), {}), ((8, 7), {}), ((8, 0), {}), ((8, 8), dict(scaling=dict(kind="no"))), ((8, 8), dict(scaling=dict(kind="linear"))), ((8, 8), dict(scaling=dict(factor=2.0))),
+    for args, kw in (((8, 8), dict(base=0.0)), ((8, 8), dict(scaling=dict(kind="linear", factor=0.0))), ((8, 8), dict(scaling=dict(kind="ramp", factor=2.0, original=-5))),
+                     ((0, 8), {}), ((8, 7), {}), ((8, 0), {}), ((8, 8), dict(scaling=dict(kind="no"))), ((8, 8), dict(scaling=dict(kind="linear"))), ((8, 8), dict(scaling=dict(factor=2.0))),
                      ((8, 2), dict(scaling=dict(kind="base", factor=2.0))), ((8, 8), dict(scaling=dict(kind="bands", factor=2.0, original=8, low=1)))):
         with pytest.raises(PtError):
             ops.rope_table(*args, device="cpu", **kw)
