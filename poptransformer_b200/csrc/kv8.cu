@@ -488,6 +488,7 @@ extern "C" int pt_rotary(const pt_rotary_args *a, void *stream) {
   PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_rotary: type %d", a->dtype);
   PT_REQUIRE(a->rows >= 0 && a->heads > 0 && a->heads <= 65535 && a->dim > 0 && a->dim <= kv8::MOST_DIM, "pt_rotary: %d rows of %d heads of %d (heads of 1 .. %d)", a->rows, a->heads, a->dim,
              kv8::MOST_DIM);
+  if (a->rows == 0) return PT_OK;
   PT_REQUIRE(a->x && a->out && a->position, "pt_rotary: null pointer argument");
   PT_REQUIRE(a->x_ld >= (long long)a->heads * a->dim && a->out_ld >= (long long)a->heads * a->dim, "pt_rotary: rows of %d and %d elements, %d heads of %d", a->x_ld, a->out_ld, a->heads, a->dim);
   const int es = kv8::elem_bytes(a->dtype);
@@ -496,7 +497,6 @@ extern "C" int pt_rotary(const pt_rotary_args *a, void *stream) {
              a->x_ld, a->out_ld);
   PT_REQUIRE(a->positions > 0 && a->rope_dims > 0, "pt_rotary: %d rotated dimensions, a table of %d positions", a->rope_dims, a->positions);
   if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->dim, "pt_rotary")) return rc;
-  if (a->rows == 0) return PT_OK;
   PT_REQUIRE((long long)a->rows * a->heads < (1ll << 30), "pt_rotary: %d rows of %d heads", a->rows, a->heads);
   const bool whole = a->dim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->x, 16) && aligned_to(a->out, 16) && (long long)a->x_ld * es % 16 == 0 && (long long)a->out_ld * es % 16 == 0;
   const kv8::Rotary p{a->rows, a->heads, a->dim, a->rope_dims, a->x_ld, a->out_ld, a->positions, a->position, (const float2 *)a->rope, a->error_flag, kv8::Divide::by(a->heads)};
@@ -513,6 +513,7 @@ extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
   PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_append: type %d", a->dtype);
   if (int rc = kv8::check_batch(a->batch, "pt_kv8_append")) return rc;
   if (int rc = kv8::check_cache(a->cache, "pt_kv8_append")) return rc;
+  if (a->batch.n_tok == 0) return PT_OK;       // (tensors without elements have no address)
   PT_REQUIRE(a->k && a->v && a->ld > 0, "pt_kv8_append: null pointer argument, or rows of %d elements", a->ld);
   PT_REQUIRE(!a->q_out || (a->q && a->n_head > 0 && a->q_out_ld >= (long long)a->n_head * a->cache.dim), "pt_kv8_append: q_out wants q and rows of %d heads of %d, got %d elements", a->n_head,
              a->cache.dim, a->q_out_ld);
@@ -526,7 +527,6 @@ extern "C" int pt_kv8_append(const pt_kv8_append_args *a, void *stream) {
   if (int rc = kv8::check_rope(a->rope, a->rope_dims, a->cache.dim, "pt_kv8_append")) return rc;
   PT_REQUIRE((long long)a->batch.n_tok * ((a->q_out ? a->n_head : 0) + 2ll * a->cache.n_kv) < (1ll << 30), "pt_kv8_append: %d tokens of %d and %d heads", a->batch.n_tok, a->n_head,
              a->cache.n_kv);
-  if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Append p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->q_out ? a->n_head : 0, a->rope_dims, a->ld, a->q_out_ld, (const float2 *)a->rope, a->error_flag,
                       kv8::Divide::by(a->cache.page_size), {}, {}, 0, 0};
   const bool whole = a->cache.dim % 16 == 0 && a->cache.vdim % 16 == 0 && a->rope_dims % 16 == 0 && aligned_to(a->rope, 16) && aligned_to(a->cache.pool, 16) && aligned_to(a->k, 16) && aligned_to(a->v, 16) &&
@@ -567,6 +567,7 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_attn: type %d", a->dtype);
   if (int rc = kv8::check_batch(a->batch, "pt_kv8_attn")) return rc;
   if (int rc = kv8::check_cache(a->cache, "pt_kv8_attn")) return rc;
+  if (a->batch.n_tok == 0) return PT_OK;
   PT_REQUIRE(a->q && a->out, "pt_kv8_attn: null pointer argument");
   PT_REQUIRE(a->n_head > 0 && a->n_head <= 65535 && a->n_head % a->cache.n_kv == 0, "pt_kv8_attn: %d heads over %d", a->n_head, a->cache.n_kv);
   PT_REQUIRE(a->q_ld >= (long long)a->n_head * a->cache.dim && a->out_ld >= (long long)a->n_head * a->cache.vdim, "pt_kv8_attn: rows of %d and %d elements, %d heads of %d and %d", a->q_ld,
@@ -578,7 +579,6 @@ extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
   PT_REQUIRE(a->window >= 0, "pt_kv8_attn: window=%d", a->window);
   PT_REQUIRE(a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f), "pt_kv8_attn: softcap=%g (0, or 1e-20 .. 1e20)", (double)a->softcap);
   PT_REQUIRE(a->scale - a->scale == 0.f, "pt_kv8_attn: scale=%g", (double)a->scale);
-  if (a->batch.n_tok == 0) return PT_OK;
   const kv8::Attn p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->n_head, a->window, a->q_ld, a->out_ld, a->scale, a->softcap, a->error_flag};
   const cudaStream_t st = as_stream(stream);
   const int width = std::max(a->cache.dim, a->cache.vdim);

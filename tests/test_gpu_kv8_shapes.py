@@ -162,3 +162,38 @@ def test_queries_that_are_no_numbers(cuda, value, fmt):
         assert out[0, 1].isnan().all()
         want[0, 1] = out[0, 1] = 0
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("plain", [False, True])
+def test_outputs_in_the_place_of_queries(cuda, plain):
+    from poptransformer_b200 import ops
+    for qpk, lengths in ((4, [5000, 3, 700]), (12, [100, 9000])):
+        s = ku.cached(ku.batch([1] * len(lengths), lengths, torch.bfloat16, torch.int8, dim=128, n_kv=2, qpk=qpk, seed=7))
+        want = ku.attend(s, s.qkv, plain=plain).clone()
+        rows = s.qkv.clone()
+        ws = ops.kv8_attn_workspace(len(lengths), s.heads, 2, 128)
+        ops.kv8_attn(s.view, rows, s.ld, s.cache, rows, s.ld, s.heads, s.scale, workspace=ws, plain=plain)
+        assert torch.equal(rows[:, :s.q_cols], want) and torch.equal(rows[:, s.q_cols:], s.qkv[:, s.q_cols:])
+
+
+def test_rotation_into_other_columns_of_the_same_rows(cuda):
+    from poptransformer_b200 import ops
+    wide = torch.randn((70, 600), device=cuda)
+    before, rope, pos = wide.clone(), ops.rope_table(70, 64, device=cuda), torch.arange(70, dtype=torch.int32, device=cuda)
+    ops.rotary(wide[:, 16:272], 4, 64, rope, pos, out=wide[:, 300:556])
+    want = ku.rotate(before[:, 16:272].cpu().reshape(70, 4, 64), rope.cpu(), pos.cpu(), 64, False).flatten(1)
+    assert torch.equal(wide[:, 300:556].cpu(), want) and torch.equal(wide[:, :300], before[:, :300]) and torch.equal(wide[:, 556:], before[:, 556:])
+
+
+def test_a_batch_without_tokens(cuda):
+    """Nothing is appended or attended to; what is cached can be unpacked."""
+    from poptransformer_b200 import ops
+    s = ku.batch([0, 0], [70, 0], torch.bfloat16, torch.int8, dim=64, seed=8)
+    pool, scales = s.pool.clone(), s.scales.clone()
+    assert append(s).shape[0] == 0 and ku.attend(s, s.qkv).shape[0] == 0
+    into = ops.PagedKVCache(2, s.n_kv, 64, 128, 64, cuda, dtype=torch.bfloat16)
+    ops.kv8_unpack(s.view, s.cache, into, error_flag=s.flag)
+    x = ku.history(s, 0, 70, 0).float().bfloat16()
+    pages = into.page_table[s.slot_host[0]].long()
+    assert torch.equal(into.pool[pages, 0].transpose(0, 1).flatten(1, 2)[:, :70], x) and (into.pool[pages, 0].transpose(0, 1).flatten(1, 2)[:, 70:] == 0).all()
+    assert torch.equal(s.pool, pool) and torch.equal(s.scales.nan_to_num(-1), scales.nan_to_num(-1)) and s.flag.item() == 0
