@@ -921,7 +921,7 @@ int pt_kv_copy_pages(const pt_kv_pool *pools_host, int n_pools, int page_size, i
 int pt_kv_move_rows(const pt_kv_pool *pools_host, int n_pools, int page_size, int max_pages, const int32_t *page_table, const pt_batch_view *batch,
                     const int32_t *path, int path_ld, const int32_t *count, int32_t *error_flag, void *stream);
 
-/* ---- paged caches of eight bits (csrc/kv8.cu) ----------------------------------------------------------------------------
+/* ---- paged caches of eight bits (csrc/kv8.cu, csrc/kv8_attn.cu) ----------------------------------------------------------------------------
  * Keys and values as bytes with a scale for every position and head.  A page of the pool is K [n_kv][page_size][dim] and then V
  * [n_kv][page_size][vdim], a byte each; its scales are fp32 [2][n_kv][page_size], K's and then V's.  A row x of one position and head is
  * kept as  byte_i = round(x_i (top / m)),  scale = m / top,  with m = max |x_i|, at least 2^-64, and top 127 (int8, rounded to nearest even) or 448

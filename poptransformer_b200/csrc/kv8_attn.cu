@@ -1,4 +1,4 @@
-// Attention of new tokens over a cache of eight bits, on tensor cores (included by kv8.cu).
+// Attention of new tokens over a cache of eight bits (kv8.cuh), on tensor cores.
 //
 // A segment is one token, one kv head and up to eight of its query heads; its keys are tiles of KT positions.  All tiles of a launch lie in one row, segment
 // after segment; every block takes an equal run of them, and every warp an equal run of its block's, so that unequal histories cost nobody a wait and warps meet
@@ -18,13 +18,19 @@
 // With x = score log2(e), v_j = bytes times vs_j, and e_j about log2 vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
 // w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once for rows of bf16 (2^-11, an eighth of what their output is rounded by) and to two parts for others (2^-21), whole down to 2^-29 of the largest and then off by
 // 2^-40 of it, however far the scales of the values lie apart.
-#pragma once
-#include <type_traits>
-
+#include "kv8.cuh"
 #include "tile_math.cuh"
 
 namespace pt {
 namespace kv8 {
+
+struct Attn {
+  Batch b;
+  Cache c;
+  int heads, window, q_ld, out_ld;
+  float scale, softcap;
+  int *error_flag;
+};
 
 constexpr int HEADS = 8, MAX_TOKENS = 1024;
 constexpr int SHORT = 3;      // tiles of a warp up to which a segment stays in one block (32 query over 8 kv heads of 128, one token: 700 positions 10.2 us so, 13.0 dealt out; 1300 13.7 either way)
@@ -781,5 +787,153 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
   }
 }
 
+// Any sizes (and 54 times the time of the tensor cores' on 48 sequences of up to 8000 positions): a block per token and head, whose warps take every fourth key each with a running maximum and sum, lanes across the dimensions.
+constexpr int PLAIN_WARPS = 4;
+template <typename T, bool E4M3> __global__ void __launch_bounds__(PLAIN_WARPS * 32) attn_plain_kernel(const T *q, T *out, const Attn p) {
+  early_start();
+  __shared__ float top[PLAIN_WARPS], total[PLAIN_WARPS], sums[PLAIN_WARPS][MOST_DIM];
+  const int tok = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.c.n_kv, g = head / (p.heads / G);
+  if (tok >= p.b.cu[p.b.n_seq]) return;
+  const int seq = p.b.tok_seq[tok], first = p.b.cu[seq], start = p.b.start[seq];
+  if (!in_table(p.c, start, p.b.cu[seq + 1] - first)) {
+    if (threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+    return;
+  }
+  const int pos = start + tok - first, from = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int *table = p.c.page_table + (size_t)p.b.slot[seq] * p.c.max_pages;
+  constexpr int PER = MOST_DIM / 32;
+  float x[PER], o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = lane + 32 * i;
+    x[i] = d < p.c.dim ? to_f(q[(size_t)tok * p.q_ld + (size_t)head * p.c.dim + d]) : 0.f;
+    o[i] = 0.f;
+  }
+  for (int j = from + warp; j <= pos; j += PLAIN_WARPS) {
+    int page = table[j / p.c.page];
+    if (page < 0) {
+      if (lane == 0 && p.error_flag) atomicExch(p.error_flag, 12);
+      page = 0;
+    }
+    const size_t row = (size_t)g * p.c.page + j % p.c.page, at = (size_t)page * 2 * G * p.c.page + row;
+    const unsigned char *k = p.c.pool + (size_t)page * p.c.page_bytes + row * p.c.dim, *v = p.c.pool + (size_t)page * p.c.page_bytes + (size_t)G * p.c.page * p.c.dim + row * p.c.vdim;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.c.dim) s = fmaf(x[i], from_byte<E4M3>(k[lane + 32 * i]), s);
+    s = warp_sum(s) * (p.c.scales[at] * p.scale);
+    if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
+    const float t = fmaxf(m, s), was = m == t ? 1.f : expf(m - t), w = expf(s - (t == -INFINITY ? 0.f : t)), wv = w * p.c.scales[at + (size_t)G * p.c.page];
+    m = t;
+    l = l * was + w;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < p.c.vdim) o[i] = o[i] * was + wv * from_byte<E4M3>(v[lane + 32 * i]);
+  }
+  if (lane == 0) { top[warp] = m; total[warp] = l; }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sums[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  float most = top[0], whole = 0.f, share[PLAIN_WARPS];
+#pragma unroll
+  for (int w = 1; w < PLAIN_WARPS; ++w) most = fmaxf(most, top[w]);
+#pragma unroll
+  for (int w = 0; w < PLAIN_WARPS; ++w) {
+    share[w] = total[w] == 0.f ? 0.f : expf(top[w] - most);
+    whole += total[w] * share[w];
+  }
+  for (int d = threadIdx.x; d < p.c.vdim; d += PLAIN_WARPS * 32) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < PLAIN_WARPS; ++w) y += total[w] == 0.f ? 0.f : sums[w][d] * share[w];
+    out[(size_t)tok * p.out_ld + (size_t)head * p.c.vdim + d] = from_f<T>(y / whole);
+  }
+}
+
+template <typename T> static cudaError_t launch_plain(const pt_kv8_attn_args &a, const Attn &p, cudaStream_t st) {
+  const auto kernel = a.cache.fmt == PT_KV8_E4M3 ? attn_plain_kernel<T, true> : attn_plain_kernel<T, false>;
+  return launch_early(kernel, Grid(dim3(a.batch.n_tok, a.n_head)), PLAIN_WARPS * 32, 0, st, (const T *)a.q, (T *)a.out, p);
+}
+// A workspace: counters, then (by the width of the heads) pieces of every block.
+static size_t workspace_bytes(int width) {
+  const size_t pieces = width > 128 ? (Shape<256>::WARPS + 2) * Shape<256>::PIECE : width > 64 ? (Shape<128>::WARPS + 2) * Shape<128>::PIECE : (Shape<64>::WARPS + 2) * Shape<64>::PIECE;
+  return sizeof(int) * COUNTERS + sizeof(float) * sm_count() * pieces;
+}
+template <int SIZE, bool FULL> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
+  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype != PT_DT_BF16;      // (weights in two fp16 parts: one would double the error of an fp16 output)
+  const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, FULL, true, 2> : attn_kernel<SIZE, FULL, true, 1>) : (wide ? attn_kernel<SIZE, FULL, false, 2> : attn_kernel<SIZE, FULL, false, 1>);
+  static std::atomic<uint64_t> allowed[4];
+  constexpr int WARPS = Shape<SIZE>::WARPS, FIXED = WARPS * Shape<SIZE>::RING;
+  const cudaError_t e = allow_smem(kernel, FIXED + (3 * MAX_TOKENS + 1) * (int)sizeof(int), allowed[2 * e4m3 + wide]);
+  if (e != cudaSuccess) return e;
+  return launch_early(kernel, Grid(sp.grid), WARPS * 32, FIXED + (3 * sp.tokens + 1) * sizeof(int), st, p, sp);
+}
+template <int SIZE> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, Split sp, cudaStream_t st) {
+  sp.parts = sp.heads + (size_t)sp.grid * Shape<SIZE>::WARPS * Shape<SIZE>::PIECE;
+  return p.c.dim == SIZE && p.c.vdim == SIZE ? launch_attn<SIZE, true>(a, p, sp, st) : launch_attn<SIZE, false>(a, p, sp, st);
+}
+
 }  // namespace kv8
 }  // namespace pt
+
+using namespace pt;
+
+extern "C" size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width) { return n_tok < 1 || n_kv < 1 || n_head < n_kv ? 0 : kv8::workspace_bytes(width); }
+
+extern "C" int pt_kv8_attn(const pt_kv8_attn_args *a, void *stream) {
+  PT_REQUIRE(a, "pt_kv8_attn: null args");
+  PT_REQUIRE(a->dtype == PT_DT_F16 || a->dtype == PT_DT_BF16 || a->dtype == PT_DT_F32, "pt_kv8_attn: type %d", a->dtype);
+  if (int rc = kv8::check_batch(a->batch, "pt_kv8_attn")) return rc;
+  if (int rc = kv8::check_cache(a->cache, "pt_kv8_attn")) return rc;
+  if (a->batch.n_tok == 0) return PT_OK;
+  PT_REQUIRE(a->q && a->out, "pt_kv8_attn: null pointer argument");
+  PT_REQUIRE(a->n_head > 0 && a->n_head <= 65535 && a->n_head % a->cache.n_kv == 0, "pt_kv8_attn: %d heads over %d", a->n_head, a->cache.n_kv);
+  PT_REQUIRE(a->q_ld >= (long long)a->n_head * a->cache.dim && a->out_ld >= (long long)a->n_head * a->cache.vdim, "pt_kv8_attn: rows of %d and %d elements, %d heads of %d and %d", a->q_ld,
+             a->out_ld, a->n_head, a->cache.dim, a->cache.vdim);
+  const int es = kv8::elem_bytes(a->dtype);
+  PT_REQUIRE((a->q == a->out && a->q_ld == a->out_ld && a->cache.dim == a->cache.vdim) || kv8::apart(a->q, a->q_ld, (long long)a->n_head * a->cache.dim, a->out, a->out_ld, (long long)a->n_head * a->cache.vdim,
+                                                                                                      a->batch.n_tok, es),
+             "pt_kv8_attn: out is q itself (with its stride and width) or apart from it");
+  PT_REQUIRE(a->window >= 0, "pt_kv8_attn: window=%d", a->window);
+  PT_REQUIRE(a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f), "pt_kv8_attn: softcap=%g (0, or 1e-20 .. 1e20)", (double)a->softcap);
+  PT_REQUIRE(a->scale - a->scale == 0.f, "pt_kv8_attn: scale=%g", (double)a->scale);
+  const kv8::Attn p{kv8::batch_of(a->batch), kv8::cache_of(a->cache), a->n_head, a->window, a->q_ld, a->out_ld, a->scale, a->softcap, a->error_flag};
+  const cudaStream_t st = as_stream(stream);
+  const int width = std::max(a->cache.dim, a->cache.vdim);
+  // (16 bytes of a row a lane, 16 positions of a page a group)
+  if (a->plain || a->cache.dim % 16 || a->cache.vdim % 16 || a->cache.page_size % 16 || !aligned_to(a->cache.pool, 16)) {
+    PT_CUDA(a->dtype == PT_DT_F32   ? kv8::launch_plain<float>(*a, p, st)
+            : a->dtype == PT_DT_F16 ? kv8::launch_plain<__half>(*a, p, st)
+                                    : kv8::launch_plain<__nv_bfloat16>(*a, p, st));
+    PT_LAUNCH_CHECK("pt_kv8_attn");
+    return PT_OK;
+  }
+  const size_t need = pt_kv8_attn_workspace_bytes(a->batch.n_tok, a->n_head, a->cache.n_kv, width);
+  PT_REQUIRE(a->workspace && aligned_to(a->workspace, 16) && a->workspace_bytes >= need, "pt_kv8_attn: %zu workspace bytes (on a multiple of 16) are wanted, got %zu", need,
+             a->workspace ? a->workspace_bytes : 0);
+  kv8::Split sp{};
+  sp.chunks = ceil_div(a->n_head / a->cache.n_kv, kv8::HEADS);
+  sp.dtype = a->dtype;
+  sp.q_whole = aligned_to(a->q, 16) && (long long)a->q_ld * es % 16 == 0;
+  sp.out_whole = aligned_to(a->out, 16) && (long long)a->out_ld * es % 16 == 0;
+  sp.counters = (int *)a->workspace;
+  sp.heads = (float *)(sp.counters + kv8::COUNTERS);
+  sp.q = a->q;
+  sp.out = a->out;
+  sp.grid = sm_count();
+  sp.segs = a->cache.n_kv * sp.chunks;
+  sp.by_segs = kv8::Divide::by(sp.segs);
+  sp.by_chunks = kv8::Divide::by(sp.chunks);
+  sp.by_page = kv8::Divide::by(p.c.page);
+  sp.by_grid = kv8::Divide::by(sp.grid);
+  // Tokens of a launch: what its blocks plan in shared memory, a counter for every segment, and tiles that an int counts.
+  const long long segs = (long long)a->cache.n_kv * sp.chunks, tiles = segs * (ceil_div(p.c.max_len, 16) + 1);
+  PT_REQUIRE(tiles < 1ll << 30, "pt_kv8_attn: %lld heads of a history of %d positions", segs, p.c.max_len);
+  const int most = (int)std::min<long long>({kv8::MAX_TOKENS, kv8::COUNTERS / segs, (1ll << 30) / tiles});
+  for (; sp.tok0 < a->batch.n_tok; sp.tok0 += most) {
+    sp.tokens = std::min(a->batch.n_tok - sp.tok0, most);
+    PT_CUDA(width > 128 ? kv8::launch_attn<256>(*a, p, sp, st) : width > 64 ? kv8::launch_attn<128>(*a, p, sp, st) : kv8::launch_attn<64>(*a, p, sp, st));
+    PT_LAUNCH_CHECK("pt_kv8_attn");
+  }
+  return PT_OK;
+}
