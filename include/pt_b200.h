@@ -974,7 +974,8 @@ int pt_kv8_append(const pt_kv8_append_args *args, void *stream);
 
 /* pt_kv8_attn: token i of sequence s attends to the cached positions up to its own, start[s] + i (which pt_kv8_append has written): out[h] = sum_j w_j v_j,
  * w = softmax(c(scale q[h] . k_j)) over the last `window` of them (0: all); softcap c: a score x becomes c tanh(x / c) (0: none).  out may be q itself where keys and values are equally wide.  Meant for few tokens a
- * sequence: every token reads its history by itself.  A negative page reads as some other page, and sets error_flag to 12. */
+ * sequence: every token reads its history by itself.  A negative page reads as some other page, and sets error_flag to 12, unless all
+ * of its positions lie in front of the window: those pages may be gone. */
 typedef struct pt_kv8_attn_args {
   pt_batch_view batch;
   pt_kv8_cache cache;

@@ -384,8 +384,9 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
           for (int u = 0; u < GROUPS; ++u) {
             int page = __shfl_sync(0xffffffffu, page_l, at + u);
             const int row = __shfl_sync(0xffffffffu, row_l, at + u);
-            if (page < 0) {
-              if (p.error_flag) atomicExch(p.error_flag, 12);
+            if (page < 0) {        // (one whose positions lie in front of the window may be gone: a tile has others of its own, and masks these)
+              const int pos = pl.pos[ahead.tok], begin = p.window > 0 ? max(0, pos - p.window + 1) : 0, at0 = (begin / KT + ahead.tile) * KT + 16 * u;
+              if (at0 + 15 >= begin && p.error_flag) atomicExch(p.error_flag, 12);
               page = 0;
             }
             const unsigned char *base = p.c.pool + (size_t)page * p.c.page_bytes, *k = base + (k_l + row * dim), *v = base + (v_l + row * vdim);

@@ -197,3 +197,20 @@ def test_a_batch_without_tokens(cuda):
     pages = into.page_table[s.slot_host[0]].long()
     assert torch.equal(into.pool[pages, 0].transpose(0, 1).flatten(1, 2)[:, :70], x) and (into.pool[pages, 0].transpose(0, 1).flatten(1, 2)[:, 70:] == 0).all()
     assert torch.equal(s.pool, pool) and torch.equal(s.scales.nan_to_num(-1), scales.nan_to_num(-1)) and s.flag.item() == 0
+
+
+@pytest.mark.parametrize("plain", [False, True])
+@pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 32), (256, 16), (96, 48)])
+def test_pages_in_front_of_the_window_may_be_gone(cuda, dim, page, fmt, plain):
+    """Pages whose positions all lie in front of every token's window are negative: the same outputs, and no error; with one page more gone there is one."""
+    counts, starts, window = [1, 1, 3, 1], [300, 60, 777, 1023], 50
+    s = ku.cached(ku.batch(counts, starts, torch.bfloat16, fmt, dim=dim, page=page, seed=dim + page))
+    want = ku.attend(s, s.qkv, window=window, plain=plain).clone()
+    gone = [max(0, n - window + 1) // page for n in starts]
+    for i, n in enumerate(gone):
+        s.page_table[s.slot_host[i], :n] = -1
+    assert torch.equal(ku.attend(s, s.qkv, window=window, plain=plain), want) and s.flag.item() == 0
+    s.page_table[s.slot_host[2], gone[2]] = -1
+    ku.attend(s, s.qkv, window=window, plain=plain)
+    assert s.flag.item() == 12
