@@ -10,14 +10,16 @@
 // bytes of four value rows (its keys).  Which dimension of the head is which k of an instruction does not matter as long as K and q agree: a lane's k are the dimensions of
 // its bytes.  Keys of int8 are multiplied as they are, with q in three parts of 8 bits (m16n8k32, whole numbers); all other bytes become fp16, exactly: E4M3 by conversion, int8 b as
 // (1024 + 128 + b) - 1152.
-// Bound by memory: 48 sequences of up to 8000 positions, 32 query over 8 kv heads of 128, 519 MB, 98 us, 5.3 TB/s; 7 TB/s from a block's first tile to its last, 780 instructions a tile of 32
-// positions, which is half of the issue slots.  Two sequences of 100,000, E4M3: 78 us.  One of 700: 10.3 us, latency.
+// Bound by memory: 48 sequences of up to 8000 positions, 32 query over 8 kv heads of 128, 519 MB, 96 us, 5.4 TB/s (105 in a long run of such calls, when the power limit
+// takes the clock from 1965 MHz to about 1700); 7 TB/s from a block's first tile to its last, 820 instructions a tile of 32 positions, which is half of the issue slots.  Two sequences of 100,000, E4M3: 79 us.
+// One of 700: 10.2 us, latency.
 //
-// Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), with PARTS = 2 a second part of what is
-// left: what is lost lies below 2^-25 of the largest.
+// Numbers.  int8: q to 2^-22 of its row's largest element.  E4M3: q in fp16 times a power of two that brings its row's largest element to [1, 2), and for rows that are not bf16 a second part of
+// what is left: what is lost lies below 2^-25 of the largest.
 // With x = score log2(e), v_j = bytes times vs_j, and e_j about log2 vs_j, a segment keeps R = max (x_j + e_j), l = sum 2^(x_j - R + 14) in 32 bits, and sums
-// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15: rounded to fp16 once for rows of bf16 (2^-11, an eighth of what their output is rounded by) and to two parts for others (2^-21), whole down to 2^-29 of the largest and then off by
-// 2^-40 of it, however far the scales of the values lie apart.
+// w_j (bytes of v_j) with w_j = 2^(x_j - R + 14) vs_j, below 2^15, in two fp16 parts: 2^-21 of a weight, whole down to 2^-29 of the largest and then off by
+// 2^-40 of it, however far the scales of the values lie apart.  (One part, 2^-11, for rows of bf16 moved outputs to the neighbouring number, 0.0011 of
+// their size altogether where two parts are 0.0001 from the plain form.  It took 98 us for the 48 sequences, 100 in a long run, where it needs less power; two parts 96 and 105.  Long sequences: 78.2, 78.6.)
 #include "kv8.cuh"
 #include "tile_math.cuh"
 
@@ -223,12 +225,12 @@ __device__ __forceinline__ Walk walk_to(int at, const Plan &pl, int segs, const 
   return w;
 }
 
-// FULL: keys and values are as wide as SIZE.  PARTS: fp16 parts of the weights (and of the queries that are fp16): 1 for rows of bf16, 2 for others.
-template <int SIZE, bool FULL, bool E4M3, int PARTS>
+// FULL: keys and values are as wide as SIZE.  QUERY_PARTS: fp16 parts of queries over E4M3 keys: 1 for rows of bf16, which have eight bits, 2 for others.
+template <int SIZE, bool FULL, bool E4M3, int QUERY_PARTS>
 __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const Attn p, const Split sp) {
   early_start();
   using S = Shape<SIZE>;
-  constexpr int QPARTS = E4M3 ? PARTS : 3, QREGS = E4M3 ? 2 : 1, NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
+  constexpr int QPARTS = E4M3 ? QUERY_PARTS : 3, QREGS = E4M3 ? 2 : 1, NW = S::WARPS, KT = S::KT, GROUPS = S::GROUPS, STAGES = S::STAGES, NK = S::NK, NV = S::NV, VB = S::VB, MT = S::MT;
   extern __shared__ __align__(128) unsigned char smem[];
   // The pieces of segments that warps begin and end with: which segments, and (R, l) of every head.
   __shared__ int scan[NW], widest[NW], front[NW], rear[NW], first_block[2], parts[2];
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
 #pragma unroll
       for (int j = 0; j < MT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.f;
       // q as B operand: lane (g, tg) holds head g's dimensions 64 i + 16 tg + .. of the byte runs that it reads of the keys.  int8: three parts of 8 bits of (127 2^14 / the row's largest) q;
-      // E4M3: fp16, after a power of two, in PARTS parts.
+      // E4M3: fp16, after a power of two, in QPARTS parts.
       uint32_t qf[QPARTS][NK * 4][QREGS];
       float by[2];          // factors of the scores of heads 2 tg and 2 tg + 1
       {
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
               for (int o = 0; o < 2; ++o) {
                 const float a = __uint_as_float(x[i][4 * c + 2 * o]) * turn, b = __uint_as_float(x[i][4 * c + 2 * o + 1]) * turn;
                 qf[0][4 * i + c][o % QREGS] = pack2(a, b);
-                if constexpr (PARTS == 2) {
+                if constexpr (QPARTS == 2) {
                   const float2 h = unpack2(qf[0][4 * i + c][o % QREGS]);
                   qf[QPARTS - 1][4 * i + c][o % QREGS] = pack2(a - h.x, b - h.y);
                 }
@@ -582,15 +584,13 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
         }
 #pragma unroll
         for (int u = 0; u < GROUPS; ++u) {
-          uint32_t wf[PARTS][2];
+          uint32_t wf[2][2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const uint32_t hi = pack2(x[u][2 * r], x[u][2 * r + 1]);
             wf[0][r] = turn8x8(hi);
-            if constexpr (PARTS == 2) {
-              const float2 f = unpack2(hi);
-              wf[PARTS - 1][r] = turn8x8(pack2(x[u][2 * r] - f.x, x[u][2 * r + 1] - f.y));
-            }
+            const float2 f = unpack2(hi);
+            wf[1][r] = turn8x8(pack2(x[u][2 * r] - f.x, x[u][2 * r + 1] - f.y));
           }
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(Shape<SIZE>::WARPS * 32, 1) attn_kernel(const 
                 widen<E4M3>(v[0][k], v[1][k], half, a0, a1);
                 widen<E4M3>(v[2][k], v[3][k], half, a2, a3);
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) mma16816(O[i * 8 + 2 * k + half], a0, a1, a2, a3, wf[q][0], wf[q][1]);
+                for (int q = 0; q < 2; ++q) mma16816(O[i * 8 + 2 * k + half], a0, a1, a2, a3, wf[q][0], wf[q][1]);
               }
           }
         }
@@ -861,11 +861,11 @@ static size_t workspace_bytes(int width) {
   return sizeof(int) * COUNTERS + sizeof(float) * sm_count() * pieces;
 }
 template <int SIZE, bool FULL> static cudaError_t launch_attn(const pt_kv8_attn_args &a, const Attn &p, const Split &sp, cudaStream_t st) {
-  const bool e4m3 = a.cache.fmt == PT_KV8_E4M3, wide = a.dtype != PT_DT_BF16;      // (weights in two fp16 parts: one would double the error of an fp16 output)
-  const auto kernel = e4m3 ? (wide ? attn_kernel<SIZE, FULL, true, 2> : attn_kernel<SIZE, FULL, true, 1>) : (wide ? attn_kernel<SIZE, FULL, false, 2> : attn_kernel<SIZE, FULL, false, 1>);
-  static std::atomic<uint64_t> allowed[4];
+  const int which = a.cache.fmt != PT_KV8_E4M3 ? 0 : a.dtype == PT_DT_BF16 ? 1 : 2;
+  const auto kernel = which == 0 ? attn_kernel<SIZE, FULL, false, 1> : which == 1 ? attn_kernel<SIZE, FULL, true, 1> : attn_kernel<SIZE, FULL, true, 2>;
+  static std::atomic<uint64_t> allowed[3];
   constexpr int WARPS = Shape<SIZE>::WARPS, FIXED = WARPS * Shape<SIZE>::RING;
-  const cudaError_t e = allow_smem(kernel, FIXED + (3 * MAX_TOKENS + 1) * (int)sizeof(int), allowed[2 * e4m3 + wide]);
+  const cudaError_t e = allow_smem(kernel, FIXED + (3 * MAX_TOKENS + 1) * (int)sizeof(int), allowed[which]);
   if (e != cudaSuccess) return e;
   return launch_early(kernel, Grid(sp.grid), WARPS * 32, FIXED + (3 * sp.tokens + 1) * sizeof(int), st, p, sp);
 }
