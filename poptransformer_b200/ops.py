@@ -452,7 +452,7 @@ def window_attn(view, qkv, qkv_ld, cache, out, out_ld, n_head, scale, window=0, 
     (a layer that reads another layer's cache).  q_norm, k_norm, rope: per-head norm and rotation of q and k; q is then rewritten.  gate: rows
     whose sigmoid multiplies the output (a view that starts at its first column).  context: an object with k, v, shared, ld, shared_dim
     and cu that names rows of the whole context as keys and values of a prompt, in place of the cache's pages (see pt_context_rows)."""
-    _wide(cache, "window_attn")
+    _wide(cache, "window_attn", qkv.element_size())
     a = WindowAttnArgs()
     a.batch, a.dtype = view, dtype_code(qkv.dtype)
     a.n_head, a.n_kv, a.dim, a.vdim = n_head, cache.n_kv, cache.head_dim, cache.v_dim
@@ -545,8 +545,9 @@ def latent_cache(rows, w, max_len, page_size=64, device="cuda", page_table=None,
 def latent_prep(view, rows, ld, q_col, kv_col, w, cq, cq_ld, cache, eps, rope, error_flag=None):
     """Norms of both latents, rotation of the shared key part, append (see pt_latent_prep).  q_col, kv_col: first columns of the query latent
     and of [latent | key part] in `rows` (kv_col None: the layer reads what another one caches); w: an object with q_rank, rank, rot_dim and the fp32 tensors q_norm, kv_norm."""
-    a = LatentPrepArgs()
     es = rows.element_size()
+    _wide(cache, "latent_prep", es)
+    a = LatentPrepArgs()
     a.batch, a.dtype, a.q_rank, a.rank, a.rot_dim, a.eps = view, dtype_code(rows.dtype), w.q_rank, w.rank, w.rot_dim, float(eps)
     a.q, a.kv, a.ld = rows.data_ptr() + q_col * es, None if kv_col is None else rows.data_ptr() + kv_col * es, ld
     a.q_norm, a.kv_norm, a.rope, a.cq, a.cq_ld = _ptr(w.q_norm), None if kv_col is None else _ptr(w.kv_norm), _ptr(rope), _ptr(cq), cq_ld
@@ -557,6 +558,7 @@ def latent_prep(view, rows, ld, q_col, kv_col, w, cq, cq_ld, cache, eps, rope, e
 
 def latent_context(view, ctx_cu, n_ctx, w, cache, shared, latent, latent_ld):
     """The cached rows of every sequence's context, one after the other (see pt_latent_context)."""
+    _wide(cache, "latent_context", latent.element_size())
     a = LatentContextArgs()
     a.batch, a.ctx_cu, a.n_ctx, a.rot_dim, a.rank = view, _ptr(ctx_cu), n_ctx, w.rot_dim, w.rank
     a.page_size, a.max_pages, a.pool, a.page_table = cache.page_size, cache.page_table.shape[1], _ptr(cache.pool), _ptr(cache.page_table)
@@ -571,6 +573,7 @@ def latent_workspace_bytes(n_tok, w, dtype):
 def latent_attn(view, q, q_ld, w, cache, out, out_ld, scale, rope, workspace, gate=None, gate_ld=0, out_cols=0, error_flag=None, plain=False, gate_per_value=False):
     """Attention over the cached latents (see pt_latent_attn).  w: an object with heads, dim, rot_dim, vdim, rank and the tensors w_k [heads,
     rank, dim] and w_v [heads, vdim, rank].  gate: a view that starts at the heads' gates (gate_per_value: one per output)."""
+    _wide(cache, "latent_attn", q.element_size())
     a = LatentAttnArgs()
     a.batch, a.dtype, a.n_head, a.dim, a.rot_dim, a.vdim, a.rank, a.scale = view, dtype_code(q.dtype), w.heads, w.dim, w.rot_dim, w.vdim, w.rank, float(scale)
     a.q, a.q_ld, a.rope, a.w_k, a.w_v = _ptr(q), q_ld, _ptr(rope), _ptr(w.w_k), _ptr(w.w_v)
@@ -793,10 +796,12 @@ def kv_cache_pipeline(state, step, updater):
 
 
 # ------------------------------------------------------------------------------------------ paged cache + attention
-def _wide(cache, who):
-    """For what reads or writes a cache in the rows' type."""
+def _wide(cache, who, es=0):
+    """For what reads or writes a cache in the rows' type, whose elements have es bytes: a pool of smaller ones ends in front of its last pages."""
     if cache.scales is not None:
         raise PtError(f"{who}: a cache of {cache.pool.dtype} is written by kv8_append and read by kv8_attn and kv8_unpack")
+    if cache.pool.element_size() < es:
+        raise PtError(f"{who}: a cache of {cache.pool.dtype} has elements of {cache.pool.element_size()} bytes, the rows' have {es}")
 
 
 class PagedKVCache:
@@ -845,7 +850,7 @@ class PagedKVCache:
 
     def export(self, step, max_len):
         """Reference-layout view [2, rows, n_kv, max_len, head_dim], newest first, zeros beyond step."""
-        _wide(self, "export")
+        _wide(self, "export", 2)
         out = torch.empty((2, self.rows, self.n_kv, max_len, self.head_dim), dtype=torch.float16, device=self.pool.device)
         check(_lib.lib().pt_kv_export(_ptr(self.pool), _ptr(self.page_table), _ptr(step), self.rows, self.n_kv, self.head_dim,
                                       self.page_size, self.max_pages, max_len, _ptr(out), _stream()), "pt_kv_export")
@@ -1086,7 +1091,7 @@ def attn_workspace(batch, n_head, head_dim, max_pages, device="cuda"):
 
 def attn_args(qkv, step, cache, out, n_head, rope_mode, softmax_mode, score_scale, rope_sin, rope_cos, workspace, error_flag, pdl=0,
               out_fp8=None, out_fp8_scale=0.0):
-    _wide(cache, "kv_append_attn")
+    _wide(cache, "kv_append_attn", qkv.element_size())
     a = AttnArgs()
     a.batch, a.n_head, a.n_kv, a.head_dim = qkv.shape[0], n_head, cache.n_kv, cache.head_dim
     a.page_size, a.max_pages, a.rope_mode, a.softmax_mode = cache.page_size, cache.max_pages, rope_mode, softmax_mode
@@ -1117,7 +1122,7 @@ def prefill_attn(qkv, cache, batch, n_tokens, start, n_head, score_scale, rope_s
     """Causal attention over a whole prompt chunk (the reference's sequence_length != 1 attention, llama2/attention.py:64-114):
     qkv fp16 [batch * n_tokens, 3 * n_head * H], row b * n_tokens + t = position start + t of sequence b.  Rotates q in place,
     appends rotated k and v to the paged cache and returns softmax(q K^T * scale + causal mask) V, [batch * n_tokens, n_head * H]."""
-    _wide(cache, "prefill_attn")
+    _wide(cache, "prefill_attn", qkv.element_size())
     if qkv.shape != (batch * n_tokens, 3 * n_head * cache.head_dim) or cache.n_kv != n_head:
         raise PtError(f"prefill_attn: qkv {tuple(qkv.shape)} does not match batch={batch} n_tokens={n_tokens} n_head={n_head} (no grouped KV heads)")
     if out is None:
