@@ -798,7 +798,7 @@ def kv_cache_pipeline(state, step, updater):
 # ------------------------------------------------------------------------------------------ paged cache + attention
 def _wide(cache, who, es=0):
     """For what reads or writes a cache in the rows' type, whose elements have es bytes: a pool of smaller ones ends in front of its last pages."""
-    if cache.scales is not None:
+    if getattr(cache, "scales", None) is not None:      # (a caller's own class need not know them)
         raise PtError(f"{who}: a cache of {cache.pool.dtype} is written by kv8_append and read by kv8_attn and kv8_unpack")
     if cache.pool.element_size() < es:
         raise PtError(f"{who}: a cache of {cache.pool.dtype} has elements of {cache.pool.element_size()} bytes, the rows' have {es}")
@@ -869,12 +869,13 @@ class PagePools:
             if c.page_size != first.page_size or c.page_table is not first.page_table and (c.page_table.data_ptr(), c.page_table.shape) != (first.page_table.data_ptr(), first.page_table.shape):
                 raise PtError("PagePools: the caches share neither page size nor page table")
         self.pools = [c.pool for c in caches]      # (keeps them alive)
-        self.scales = [c.scales for c in caches if c.scales is not None]
+        scaled = [c for c in caches if getattr(c, "scales", None) is not None]
+        self.scales = [c.scales for c in scaled]
         self.page_size, self.page_table = first.page_size, first.page_table
         self.n_pages = min(t.shape[0] for t in self.pools)
         pools = [_lib.KvPool(_ptr(c.pool), c.n_kv, c.head_dim, c.v_dim, c.pool.element_size()) for c in caches]
         # Scales are pools of one fp32 value a position.  They have a launch of their own: the pools of a launch are copied in the unit that divides the rows of all of them.
-        small = [_lib.KvPool(_ptr(c.scales), c.n_kv, 1, 1, 4) for c in caches if c.scales is not None]
+        small = [_lib.KvPool(_ptr(c.scales), c.n_kv, 1, 1, 4) for c in scaled]
         self._pools = [(_lib.KvPool * len(p))(*p) for p in (pools, small) if p]
 
     def copy_pages(self, src, dst, error_flag=None):

@@ -1,8 +1,10 @@
 """Caches of eight bits and of other widths than the rows': what the calls beside them say before any launch."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from poptransformer_b200 import ops
+from poptransformer_b200 import _lib, ops
 from poptransformer_b200._lib import PtError
 
 
@@ -41,3 +43,33 @@ def test_a_pool_of_smaller_elements_than_the_rows_is_refused():
                 call()
     with pytest.raises(PtError, match="export.*elements of"):
         cache(torch.uint8).export(torch.zeros(1, dtype=torch.int32), 8)
+
+
+def test_cache_objects_of_a_callers_own_need_no_scales(monkeypatch):
+    """What the calls read of a cache of 16 or 32 bits is what they read before there were others."""
+    monkeypatch.setattr(ops, "_ptr", lambda t: None if t is None else t.data_ptr())
+
+    class Taken(Exception):
+        pass
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*args):
+                raise Taken(name)
+            return call
+
+    monkeypatch.setattr(ops._lib, "lib", Library)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    full = cache(torch.float16)
+    own = SimpleNamespace(**{n: getattr(full, n) for n in ("n_kv", "head_dim", "v_dim", "page_size", "max_pages", "max_len", "pool", "page_table")})
+    w = SimpleNamespace(q_rank=8, rank=8, rot_dim=8, dim=8, vdim=8, heads=2, q_norm=None, kv_norm=None, w_k=None, w_v=None)
+    view, step = _lib.BatchView(1, 1), torch.zeros(1, dtype=torch.int32)
+    wide = torch.zeros((1, 3 * 2 * 64), dtype=torch.float16)
+    for call, name in ((lambda: ops.window_attn(view, wide, 384, own, wide, 384, 2, 1.0), "pt_window_attn"), (lambda: ops.kv_append_attn(wide, step, own, 2, workspace=wide), "pt_kv_append_attn"),
+                       (lambda: ops.prefill_attn(wide, own, 1, 1, 0, 2, 1.0, None, None), "pt_prefill_attn"), (lambda: ops.tree_attn(view, wide, 384, own, wide, 384, 2, 1.0), "pt_tree_attn"),
+                       (lambda: ops.latent_prep(view, wide, 384, 0, 0, w, wide, 384, own, 0.0, None), "pt_latent_prep"),
+                       (lambda: ops.latent_context(view, step, 1, w, own, wide, wide, 384), "pt_latent_context"),
+                       (lambda: ops.latent_attn(view, wide, 384, w, own, wide, 384, 1.0, None, wide), "pt_latent_attn"),
+                       (lambda: ops.PagePools([own]).copy_pages(step, step), "pt_kv_copy_pages")):
+        with pytest.raises(Taken, match=name):
+            call()
