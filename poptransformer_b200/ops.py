@@ -810,7 +810,8 @@ class PagedKVCache:
     are handed out on demand (cache.SequenceSlots) instead of max_len tokens per row.
 
     dtype torch.int8 or torch.float8_e4m3fn: a cache of eight bits, with fp32 `scales` [pages, 2, n_kv, page_size] of every position and head (K's and
-    V's), which kv8_append writes and kv8_attn and kv8_unpack read; PagePools serves both kinds, the other kernels want caches of the rows' type."""
+    V's), which kv8_append writes and kv8_attn and kv8_unpack read; PagePools serves both kinds, the other kernels want caches of the rows' type.  Pages of bytes that
+    a program fills and reads by itself, of any widths and without scales, are torch.uint8: PagePools copies and moves them like the others."""
 
     def __init__(self, rows, n_kv, head_dim, max_len, page_size=64, device="cuda", page_table=None, extra_pages=0, v_dim=None, dtype=torch.float16,
                  n_pages=None, pool=None, scales=None):
@@ -835,9 +836,9 @@ class PagedKVCache:
         self.scales = self.kv8 = None
         if dtype in KV8_FORMATS:
             if not 1 <= min(head_dim, self.v_dim) <= max(head_dim, self.v_dim) <= 256:
-                raise PtError(f"PagedKVCache: eight bits want heads of 1 to 256 dimensions, got {head_dim} and {self.v_dim}")
+                raise PtError(f"PagedKVCache: eight bits want heads of 1 to 256 dimensions, got {head_dim} and {self.v_dim} (bytes of any kind, without scales, are a pool of torch.uint8)")
             if (scales is None) != (pool is None):
-                raise PtError("PagedKVCache: a pool of eight bits and its scales are given together")
+                raise PtError("PagedKVCache: a pool of eight bits and its scales are given together (bytes of any kind, without scales, are a pool of torch.uint8)")
             shape = (self.pool.shape[0], 2, n_kv, page_size)
             if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != shape or not scales.is_contiguous() or scales.device != self.pool.device):
                 raise PtError(f"PagedKVCache: scales {scales.dtype} {tuple(scales.shape)} on {scales.device}, expected contiguous float32 {shape} on {self.pool.device}")

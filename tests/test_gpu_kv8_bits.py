@@ -1,4 +1,4 @@
-"""Attention over caches of eight bits: outputs of 16 bits are the exact ones, rounded once, but for what sums in 32 bits lose."""
+"""Caches of eight bits: outputs of 16 bits are the exact ones, rounded once, but for what sums in 32 bits lose; pages of bytes without scales."""
 from types import SimpleNamespace
 
 import pytest
@@ -24,3 +24,14 @@ def test_rows_of_bf16_have_weights_of_more_bits_than_their_output(cuda, fmt, dim
     off = (out - want).abs()
     bad = off > tol + torch.finfo(torch.bfloat16).eps / 2 * want
     assert not bad.any(), (int(bad.sum()), bad.numel(), (off / want).max().item())
+
+
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (576, 0), (300, 17)])
+def test_pages_of_bytes_are_copied(cuda, dim, vdim):
+    from poptransformer_b200 import ops
+    kv = ops.PagedKVCache(2, 3, dim, 128, 64, cuda, v_dim=vdim, dtype=torch.uint8)
+    kv.pool.random_(0, 256)
+    want = kv.pool.clone()
+    want[3] = want[0]
+    ops.PagePools([kv]).copy_pages(ku.ints([0]), ku.ints([3]))
+    assert torch.equal(kv.pool, want)

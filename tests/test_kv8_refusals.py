@@ -73,3 +73,17 @@ def test_cache_objects_of_a_callers_own_need_no_scales(monkeypatch):
                        (lambda: ops.PagePools([own]).copy_pages(step, step), "pt_kv_copy_pages")):
         with pytest.raises(Taken, match=name):
             call()
+
+
+def test_pages_of_bytes_without_scales():
+    """A program's own bytes (any widths, no scales) are torch.uint8, and the refusals of eight bits say so."""
+    for dtype in (torch.int8, torch.float8_e4m3fn):
+        made = cache(dtype)
+        for kw in (dict(pool=made.pool), dict(v_dim=0), dict(v_dim=300)):
+            with pytest.raises(PtError, match="torch.uint8"):
+                cache(dtype, **kw)
+        own = cache(torch.uint8, pool=made.pool.view(torch.uint8))
+        assert own.scales is None and own.pool.data_ptr() == made.pool.data_ptr()
+    assert cache(torch.uint8, v_dim=0).pool.shape == (4, 2 * 64 * 64) and cache(torch.uint8, v_dim=300).pool.shape == (4, 2 * 64 * 364)
+    with pytest.raises(PtError, match="is wanted"):
+        ops._kv8(cache(torch.uint8), "kv8_attn")
