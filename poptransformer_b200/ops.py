@@ -994,19 +994,24 @@ def rotary(x, heads, dim, rope, positions, out=None, rope_dims=None, interleaved
 
 
 def _kv8(cache, who):
-    """The structure of a cache of eight bits.  (Made once: its tensors are the same from call to call.)"""
-    pool, scales, table, made = cache.pool, cache.scales, cache.page_table, cache.kv8
-    if made is not None and made[0] is pool and made[1] is scales and made[2] is table and made[4] == (pool.data_ptr(), scales.data_ptr(), table.data_ptr()):
+    """The structure of a cache of eight bits.  (Made once, and again where any of what is in it has changed.)"""
+    pool, scales, table, made = cache.pool, getattr(cache, "scales", None), cache.page_table, getattr(cache, "kv8", None)
+    if made is not None and made[0] is pool and made[1] is scales and made[2] is table and made[4] == (pool.data_ptr(), scales.data_ptr(), table.data_ptr()) and \
+            made[5] == (cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.size(-1), cache.max_len):
         return made[3]
     fmt = KV8_FORMATS.get(pool.dtype)
     if fmt is None:
         raise PtError(f"{who}: a cache of {pool.dtype}; int8 or float8_e4m3fn is wanted")
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] * cache.page_size < cache.max_len:
         raise PtError(f"{who}: the page table is int32 [slots, pages of {cache.max_len} positions], got {table.dtype} {tuple(table.shape)}")
+    rows = cache.n_kv * cache.page_size
+    if pool.dim() == 0 or pool.numel() != pool.shape[0] * rows * (cache.head_dim + cache.v_dim) or scales.dtype != torch.float32 or scales.numel() != pool.shape[0] * rows * 2:
+        raise PtError(f"{who}: pages of {cache.page_size} positions of {cache.n_kv} heads of {cache.head_dim} and {cache.v_dim}, got {tuple(pool.shape)} with scales {scales.dtype} {tuple(scales.shape)}")
     if not pool.get_device() == scales.get_device() == table.get_device():
         raise PtError(f"{who}: pool on {pool.device}, scales on {scales.device}, page table on {table.device}")
-    made = Kv8Cache(_ptr(pool), _ptr(scales), _ptr(table), fmt, cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len)
-    cache.kv8 = (pool, scales, table, made, (made.pool, made.scales, made.page_table))
+    sizes = cache.n_kv, cache.head_dim, cache.v_dim, cache.page_size, table.shape[1], cache.max_len
+    made = Kv8Cache(_ptr(pool), _ptr(scales), _ptr(table), fmt, *sizes)
+    cache.kv8 = (pool, scales, table, made, (made.pool, made.scales, made.page_table), sizes)
     return made
 
 

@@ -87,3 +87,30 @@ def test_pages_of_bytes_without_scales():
     assert cache(torch.uint8, v_dim=0).pool.shape == (4, 2 * 64 * 64) and cache(torch.uint8, v_dim=300).pool.shape == (4, 2 * 64 * 364)
     with pytest.raises(PtError, match="is wanted"):
         ops._kv8(cache(torch.uint8), "kv8_attn")
+
+
+def test_a_changed_cache_is_looked_at_again(monkeypatch):
+    """The structure that the kernels get is kept from call to call, and says what the cache says now."""
+    monkeypatch.setattr(ops, "_ptr", lambda t: None if t is None else t.data_ptr())
+    c = cache()
+    first = ops._kv8(c, "kv8_attn")
+    assert ops._kv8(c, "kv8_attn") is first and first.max_len == 128 and first.max_pages == 2
+    c.max_len = 100                                   # positions from 100 on are refused from now on
+    assert ops._kv8(c, "kv8_attn").max_len == 100
+    c.max_len = 129                                   # more than the table has pages for
+    with pytest.raises(PtError, match="page table"):
+        ops._kv8(c, "kv8_attn")
+    c.max_len, table = 128, torch.zeros((2, 5), dtype=torch.int32)
+    c.page_table = table
+    assert ops._kv8(c, "kv8_attn").max_pages == 5
+    table.resize_(2, 2)                               # the same tensor at the same place
+    assert ops._kv8(c, "kv8_attn").max_pages == 2
+    c.page_size, c.max_len = 32, 64                   # (two pages of 32)
+    with pytest.raises(PtError, match="pages of 32 positions"):
+        ops._kv8(c, "kv8_attn")
+    c.n_kv = 4                                        # the same bytes, as twice the heads of half of the positions
+    made = ops._kv8(c, "kv8_attn")
+    assert (made.n_kv, made.page_size, made.max_len) == (4, 32, 64)
+    c.head_dim = 65
+    with pytest.raises(PtError, match="heads of 65 and 64"):
+        ops._kv8(c, "kv8_attn")
