@@ -953,7 +953,7 @@ def _here(who, *tensors):
 
 
 def _rope_ok(who, rope, rope_dims, positions):
-    if rope_dims and (rope is None or rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[0] < positions or rope.shape[1] * 2 != rope_dims or rope.shape[2] != 2):
+    if rope is None or (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[0] < positions or rope.shape[1] * 2 != rope_dims or rope.shape[2] != 2):
         raise PtError(f"{who}: {rope_dims} rotated dimensions want float32 rope [{positions} positions or more, {rope_dims // 2}, 2], got "
                       f"{None if rope is None else (rope.dtype, tuple(rope.shape))}")
 
@@ -1020,15 +1020,18 @@ def _rows_fit(who, name, t, rows, width, ld):
         raise PtError(f"{who}: {name} has {t.numel()} elements, {rows} rows of {width} at a stride of {ld} are wanted")
 
 
-def kv8_append(view, rows, ld, cache, n_head=0, rope=None, rope_dims=0, interleaved=False, q_out=None, q_out_ld=0, error_flag=None):
+def kv8_append(view, rows, ld, cache, n_head=0, rope=None, rope_dims=None, interleaved=False, q_out=None, q_out_ld=0, error_flag=None):
     """Keys (rotated) and values of the packed tokens of `view` go to a cache of eight bits (see pt_kv8_append).  Rows hold [q | k | v] of n_head query heads, or [k | v] with n_head = 0.  q_out: where
-    the rotated queries go, rows of q_out_ld (`rows` itself rotates them in place).  rope: as rope_table makes it, of cache.max_len positions or more."""
+    the rotated queries go, rows of q_out_ld (`rows` itself rotates them in place).  rope: as rope_table makes it, of cache.max_len positions or more.  rope_dims: rotated dimensions at the front of a head (None: the
+    table's; without a table nothing turns)."""
     n_tok, n_kv, dim, vdim, es, dtype = view.n_tok, cache.n_kv, cache.head_dim, cache.v_dim, rows.element_size(), rows.dtype
     now = torch._C._cuda_getDevice() if rows.is_cuda else -1
     if not (rows.get_device() == cache.pool.get_device() == view.keep[0].get_device() == now >= 0 and (rope is None or rope.get_device() == now) and (q_out is None or q_out.get_device() == now)
             and (error_flag is None or error_flag.get_device() == now)):
         _here("kv8_append", rows, cache.pool, *view.keep, rope, q_out, error_flag)
-    if rope_dims:
+    if rope_dims is None:
+        rope_dims = 2 * rope.shape[1] if rope is not None and rope.dim() == 3 else 0
+    if rope_dims or rope is not None:
         _rope_ok("kv8_append", rope, rope_dims, cache.max_len)
     _rows_fit("kv8_append", "rows", rows, n_tok, (n_head + n_kv) * dim + n_kv * vdim, ld)
     to = None

@@ -35,3 +35,13 @@ def test_pages_of_bytes_are_copied(cuda, dim, vdim):
     want[3] = want[0]
     ops.PagePools([kv]).copy_pages(ku.ints([0]), ku.ints([3]))
     assert torch.equal(kv.pool, want)
+
+
+@pytest.mark.parametrize("rot", [32, 64])
+def test_appending_turns_what_the_table_turns(cuda, rot):
+    from poptransformer_b200 import ops
+    s = ku.batch([5, 2], [10, 70], torch.float16, torch.int8, rot=rot, seed=rot)
+    pool, scales, q = ku.appended(s)
+    out = torch.empty((s.n_tok, s.q_cols), dtype=s.dtype, device=cuda)
+    ops.kv8_append(s.view, s.qkv, s.ld, s.cache, s.heads, rope=s.rope, q_out=out, q_out_ld=s.q_cols, error_flag=s.flag)
+    assert torch.equal(s.pool.view(torch.uint8).cpu(), pool) and torch.equal(s.scales.cpu().nan_to_num(-1), scales.nan_to_num(-1)) and torch.equal(out.cpu(), q.to(s.dtype)) and s.flag.item() == 0

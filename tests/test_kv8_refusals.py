@@ -114,3 +114,29 @@ def test_a_changed_cache_is_looked_at_again(monkeypatch):
     c.head_dim = 65
     with pytest.raises(PtError, match="heads of 65 and 64"):
         ops._kv8(c, "kv8_attn")
+
+
+def test_a_table_of_angles_says_how_much_turns(monkeypatch):
+    """kv8_append rotates as wide as its table is, like rotary; a width that is not the table's is refused, 0 too."""
+    monkeypatch.setattr(ops, "_ptr", lambda t: None if t is None else t.data_ptr())
+    monkeypatch.setattr(ops, "_here", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    seen = []
+
+    class Library:
+        def pt_kv8_append(self, a, stream):
+            seen.append(a._obj.rope_dims)
+            return 0
+
+    monkeypatch.setattr(ops._lib, "lib", Library)
+    c, i = cache(), torch.zeros(2, dtype=torch.int32)
+    view = _lib.BatchView(1, 1)
+    view.keep = (i, i, i, i)
+    x, rope = torch.zeros((1, 6 * 64), dtype=torch.float16), ops.rope_table(128, 32, device="cpu")
+    for kw, dims in ((dict(rope=rope), 32), (dict(rope=rope, rope_dims=32), 32), (dict(), 0), (dict(rope_dims=0), 0), (dict(rope_dims=None), 0)):
+        ops.kv8_append(view, x, 384, c, 2, **kw)
+        assert seen.pop() == dims
+    for kw in (dict(rope=rope, rope_dims=0), dict(rope=rope, rope_dims=64), dict(rope_dims=32), dict(rope=rope[:100]), dict(rope=rope.double()), dict(rope=rope[0]), dict(rope=rope[:, 0, 0])):
+        with pytest.raises(PtError, match="rotated dimensions"):
+            ops.kv8_append(view, x, 384, c, 2, **kw)
+    assert not seen
