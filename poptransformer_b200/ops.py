@@ -969,9 +969,11 @@ def _row_ld(who, name, t, rows, width):
 def rotary(x, heads, dim, rope, positions, out=None, rope_dims=None, interleaved=False, inverse=False, error_flag=None):
     """Rows of heads rotated by their positions (see pt_rotary): x [rows, heads * dim or more], whose rows may lie apart (a part of wider rows), positions int32 [rows], rope as rope_table makes
     it.  out: None rotates x itself.  rope_dims: rotated dimensions at the front of a head (None: the table's).  interleaved: pairs are neighbours.  inverse: by
-    the negative angles, which takes the gradient of the output to that of x."""
+    the negative angles, which takes the gradient of the output to that of x.  The call records no gradient: a tensor that wants one is refused while gradients are recorded."""
     rows, table, dtype = x.shape[0], rope.shape, x.dtype
     out = x if out is None else out
+    if (x.requires_grad or out.requires_grad) and torch.is_grad_enabled():
+        raise PtError("rotary: the tensor wants a gradient, which this call does not record: call it under torch.no_grad(), on the detached rows, and on the gradient with inverse=True")
     rope_dims = table[1] * 2 if rope_dims is None else rope_dims
     now = torch._C._cuda_getDevice() if x.is_cuda else -1
     # (One look at what is right, the same again with words where it is not: a launch takes less time than the checks one by one.)

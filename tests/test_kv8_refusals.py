@@ -140,3 +140,16 @@ def test_a_table_of_angles_says_how_much_turns(monkeypatch):
         with pytest.raises(PtError, match="rotated dimensions"):
             ops.kv8_append(view, x, 384, c, 2, **kw)
     assert not seen
+
+
+def test_rotary_refuses_rows_that_want_a_gradient():
+    """The call records none; without recording, such rows are as good as others."""
+    rope, at = ops.rope_table(4, 64, device="cpu"), torch.zeros(1, dtype=torch.int32)
+    leaf, plain = torch.zeros((1, 64), requires_grad=True), torch.zeros((1, 64))
+    for x, out in ((leaf, None), (leaf * 2.0, None), (leaf, plain), (plain, leaf)):
+        with pytest.raises(PtError, match="wants a gradient"):
+            ops.rotary(x, 1, 64, rope, at, out=out)
+        with torch.no_grad(), pytest.raises(PtError, match="device"):           # (the next check: everything is on the CPU here)
+            ops.rotary(x, 1, 64, rope, at, out=out)
+    with pytest.raises(PtError, match="device"):
+        ops.rotary(leaf.detach(), 1, 64, rope, at)
