@@ -1078,7 +1078,8 @@ def kv8_attn(view, q, q_ld, cache, out, out_ld, n_head, scale, window=0, softcap
 
 def kv8_unpack(view, cache, into, error_flag=None):
     """All positions of the sequences of `view`, the cached and the new ones, from a cache of eight bits into the pages of one of 16 or 32 bits (`into`: same heads, its own table with the same slots), for
-    the kernels that read those: a prompt's window_attn(append=False), for instance (see pt_kv8_unpack)."""
+    the kernels that read those (see pt_kv8_unpack): window_attn(append=False) for a prompt, whose rows and pages are bf16 or fp32 (queries of fp16 go with fp32 pages, and lose nothing);
+    tree_attn for chunks of up to 256 tokens of any type, which puts the chunk's own keys and values into those pages."""
     _wide(into, "kv8_unpack (into)")
     pool, table = into.pool, into.page_table
     if into.n_kv != cache.n_kv or into.head_dim != cache.head_dim or into.v_dim != cache.v_dim:
