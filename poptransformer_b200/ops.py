@@ -913,8 +913,8 @@ def rope_table(positions, dims, base=10000.0, scaling=None, device="cuda"):
       "bands":  pairs that turn less than `low` times over `original` are divided by `factor`, those that turn more than `high` times are left, in proportion to their turns between."""
     if dims <= 0 or dims % 2 or positions <= 0:
         raise PtError(f"rope_table: {positions} positions of {dims} dimensions (an even number)")
-    if base <= 0 or any(not float(v) > 0 for k, v in (scaling or {}).items() if k != "kind"):
-        raise PtError(f"rope_table: base {base} and scaling {scaling} are positive")
+    if any(not 0 < float(v) < math.inf for v in [base] + [v for k, v in (scaling or {}).items() if k != "kind"]):
+        raise PtError(f"rope_table: base {base} and scaling {scaling} are positive numbers")
     kind, s, magnitude = (scaling or {}).get("kind"), dict(scaling or {}), 1.0
     i = torch.arange(dims // 2, dtype=torch.float64, device=device)
     try:
@@ -927,12 +927,16 @@ def rope_table(positions, dims, base=10000.0, scaling=None, device="cuda"):
             f = f / float(s["factor"])
         elif kind == "ramp":
             factor, original = float(s["factor"]), float(s["original"])
+            if base <= 1 or float(s.get("slow", 1)) >= float(s.get("fast", 32)):
+                raise PtError(f"rope_table: a ramp wants a base above 1 and slow below fast, got base {base} and {scaling}")
             pair = lambda turns: dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
             lo, hi = max(math.floor(pair(float(s.get("fast", 32)))), 0), min(math.ceil(pair(float(s.get("slow", 1)))), dims - 1)
             kept = 1.0 - ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
             f = f / factor * (1.0 - kept) + f * kept
             magnitude = float(s.get("magnitude", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
         elif kind == "bands":
+            if float(s["low"]) >= float(s["high"]):
+                raise PtError(f"rope_table: bands want low below high, got {scaling}")
             turns = float(s["original"]) * f / (2 * math.pi)
             kept = ((turns - float(s["low"])) / (float(s["high"]) - float(s["low"]))).clamp(0, 1)
             f = f / float(s["factor"]) * (1.0 - kept) + f * kept

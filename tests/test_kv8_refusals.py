@@ -1,4 +1,5 @@
 """Caches of eight bits and of other widths than the rows': what the calls beside them say before any launch."""
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -153,3 +154,15 @@ def test_rotary_refuses_rows_that_want_a_gradient():
             ops.rotary(x, 1, 64, rope, at, out=out)
     with pytest.raises(PtError, match="device"):
         ops.rotary(leaf.detach(), 1, 64, rope, at)
+
+
+def test_tables_of_angles_that_would_be_no_numbers():
+    """Sizes that are no finite numbers, and bounds that leave nothing between them or stand in the wrong order."""
+    for kw in (dict(base=math.nan), dict(base=math.inf), dict(scaling=dict(kind="linear", factor=math.inf)), dict(scaling=dict(kind="base", factor=math.nan)),
+               dict(scaling=dict(kind="bands", factor=2.0, original=64, low=4.0, high=4.0)), dict(scaling=dict(kind="bands", factor=2.0, original=64, low=4.0, high=1.0)),
+               dict(base=1.0, scaling=dict(kind="ramp", factor=2.0, original=64)), dict(base=0.5, scaling=dict(kind="ramp", factor=2.0, original=64)),
+               dict(scaling=dict(kind="ramp", factor=2.0, original=64, slow=32, fast=32)), dict(scaling=dict(kind="ramp", factor=2.0, original=64, slow=40))):
+        with pytest.raises(PtError, match="rope_table"):
+            ops.rope_table(8, 8, device="cpu", **kw)
+    for kw in (dict(base=0.5), dict(base=1.0), dict(scaling=dict(kind="bands", factor=2.0, original=64, low=1.0, high=4.0)), dict(scaling=dict(kind="ramp", factor=1.0, original=64))):
+        assert ops.rope_table(8, 8, device="cpu", **kw).isfinite().all()
