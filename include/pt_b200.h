@@ -966,7 +966,7 @@ typedef struct pt_kv8_append_args {
   const void *q, *k, *v;
   int ld;
   void *q_out;            /* or NULL: q is not looked at                             */
-  int q_out_ld, rope_dims, interleaved;
+  int q_out_ld, rope_dims, interleaved;   /* rope_dims 0: nothing turns             */
   const float *rope;      /* fp32 [max_len, rope_dims / 2, 2]                        */
   int32_t *error_flag;
 } pt_kv8_append_args;
@@ -975,7 +975,11 @@ int pt_kv8_append(const pt_kv8_append_args *args, void *stream);
 /* pt_kv8_attn: token i of sequence s attends to the cached positions up to its own, start[s] + i (which pt_kv8_append has written): out[h] = sum_j w_j v_j,
  * w = softmax(c(scale q[h] . k_j)) over the last `window` of them (0: all); softcap c: a score x becomes c tanh(x / c) (0: none).  out may be q itself where keys and values are equally wide.  Meant for few tokens a
  * sequence: every token reads its history by itself.  A negative page reads as some other page, and sets error_flag to 12, unless all
- * of its positions lie in front of the window: those pages may be gone. */
+ * of its positions lie in front of the window: those pages may be gone.
+ * All sums are in 32 bits.  The kernel for any sizes (plain, heads or pages that are no multiple of 16) has everything else in 32 bits too.  The others multiply the bytes as they are; weights are two fp16
+ * parts (2^-21 of a weight); queries are kept to 2^-22 of the largest element of their head over int8 keys, and over E4M3 keys to 2^-25 of it (bf16: whole).  Rows of fp32 whose queries have single large elements
+ * lose by that: with one of 30 times the others 5e-6 of the output's size, where 32 bits lose 2e-6.
+ * A query with a NaN or an infinity has outputs that are NaN, but for an infinity under a softcap: the kernel for any sizes, and bf16 over E4M3, see a score of -c or c, the others NaN. */
 typedef struct pt_kv8_attn_args {
   pt_batch_view batch;
   pt_kv8_cache cache;
@@ -995,7 +999,8 @@ size_t pt_kv8_attn_workspace_bytes(int n_tok, int n_head, int n_kv, int width); 
 int pt_kv8_attn(const pt_kv8_attn_args *args, void *stream);
 
 /* pt_kv8_unpack: positions 0 .. start[s] + tokens - 1 of every sequence <- byte * scale, rounded once, in another pool's pages (K [n_kv][into_page_size][dim]
- * and then V [n_kv][into_page_size][vdim]), which have a table of their own with the same slots: for kernels that read caches of the rows' type. */
+ * and then V [n_kv][into_page_size][vdim]), which have a table of their own with the same slots: for kernels that read caches of the rows' type.  (A prompt that reads them in 16 bits sees keys and
+ * values that are rounded once more than those of pt_kv8_attn; in fp32 they are the same.)  The launch goes by max_len, not by the lengths, which are on the device: a limit far above them costs time. */
 typedef struct pt_kv8_unpack_args {
   pt_batch_view batch;
   pt_kv8_cache cache;

@@ -39,7 +39,8 @@ struct Rotary {
 };
 // LANES lanes (16 elements each) for a head of a row; a thread has one.  Bound by memory: rows in and out once.  So nothing waits for the position before the row has been asked for, and no lane
 // loops (4000 rows of 34 heads of 128, half of each turned: 13.3 us, 5.3 TB/s; a block a row, whose lanes went
-// through its heads in turn with the angles in registers, 16.1).
+// through its heads in turn with the angles in registers, 16.1).  Rotated parts, heads or addresses that are no multiples of 16 go element by element: 4000 rows of 34 heads of 80, 20 of each turned, 55 us
+// (neighbours 62) for 6.7 of bytes.
 template <typename T, int LANES, bool WHOLE, bool INVERSE, bool NEIGHBOURS>
 __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const T *x, T *out, const Rotary p) {
   early_start();
@@ -167,7 +168,7 @@ __device__ __forceinline__ void append_rows(const T *src, T *q_out, const Append
 }
 // Bound by memory, and before that by the way to a token's place (sequence, position, page, angles), which is gone once for all of a lane's rows, after they have been asked for.  11,000 tokens
 // of 32 + 8 + 8 heads of 128, 250 MB: 46.0 us, 5.4 TB/s; a row a lane 69.7, two rows of any kind 59.0 (selects and addresses of three kinds).  Where there is less than a wave of rows one is
-// faster: a token 2.4 us.
+// faster: a token 2.4 us.  Element by element (as in the rotation; heads of 80, 20 of each turned) 204 us for 23 of bytes; heads of 80 that turn whole 40.
 template <typename T, int LANES, int ROWS, bool WHOLE, bool NEIGHBOURS, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 4) append_kernel(const T *q, const T *k, const T *v, T *q_out, const Append p) {
   early_start();
@@ -197,6 +198,7 @@ template <bool E4M3> __device__ __forceinline__ void from_word(uint32_t w, float
 }
 // Block: rows_each positions of a sequence, keys or values of heads_each heads.  Bound by memory: a thread finds its places once and asks for four heads' bytes together, and a warp's stores are whole
 // sectors.  4 sequences of up to 16500 positions, 8 heads of 128, E4M3 to fp16, 299 MB: 49.7 us, 6.0 TB/s (a block a head, which found its places again, 63.4; stores of half sectors 60.4).
+// Blocks are launched for what the tables can hold: 8 sequences of 700 positions 6.2 us, in tables of 131072 136.
 template <typename T, bool WHOLE, bool E4M3> __global__ void __launch_bounds__(THREADS) unpack_kernel(T *into, const Unpack p) {
   early_start();
   const int parts = gridDim.z / 2;

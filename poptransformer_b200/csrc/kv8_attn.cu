@@ -35,8 +35,8 @@ struct Attn {
 };
 
 constexpr int HEADS = 8, MAX_TOKENS = 1024;
-constexpr int SHORT = 3;      // tiles of a warp up to which a segment stays in one block (32 query over 8 kv heads of 128, one token: 700 positions 10.2 us so, 13.0 dealt out; 1300 13.7 either way)
-constexpr int ALIGNED = 6;    // ... and up to which a block has whole segments (64 sequences of 300 positions 21.0 us dealt out evenly, so 18.6; of 2000 48.5 and 45.7; from 9 on the blocks' loads differ too much)
+constexpr int SHORT = 3;      // tiles of a warp up to which a segment stays in one block (32 query over 8 kv heads of 128, one token: 700 positions 10.2 us so, 13.0 dealt out; 1300 13.7 either way; both limits were measured at this width alone)
+constexpr int ALIGNED = 6;    // ... and up to which a block has whole segments (64 sequences of 300 positions 21.0 us dealt out evenly, so 19.2; of 2000 48.5 and 46.3; from 9 on the blocks' loads differ too much)
 constexpr int COUNTERS = 1 << 16;      // of a workspace, always in front: whichever calls share one, nothing else is written there
 
 // SIZE: the widest head, 64, 128 or 256.

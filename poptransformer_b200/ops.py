@@ -859,7 +859,7 @@ class PagedKVCache:
 
 
 class PagePools:
-    """The pools of a model's layers, which share one page numbering (and page table): what is copied or moved is copied in all of them by one launch."""
+    """The pools of a model's layers, which share one page numbering (and page table): what is copied or moved is copied in all of them by one launch (and the scales of caches of eight bits by one more)."""
 
     def __init__(self, caches):
         caches = list(caches)
